@@ -45,6 +45,10 @@ extern "C" {
    of this library with no counterpart in the reference or the GGUF; the same
    bytes per row, the same results as QMAG_TYPE_Q6_K). */
 #define QMAG_TYPE_Q6_K_R 270
+/* Activation types of the attention entries (GGML's type ids). */
+#define QMAG_TYPE_F32 0
+#define QMAG_TYPE_F16 1
+#define QMAG_TYPE_BF16 30
 
 #define QMAG_OK 0
 #define QMAG_ERR_HIP (-1)      /* a HIP runtime call failed                  */
@@ -130,7 +134,8 @@ int qmag_event_elapsed(int a, int b, float *ms);
    the library stream.  Kernel ids: 0 router, 1 top-k/Q8_K(x), 2 gate/up,
    3 Q8_K(h), 4 down+combine, 5 fused decode, 6 matvec (matmul entries),
    7 Q8_K quantisation (every launch of it), 8 grouping (prefill), 9 combine
-   (prefill).  qmag_prof_read synchronises and
+   (prefill), 10 rotary positions, 11 cache bookkeeping, append and read,
+   12 attention (both launches of a call).  qmag_prof_read synchronises and
    returns the launch count and summed milliseconds of one id. */
 int qmag_prof_enable(int on);
 int qmag_prof_read(int kernel_id, long *count, double *total_ms);
@@ -469,6 +474,144 @@ int qmag_sampler_candidates_dev(int n_vocab, const float *logits, const qmag_sam
    calls again. */
 int qmag_sampler_sample_dev(int n_vocab, const float *logits, qmag_sampler *s, int max_k, float top_p,
                             int *token);
+
+/* ------------------------------------------------------------------------ */
+/* Attention: rotary positions, a paged 4-bit cache, attention over it and   */
+/* over whole prompts                                                        */
+/* ------------------------------------------------------------------------ */
+
+/* What a program calls between the projections (qmag_matmul_group_dev) and
+   the MoE layer to keep a sequence on the device:
+
+     prompt   rope -> attn_prompt, and kv4_append for the tokens to come
+     decode   kv_assign -> rope -> kv4_append -> attn_kv4
+
+   Device pointers throughout, ordered on the library stream, one host thread
+   at a time, as the other device entries.  Activations are f32, f16 or bf16
+   (`type`: QMAG_TYPE_F32 / _F16 / _BF16), one type for all of a call's views.
+   f32 calls keep fp32 accuracy (about 2^-22 of a row's largest value in each
+   operand); 16-bit calls hold weights to the type's own bits and round the
+   result once.  Scores, sums and maxima are fp32. */
+
+/* Heads in memory: value c of head h of token t lies at
+   ptr[t * token_stride + h * head_stride + c], strides in values.  q of the
+   engine's attention layer, which lies beside its gate: {d_q, N_HEAD,
+   2 * N_HEAD * N_EMBD_HEAD, 2 * N_EMBD_HEAD}.  Any strides; ptr and strides of
+   whole 16 bytes are the fast form.  Views that are written hold each value
+   once and overlap no view that is read, except where said. */
+#define QMAG_MAX_HEADS 4096
+typedef struct qmag_heads {
+    void *ptr;
+    int n_head;
+    int64_t token_stride, head_stride;
+} qmag_heads;
+
+/* Rotary positions with several axes (rope_imrope, nn.c:841-861; time, height
+   and width of images and video).  The first n_rot values of each head turn in
+   pairs, pair i by pos[axis][t] * theta^(-2 i / n_rot); the others stay. */
+#define QMAG_ROPE_MAX_DIM 1024
+typedef struct qmag_rope {
+    int head_dim;       /* 2..QMAG_ROPE_MAX_DIM */
+    int n_rot;          /* even, 2..min(head_dim, 256) */
+    int n_axes;         /* 1..4 */
+    int sections[4];    /* pairs of each axis, n_rot / 2 together */
+    int interleaved;    /* 0: the axes' pairs in runs; 1: in turns, an axis whose pairs are used up passed over */
+    int adjacent;       /* 0: pair i is values i and i + n_rot / 2; 1: values 2 i and 2 i + 1 */
+    double theta;       /* > 0 */
+} qmag_rope;
+/* pos: i32 [n_axes][T].  src -> dst for n_views (1 or 2: q and k) views; a dst
+   equal to its src turns in place.  Angles are formed in 64 bits. */
+int qmag_rope_dev(const qmag_rope *r, const int *pos, int T, int type, const qmag_heads *src, const qmag_heads *dst,
+                  int n_views);
+
+/* The blocks of a paged cache: table[i][c] is the block that holds tokens
+   c * block_size .. of sequence i; blocks nobody holds are
+   free_list[0 .. n_free), n_free a word on the device. */
+#define QMAG_KV_MAX_SEQ 4096
+typedef struct qmag_kv_table {
+    int n_seq;          /* 0..QMAG_KV_MAX_SEQ */
+    int max_blocks;     /* columns */
+    int block_size;     /* tokens of a block: a power of two from 16 to 256 */
+    int n_block;        /* blocks of the cache; n_block * block_size < 2^31 */
+    int *table;         /* i32 [n_seq][max_blocks] */
+    int *free_list;     /* i32 [n_block] (not used by qmag_attn_kv4_dev) */
+} qmag_kv_table;
+
+/* What the bookkeeping calls leave in *status (device): */
+#define QMAG_KV_OK 0
+#define QMAG_KV_FULL 1    /* too few free blocks */
+#define QMAG_KV_ROW 2     /* a sequence of more than max_blocks blocks */
+#define QMAG_KV_LENGTH 3  /* a negative length, or more new tokens than T */
+#define QMAG_KV_LIST 4    /* n_free outside 0..n_block, or more blocks given back than the list has room for */
+
+/* Blocks of ended sequences go back: for each i with ended[i] != 0, in
+   ascending order, table[i]'s ceil(len[i] / block_size) blocks are appended to
+   the free list and len_next[i] = 0; other lengths are copied.  len_next and
+   n_free_next are places of their own (a step may then be issued again).  With
+   a status other than 0 nothing is given back, len_next = len and
+   *n_free_next = *n_free. */
+int qmag_kv_release_dev(const qmag_kv_table *t, const int *len, const int *ended, const int *n_free, int *len_next,
+                        int *n_free_next, int *status);
+
+/* Blocks for new tokens: sequence i, which holds len[i] tokens, gets n_new[i]
+   more.  Blocks are taken from the end of the free list, by ascending sequence
+   and column, and written to the table.  Token t = cu[i] + j (cu: i32
+   [n_seq + 1], the sums of n_new) is token pos[t] = len[i] + j of sequence i and
+   goes to slot[t] = block * block_size + place in the block.  slot and pos have T
+   entries; those behind the last token get slot -1 and pos 0.  len_next[i] =
+   len[i] + n_new[i].  With a status other than 0 no block is taken, every slot
+   is -1, cu is 0, and len_next and *n_free_next are as before. */
+int qmag_kv_assign_dev(const qmag_kv_table *t, const int *len, const int *n_new, const int *n_free, int T, int *slot,
+                       int *pos, int *cu, int *len_next, int *n_free_next, int *status);
+
+/* A cache held in 4 bits.  A block holds for each kv head [K codes | K scales |
+   V codes | V scales] of its block_size tokens: per token head_dim / 2 bytes of
+   codes and per 64 values a step d and a minimum m in fp16 (d first); a value is
+   d * code + m.  m = fp16(min), d = fp16((max - min) / 15), code = (x - m) / d to
+   the nearest even whole number within 0..15, each step in fp32 as written; m
+   and d saturate, and 64 values with an infinity or a NaN among them are all
+   NaN.  Codes of a token's K row: dword h * head_dim / 32 + 2 g + s holds channels
+   64 g + 32 s + 8 h .. + 7, lowest bits first; of its V row: 16-bit word
+   i * head_dim / 64 + g holds channels 64 g + 4 i .. + 3. */
+typedef struct qmag_kv4 {
+    void *data;         /* n_block * qmag_kv4_block_bytes, 16-byte aligned */
+    int n_block;
+    int block_size;     /* a power of two from 16 to 256 */
+    int n_kv;           /* kv heads */
+    int head_dim;       /* 64, 128 or 256 */
+} qmag_kv4;
+/* Bytes of a block (data and n_block are not read); needs no GPU. */
+int qmag_kv4_block_bytes(const qmag_kv4 *c, size_t *bytes);
+/* K and V of T tokens (n_kv heads each) into their slots; a token whose slot is
+   outside the cache (-1: a padded one) is left out.  A slot named twice holds
+   one of the tokens, or parts of both. */
+int qmag_kv4_append_dev(const qmag_kv4 *c, int type, const qmag_heads *k, const qmag_heads *v, const int *slot, int T);
+/* The values the cache holds for T slots, f32 [T][n_kv][head_dim] each; zeros
+   for a slot outside it. */
+int qmag_kv4_read_dev(const qmag_kv4 *c, const int *slot, int T, float *k, float *v);
+
+/* Attention of the newest tokens over the cache (attn_worker over its 4-bit
+   tier, nn.c:1215-1453).  Sequence i has len[i] tokens in the cache (the newest
+   among them) and rows cu[i] .. cu[i + 1] - 1 of q ask: row j of its n is token
+   len[i] - n + j and sees the tokens up to itself.  T: rows of q and out; heads
+   of q share kv heads in runs of q->n_head / n_kv.  A row that sees nothing is
+   zero, and so a row ahead of its sequence; rows behind cu[n_seq] are left as
+   they were.  A table entry outside the cache stands for tokens that are not
+   there.  What the cache holds where a row does not see has no effect on it.
+   t->n_block and block_size are the cache's; max_blocks * block_size <= 2^30.
+   Sequences are split over the chip by their lengths and joined in a fixed
+   order: equal calls give equal bits. */
+#define QMAG_ATTN_MAX_TOKENS (1 << 22)
+int qmag_attn_kv4_dev(const qmag_kv4 *c, const qmag_kv_table *t, int type, const qmag_heads *q, const qmag_heads *out,
+                      const int *cu, const int *len, int T, float scale);
+
+/* Causal attention over n_seq prompts packed one behind another: sequence i is
+   rows cu[i] .. cu[i + 1] - 1 of q, k, v and out (cu ascending, cu[n_seq] <= T;
+   empty sequences are fine; rows behind cu[n_seq] are left as they were).  Heads
+   of q share kv heads in runs of q->n_head / k->n_head.  Infinities and NaN at
+   keys that a row does not see have no effect on it. */
+int qmag_attn_prompt_dev(int type, int head_dim, const qmag_heads *q, const qmag_heads *k, const qmag_heads *v,
+                         const qmag_heads *out, const int *cu, int n_seq, int T, float scale);
 
 /* ------------------------------------------------------------------------ */
 /* Synthetic inputs (bench/test utilities; not part of the reference)        */

@@ -1,0 +1,483 @@
+// qmag_attn.hip -- causal attention over whole prompts, packed one behind
+// another, heads in groups that share K and V (the role of attn_worker on a
+// prompt chunk, src/nn.c:1215-1453).
+//
+//   o_i = sum_{j <= i} p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - max_i)
+//
+// Two launches.  The first lays K and V out in tiles of 32 keys of one sequence
+// and kv head, in the order the second's LDS wants them, rows behind a
+// sequence's end zero.  The second takes 128 queries of a head per workgroup,
+// 32 to a wave, and passes over the tiles once with a running maximum and sum.
+//
+// 16-bit calls multiply in their own type.  fp32 calls are carried by the fp16
+// matrix cores, 16 times the fp32 ones' rate: every row of Q, K and V is scaled
+// by a power of two (exact) and split into two fp16 parts, x = hi + lo to 22
+// bits, and a product is hi hi + hi lo + lo hi.
+//
+// S^T = K Q^T by v_mfma_f32_32x32x16 leaves a lane with one query (n = lane % 32)
+// and keys 8 (r / 4) + 4 (lane / 32) + r % 4 of a tile; O^T = V^T P^T takes the
+// weights as they are when V's keys are read in that order, so they never leave
+// their lane.  V^T comes from row-major LDS by transposing reads.
+#include "qmag_attn.h"
+
+namespace qmag {
+
+constexpr int AP_WG = 256;
+constexpr int AP_ROWS = 128;              // queries of a workgroup
+constexpr int AP_KEYS = 32;               // keys of a tile
+
+struct ApArgs {
+    const void *q, *k, *v;
+    void *out;
+    int64_t qt, qh, kt, kh, vt, vh, ot, oh;
+    const int *cu;
+    uint8_t *img;                         // [n_kv][tiles][K image | V image]
+    float *scale;                         // [n_kv][tiles][32 of K | 32 of V], fp32 calls
+    int *odd;                             // [n_kv][tiles]: V holds an infinity or a NaN
+    int n_seq, T, tiles, n_kv, G;
+    float sc;                             // scale * log2 e
+    int q_vec, k_vec, v_vec, o_vec;
+};
+
+// Sequence i's rows, and its first tile: floor(cu / 32) + i leaves every
+// sequence the tiles it needs, whatever the lengths.
+__device__ __forceinline__ void ap_seq(const ApArgs &A, int i, int *a, int *n)
+{
+    *a = min(max(A.cu[i], 0), A.T);
+    *n = max(min(max(A.cu[i + 1], 0), A.T) - *a, 0);
+}
+
+// The sequence and part of it that hold unit `want` of `per` rows each; last:
+// counted from the end.  Found by the calling wave alone.
+__device__ __forceinline__ bool ap_find(const ApArgs &A, int want, int per, bool last, int *seq, int *part, int *a, int *n)
+{
+    const int lane = lane_id();
+    int x, len;
+    if (last) {
+        long long all = 0;
+        for (int i = lane; i < A.n_seq; i += 64) {
+            ap_seq(A, i, &x, &len);
+            all += (len + per - 1) / per;
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+        if (want >= all) return false;
+        want = (int)min(all - 1 - want, (long long)INT32_MAX);
+    }
+    long long before = 0;
+    for (int base = 0; base < A.n_seq; base += 64) {
+        const int i = base + lane;
+        x = len = 0;
+        if (i < A.n_seq) ap_seq(A, i, &x, &len);
+        const int mine = (len + per - 1) / per;
+        long long incl = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const long long v = __shfl_up(incl, d);
+            if (lane >= d) incl += v;
+        }
+        const unsigned long long hit = __ballot(want < before + incl);
+        if (hit) {
+            const int at = __ffsll(hit) - 1;
+            *seq = base + at;
+            *a = __builtin_amdgcn_readlane(x, at);
+            *n = __builtin_amdgcn_readlane(len, at);
+            *part = (int)(want - before - __shfl(incl - mine, at));
+            return true;
+        }
+        before += __shfl(incl, 63);
+    }
+    return false;
+}
+
+// 16-byte chunks of an image row are exchanged by key so that neither the rows
+// of K's reads (one chunk of 32 keys) nor those of V's (32 bytes of 4 keys)
+// meet in a bank.
+template <int D>
+__device__ __forceinline__ int k_chunk(int key, int c) { return c ^ (key & 7); }
+template <int D>
+__device__ __forceinline__ int v_chunk(int key, int c)
+{
+    return c ^ ((((key & 3) << 1) | ((key & 4) << 1)) & (D / 8 - 1));
+}
+
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The exponent a row is scaled by: its largest finite value to 2^14 .. 2^15.
+__device__ __forceinline__ int row_exp(float top) { return min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127); }
+
+template <class T> struct ApOperand { using E = _Float16; using V = half8; };
+template <> struct ApOperand<TBF16> { using E = __bf16; using V = bf168; };
+
+__device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(bf168 a, bf168 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// ---------------------------------------------------------------- tiles ----
+template <class T, int D>
+__global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
+{
+    using S = typename T::S;
+    using E = typename ApOperand<T>::E;
+    using V8 = typename ApOperand<T>::V;
+    constexpr int NS = sizeof(S) == 4 ? 2 : 1;
+    constexpr int CH = D / 8, ROWS = AP_WG / CH;
+    constexpr int PLANE = AP_KEYS * D;
+    int seq, part, a, n;
+    if (!ap_find(A, blockIdx.x, AP_KEYS, false, &seq, &part, &a, &n)) return;
+    const int kvh = blockIdx.y;
+    const int64_t tile = (int64_t)kvh * A.tiles + a / AP_KEYS + seq + part;
+    E *img = (E *)A.img + tile * 2 * NS * PLANE;
+    const int c = threadIdx.x % CH;
+    int odd = 0;
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+        const S *base = (const S *)(w ? A.v : A.k) + kvh * (w ? A.vh : A.kh);
+        const int64_t stride = w ? A.vt : A.kt;
+        for (int key = threadIdx.x / CH; key < AP_KEYS; key += ROWS) {
+            const int t = part * AP_KEYS + key;
+            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (t < n) load8<T>(base + (int64_t)(a + t) * stride + 8 * c, w ? A.v_vec : A.k_vec, x);
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool fine = fabsf(x[i]) <= 3.402823466e38f;
+                top = fmaxf(top, fine ? fabsf(x[i]) : 0.0f);
+                // V's infinities and NaN are added where they are seen, not multiplied
+                if (w && !fine) odd = 1, x[i] = 0.0f;
+            }
+            E *row = img + w * NS * PLANE + key * D + 8 * (w ? v_chunk<D>(key, c) : k_chunk<D>(key, c));
+            V8 hi, lo;
+            if constexpr (NS == 2) {
+                const int e = row_exp(group_max<CH>(top));
+                const float up = pow2i(14 - e);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = rounded(x[i] * up);
+                    hi[i] = (E)y;
+                    lo[i] = fabsf((float)hi[i]) <= 65504.0f ? (E)(y - (float)hi[i]) : (E)0.0f;
+                }
+                *(V8 *)(row + PLANE) = lo;
+                if (c == 0) A.scale[tile * 2 * AP_KEYS + w * AP_KEYS + key] = pow2i(e - 14);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) hi[i] = (E)x[i];
+            }
+            *(V8 *)row = hi;
+        }
+    }
+    odd = __syncthreads_or(odd);
+    if (threadIdx.x == 0) A.odd[tile] = odd;
+}
+
+// ------------------------------------------------------------- attention ----
+template <class T, int D>
+__global__ void __launch_bounds__(AP_WG, 1) attn_prompt_kernel(ApArgs A)
+{
+    using S = typename T::S;
+    using E = typename ApOperand<T>::E;
+    using V8 = typename ApOperand<T>::V;
+    constexpr int NS = sizeof(S) == 4 ? 2 : 1;
+    constexpr int PLANE = AP_KEYS * D;
+    constexpr int TILE = 2 * NS * PLANE;          // values of a tile, K and V
+    constexpr int KS = D / 16;                    // steps of 16 channels
+    constexpr int DT = D / 32;                    // 32-channel parts of the output
+    __shared__ __attribute__((aligned(16))) E lds[2][TILE];
+    __shared__ __attribute__((aligned(16))) float lsc[2][NS == 2 ? 2 * AP_KEYS : 4];
+
+    int seq, part, a, len;
+    if (!ap_find(A, blockIdx.x, AP_ROWS, true, &seq, &part, &a, &len)) return;
+    const int head = blockIdx.y, kvh = head / A.G;
+    const int wave = threadIdx.x >> 6, lane = lane_id(), n = lane & 31, h = lane >> 5;
+    const int q0 = part * AP_ROWS + wave * 32, qi = q0 + n;
+
+    // ---- queries
+    V8 qh[KS], ql[NS == 2 ? KS : 1];
+    float rs = A.sc;
+    {
+        const S *qp = (const S *)A.q + (int64_t)(a + min(qi, len - 1)) * A.qt + head * A.qh;
+        if constexpr (NS == 2) {
+            float x[KS][8], top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                load8<T>(qp + 16 * k + 8 * h, A.q_vec, x[k]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[k][i]));
+            }
+            auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const int e = row_exp(fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])));
+            const float up = pow2i(14 - e);
+            rs = A.sc * pow2i(e - 14);
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = rounded(x[k][i] * up);
+                    qh[k][i] = (E)y;
+                    ql[k][i] = (E)(y - (float)qh[k][i]);
+                }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                float x[8];
+                load8<T>(qp + 16 * k + 8 * h, A.q_vec, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) qh[k][i] = (E)x[i];
+            }
+        }
+    }
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    int ve = -127;                                 // fp32: the row's weights carry 2^(7 - ve) and V's power of two
+
+    const int64_t tile0 = (int64_t)kvh * A.tiles + a / AP_KEYS + seq;
+    const int n_tile = min(part * AP_ROWS + AP_ROWS, len);
+    const int tiles = (n_tile + AP_KEYS - 1) / AP_KEYS;
+    const uint4 *src = (const uint4 *)((const E *)A.img + tile0 * TILE);
+    constexpr int PIECES = TILE * (int)sizeof(E) / 16;
+
+    auto load = [&](int kt, int b) {
+        // 1 KB of the image per wave and instruction, straight into LDS
+#pragma unroll
+        for (int i = 0; i < PIECES / AP_WG; i++) {
+            const int at = i * AP_WG + wave * 64;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (int64_t)kt * PIECES + at + lane),
+                                             (__attribute__((address_space(3))) void *)((uint4 *)lds[b] + at), 16, 0, 0);
+        }
+        if constexpr (NS == 2)
+            if (threadIdx.x < 2 * AP_KEYS) lsc[b][threadIdx.x] = A.scale[(tile0 + kt) * 2 * AP_KEYS + threadIdx.x];
+    };
+
+    load(0, 0);
+    for (int kt = 0; kt < tiles; kt++) {
+        const int b = kt & 1;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (kt + 1 < tiles) load(kt + 1, b ^ 1);
+        const int k0 = kt * AP_KEYS;
+        if (k0 > q0 + 31 || q0 >= len) continue;   // behind every query of the wave
+        const E *K = lds[b], *V = lds[b] + NS * PLANE;
+
+        // ---- scores
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const E *p = K + n * D + 8 * k_chunk<D>(n, 2 * k + h);
+            const V8 kh = *(const V8 *)p;
+            s = mfma(kh, qh[k], s);
+            if constexpr (NS == 2) {
+                const V8 kl = *(const V8 *)(p + PLANE);
+                s = mfma(kh, ql[k], s);
+                s = mfma(kl, qh[k], s);
+            }
+        }
+        float vp[NS == 2 ? 16 : 1];                // V's powers of two
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            if constexpr (NS == 2) {
+                const float4 ks = *(const float4 *)&lsc[b][8 * g + 4 * h], vs = *(const float4 *)&lsc[b][AP_KEYS + 8 * g + 4 * h];
+                s[4 * g] *= rs * ks.x, s[4 * g + 1] *= rs * ks.y, s[4 * g + 2] *= rs * ks.z, s[4 * g + 3] *= rs * ks.w;
+                vp[4 * g] = vs.x, vp[4 * g + 1] = vs.y, vp[4 * g + 2] = vs.z, vp[4 * g + 3] = vs.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[4 * g + i] *= rs;
+            }
+        }
+        const bool edge = k0 + 31 > q0;            // some query does not see some key (keys behind the end are behind every query)
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const bool seen = k0 + 8 * (i >> 2) + 4 * h + (i & 3) <= qi;
+                s[i] = seen ? s[i] : -INFINITY;
+                if constexpr (NS == 2) vp[i] = seen ? vp[i] : 0.0f;
+            }
+        }
+
+        // ---- running maximum: moved only when a weight would pass 2^8
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        {
+            auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        }
+        float f = 1.0f;
+        bool move = top > m + 8.0f;
+        if (__any(move)) {
+            const float mn = fmaxf(m, top);
+            f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+        }
+        if constexpr (NS == 2) {
+            float vt = vp[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) vt = fmaxf(vt, vp[i]);
+            auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(vt), __float_as_uint(vt), false, false);
+            vt = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+            const int e = max((int)(__float_as_uint(vt) >> 23) - 127, -126);
+            if (e > ve) {
+                f *= ve == -127 ? 0.0f : pow2i(max(ve - e, -126));
+                ve = e;
+                move = true;
+            }
+        }
+        if (__any(move)) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= f;
+        }
+        const float ms = m == -INFINITY ? 0.0f : m;
+        V8 ph[2], pl[NS == 2 ? 2 : 1];
+        const float pv = NS == 2 ? pow2i(min(7 - ve, 127)) : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float p = __builtin_amdgcn_exp2f(s[i] - ms);
+            l += p;
+            if constexpr (NS == 2) {
+                p = rounded(p * (vp[i] * pv));
+                ph[i >> 3][i & 7] = (E)p;
+                pl[i >> 3][i & 7] = (E)(p - (float)ph[i >> 3][i & 7]);
+            } else {
+                ph[i >> 3][i & 7] = (E)p;
+            }
+        }
+
+        // ---- output
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                // four keys of 16 channels to every 16 lanes; a lane gets one channel's
+                const int key = 16 * st + 4 * h + ((lane & 15) >> 2), c = 32 * d + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+                union { s16x4 r[2]; V8 v; } vh, vl;
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int kk = key + 8 * u;
+                    const E *p = V + kk * D + 8 * v_chunk<D>(kk, c >> 3) + (c & 7);
+                    vh.r[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+                    if constexpr (NS == 2)
+                        vl.r[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + PLANE));
+                }
+                o[d] = mfma(vh.v, ph[st], o[d]);
+                if constexpr (NS == 2) {
+                    o[d] = mfma(vh.v, pl[st], o[d]);
+                    o[d] = mfma(vl.v, ph[st], o[d]);
+                }
+            }
+
+        // ---- infinities and NaN of V, to the rows that see them
+        if (A.odd[tile0 + kt]) {
+            for (int k = 0; k < AP_KEYS && k0 + k < len; k++) {
+                const S *vr = (const S *)A.v + (int64_t)(a + k0 + k) * A.vt + kvh * A.vh;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float x = T::up(vr[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
+                        o[d][i] += k0 + k <= qi && !(fabsf(x) <= 3.402823466e38f) ? x : 0.0f;
+                    }
+            }
+        }
+    }
+
+    if (qi >= len) return;
+    {
+        auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    float inv = 1.0f / l;                          // every row sees itself
+    S *op = (S *)A.out + (int64_t)(a + qi) * A.ot + head * A.oh;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                y[i] = o[d][4 * g + i] * inv;
+                if constexpr (NS == 2) y[i] = ldexpf(y[i], ve - 7);
+            }
+            store4<T>(op + 32 * d + 8 * g + 4 * h, A.o_vec, y);
+        }
+}
+
+template <class T, int D>
+static int ap_launch(ApArgs A, hipStream_t s)
+{
+    constexpr int NS = sizeof(typename T::S) == 4 ? 2 : 1;
+    constexpr size_t TILE = 2 * NS * AP_KEYS * D * 2;
+    A.tiles = A.T / AP_KEYS + A.n_seq;
+    const size_t n = (size_t)A.tiles * A.n_kv;
+    int st;
+    uint8_t *ws = (uint8_t *)workspace(WS_ATTN, n * (TILE + (NS == 2 ? 2 * AP_KEYS * sizeof(float) : 0) + sizeof(int)), &st);
+    if (st) return st;
+    A.img = ws;
+    A.scale = (float *)(ws + n * TILE);
+    A.odd = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
+    prompt_tiles_kernel<T, D><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv), AP_WG, 0, s>>>(A);
+    attn_prompt_kernel<T, D><<<dim3((unsigned)(A.T / AP_ROWS + A.n_seq), (unsigned)(A.n_kv * A.G)), AP_WG, 0, s>>>(A);
+    return QMAG_OK;
+}
+
+}  // namespace qmag
+
+using namespace qmag;
+
+extern "C" int qmag_attn_prompt_dev(int type, int head_dim, const qmag_heads *q, const qmag_heads *k, const qmag_heads *v,
+                                    const qmag_heads *out, const int *cu, int n_seq, int T, float scale)
+{
+    int st;
+    if (!q || !k || !v || !out) return fail(QMAG_ERR_ARG, "attn_prompt: null pointer");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return fail(QMAG_ERR_ARG, "attn_prompt: head_dim %d (64, 128 or 256)", head_dim);
+    if (T < 0 || T > QMAG_ATTN_MAX_TOKENS || n_seq < 0 || n_seq > QMAG_KV_MAX_SEQ)
+        return fail(QMAG_ERR_ARG, "attn_prompt: T=%d n_seq=%d", T, n_seq);
+    if ((st = check_heads("attn_prompt q", q, type, head_dim, T, false))) return st;
+    if ((st = check_heads("attn_prompt k", k, type, head_dim, T, false))) return st;
+    if ((st = check_heads("attn_prompt v", v, type, head_dim, T, false))) return st;
+    if ((st = check_heads("attn_prompt out", out, type, head_dim, T, true))) return st;
+    if (k->n_head < 1 || k->n_head != v->n_head || q->n_head < 1 || q->n_head != out->n_head || q->n_head % k->n_head)
+        return fail(QMAG_ERR_ARG, "attn_prompt: %d query, %d key, %d value and %d output heads", q->n_head, k->n_head,
+                    v->n_head, out->n_head);
+    if (T > 0 && n_seq > 0 && (!cu || (uintptr_t)cu % 4)) return fail(QMAG_ERR_ARG, "attn_prompt: cu is null or not aligned");
+    const int size = attn_type_size(type);
+    if (heads_overlap(q, out, size, head_dim, T) || heads_overlap(k, out, size, head_dim, T) ||
+        heads_overlap(v, out, size, head_dim, T))
+        return fail(QMAG_ERR_ARG, "attn_prompt: the output overlaps an input");
+    if ((st = require_ready())) return st;
+    if (T == 0 || n_seq == 0) return QMAG_OK;
+    DeviceScope dev;
+    if (dev.st) return dev.st;
+    ApArgs A = {};
+    A.q = q->ptr, A.k = k->ptr, A.v = v->ptr, A.out = out->ptr;
+    A.qt = q->token_stride, A.qh = q->head_stride, A.kt = k->token_stride, A.kh = k->head_stride;
+    A.vt = v->token_stride, A.vh = v->head_stride, A.ot = out->token_stride, A.oh = out->head_stride;
+    A.cu = cu;
+    A.n_seq = n_seq;
+    A.T = T;
+    A.n_kv = k->n_head;
+    A.G = q->n_head / k->n_head;
+    A.sc = scale * 1.44269504088896340736f;
+    A.q_vec = heads_aligned(q, type), A.k_vec = heads_aligned(k, type), A.v_vec = heads_aligned(v, type);
+    A.o_vec = heads_aligned(out, type);
+    hipStream_t s = ctx().stream;
+    prof_begin(PROF_ATTN, s);
+    st = with_type(type, [&](auto t) {
+        using TT = decltype(t);
+        if (head_dim == 64) return ap_launch<TT, 64>(A, s);
+        if (head_dim == 128) return ap_launch<TT, 128>(A, s);
+        return ap_launch<TT, 256>(A, s);
+    });
+    prof_end(PROF_ATTN, s);
+    if (st) return st;
+    QMAG_HIP(hipGetLastError());
+    return QMAG_OK;
+}

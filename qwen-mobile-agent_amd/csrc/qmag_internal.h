@@ -51,6 +51,7 @@ enum WsSlot {
     WS_SAMP,                        // sampler: per-chunk candidates and the merged list
     WS_HOSTIO,                      // qmag_moe_ffn_host: the device copies of x and out
     WS_F32PART,                     // fp32 matmul rows longer than one LDS chunk: per-chunk partials
+    WS_ATTN,                        // attention: partial results over a cache, tiles of a prompt's K and V
     WS_COUNT
 };
 void *workspace(int slot, size_t bytes, int *status);
@@ -58,7 +59,7 @@ void *workspace(int slot, size_t bytes, int *status);
 // ---- per-kernel event timing (qmag_prof_*) ----
 enum ProfId {
     PROF_ROUTER = 0, PROF_TOPK, PROF_GATEUP, PROF_HQUANT, PROF_DOWN, PROF_FUSED, PROF_MATVEC, PROF_Q8K,
-    PROF_GROUP, PROF_COMBINE,
+    PROF_GROUP, PROF_COMBINE, PROF_ROPE, PROF_KV, PROF_ATTN,
     PROF_COUNT
 };
 bool prof_on();

@@ -1,0 +1,221 @@
+// qmag_kv4.hip -- tokens' K and V into the 4-bit cache, and the values it holds.
+//
+// 64 consecutive values of a head share a minimum m and a step d, both fp16:
+//   m = fp16(min), d = fp16((max - min) / 15), code = clamp(rne((x - m) / d), 0, 15),
+// every step in fp32 as written, so that the codes do not depend on who forms
+// them.  m and d saturate at fp16's largest value; a group that holds an
+// infinity or a NaN stands for NaN throughout (d NaN).
+//
+// A thread takes 8 values of one head of one token; a group is 8 threads, its
+// minimum and maximum three lane exchanges.  Memory bound: each value is read
+// once, each code written once.
+#include "qmag_attn.h"
+
+namespace qmag {
+
+constexpr int KV4_WG = 256;
+
+// where the 8 codes from channel 8 * e of a token's row lie (K: one dword)
+template <int D>
+__device__ __forceinline__ int k_dword_at(int e)
+{
+    const int g = e >> 3, s = (e >> 2) & 1, h = e & 3;
+    return h * (D / 8) + g * 8 + s * 4;
+}
+// V: four channels each in 16 bits, channels 4 * i of group g
+template <int D>
+__device__ __forceinline__ int v_short_at(int g, int i)
+{
+    return i * (D / 32) + g * 2;
+}
+
+struct Kv4Args {
+    uint8_t *data;
+    int n_slot, shift, n_kv;
+    int64_t half;                 // bytes of K, or of V, of a head in a block
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(KV4_WG) kv4_append_kernel(Kv4Args c, qmag_heads K, qmag_heads V, const int *slot, int n_tok,
+                                                            bool vec)
+{
+    constexpr int PER = D / 8;                       // threads of a head
+    constexpr int ROWS = KV4_WG / PER;
+    const int e = threadIdx.x % PER, g = e >> 3;
+    const int64_t rows = (int64_t)n_tok * c.n_kv * 2;
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < rows; r0 += (int64_t)gridDim.x * ROWS) {
+        // rows: K of every head of a token, then V
+        const int64_t row = r0 + threadIdx.x / PER;
+        if (row >= rows) continue;                   // whole groups of lanes leave together
+        const int64_t t = row / (2 * c.n_kv);
+        const int w = (int)(row - t * 2 * c.n_kv), is_v = w >= c.n_kv, head = is_v ? w - c.n_kv : w;
+        const int sl = slot[t];
+        if (sl < 0 || sl >= c.n_slot) continue;
+        const qmag_heads &H = is_v ? V : K;
+        float x[8];
+        load8<T>((const typename T::S *)H.ptr + t * H.token_stride + head * H.head_stride + 8 * e, vec, x);
+        float lo = x[0], hi = x[0];
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            lo = fminf(lo, x[i]);
+            hi = fmaxf(hi, x[i]);
+            ok = ok && fabsf(x[i]) <= 3.402823466e38f;
+        }
+        lo = group_min<8>(lo);
+        hi = group_max<8>(hi);
+        const bool group_ok = group_min<8>(ok ? 1.0f : 0.0f) > 0.0f;
+        const _Float16 m = (_Float16)fminf(fmaxf(lo, -65504.0f), 65504.0f);
+        const _Float16 d = (_Float16)fminf((hi - lo) / 15.0f, 65504.0f);
+        const float mf = (float)m, df = (float)d;
+        uint32_t code[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            code[i] = group_ok && df > 0.0f ? (uint32_t)fminf(fmaxf(rintf((x[i] - mf) / df), 0.0f), 15.0f) : 0u;
+        uint32_t dword = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) dword |= code[i] << (4 * i);
+        const int64_t blk = sl >> c.shift;
+        const int off = sl & ((1 << c.shift) - 1);
+        uint8_t *base = c.data + (blk * c.n_kv + head) * 2 * c.half + (is_v ? c.half : 0);
+        uint8_t *codes = base + off * (D / 2);
+        if (is_v) {
+            *(uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7))) = (uint16_t)dword;
+            *(uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7) + 1)) = (uint16_t)(dword >> 16);
+        } else {
+            *(uint32_t *)(codes + k_dword_at<D>(e)) = dword;
+        }
+        if ((e & 7) == 0) {
+            const uint32_t dm = group_ok ? (uint32_t)__builtin_bit_cast(uint16_t, d) |
+                                               ((uint32_t)__builtin_bit_cast(uint16_t, m) << 16)
+                                         : 0x7E00u;
+            *(uint32_t *)(base + ((int64_t)(D / 2) << c.shift) + (off * (D / KV4_GROUP) + g) * 4) = dm;
+        }
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(KV4_WG) kv4_read_kernel(Kv4Args c, const int *slot, int n_tok, float *ko, float *vo, bool vec)
+{
+    constexpr int PER = D / 8;
+    constexpr int ROWS = KV4_WG / PER;
+    const int e = threadIdx.x % PER, g = e >> 3;
+    const int64_t rows = (int64_t)n_tok * c.n_kv * 2;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / PER; row < rows; row += (int64_t)gridDim.x * ROWS) {
+        const int64_t t = row / (2 * c.n_kv);
+        const int w = (int)(row - t * 2 * c.n_kv), is_v = w >= c.n_kv, head = is_v ? w - c.n_kv : w;
+        const int sl = slot[t];
+        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (sl >= 0 && sl < c.n_slot) {
+            const int64_t blk = sl >> c.shift;
+            const int off = sl & ((1 << c.shift) - 1);
+            const uint8_t *base = c.data + (blk * c.n_kv + head) * 2 * c.half + (is_v ? c.half : 0);
+            const uint8_t *codes = base + off * (D / 2);
+            uint32_t dword;
+            if (is_v)
+                dword = *(const uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7))) |
+                        ((uint32_t)*(const uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7) + 1)) << 16);
+            else
+                dword = *(const uint32_t *)(codes + k_dword_at<D>(e));
+            const uint32_t dm = *(const uint32_t *)(base + ((int64_t)(D / 2) << c.shift) + (off * (D / KV4_GROUP) + g) * 4);
+            const float d = h2f(dm & 0xFFFFu), m = h2f(dm >> 16);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = fmaf(d, (float)((dword >> (4 * i)) & 15u), m);
+        }
+        float *o = (is_v ? vo : ko) + (t * c.n_kv + head) * D + 8 * e;
+        const float a[4] = {y[0], y[1], y[2], y[3]}, b[4] = {y[4], y[5], y[6], y[7]};
+        store4<TF32>(o, vec, a);
+        store4<TF32>(o + 4, vec, b);
+    }
+}
+
+static Kv4Args kv4_args(const qmag_kv4 *c)
+{
+    int shift = 0;
+    while ((1 << shift) < c->block_size) shift++;
+    return {(uint8_t *)c->data, c->n_block * c->block_size, shift, c->n_kv, kv4_half_bytes(c->block_size, c->head_dim)};
+}
+
+template <class F>
+static int with_dim(int dim, F f)
+{
+    if (dim == 64) return f(std::integral_constant<int, 64>{});
+    if (dim == 128) return f(std::integral_constant<int, 128>{});
+    return f(std::integral_constant<int, 256>{});
+}
+
+// workgroups for `rows` heads of `dim` values, at most 16 for each CU
+static unsigned kv4_grid(int64_t rows, int dim)
+{
+    const int64_t per = KV4_WG / (dim / 8), wgs = (rows + per - 1) / per;
+    return (unsigned)(wgs < 4096 ? wgs : 4096);
+}
+
+}  // namespace qmag
+
+using namespace qmag;
+
+extern "C" int qmag_kv4_block_bytes(const qmag_kv4 *c, size_t *bytes)
+{
+    if (!c || !bytes) return fail(QMAG_ERR_ARG, "kv4_block_bytes: null pointer");
+    qmag_kv4 shape = *c;
+    shape.data = (void *)16;             // the shape alone is asked for
+    if (shape.n_block < 1) shape.n_block = 1;
+    int st = check_kv4(&shape);
+    if (st) return st;
+    *bytes = (size_t)(2 * kv4_half_bytes(c->block_size, c->head_dim)) * (size_t)c->n_kv;
+    return QMAG_OK;
+}
+
+extern "C" int qmag_kv4_append_dev(const qmag_kv4 *c, int type, const qmag_heads *k, const qmag_heads *v, const int *slot,
+                                   int T)
+{
+    int st = check_kv4(c);
+    if (st) return st;
+    if (!k || !v || T < 0 || (T > 0 && (!slot || (uintptr_t)slot % 4)))
+        return fail(QMAG_ERR_ARG, "kv4_append: T=%d or a null or unaligned pointer", T);
+    if ((st = check_heads("kv4_append k", k, type, c->head_dim, T, false))) return st;
+    if ((st = check_heads("kv4_append v", v, type, c->head_dim, T, false))) return st;
+    if (k->n_head != c->n_kv || v->n_head != c->n_kv)
+        return fail(QMAG_ERR_ARG, "kv4_append: %d and %d heads for a cache of %d", k->n_head, v->n_head, c->n_kv);
+    if ((st = require_ready())) return st;
+    if (T == 0) return QMAG_OK;
+    const bool vec = heads_aligned(k, type) && heads_aligned(v, type);
+    DeviceScope dev;
+    if (dev.st) return dev.st;
+    hipStream_t s = ctx().stream;
+    const unsigned grid = kv4_grid((int64_t)T * c->n_kv * 2, c->head_dim);
+    prof_begin(PROF_KV, s);
+    with_type(type, [&](auto t) {
+        return with_dim(c->head_dim, [&](auto d) {
+            kv4_append_kernel<decltype(t), decltype(d)::value><<<grid, KV4_WG, 0, s>>>(kv4_args(c), *k, *v, slot, T, vec);
+            return 0;
+        });
+    });
+    prof_end(PROF_KV, s);
+    QMAG_HIP(hipGetLastError());
+    return QMAG_OK;
+}
+
+extern "C" int qmag_kv4_read_dev(const qmag_kv4 *c, const int *slot, int T, float *k, float *v)
+{
+    int st = check_kv4(c);
+    if (st) return st;
+    if (T < 0 || (T > 0 && (!slot || !k || !v || ((uintptr_t)slot | (uintptr_t)k | (uintptr_t)v) % 4)))
+        return fail(QMAG_ERR_ARG, "kv4_read: T=%d or a null or unaligned pointer", T);
+    if ((st = require_ready())) return st;
+    if (T == 0) return QMAG_OK;
+    const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
+    DeviceScope dev;
+    if (dev.st) return dev.st;
+    hipStream_t s = ctx().stream;
+    const unsigned grid = kv4_grid((int64_t)T * c->n_kv * 2, c->head_dim);
+    prof_begin(PROF_KV, s);
+    with_dim(c->head_dim, [&](auto d) {
+        kv4_read_kernel<decltype(d)::value><<<grid, KV4_WG, 0, s>>>(kv4_args(c), slot, T, k, v, vec);
+        return 0;
+    });
+    prof_end(PROF_KV, s);
+    QMAG_HIP(hipGetLastError());
+    return QMAG_OK;
+}

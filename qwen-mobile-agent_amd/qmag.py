@@ -19,6 +19,7 @@ QK_K = 256
 TYPE_Q4_K = 12
 TYPE_Q6_K = 14
 TYPE_Q6_K_R = 270          # Q6_K rows repacked by qmag_repack_q6k_dev (same bytes per row)
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30       # activations of the attention entries
 BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210, TYPE_Q6_K_R: 210}
 
 P = C.c_void_p
@@ -90,6 +91,14 @@ SIGNATURES = {
     "qmag_gguf_expert_record_bytes": (C.c_int, [P, C.POINTER(C.c_size_t)]),
     "qmag_sampler_candidates_dev": (C.c_int, [C.c_int, P, P, P, P, C.c_int]),
     "qmag_sampler_sample_dev": (C.c_int, [C.c_int, P, P, C.c_int, C.c_float, P]),
+    "qmag_rope_dev": (C.c_int, [P, P, C.c_int, C.c_int, P, P, C.c_int]),
+    "qmag_kv_release_dev": (C.c_int, [P] * 7),
+    "qmag_kv_assign_dev": (C.c_int, [P, P, P, P, C.c_int, P, P, P, P, P, P]),
+    "qmag_kv4_block_bytes": (C.c_int, [P, C.POINTER(C.c_size_t)]),
+    "qmag_kv4_append_dev": (C.c_int, [P, C.c_int, P, P, P, C.c_int]),
+    "qmag_kv4_read_dev": (C.c_int, [P, P, C.c_int, P, P]),
+    "qmag_attn_kv4_dev": (C.c_int, [P, P, C.c_int, P, P, P, P, C.c_int, C.c_float]),
+    "qmag_attn_prompt_dev": (C.c_int, [C.c_int, C.c_int, P, P, P, P, P, C.c_int, C.c_int, C.c_float]),
     "qmag_synth_normal": (C.c_int, [C.c_uint64, C.c_size_t, C.c_float, C.c_float, P]),
     "qmag_synth_weights": (C.c_int, [C.c_uint64, C.c_size_t, C.c_float, C.c_int, P]),
     "qmag_quantize_dev": (C.c_int, [P, C.c_size_t, C.c_int, P]),
@@ -334,6 +343,77 @@ def moe_last_stage(n_expert: int, n_used: int, n_ff: int, n_tok: int = 0):
     return dict(logits=logits, sel=sel, w=w, gs=gs, h=h)
 
 
+class Heads(C.Structure):
+    """qmag_heads: value c of head h of token t at ptr[t * token_stride + h * head_stride + c]."""
+    _fields_ = [("ptr", P), ("n_head", C.c_int), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+def heads(*views):
+    """An array of qmag_heads from (ptr, n_head, token_stride, head_stride) tuples."""
+    return (Heads * len(views))(*[Heads(*v) for v in views])
+
+
+class Rope(C.Structure):
+    """qmag_rope"""
+    _fields_ = [("head_dim", C.c_int), ("n_rot", C.c_int), ("n_axes", C.c_int), ("sections", C.c_int * 4),
+                ("interleaved", C.c_int), ("adjacent", C.c_int), ("theta", C.c_double)]
+
+    @classmethod
+    def make(cls, head_dim, n_rot, sections, interleaved=False, adjacent=False, theta=1e4):
+        return cls(head_dim, n_rot, len(sections), (C.c_int * 4)(*sections), int(interleaved), int(adjacent), theta)
+
+
+class KvTable(C.Structure):
+    """qmag_kv_table"""
+    _fields_ = [("n_seq", C.c_int), ("max_blocks", C.c_int), ("block_size", C.c_int), ("n_block", C.c_int), ("table", P),
+                ("free_list", P)]
+
+
+class Kv4(C.Structure):
+    """qmag_kv4"""
+    _fields_ = [("data", P), ("n_block", C.c_int), ("block_size", C.c_int), ("n_kv", C.c_int), ("head_dim", C.c_int)]
+
+
+KV_OK, KV_FULL, KV_ROW, KV_LENGTH, KV_LIST = range(5)
+
+
+def rope_dev(rope: Rope, pos_ptr: int, T: int, type: int, src, dst) -> None:
+    """src, dst: heads() of one or two views (q, k)."""
+    check(lib().qmag_rope_dev(C.byref(rope), pos_ptr, T, type, src, dst, len(src)))
+
+
+def kv_release_dev(t: KvTable, len_ptr, ended_ptr, n_free_ptr, len_next_ptr, n_free_next_ptr, status_ptr) -> None:
+    check(lib().qmag_kv_release_dev(C.byref(t), len_ptr, ended_ptr, n_free_ptr, len_next_ptr, n_free_next_ptr, status_ptr))
+
+
+def kv_assign_dev(t: KvTable, len_ptr, n_new_ptr, n_free_ptr, T, slot_ptr, pos_ptr, cu_ptr, len_next_ptr,
+                  n_free_next_ptr, status_ptr) -> None:
+    check(lib().qmag_kv_assign_dev(C.byref(t), len_ptr, n_new_ptr, n_free_ptr, T, slot_ptr, pos_ptr, cu_ptr, len_next_ptr,
+                                   n_free_next_ptr, status_ptr))
+
+
+def kv4_block_bytes(c: Kv4) -> int:
+    n = C.c_size_t()
+    check(lib().qmag_kv4_block_bytes(C.byref(c), C.byref(n)))
+    return n.value
+
+
+def kv4_append_dev(c: Kv4, type: int, k, v, slot_ptr: int, T: int) -> None:
+    check(lib().qmag_kv4_append_dev(C.byref(c), type, k, v, slot_ptr, T))
+
+
+def kv4_read_dev(c: Kv4, slot_ptr: int, T: int, k_ptr: int, v_ptr: int) -> None:
+    check(lib().qmag_kv4_read_dev(C.byref(c), slot_ptr, T, k_ptr, v_ptr))
+
+
+def attn_kv4_dev(c: Kv4, t: KvTable, type: int, q, out, cu_ptr: int, len_ptr: int, T: int, scale: float) -> None:
+    check(lib().qmag_attn_kv4_dev(C.byref(c), C.byref(t), type, q, out, cu_ptr, len_ptr, T, scale))
+
+
+def attn_prompt_dev(type: int, head_dim: int, q, k, v, out, cu_ptr: int, n_seq: int, T: int, scale: float) -> None:
+    check(lib().qmag_attn_prompt_dev(type, head_dim, q, k, v, out, cu_ptr, n_seq, T, scale))
+
+
 def synth_normal(seed: int, n: int, mean: float, std: float, out_ptr: int) -> None:
     check(lib().qmag_synth_normal(C.c_uint64(seed), n, mean, std, out_ptr))
 
@@ -347,7 +427,7 @@ def quantize_dev(x_ptr: int, n: int, wtype: int, out_ptr: int) -> None:
 
 
 PROF_IDS = {"router": 0, "topk": 1, "gateup": 2, "hquant": 3, "down": 4, "fused": 5, "matvec": 6,
-            "q8k": 7, "group": 8, "combine": 9}
+            "q8k": 7, "group": 8, "combine": 9, "rope": 10, "kv": 11, "attn": 12}
 
 
 def prof_enable(on: bool) -> None:
