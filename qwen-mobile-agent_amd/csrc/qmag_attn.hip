@@ -18,12 +18,13 @@
 // and keys 8 (r / 4) + 4 (lane / 32) + r % 4 of a tile; O^T = V^T P^T takes the
 // weights as they are when V's keys are read in that order, so they never leave
 // their lane.  V^T comes from row-major LDS by transposing reads.
+#include <type_traits>
+
 #include "qmag_attn.h"
 
 namespace qmag {
 
 constexpr int AP_WG = 256;
-constexpr int AP_ROWS = 128;              // queries of a workgroup
 constexpr int AP_KEYS = 32;               // keys of a tile
 
 struct ApArgs {
@@ -90,21 +91,30 @@ __device__ __forceinline__ bool ap_find(const ApArgs &A, int want, int per, bool
     return false;
 }
 
-// 16-byte chunks of an image row are exchanged by key so that neither the rows
-// of K's reads (one chunk of 32 keys) nor those of V's (32 bytes of 4 keys)
-// meet in a bank.
+// 16-byte chunks of an image row are exchanged by key so that the rows of a
+// read keep apart in LDS's 64 banks (256 bytes): 8 keys' chunk for K, and for V
+// 64 bytes of 4 keys (of half a row where a row is 128 bytes).
 template <int D>
 __device__ __forceinline__ int k_chunk(int key, int c) { return c ^ (key & 7); }
 template <int D>
-__device__ __forceinline__ int v_chunk(int key, int c)
-{
-    return c ^ ((((key & 3) << 1) | ((key & 4) << 1)) & (D / 8 - 1));
-}
+__device__ __forceinline__ int v_chunk(int key, int c) { return c ^ (D == 64 ? (key & 2) << 1 : (key & 3) << 2); }
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // The exponent a row is scaled by: its largest finite value to 2^14 .. 2^15.
 __device__ __forceinline__ int row_exp(float top) { return min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127); }
+
+// over the two lanes that hold a query
+__device__ __forceinline__ float half_max(float v)
+{
+    auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float half_sum(float v)
+{
+    auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
 
 template <class T> struct ApOperand { using E = _Float16; using V = half8; };
 template <> struct ApOperand<TBF16> { using E = __bf16; using V = bf168; };
@@ -170,8 +180,9 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
 }
 
 // ------------------------------------------------------------- attention ----
-template <class T, int D>
-__global__ void __launch_bounds__(AP_WG, 1) attn_prompt_kernel(ApArgs A)
+// NW waves of 32 queries; KT tiles of keys to a barrier; WE waves to a SIMD.
+template <class T, int D, int NW, int KT, int WE>
+__global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 {
     using S = typename T::S;
     using E = typename ApOperand<T>::E;
@@ -181,20 +192,46 @@ __global__ void __launch_bounds__(AP_WG, 1) attn_prompt_kernel(ApArgs A)
     constexpr int TILE = 2 * NS * PLANE;          // values of a tile, K and V
     constexpr int KS = D / 16;                    // steps of 16 channels
     constexpr int DT = D / 32;                    // 32-channel parts of the output
-    __shared__ __attribute__((aligned(16))) E lds[2][TILE];
-    __shared__ __attribute__((aligned(16))) float lsc[2][NS == 2 ? 2 * AP_KEYS : 4];
+    constexpr int ROWS = 32 * NW;
+    constexpr int AHEAD = 2;                      // steps that LDS is read ahead of the products
+    __shared__ __attribute__((aligned(16))) E lds[2][KT * TILE];
+    __shared__ __attribute__((aligned(16))) float lsc[2][NS == 2 ? KT * 2 * AP_KEYS : 4];
 
+    // Workgroups go to the 8 XCDs in turn.  An XCD takes consecutive eighths of
+    // heads (a head's units counted from its longest rows, every eighth), so that
+    // it finds the K and V its heads share in its L2, and goes through all of
+    // them from the longest rows to the shortest.
+    const unsigned heads = (unsigned)(A.n_kv * A.G), i8 = blockIdx.x >> 3, v8 = (blockIdx.x & 7) * heads + i8 % heads;
+    const int head = (int)(v8 >> 3), unit = (int)(8 * (i8 / heads) + (v8 & 7)), kvh = head / A.G;
     int seq, part, a, len;
-    if (!ap_find(A, blockIdx.x, AP_ROWS, true, &seq, &part, &a, &len)) return;
-    const int head = blockIdx.y, kvh = head / A.G;
-    const int wave = threadIdx.x >> 6, lane = lane_id(), n = lane & 31, h = lane >> 5;
-    const int q0 = part * AP_ROWS + wave * 32, qi = q0 + n;
+    if (!ap_find(A, unit, ROWS, true, &seq, &part, &a, &len)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), n = lane & 31, h = lane >> 5;
+    const int q0 = part * ROWS + wave * 32, qi = q0 + n;      // the wave's first query, the lane's
 
-    // ---- queries
+    const int64_t tile0 = (int64_t)kvh * A.tiles + a / AP_KEYS + seq;
+    const int tiles = (min(part * ROWS + ROWS, len) + AP_KEYS - 1) / AP_KEYS;
+    const uint4 *src = (const uint4 *)((const E *)A.img + tile0 * TILE);
+    constexpr int PIECES = KT * TILE * (int)sizeof(E) / 16;
+    auto load = [&](int step, int b) {
+        // 1 KB of the image per wave and instruction, straight into LDS
+#pragma unroll
+        for (int i = 0; i < PIECES / (64 * NW); i++) {
+            const int at = i * 64 * NW + wave * 64;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (int64_t)step * PIECES + at + lane),
+                                             (__attribute__((address_space(3))) void *)((uint4 *)lds[b] + at), 16, 0, 0);
+        }
+        if constexpr (NS == 2)
+            if (threadIdx.x < KT * 2 * AP_KEYS)
+                lsc[b][threadIdx.x] = A.scale[(tile0 + (int64_t)step * KT) * 2 * AP_KEYS + threadIdx.x];
+    };
+    load(0, 0);
+
+    // ---- queries; a negative scale turns their sign
     V8 qh[KS], ql[NS == 2 ? KS : 1];
-    float rs = A.sc;
+    float rs = fabsf(A.sc);
     {
         const S *qp = (const S *)A.q + (int64_t)(a + min(qi, len - 1)) * A.qt + head * A.qh;
+        const float sign = A.sc < 0.0f ? -1.0f : 1.0f;
         if constexpr (NS == 2) {
             float x[KS][8], top = 0.0f;
 #pragma unroll
@@ -203,10 +240,9 @@ __global__ void __launch_bounds__(AP_WG, 1) attn_prompt_kernel(ApArgs A)
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[k][i]));
             }
-            auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            const int e = row_exp(fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1])));
-            const float up = pow2i(14 - e);
-            rs = A.sc * pow2i(e - 14);
+            const int e = row_exp(half_max(top));
+            const float up = sign * pow2i(14 - e);
+            rs *= pow2i(e - 14);
 #pragma unroll
             for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -221,125 +257,106 @@ __global__ void __launch_bounds__(AP_WG, 1) attn_prompt_kernel(ApArgs A)
                 float x[8];
                 load8<T>(qp + 16 * k + 8 * h, A.q_vec, x);
 #pragma unroll
-                for (int i = 0; i < 8; i++) qh[k][i] = (E)x[i];
+                for (int i = 0; i < 8; i++) qh[k][i] = (E)(x[i] * sign);
             }
         }
     }
 
     f32x16 o[DT];
+    float m = -3e38f, l = 0.0f;                    // running maximum (of scaled scores), sum
+    int ve = -127;                                 // fp32: the row's weights carry 2^(7 - ve) and V's power of two
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    int ve = -127;                                 // fp32: the row's weights carry 2^(7 - ve) and V's power of two
 
-    const int64_t tile0 = (int64_t)kvh * A.tiles + a / AP_KEYS + seq;
-    const int n_tile = min(part * AP_ROWS + AP_ROWS, len);
-    const int tiles = (n_tile + AP_KEYS - 1) / AP_KEYS;
-    const uint4 *src = (const uint4 *)((const E *)A.img + tile0 * TILE);
-    constexpr int PIECES = TILE * (int)sizeof(E) / 16;
-
-    auto load = [&](int kt, int b) {
-        // 1 KB of the image per wave and instruction, straight into LDS
+    // a lane's places in a tile: chunk 2 k + h of K's row n, four keys of 16
+    // channels of V to every 16 lanes
+    int k_at[4], v_at[4];
 #pragma unroll
-        for (int i = 0; i < PIECES / AP_WG; i++) {
-            const int at = i * AP_WG + wave * 64;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (int64_t)kt * PIECES + at + lane),
-                                             (__attribute__((address_space(3))) void *)((uint4 *)lds[b] + at), 16, 0, 0);
-        }
-        if constexpr (NS == 2)
-            if (threadIdx.x < 2 * AP_KEYS) lsc[b][threadIdx.x] = A.scale[(tile0 + kt) * 2 * AP_KEYS + threadIdx.x];
-    };
+    for (int i = 0; i < 4; i++) {
+        k_at[i] = n * D + 8 * k_chunk<D>(n, 2 * i + h);
+        const int key = 4 * h + ((lane & 15) >> 2), c = 32 * i + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        v_at[i] = NS * PLANE + key * D + 8 * v_chunk<D>(key, c >> 3) + (c & 7);
+    }
 
-    load(0, 0);
-    for (int kt = 0; kt < tiles; kt++) {
-        const int b = kt & 1;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (kt + 1 < tiles) load(kt + 1, b ^ 1);
-        const int k0 = kt * AP_KEYS;
-        if (k0 > q0 + 31 || q0 >= len) continue;   // behind every query of the wave
-        const E *K = lds[b], *V = lds[b] + NS * PLANE;
-
+    // One tile of 32 keys; EDGE: the one whose keys are the wave's own tokens.
+    auto tile = [&](const E *K, const float *sc, auto EDGE) {
         // ---- scores
         f32x16 s;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            const E *p = K + n * D + 8 * k_chunk<D>(n, 2 * k + h);
+            const E *p = K + k_at[k & 3] + 64 * (k >> 2);
             const V8 kh = *(const V8 *)p;
-            s = mfma(kh, qh[k], s);
             if constexpr (NS == 2) {
                 const V8 kl = *(const V8 *)(p + PLANE);
                 s = mfma(kh, ql[k], s);
                 s = mfma(kl, qh[k], s);
             }
+            s = mfma(kh, qh[k], s);
         }
+        // K is read AHEAD steps ahead of its products
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * NS, 0);
+#pragma unroll
+        for (int k = 0; k < KS - AHEAD; k++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NS == 2 ? 3 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, NS, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * (NS == 2 ? 3 : 1), 0);
         float vp[NS == 2 ? 16 : 1];                // V's powers of two
+        if constexpr (NS == 2) {
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            if constexpr (NS == 2) {
-                const float4 ks = *(const float4 *)&lsc[b][8 * g + 4 * h], vs = *(const float4 *)&lsc[b][AP_KEYS + 8 * g + 4 * h];
-                s[4 * g] *= rs * ks.x, s[4 * g + 1] *= rs * ks.y, s[4 * g + 2] *= rs * ks.z, s[4 * g + 3] *= rs * ks.w;
+            for (int g = 0; g < 4; g++) {
+                const float4 ks = *(const float4 *)(sc + 8 * g + 4 * h), vs = *(const float4 *)(sc + AP_KEYS + 8 * g + 4 * h);
+                s[4 * g] *= rs * ks.x, s[4 * g + 1] *= rs * ks.y;
+                s[4 * g + 2] *= rs * ks.z, s[4 * g + 3] *= rs * ks.w;
                 vp[4 * g] = vs.x, vp[4 * g + 1] = vs.y, vp[4 * g + 2] = vs.z, vp[4 * g + 3] = vs.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[4 * g + i] *= rs;
             }
         }
-        const bool edge = k0 + 31 > q0;            // some query does not see some key (keys behind the end are behind every query)
-        if (edge) {
+        if constexpr (EDGE.value) {                // (keys behind the end are behind every query)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const bool seen = k0 + 8 * (i >> 2) + 4 * h + (i & 3) <= qi;
+                const bool seen = 8 * (i >> 2) + 4 * h + (i & 3) <= n;
                 s[i] = seen ? s[i] : -INFINITY;
                 if constexpr (NS == 2) vp[i] = seen ? vp[i] : 0.0f;
             }
         }
-
         // ---- running maximum: moved only when a weight would pass 2^8
+        const float r = NS == 2 ? 1.0f : rs;
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-        {
-            auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-            top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-        }
+        top = half_max(top) * r;
         float f = 1.0f;
         bool move = top > m + 8.0f;
-        if (__any(move)) {
-            const float mn = fmaxf(m, top);
-            f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= f;
-        }
         if constexpr (NS == 2) {
             float vt = vp[0];
 #pragma unroll
             for (int i = 1; i < 16; i++) vt = fmaxf(vt, vp[i]);
-            auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(vt), __float_as_uint(vt), false, false);
-            vt = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-            const int e = max((int)(__float_as_uint(vt) >> 23) - 127, -126);
+            const int e = max((int)(__float_as_uint(half_max(vt)) >> 23) - 127, -126);
             if (e > ve) {
-                f *= ve == -127 ? 0.0f : pow2i(max(ve - e, -126));
+                f = ve == -127 ? 0.0f : pow2i(max(ve - e, -126));
                 ve = e;
                 move = true;
             }
         }
         if (__any(move)) {
+            const float mn = fmaxf(m, top), g = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= g;
+            f *= g;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= f;
         }
-        const float ms = m == -INFINITY ? 0.0f : m;
-        V8 ph[2], pl[NS == 2 ? 2 : 1];
         const float pv = NS == 2 ? pow2i(min(7 - ve, 127)) : 1.0f;
+        V8 ph[2], pl[NS == 2 ? 2 : 1];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            float p = __builtin_amdgcn_exp2f(s[i] - ms);
+            float p = __builtin_amdgcn_exp2f(NS == 2 ? s[i] - m : fmaf(s[i], r, -m));
             l += p;
             if constexpr (NS == 2) {
                 p = rounded(p * (vp[i] * pv));
@@ -349,51 +366,71 @@ __global__ void __launch_bounds__(AP_WG, 1) attn_prompt_kernel(ApArgs A)
                 ph[i >> 3][i & 7] = (E)p;
             }
         }
-
         // ---- output
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int st = 0; st < 2; st++) {
-                // four keys of 16 channels to every 16 lanes; a lane gets one channel's
-                const int key = 16 * st + 4 * h + ((lane & 15) >> 2), c = 32 * d + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
                 union { s16x4 r[2]; V8 v; } vh, vl;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const int kk = key + 8 * u;
-                    const E *p = V + kk * D + 8 * v_chunk<D>(kk, c >> 3) + (c & 7);
+                    const E *p = K + v_at[d & 3] + 128 * (d >> 2) + (16 * st + 8 * u) * D;
                     vh.r[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
                     if constexpr (NS == 2)
                         vl.r[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + PLANE));
                 }
-                o[d] = mfma(vh.v, ph[st], o[d]);
                 if constexpr (NS == 2) {
                     o[d] = mfma(vh.v, pl[st], o[d]);
                     o[d] = mfma(vl.v, ph[st], o[d]);
                 }
+                o[d] = mfma(vh.v, ph[st], o[d]);
             }
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * 2 * NS, 0);
+#pragma unroll
+        for (int k = 0; k < 2 * DT - AHEAD; k++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NS == 2 ? 3 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * NS, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * (NS == 2 ? 3 : 1), 0);
+    };
 
-        // ---- infinities and NaN of V, to the rows that see them
-        if (A.odd[tile0 + kt]) {
-            for (int k = 0; k < AP_KEYS && k0 + k < len; k++) {
-                const S *vr = (const S *)A.v + (int64_t)(a + k0 + k) * A.vt + kvh * A.vh;
+    const int mine = q0 < len ? q0 / AP_KEYS : -1;           // the wave's last tile
+    const int steps = (tiles + KT - 1) / KT;
+    for (int step = 0; step < steps; step++) {
+        const int b = step & 1;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (step + 1 < steps) load(step + 1, b ^ 1);
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float x = T::up(vr[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
-                        o[d][i] += k0 + k <= qi && !(fabsf(x) <= 3.402823466e38f) ? x : 0.0f;
-                    }
-            }
+        for (int i = 0; i < KT; i++) {
+            const int kt = step * KT + i;
+            const float *sc = lsc[b] + (NS == 2 ? i * 2 * AP_KEYS : 0);
+            if (kt < mine) tile(lds[b] + i * TILE, sc, std::false_type{});
+            else if (kt == mine) tile(lds[b] + i * TILE, sc, std::true_type{});
         }
     }
-
     if (qi >= len) return;
-    {
-        auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-        l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+
+    // ---- infinities and NaN of V, to the rows that see them: whatever else a
+    // row sums, they decide its result, so they are added to it at the end
+    const float inv = 1.0f / half_sum(l);          // every row sees itself
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] *= inv;
+    for (int t = 0; t <= mine; t++) {
+        if (!A.odd[tile0 + t]) continue;
+        for (int k = t * AP_KEYS; k < min(t * AP_KEYS + AP_KEYS, qi + 1); k++) {
+            const S *vr = (const S *)A.v + (int64_t)(a + k) * A.vt + kvh * A.vh;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float x = T::up(vr[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
+                    o[d][i] += fabsf(x) <= 3.402823466e38f ? 0.0f : x;
+                }
+        }
     }
-    float inv = 1.0f / l;                          // every row sees itself
     S *op = (S *)A.out + (int64_t)(a + qi) * A.ot + head * A.oh;
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -401,10 +438,7 @@ __global__ void __launch_bounds__(AP_WG, 1) attn_prompt_kernel(ApArgs A)
         for (int g = 0; g < 4; g++) {
             float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                y[i] = o[d][4 * g + i] * inv;
-                if constexpr (NS == 2) y[i] = ldexpf(y[i], ve - 7);
-            }
+            for (int i = 0; i < 4; i++) y[i] = NS == 2 ? ldexpf(o[d][4 * g + i], ve - 7) : o[d][4 * g + i];
             store4<T>(op + 32 * d + 8 * g + 4 * h, A.o_vec, y);
         }
 }
@@ -415,7 +449,7 @@ static int ap_launch(ApArgs A, hipStream_t s)
     constexpr int NS = sizeof(typename T::S) == 4 ? 2 : 1;
     constexpr size_t TILE = 2 * NS * AP_KEYS * D * 2;
     A.tiles = A.T / AP_KEYS + A.n_seq;
-    const size_t n = (size_t)A.tiles * A.n_kv;
+    const size_t n = (size_t)A.tiles * A.n_kv + 8;         // a barrier's tiles may reach past the last one
     int st;
     uint8_t *ws = (uint8_t *)workspace(WS_ATTN, n * (TILE + (NS == 2 ? 2 * AP_KEYS * sizeof(float) : 0) + sizeof(int)), &st);
     if (st) return st;
@@ -423,7 +457,10 @@ static int ap_launch(ApArgs A, hipStream_t s)
     A.scale = (float *)(ws + n * TILE);
     A.odd = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
     prompt_tiles_kernel<T, D><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv), AP_WG, 0, s>>>(A);
-    attn_prompt_kernel<T, D><<<dim3((unsigned)(A.T / AP_ROWS + A.n_seq), (unsigned)(A.n_kv * A.G)), AP_WG, 0, s>>>(A);
+    constexpr int NW = 4, KT = D == 64 ? 2 : 1, WE = NS == 2 && D == 256 ? 1 : 2;
+    const int64_t wgs = (((int64_t)A.T / (32 * NW) + A.n_seq + 7) / 8 * 8) * A.n_kv * A.G;
+    if (wgs > UINT32_MAX / (64 * NW)) return fail(QMAG_ERR_ARG, "attn_prompt: %lld workgroups", (long long)wgs);
+    attn_prompt_kernel<T, D, NW, KT, WE><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
     return QMAG_OK;
 }
 
