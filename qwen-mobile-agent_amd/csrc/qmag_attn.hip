@@ -92,38 +92,56 @@ __device__ __forceinline__ bool ap_find(const ApArgs &A, int want, int per, bool
 }
 
 // 16-byte chunks of an image row are exchanged by key so that the rows of a
-// read keep apart in LDS's 64 banks (256 bytes): 8 keys' chunk for K, and for V
-// 64 bytes of 4 keys (of half a row where a row is 128 bytes).
+// read keep apart in LDS's 64 banks (256 bytes): for K 16 keys' chunk; for V 64
+// bytes of 4 keys, or 32 bytes of 8 with 16 queries.  (Where a row is 128 bytes,
+// only keys of one parity share banks.)
 template <int D>
-__device__ __forceinline__ int k_chunk(int key, int c) { return c ^ (key & 7); }
-template <int D>
-__device__ __forceinline__ int v_chunk(int key, int c) { return c ^ (D == 64 ? (key & 2) << 1 : (key & 3) << 2); }
+__device__ __forceinline__ int k_chunk(int key, int c) { return c ^ (D == 64 ? (key >> 1) & 7 : key & 15); }
+template <int D, int QW>
+__device__ __forceinline__ int v_chunk(int key, int c)
+{
+    if (QW == 32) return c ^ (D == 64 ? (key & 2) << 1 : (key & 3) << 2);
+    return c ^ (D == 64 ? (key & 6) : (key & 7) << 1);
+}
 
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // The exponent a row is scaled by: its largest finite value to 2^14 .. 2^15.
 __device__ __forceinline__ int row_exp(float top) { return min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127); }
 
-// over the two lanes that hold a query
-__device__ __forceinline__ float half_max(float v)
+// over the lanes that hold a query: two of 32 queries, four of 16
+template <int QW>
+__device__ __forceinline__ float query_max(float v)
 {
+    if (QW == 16) {
+        auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    }
     auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
-__device__ __forceinline__ float half_sum(float v)
+template <int QW>
+__device__ __forceinline__ float query_sum(float v)
 {
+    if (QW == 16) {
+        auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
     auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
+// what a call of type T multiplies
 template <class T> struct ApOperand { using E = _Float16; using V = half8; };
 template <> struct ApOperand<TBF16> { using E = __bf16; using V = bf168; };
 
 __device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma(bf168 a, bf168 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(bf168 a, bf168 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 // ---------------------------------------------------------------- tiles ----
-template <class T, int D>
+template <class T, int D, int QW>
 __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
 {
     using S = typename T::S;
@@ -155,7 +173,7 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
                 // V's infinities and NaN are added where they are seen, not multiplied
                 if (w && !fine) odd = 1, x[i] = 0.0f;
             }
-            E *row = img + w * NS * PLANE + key * D + 8 * (w ? v_chunk<D>(key, c) : k_chunk<D>(key, c));
+            E *row = img + w * NS * PLANE + key * D + 8 * (w ? v_chunk<D, QW>(key, c) : k_chunk<D>(key, c));
             V8 hi, lo;
             if constexpr (NS == 2) {
                 const int e = row_exp(group_max<CH>(top));
@@ -180,8 +198,9 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
 }
 
 // ------------------------------------------------------------- attention ----
-// NW waves of 32 queries; KT tiles of keys to a barrier; WE waves to a SIMD.
-template <class T, int D, int NW, int KT, int WE>
+// NW waves of QW queries; KT tiles of keys to a barrier; LDS read AHEAD steps
+// ahead of the products; WE waves to a SIMD.
+template <class T, int D, int NW, int QW, int KT, int AHEAD, int WE>
 __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 {
     using S = typename T::S;
@@ -190,10 +209,14 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
     constexpr int PLANE = AP_KEYS * D;
     constexpr int TILE = 2 * NS * PLANE;          // values of a tile, K and V
-    constexpr int KS = D / 16;                    // steps of 16 channels
-    constexpr int DT = D / 32;                    // 32-channel parts of the output
-    constexpr int ROWS = 32 * NW;
-    constexpr int AHEAD = 2;                      // steps that LDS is read ahead of the products
+    // a product takes KW channels of 32 (QW = 16: twice 16) keys, or PK keys of QW channels
+    using Acc = std::conditional_t<QW == 32, f32x16, f32x4>;
+    constexpr int R = QW == 32 ? 16 : 4;          // values of it in a lane
+    constexpr int NA = 32 / QW, NV = QW / 2;      // such scores of a tile, and a lane's scores
+    constexpr int KW = QW == 32 ? 16 : 32, KS = D / KW;
+    constexpr int DT = D / QW;                    // QW-channel parts of the output
+    constexpr int PK = KW, PS = 32 / PK;
+    constexpr int ROWS = QW * NW;
     __shared__ __attribute__((aligned(16))) E lds[2][KT * TILE];
     __shared__ __attribute__((aligned(16))) float lsc[2][NS == 2 ? KT * 2 * AP_KEYS : 4];
 
@@ -205,8 +228,8 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     const int head = (int)(v8 >> 3), unit = (int)(8 * (i8 / heads) + (v8 & 7)), kvh = head / A.G;
     int seq, part, a, len;
     if (!ap_find(A, unit, ROWS, true, &seq, &part, &a, &len)) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), n = lane & 31, h = lane >> 5;
-    const int q0 = part * ROWS + wave * 32, qi = q0 + n;      // the wave's first query, the lane's
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), n = lane & (QW - 1), h = lane / QW;
+    const int q0 = part * ROWS + wave * QW, qi = q0 + n;      // the wave's first query, the lane's
 
     const int64_t tile0 = (int64_t)kvh * A.tiles + a / AP_KEYS + seq;
     const int tiles = (min(part * ROWS + ROWS, len) + AP_KEYS - 1) / AP_KEYS;
@@ -236,11 +259,11 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             float x[KS][8], top = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                load8<T>(qp + 16 * k + 8 * h, A.q_vec, x[k]);
+                load8<T>(qp + KW * k + 8 * h, A.q_vec, x[k]);
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[k][i]));
             }
-            const int e = row_exp(half_max(top));
+            const int e = row_exp(query_max<QW>(top));
             const float up = sign * pow2i(14 - e);
             rs *= pow2i(e - 14);
 #pragma unroll
@@ -255,61 +278,71 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 float x[8];
-                load8<T>(qp + 16 * k + 8 * h, A.q_vec, x);
+                load8<T>(qp + KW * k + 8 * h, A.q_vec, x);
 #pragma unroll
                 for (int i = 0; i < 8; i++) qh[k][i] = (E)(x[i] * sign);
             }
         }
     }
 
-    f32x16 o[DT];
+    Acc o[DT];
     float m = -3e38f, l = 0.0f;                    // running maximum (of scaled scores), sum
     int ve = -127;                                 // fp32: the row's weights carry 2^(7 - ve) and V's power of two
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+        for (int i = 0; i < R; i++) o[d][i] = 0.0f;
 
-    // a lane's places in a tile: chunk 2 k + h of K's row n, four keys of 16
-    // channels of V to every 16 lanes
-    int k_at[4], v_at[4];
+    // a lane's places in a tile: its chunk of K's row n, four keys of 16 channels
+    // of V to every 16 lanes
+    constexpr int KV = QW == 32 ? 8 : 4, VV = QW == 32 ? 4 : 8;      // places that differ by more than a constant
+    int k_at[KV], v_at[VV];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        k_at[i] = n * D + 8 * k_chunk<D>(n, 2 * i + h);
-        const int key = 4 * h + ((lane & 15) >> 2), c = 32 * i + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-        v_at[i] = NS * PLANE + key * D + 8 * v_chunk<D>(key, c >> 3) + (c & 7);
+    for (int i = 0; i < KV; i++) k_at[i] = n * D + 8 * k_chunk<D>(n, (KW / 8 * i + h) % (D / 8));
+#pragma unroll
+    for (int i = 0; i < VV; i++) {
+        const int key = 4 * h + ((lane & 15) >> 2), c = QW * i + (QW == 32 ? ((lane >> 4) & 1) * 16 : 0) + (lane & 3) * 4;
+        v_at[i] = NS * PLANE + key * D + 8 * v_chunk<D, QW>(key, c >> 3) + (c & 7);
     }
 
-    // One tile of 32 keys; EDGE: the one whose keys are the wave's own tokens.
+    // One tile of 32 keys; EDGE: the one that holds the wave's own tokens.
     auto tile = [&](const E *K, const float *sc, auto EDGE) {
         // ---- scores
-        f32x16 s;
+        Acc sa[NA];
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+        for (int w = 0; w < NA; w++)
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const E *p = K + k_at[k & 3] + 64 * (k >> 2);
-            const V8 kh = *(const V8 *)p;
-            if constexpr (NS == 2) {
-                const V8 kl = *(const V8 *)(p + PLANE);
-                s = mfma(kh, ql[k], s);
-                s = mfma(kl, qh[k], s);
+            for (int i = 0; i < R; i++) sa[w][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int w = 0; w < NA; w++) {
+                const E *p = K + k_at[k % KV] + 128 * (k / KV) + w * 16 * D;
+                const V8 kh = *(const V8 *)p;
+                if constexpr (NS == 2) {
+                    const V8 kl = *(const V8 *)(p + PLANE);
+                    sa[w] = mfma(kh, ql[k], sa[w]);
+                    sa[w] = mfma(kl, qh[k], sa[w]);
+                }
+                sa[w] = mfma(kh, qh[k], sa[w]);
             }
-            s = mfma(kh, qh[k], s);
-        }
         // K is read AHEAD steps ahead of its products
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * NS, 0);
 #pragma unroll
-        for (int k = 0; k < KS - AHEAD; k++) {
+        for (int k = 0; k < KS * NA - AHEAD; k++) {
             __builtin_amdgcn_sched_group_barrier(0x008, NS == 2 ? 3 : 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, NS, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * (NS == 2 ? 3 : 1), 0);
-        float vp[NS == 2 ? 16 : 1];                // V's powers of two
+        float s[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) s[i] = sa[i / R][i % R];
+        constexpr int KG = QW == 32 ? 8 : 16;      // a lane's keys: KG g + 4 h + 0 .. 3
+        float vp[NS == 2 ? NV : 1];                // V's powers of two
         if constexpr (NS == 2) {
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const float4 ks = *(const float4 *)(sc + 8 * g + 4 * h), vs = *(const float4 *)(sc + AP_KEYS + 8 * g + 4 * h);
+            for (int g = 0; g < NV / 4; g++) {
+                const float4 ks = *(const float4 *)(sc + KG * g + 4 * h), vs = *(const float4 *)(sc + AP_KEYS + KG * g + 4 * h);
                 s[4 * g] *= rs * ks.x, s[4 * g + 1] *= rs * ks.y;
                 s[4 * g + 2] *= rs * ks.z, s[4 * g + 3] *= rs * ks.w;
                 vp[4 * g] = vs.x, vp[4 * g + 1] = vs.y, vp[4 * g + 2] = vs.z, vp[4 * g + 3] = vs.w;
@@ -317,8 +350,8 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         }
         if constexpr (EDGE.value) {                // (keys behind the end are behind every query)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const bool seen = 8 * (i >> 2) + 4 * h + (i & 3) <= n;
+            for (int i = 0; i < NV; i++) {
+                const bool seen = KG * (i >> 2) + 4 * h + (i & 3) <= qi % AP_KEYS;
                 s[i] = seen ? s[i] : -INFINITY;
                 if constexpr (NS == 2) vp[i] = seen ? vp[i] : 0.0f;
             }
@@ -327,15 +360,15 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         const float r = NS == 2 ? 1.0f : rs;
         float top = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-        top = half_max(top) * r;
+        for (int i = 1; i < NV; i++) top = fmaxf(top, s[i]);
+        top = query_max<QW>(top) * r;
         float f = 1.0f;
         bool move = top > m + 8.0f;
         if constexpr (NS == 2) {
             float vt = vp[0];
 #pragma unroll
-            for (int i = 1; i < 16; i++) vt = fmaxf(vt, vp[i]);
-            const int e = max((int)(__float_as_uint(half_max(vt)) >> 23) - 127, -126);
+            for (int i = 1; i < NV; i++) vt = fmaxf(vt, vp[i]);
+            const int e = max((int)(__float_as_uint(query_max<QW>(vt)) >> 23) - 127, -126);
             if (e > ve) {
                 f = ve == -127 ? 0.0f : pow2i(max(ve - e, -126));
                 ve = e;
@@ -350,12 +383,12 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] *= f;
+                for (int i = 0; i < R; i++) o[d][i] *= f;
         }
         const float pv = NS == 2 ? pow2i(min(7 - ve, 127)) : 1.0f;
-        V8 ph[2], pl[NS == 2 ? 2 : 1];
+        V8 ph[PS], pl[NS == 2 ? PS : 1];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < NV; i++) {
             float p = __builtin_amdgcn_exp2f(NS == 2 ? s[i] - m : fmaf(s[i], r, -m));
             l += p;
             if constexpr (NS == 2) {
@@ -370,11 +403,11 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
-            for (int st = 0; st < 2; st++) {
+            for (int st = 0; st < PS; st++) {
                 union { s16x4 r[2]; V8 v; } vh, vl;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const E *p = K + v_at[d & 3] + 128 * (d >> 2) + (16 * st + 8 * u) * D;
+                    const E *p = K + v_at[d % VV] + 128 * (d / VV) + (PK * st + KG * u) * D;
                     vh.r[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
                     if constexpr (NS == 2)
                         vl.r[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(p + PLANE));
@@ -387,7 +420,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             }
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * 2 * NS, 0);
 #pragma unroll
-        for (int k = 0; k < 2 * DT - AHEAD; k++) {
+        for (int k = 0; k < PS * DT - AHEAD; k++) {
             __builtin_amdgcn_sched_group_barrier(0x008, NS == 2 ? 3 : 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, 2 * NS, 0);
         }
@@ -413,11 +446,12 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 
     // ---- infinities and NaN of V, to the rows that see them: whatever else a
     // row sums, they decide its result, so they are added to it at the end
-    const float inv = 1.0f / half_sum(l);          // every row sees itself
+    const float inv = 1.0f / query_sum<QW>(l);          // every row sees itself
+    constexpr int CG = QW == 32 ? 8 : 0;           // a lane's channels: QW d + CG g + 4 h + 0 .. 3
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] *= inv;
+        for (int i = 0; i < R; i++) o[d][i] *= inv;
     for (int t = 0; t <= mine; t++) {
         if (!A.odd[tile0 + t]) continue;
         for (int k = t * AP_KEYS; k < min(t * AP_KEYS + AP_KEYS, qi + 1); k++) {
@@ -425,8 +459,8 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float x = T::up(vr[32 * d + 8 * (i >> 2) + 4 * h + (i & 3)]);
+                for (int i = 0; i < R; i++) {
+                    const float x = T::up(vr[QW * d + CG * (i >> 2) + 4 * h + (i & 3)]);
                     o[d][i] += fabsf(x) <= 3.402823466e38f ? 0.0f : x;
                 }
         }
@@ -435,33 +469,42 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
+        for (int g = 0; g < R / 4; g++) {
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = NS == 2 ? ldexpf(o[d][4 * g + i], ve - 7) : o[d][4 * g + i];
-            store4<T>(op + 32 * d + 8 * g + 4 * h, A.o_vec, y);
+            store4<T>(op + QW * d + CG * g + 4 * h, A.o_vec, y);
         }
 }
 
-template <class T, int D>
-static int ap_launch(ApArgs A, hipStream_t s)
+template <class T, int D, int NW, int QW, int KT, int AHEAD, int WE>
+static int ap_run(ApArgs A, hipStream_t s)
 {
     constexpr int NS = sizeof(typename T::S) == 4 ? 2 : 1;
     constexpr size_t TILE = 2 * NS * AP_KEYS * D * 2;
     A.tiles = A.T / AP_KEYS + A.n_seq;
     const size_t n = (size_t)A.tiles * A.n_kv + 8;         // a barrier's tiles may reach past the last one
+    const int64_t wgs = (((int64_t)A.T / (QW * NW) + A.n_seq + 7) / 8 * 8) * A.n_kv * A.G;
+    if (wgs > UINT32_MAX / (64 * NW)) return fail(QMAG_ERR_ARG, "attn_prompt: %lld workgroups", (long long)wgs);
     int st;
     uint8_t *ws = (uint8_t *)workspace(WS_ATTN, n * (TILE + (NS == 2 ? 2 * AP_KEYS * sizeof(float) : 0) + sizeof(int)), &st);
     if (st) return st;
     A.img = ws;
     A.scale = (float *)(ws + n * TILE);
     A.odd = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
-    prompt_tiles_kernel<T, D><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv), AP_WG, 0, s>>>(A);
-    constexpr int NW = 4, KT = D == 64 ? 2 : 1, WE = NS == 2 && D == 256 ? 1 : 2;
-    const int64_t wgs = (((int64_t)A.T / (32 * NW) + A.n_seq + 7) / 8 * 8) * A.n_kv * A.G;
-    if (wgs > UINT32_MAX / (64 * NW)) return fail(QMAG_ERR_ARG, "attn_prompt: %lld workgroups", (long long)wgs);
-    attn_prompt_kernel<T, D, NW, KT, WE><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
+    prompt_tiles_kernel<T, D, QW><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv), AP_WG, 0, s>>>(A);
+    attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
     return QMAG_OK;
+}
+
+template <class T, int D>
+static int ap_launch(const ApArgs &A, hipStream_t s)
+{
+    constexpr bool F32 = sizeof(typename T::S) == 4;
+    const int64_t wgs = ((int64_t)A.T / 128 + A.n_seq) * A.n_kv * A.G;
+    if (wgs < (F32 && D == 256 ? 1 : 4) * (int64_t)ctx().n_cu) return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);
+    if constexpr (F32 || D == 256) return ap_run<T, D, 8, 16, D == 64 ? 2 : 1, F32 && D == 128 ? 2 : 3, F32 && D == 128 ? 4 : 2>(A, s);
+    else return ap_run<T, D, 4, 32, D == 64 ? 2 : 1, 3, 2>(A, s);
 }
 
 }  // namespace qmag
