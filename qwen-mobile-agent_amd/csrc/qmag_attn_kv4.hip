@@ -9,10 +9,13 @@
 // the code, and one subtraction for two values leaves code - 8.  No code is
 // rounded, and no step or minimum touches the operand.  The 8 keeps the two sums
 // below small: with codes from 0 to 15 they were each tens of times the result,
-// which cost a digit (1e-5 of the result against 1e-6).  (The nibble alone is an
-// fp16 subnormal, two instructions less for four values, but the matrix cores
-// align subnormal products as if their leading zeros were digits: the sums came
-// out 10 bits short, 3e-4 of the result.)
+// which cost a digit (1e-5 of the result against 1e-6).
+// bf16 calls (RAW) take the nibble alone, an fp16 subnormal (code * 2^-24, or
+// * 2^-20 in the upper half of a byte, made up for exactly): five instructions for
+// eight codes instead of nine.  The matrix cores align subnormal products as if
+// their leading zeros were digits, so the sums are 10 bits short: 3e-4 of the
+// result, a fifth of what bf16's own rounding of it takes (2^-9, 1.7e-3 in the
+// mean), but more than fp16's.
 //   scores   S = K Q^T per 64 channels on codes, then d S + (m + 8 d) sum(q) in fp32;
 //   output   O^T = V^T P'^T with P' = p d: the step of a token and group is
 //            folded into the softmax weight, the rest adds sum_t p (m + 8 d).
@@ -30,11 +33,11 @@
 // from the lengths on the device.  The chunk is the same for all sequences, so
 // that a long one among short ones is spread over the chip; partial results of
 // split sequences are joined by a second launch.
+#include <type_traits>
+
 #include "qmag_attn.h"
 
 namespace qmag {
-
-constexpr int AK_WG = 256;
 
 struct AkArgs {
     const uint8_t *data;
@@ -71,55 +74,63 @@ __device__ __forceinline__ int ak_groups(const AkArgs &A, int nq, int RG)
 }
 
 // The sequence of item `want` (by_token: of row `want` of q), found by the
-// calling wave alone.  False if there is none.
+// calling wave alone.  False if there is none.  (The caps only meet lengths that
+// are none, and keep their sums in range; the host refuses 2^23 groups.)
 template <int RG, int STEP>
 __device__ __forceinline__ bool ak_find(const AkArgs &A, int want, bool by_token, AkPlan *P)
 {
     const int lane = lane_id();
-    unsigned long long cost = 0;
-    int q0, nq, len;
+    int q0 = 0, nq = 0, len = 0;
+    if (lane < A.n_seq) ak_seq(A, lane, &q0, &nq, &len);
     P->chunk = 1 << 30;                            // no sequence is longer
     if (A.min_chunk) {
-        for (int i = lane; i < A.n_seq; i += 64) {
-            ak_seq(A, i, &q0, &nq, &len);
-            cost += (unsigned long long)ak_groups(A, nq, RG) * (unsigned)len;
+        float cost = (float)ak_groups(A, nq, RG) * (float)len;       // the same for whoever forms it
+        for (int i = 64 + lane; i < A.n_seq; i += 64) {
+            int x, n, l;
+            ak_seq(A, i, &x, &n, &l);
+            cost += (float)ak_groups(A, n, RG) * (float)l;
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) cost += __shfl_xor(cost, d);
-        const unsigned long long c = (cost + A.target - 1) / (unsigned)A.target;
-        const unsigned long long r = (max(c, (unsigned long long)A.min_chunk) + STEP - 1) / STEP * STEP;
-        P->chunk = (int)min(r, 1ull << 30);
+        const float c = fminf(group_sum<64>(cost) / (float)A.target, 1073741824.0f);
+        P->chunk = __builtin_amdgcn_readfirstlane(max((int)c / STEP * STEP + STEP, A.min_chunk));
     }
-    long long items = 0;
+    int items = 0;
     for (int base = 0; base < A.n_seq; base += 64) {
-        const int i = base + lane;
-        q0 = nq = len = 0;
-        if (i < A.n_seq) ak_seq(A, i, &q0, &nq, &len);
+        if (base) {
+            q0 = nq = len = 0;
+            if (base + lane < A.n_seq) ak_seq(A, base + lane, &q0, &nq, &len);
+        }
         const int split = max(1, (int)(((unsigned)len + (unsigned)P->chunk - 1u) / (unsigned)P->chunk));
-        const long long mine = (long long)ak_groups(A, nq, RG) * split;
-        long long incl = mine;
+        const int mine = (int)min((long long)ak_groups(A, nq, RG) * split, 1ll << 23);
+        int incl = mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const long long v = __shfl_up(incl, d);
+            const int v = __shfl_up(incl, d);
             if (lane >= d) incl += v;
         }
         const bool here = by_token ? want >= q0 && want < q0 + nq : want < items + incl;
         const unsigned long long hit = __ballot(here);
         if (hit) {
-            const int at = __ffsll(hit) - 1;
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll(hit) - 1);
             P->seq = base + at;
             P->q0 = __builtin_amdgcn_readlane(q0, at);
             P->nq = __builtin_amdgcn_readlane(nq, at);
             P->len = __builtin_amdgcn_readlane(len, at);
             P->n_split = __builtin_amdgcn_readlane(split, at);
+            P->item0 = items + __builtin_amdgcn_readlane(incl - mine, at);
             // lengths that overlap make more items than there are workgroups
-            if (items + __shfl(incl, at) > A.max_items && by_token) return false;
-            P->item0 = (int)(items + __shfl(incl - mine, at));
-            return true;
+            return !by_token || items + __builtin_amdgcn_readlane(incl, at) <= A.max_items;
         }
-        items += __shfl(incl, 63);
+        items = min(items + __builtin_amdgcn_readlane(incl, 63), 1 << 30);
     }
     return false;
+}
+
+// Where row r of a group of RG rows has its partial results: a row's parts one
+// behind another (16 KB apart, as the workgroups write them, they would all lie
+// in one memory channel: joining 256 of them took 14 us against 3).
+__device__ __forceinline__ int64_t ak_part(const AkArgs &A, const AkPlan &P, int kvh, int group, int RG, int r)
+{
+    return ((int64_t)kvh * A.max_items + P.item0 + (int64_t)group * P.n_split) * RG + (int64_t)r * P.n_split;
 }
 
 // max and sum over the four lanes that hold a row
@@ -153,32 +164,48 @@ union Frag {
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Nibbles 0 and 4 of w (of each half dword), or 1 and 5, less 8, as fp16.
-__device__ __forceinline__ uint32_t even_codes(uint32_t w)
-{
-    const half2v v = __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) - (half2v){(_Float16)1032.0f, (_Float16)1032.0f};
-    return __builtin_bit_cast(uint32_t, v);
-}
-__device__ __forceinline__ uint32_t odd_codes(uint32_t w)
-{
-    const half2v v = __builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x54005400u) - (half2v){(_Float16)72.0f, (_Float16)72.0f};
-    return __builtin_bit_cast(uint32_t, v);
-}
+// What turns nibbles into fp16: masks and exponents in registers of both kinds,
+// so that the two go into one instruction.
+struct Nibbles {
+    uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, e1024 = 0x64006400u, e64 = 0x54005400u;
+    // nibbles 0 and 4 of w (of each half dword), or 1 and 5: raw, or less 8, as fp16
+    __device__ __forceinline__ Nibbles()
+    {
+        asm("" : "+s"(lo), "+s"(hi));
+        asm("" : "+v"(e1024), "+v"(e64));
+    }
+    template <bool RAW>
+    __device__ __forceinline__ uint32_t even(uint32_t w) const
+    {
+        if (RAW) return w & lo;
+        const half2v v = __builtin_bit_cast(half2v, (w & lo) | e1024) - (half2v){(_Float16)1032.0f, (_Float16)1032.0f};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+    template <bool RAW>
+    __device__ __forceinline__ uint32_t odd(uint32_t w) const
+    {
+        if (RAW) return w & hi;
+        const half2v v = __builtin_bit_cast(half2v, (w & hi) | e64) - (half2v){(_Float16)72.0f, (_Float16)72.0f};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+};
 
 // Eight nibbles as eight fp16 values, in the order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ half8 k_frag(uint32_t w)
+template <bool RAW>
+__device__ __forceinline__ half8 k_frag(const Nibbles &N, uint32_t w)
 {
     Frag f;
-    f.u[0] = even_codes(w);
-    f.u[1] = odd_codes(w);
-    f.u[2] = even_codes(w >> 8);
-    f.u[3] = odd_codes(w >> 8);
+    f.u[0] = N.template even<RAW>(w);
+    f.u[1] = N.template odd<RAW>(w);
+    f.u[2] = N.template even<RAW>(w >> 8);
+    f.u[3] = N.template odd<RAW>(w >> 8);
     return f.h;
 }
 
-// d, and m + 8 d, the value of code 8
+// d, and m + 8 d, the value of code 8 (RAW: m, of code 0)
 __device__ __forceinline__ float step_of(uint32_t dm) { return h2f(dm & 0xFFFFu); }
-__device__ __forceinline__ float mid_of(uint32_t dm) { return fmaf(8.0f, h2f(dm & 0xFFFFu), h2f(dm >> 16)); }
+template <bool RAW>
+__device__ __forceinline__ float mid_of(uint32_t dm) { return RAW ? h2f(dm >> 16) : fmaf(8.0f, h2f(dm & 0xFFFFu), h2f(dm >> 16)); }
 
 // (hi, lo) fp16 parts of eight values; NS == 1: hi alone, to nearest
 template <int NS>
@@ -211,32 +238,475 @@ __device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&o)[N])
     }
 }
 
-// SPLITW: the four waves take the tiles of a chunk in turn for the same 16
-// rows and join at the end; otherwise each has 16 rows of its own.
-template <class T, int D, bool SPLITW>
-__global__ void __launch_bounds__(AK_WG, 2) attn_kv4_kernel(AkArgs A)
+// Bytes of a wave's tile of 32 tokens in LDS: K codes, V codes, scales of both.
+template <int D>
+constexpr int ak_tile() { return 36 * D; }
+
+// A group of 16 rows against a chunk of the cache: the NW waves take its tiles
+// of 32 tokens in turn and join at the end.  Each wave keeps its next tiles in
+// flight from memory to its own part of LDS (NB tiles, no registers, no
+// barriers); a lane later reads back little more than what it asked for itself.
+template <class T, int D, int NB, int NW>
+__global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typename T::S) == 4 ? 3 : 4) attn_kv4_kernel(AkArgs A)
 {
     using S = typename T::S;
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
+    constexpr bool RAW = std::is_same_v<T, TBF16>;
     constexpr int NG = D / 64;
-    constexpr int RG = SPLITW ? 16 : 64;
+    constexpr int RG = 16, STEP = 32 * NW;
     constexpr int VD = (D + 127) / 128;            // dwords of a lane's V codes of a token
-    constexpr int LROW = D + 4;                    // LDS row of the join
-    __shared__ float join[SPLITW ? 4 * 16 * LROW : 1];
-    __shared__ float join_m[4][16], join_l[4][16];
+    constexpr int TILE = ak_tile<D>();
+    constexpr int LROW = D + 4;                    // row of the join
+    constexpr int LDS = NW * NB * TILE > NW * 16 * LROW * 4 ? NW * NB * TILE : NW * 16 * LROW * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    __shared__ float join_m[NW][16], join_l[NW][16];
 
     const int kvh = blockIdx.y, item = blockIdx.x;
-    const int wave = threadIdx.x >> 6, lane = lane_id(), n = lane & 15, h = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, h = lane >> 4;
     AkPlan P;
-    if (!ak_find<RG, SPLITW ? 128 : 32>(A, item, false, &P)) return;
+    if (!ak_find<RG, STEP>(A, item, false, &P)) return;
     const int local = item - P.item0, split = local % P.n_split, group = local / P.n_split;
-    const int rows = P.nq * A.G;
-    const int r0 = group * RG + (SPLITW ? 0 : wave * 16);
-    if (!SPLITW && r0 >= rows) return;
+    const int rows = P.nq * A.G, r0 = group * RG;
 
-    // ---- queries
+    // ---- the range of tokens
     const int row = r0 + n, j = min(row, rows - 1) / A.G, gh = min(row, rows - 1) - j * A.G;
     const bool live = row < rows;
+    const int past = P.len - P.nq;                 // tokens before the first query's own
+    const int lim = live ? past + j : INT32_MAX;   // the last token the row sees
+    const int j_last = (min(r0 + 16, rows) - 1) / A.G, open = past + r0 / A.G;
+    const int c0 = split * P.chunk + 32 * wave;
+    const int c1 = min(min(P.len, split * P.chunk + P.chunk), past + j_last + 1);
+    // (read as constants: no kernel writes the table while this one runs)
+    const auto *table = (const __attribute__((address_space(4))) int *)(A.table + P.seq * (int64_t)A.max_blocks);
+    const int64_t block_stride = 2 * A.half * A.n_kv;
+    const uint8_t *head = A.data + kvh * 2 * A.half;
+    const int64_t codes = (int64_t)(D / 2) << A.shift;
+    uint8_t *ring = lds + wave * NB * TILE;
+
+    // ---- tiles from memory: where in a half (16 tokens, within a block) a lane's pieces lie
+    int k_from, v_from, s_from;
+    bool k_up = false, v_up = false, s_up;         // the lane's piece is of the upper half
+    if constexpr (D == 256) {
+        k_from = (lane & 15) * 128 + (lane >> 4) * 32;
+        v_from = (4 * ((lane >> 3) & 3) + (lane >> 5)) * 128 + (lane & 7) * 16;
+    } else if constexpr (D == 128) {
+        k_from = (lane & 15) * 64 + (lane >> 4) * 16;
+        v_from = (4 * ((lane >> 2) & 3) + (lane >> 4)) * 64 + (lane & 3) * 16;
+    } else {
+        k_from = (lane & 15) * 32 + ((lane >> 4) & 1) * 16;
+        v_from = (4 * ((lane >> 1) & 3) + ((lane >> 3) & 3)) * 32 + (lane & 1) * 16;
+        k_up = v_up = lane >= 32;
+    }
+    {
+        const int w = lane / (8 * NG), c = lane % (8 * NG);
+        s_up = c >= 4 * NG;
+        s_from = (w ? (int)A.half : 0) + (int)codes + (c % (4 * NG)) * 16;
+    }
+    constexpr int LOADS = (D == 256 ? 8 : D == 128 ? 4 : 2) + 1;
+    uint32_t gone = 0;                             // two bits a tile in flight: a half whose block is none
+    auto dma = [&](const uint8_t *from, uint8_t *to) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                         (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+    };
+    auto issue = [&](int t0, int slot) {
+        const uint8_t *kb[2];
+        int off[2];
+        uint32_t bad = 0;
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const int t = t0 + 16 * a;
+            const int id = table[min(t >> A.shift, A.max_blocks - 1)];
+            const bool there = id >= 0 && id < A.n_block;
+            bad |= there ? 0u : 1u << a;
+            kb[a] = head + (there ? id : 0) * block_stride;
+            off[a] = t & ((1 << A.shift) - 1);
+        }
+        gone = (gone >> 2) | (bad << (2 * (NB - 1)));
+        uint8_t *to = ring + slot * TILE;
+        const uint8_t *k[2] = {kb[0] + off[0] * (D / 2), kb[1] + off[1] * (D / 2)};
+        if constexpr (D == 64) {
+            dma((k_up ? k[1] : k[0]) + (uint32_t)k_from, to);
+            dma((v_up ? k[1] : k[0]) + A.half + (uint32_t)v_from, to + 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 64; i++)       // D = 256: (half, piece), 128: half
+                dma(k[D == 256 ? i >> 1 : i] + (D == 256 ? 16 * (i & 1) : 0) + (uint32_t)k_from, to + 1024 * i);
+#pragma unroll
+            for (int i = 0; i < D / 64; i++)
+                dma(k[D == 256 ? i >> 1 : i] + A.half + (D == 256 ? 256 * (i & 1) : 0) + (uint32_t)v_from, to + 16 * D + 1024 * i);
+        }
+        if (lane < 16 * NG) dma((s_up ? kb[1] + off[1] * (NG * 4) : kb[0] + off[0] * (NG * 4)) + s_from, to + 32 * D);
+    };
+    float x[NG][2][8];                             // the row's queries, under way before the tiles
+    {
+        const S *qp = (const S *)A.q + (P.q0 + j) * A.qt + (kvh * A.G + gh) * A.qh;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int s = 0; s < 2; s++) load8<T>(qp + g * 64 + s * 32 + h * 8, A.q_vec, x[g][s]);
+    }
+#pragma unroll
+    for (int i = 0; i < NB - 1; i++)
+        if (c0 + i * STEP < c1) issue(c0 + i * STEP, i);
+        else gone >>= 2;
+
+    const Nibbles N;
+    // ---- queries
+    half8 qh[NG][2], ql[NS == 2 ? NG : 1][2];
+    float qs[NG], rs;
+    {
+        float top = 0.0f;
+#pragma unroll
+        for (int g = 0; g < NG; g++)
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[g][s][i]));
+        // the row's largest value to 2^14 .. 2^15: exact, and undone by rs
+        const int e = min(max((int)(__float_as_uint(row_max(top)) >> 23) - 127, -100), 127);
+        const float up = exp2i(14 - e);
+        rs = (RAW ? exp2i(min(e, 113) - 14 + 24) : exp2i(e - 14)) * A.scale;      // (beyond 2^113 weights are 0 or 1 in any case)
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[g][s][i] *= up;
+                    sum += x[g][s][i];
+                    f[2 * (i & 3) + (i >> 2)] = x[g][s][i] * (RAW && (i & 1) ? 0.0625f : 1.0f);     // nibble i's place in a fragment
+                }
+                split8<NS>(f, &qh[g][s], &ql[NS == 2 ? g : 0][s]);
+            }
+            qs[g] = row_sum(sum) * (RAW ? 0x1p-24f : 1.0f);
+        }
+    }
+
+    f32x4 o[NG][4];
+    float vs[NG], l = 0.0f, m = -INFINITY;
+    int ve = -1;                                   // the row's weights carry 2^(21 - ve)
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        vs[g] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[g][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    int slot = 0;
+    for (int t0 = c0; t0 < c1; t0 += STEP) {
+        // this tile's pieces are in once no more than the next ones' are under way
+        if (NB > 2 && t0 + STEP < c1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t0 + (NB - 1) * STEP < c1) issue(t0 + (NB - 1) * STEP, slot == 0 ? NB - 1 : slot - 1);
+        else gone >>= 2;
+        const uint32_t bad = gone & 3;
+        const uint8_t *tile = ring + slot * TILE;
+        slot = slot + 1 == NB ? 0 : slot + 1;
+
+        // ---- scores
+        float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            uint32_t kc[D / 32], dm[4][NG];
+            if constexpr (D == 64) load_dwords(tile + (a * 32 + (h >> 1) * 16 + n) * 16 + (h & 1) * 8, kc);
+            else {
+#pragma unroll
+                for (int i = 0; i < D / 128; i++) {
+                    const uint4 v = *(const uint4 *)(tile + ((a * (D / 128) + i) * 64 + lane) * 16);
+                    kc[4 * i] = v.x, kc[4 * i + 1] = v.y, kc[4 * i + 2] = v.z, kc[4 * i + 3] = v.w;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) load_dwords(tile + 32 * D + (16 * a + 4 * h + r) * (NG * 4), dm[r]);
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    const half8 kf = k_frag<RAW>(N, kc[2 * g + st]);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g][st], acc, 0, 0, 0);
+                    if constexpr (NS == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g][st], acc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float d = step_of(dm[r][g]), mid = mid_of<RAW>(dm[r][g]);
+                    s[4 * a + r] = fmaf(d, acc[r], fmaf(mid, qs[g], s[4 * a + r]));
+                }
+            }
+        }
+        uint32_t vdm[8][NG];
+#pragma unroll
+        for (int i = 0; i < 8; i++) load_dwords(tile + 32 * D + 128 * NG + (16 * (i >> 2) + 4 * h + (i & 3)) * (NG * 4), vdm[i]);
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; i++) s[i] *= rs;
+        if (bad || t0 + 31 > open) {
+            // a token the row does not see has no weight, whatever the cache holds there
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int a = i >> 2, tk = t0 + 16 * a + 4 * h + (i & 3);
+                const bool seen = tk <= lim && tk < c1 && !((bad >> a) & 1);
+                s[i] = seen ? s[i] : -INFINITY;
+#pragma unroll
+                for (int g = 0; g < NG; g++) vdm[i][g] = seen ? vdm[i][g] : 0u;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = fmaxf(top, s[i]);
+        top = row_max(top);
+
+        // ---- running maximum: moved only when a weight would pass 2^8
+        if (__any(top > m + 8.0f)) {
+            const float mn = fmaxf(m, top);
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                vs[g] *= f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[g][i] *= f;
+            }
+        }
+        const float ms = m == -INFINITY ? 0.0f : m;
+        // ---- the largest step the row has seen sets the power of two of its weights
+        typedef short s16x2 __attribute__((ext_vector_type(2)));
+        s16x2 dt = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) dt = __builtin_elementwise_max(dt, __builtin_bit_cast(s16x2, vdm[i][g]));
+        const int de = row_max_i(min((int)dt[0] >> 10, 30));
+        if (__any(de > ve)) {
+            const int en = max(de, ve);
+            const float f = ve < 0 ? 0.0f : exp2i(ve - en);
+            ve = en;
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[g][i] *= f;
+        }
+        const float pf = exp2i(21 - ve);
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = __builtin_amdgcn_exp2f(s[i] - ms);
+            l += p[i];
+        }
+
+        // ---- output
+        uint32_t vc[8][VD];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint8_t *v = tile + 16 * D + (i * 4 + h) * (D / 2) + n * (D / 32);
+            if constexpr (D == 64) vc[i][0] = *(const uint16_t *)v;
+            else load_dwords(v, vc[i]);
+        }
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[i] = p[i] * pf * step_of(vdm[i][g]);
+                vs[g] = fmaf(p[i], mid_of<RAW>(vdm[i][g]), vs[g]);
+            }
+            half8 ph, pl;
+            split8<NS>(x, &ph, &pl);
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                // byte b of group g: channels 4 n + 2 b and the next of every token
+                Frag even, odd;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int at = 2 * (g & 1) + b;
+                    const uint32_t w = __builtin_amdgcn_perm(vc[2 * k + 1][g >> 1], vc[2 * k][g >> 1],
+                                                             0x0C040C00u + 0x00010001u * (uint32_t)at);
+                    even.u[k] = N.template even<RAW>(w);
+                    odd.u[k] = N.template odd<RAW>(w);
+                }
+                o[g][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even.h, ph, o[g][2 * b], 0, 0, 0);
+                o[g][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd.h, ph, o[g][2 * b + 1], 0, 0, 0);
+                if constexpr (NS == 2) {
+                    o[g][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even.h, pl, o[g][2 * b], 0, 0, 0);
+                    o[g][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd.h, pl, o[g][2 * b + 1], 0, 0, 0);
+                }
+            }
+        }
+    }
+
+    // ---- the waves' shares; a lane's row: channels 64 g + 4 (4 h + r) + i in o[g][i][r]
+    l = row_sum(l);
+    const float back = exp2i(max(ve, 0) - 21) * (RAW ? 0x1p24f : 1.0f), back1 = back * (RAW ? 0.0625f : 1.0f);
+    if (h == 0) {
+        join_m[wave][n] = m;
+        join_l[wave][n] = l;
+    }
+    __syncthreads();                               // no wave reads its tiles any more either
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; w++) all = fmaxf(all, join_m[w][n]);
+    float share = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - all);
+    if (m == -INFINITY && l != 0.0f) share = l;    // a NaN weight leaves m at -inf: let it through
+    float *join = (float *)lds, *mine = join + (wave * 16 + n) * LROW;
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+        const float add = row_sum(vs[g]);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            *(float4 *)(mine + 64 * g + 4 * (4 * h + r)) =
+                make_float4(fmaf(o[g][0][r], back, add) * share, fmaf(o[g][1][r], back1, add) * share,
+                            fmaf(o[g][2][r], back, add) * share, fmaf(o[g][3][r], back1, add) * share);
+    }
+    __syncthreads();
+    // 4 NW threads a row, four channels at a time
+    constexpr int PER = 4 * NW, CP = D / (4 * PER) > 0 ? D / (4 * PER) : 1;
+    const int rr = threadIdx.x / PER, cc = threadIdx.x % PER;
+    if (r0 + rr >= rows) return;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) M = fmaxf(M, join_m[w][rr]);
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+        const float mw = join_m[w][rr], lw = join_l[w][rr];
+        L += mw == -INFINITY ? (lw != 0.0f ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - M);
+    }
+    const int jj = (r0 + rr) / A.G, hh = r0 + rr - jj * A.G;
+    S *op = (S *)A.out + (P.q0 + jj) * A.ot + (kvh * A.G + hh) * A.oh;
+    const int64_t at = ak_part(A, P, kvh, group, RG, rr) + split;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int cb = 0; cb < CP; cb++) {
+        const int c = 4 * (cb * PER + cc);
+        if (c >= D) break;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float4 f = *(const float4 *)(join + (w * 16 + rr) * LROW + c);
+            v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+        }
+        if (P.n_split == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] *= inv;
+            store4<T>(op + c, A.o_vec, v);
+        } else {
+            store4<TF32>(A.part + at * D + c, true, v);
+        }
+    }
+    if (P.n_split > 1 && cc == 0) {
+        A.ml[2 * at] = M;
+        A.ml[2 * at + 1] = L;
+    }
+}
+
+// Many rows to a sequence: NW waves of 16 rows each against a chunk of the cache.
+// A tile of 32 tokens comes from memory to LDS as it lies there, is turned into
+// fp16 codes once for all the waves (K and V row by row, in the order the
+// products read them), and then serves as a tile of a prompt does; memory is two
+// tiles ahead, the codes one, and a tile costs one barrier.
+template <class T, int D, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) attn_kv4_rows_kernel(AkArgs A)
+{
+    using S = typename T::S;
+    constexpr int NS = sizeof(S) == 4 ? 2 : 1;
+    constexpr bool RAW = false;                    // the codes are formed once: no need to save there
+    constexpr int NG = D / 64;
+    constexpr int RG = 16 * NW, STEP = 32;
+    constexpr int TILE = ak_tile<D>(), IMG = 32 * D, SC = 4 * D;   // bytes, values, bytes
+    __shared__ __attribute__((aligned(16))) uint8_t raw[2][TILE];
+    __shared__ __attribute__((aligned(16))) _Float16 ik[2][IMG], iv[2][IMG];
+    __shared__ __attribute__((aligned(16))) uint8_t isc[2][SC];    // scales of K, then of V: [32][NG] each
+
+    const int kvh = blockIdx.y, item = blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, h = lane >> 4;
+    AkPlan P;
+    if (!ak_find<RG, STEP>(A, item, false, &P)) return;
+    const int local = item - P.item0, split = local % P.n_split, group = local / P.n_split;
+    const int rows = P.nq * A.G, r0 = group * RG + wave * 16;
+
+    // ---- the range of tokens
+    const int row = r0 + n, j = min(row, rows - 1) / A.G, gh = min(row, rows - 1) - j * A.G;
+    const bool live = row < rows;
+    const int past = P.len - P.nq;                 // tokens before the first query's own
+    const int lim = live ? past + j : INT32_MAX;   // the last token the row sees
+    const int open = past + min(r0, rows - 1) / A.G;
+    const int c0 = split * P.chunk, c1 = min(P.len, c0 + P.chunk);
+    const int all = min(c1, past + (min(group * RG + RG, rows) - 1) / A.G + 1);        // what any row sees
+    const int mine = r0 < rows ? min(c1, past + (min(r0 + 16, rows) - 1) / A.G + 1) : c0;   // what the wave's see
+    const auto *table = (const __attribute__((address_space(4))) int *)(A.table + P.seq * (int64_t)A.max_blocks);
+    const int64_t block_stride = 2 * A.half * A.n_kv;
+    const uint8_t *head = A.data + kvh * 2 * A.half;
+    const int codes = (D / 2) << A.shift;
+
+    // ---- tiles from memory, 16-byte pieces in the order [K codes | V codes | K scales | V scales], halves in turn
+    constexpr int PIECES = TILE / 16;
+    uint32_t gone = 0;                             // two bits a tile: a half whose block is none
+    auto issue = [&](int t0, int b) {
+        const uint8_t *kb[2];
+        int off[2];
+        uint32_t bad = 0;
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const int t = t0 + 16 * a;
+            const int id = table[min(t >> A.shift, A.max_blocks - 1)];
+            const bool there = id >= 0 && id < A.n_block;
+            bad |= there ? 0u : 1u << a;
+            kb[a] = head + (there ? id : 0) * block_stride;
+            off[a] = t & ((1 << A.shift) - 1);
+        }
+        gone = (gone >> 2) | (bad << 4);
+#pragma unroll
+        for (int w = 0; w < (PIECES + 64 * NW - 1) / (64 * NW); w++) {
+            const int p0 = (w * NW + wave) * 64, p = p0 + lane;
+            if (p >= PIECES) break;
+            const bool sc = p >= 2 * D;
+            const int q = sc ? p - 2 * D : p, per = sc ? D / 16 : D / 2;       // pieces of a half
+            const int v = q >= 2 * per, a = (q / per) & 1, x = q % per;
+            const uint8_t *from = (a ? kb[1] : kb[0]) + (v ? A.half : 0) + (sc ? codes + (a ? off[1] : off[0]) * (NG * 4) : (a ? off[1] : off[0]) * (D / 2)) + 16 * x;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                             (__attribute__((address_space(3))) void *)(raw[b] + 16 * p0), 16, 0, 0);
+        }
+    };
+    const Nibbles N;
+    auto unpack = [&](int b) {
+#pragma unroll
+        for (int w = 0; w < (PIECES + 64 * NW - 1) / (64 * NW); w++) {
+            const int p = w * 64 * NW + (int)threadIdx.x;
+            if (p >= PIECES) break;
+            const uint4 x = *(const uint4 *)(raw[b] + 16 * p);
+            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+            if (p < D) {                           // K: dword h * D / 32 + 2 g + s of a row
+                const int t = p / (D / 32), d0 = 4 * (p % (D / 32));
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int hh = (d0 + i) / (D / 32), gs = (d0 + i) % (D / 32);
+                    *(half8 *)(ik[b] + t * D + 8 * (D == 64 ? (4 * gs + hh) ^ ((t >> 1) & 7) : (4 * gs + hh) ^ (t & 15))) =
+                        k_frag<RAW>(N, u[i]);
+                }
+            } else if (p < 2 * D) {                // V: 16-bit word i * NG + g of a row, four channels
+                const int t = (p - D) / (D / 32), w0 = 8 * ((p - D) % (D / 32));
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t c = i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xFFFFu;
+                    const int ii = (w0 + i) / NG, g = (w0 + i) % NG, ch = 8 * g + (ii >> 1);
+                    union { uint32_t u[2]; s16x4 v; } y;
+                    y.u[0] = N.template even<RAW>(c | (c << 12));
+                    y.u[1] = N.template even<RAW>((c >> 8) | (c << 4));
+                    *(s16x4 *)(iv[b] + t * D + 8 * (D == 64 ? ch ^ (t & 6) : ch ^ ((t & 7) << 1)) + 4 * (ii & 1)) = y.v;
+                }
+            } else {
+                *(uint4 *)(isc[b] + 16 * (p - 2 * D)) = x;
+            }
+        }
+    };
+    auto arrived = [&]() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    if (c0 < all) issue(c0, 0);
+
+    // ---- queries
     half8 qh[NG][2], ql[NS == 2 ? NG : 1][2];
     float qs[NG], rs;
     {
@@ -272,20 +742,7 @@ __global__ void __launch_bounds__(AK_WG, 2) attn_kv4_kernel(AkArgs A)
         }
     }
 
-    // ---- the range of tokens
-    const int past = P.len - P.nq;                 // tokens before the first query's own
-    const int lim = live ? past + j : INT32_MAX;   // the last token the row sees
-    const int j_last = (min(r0 + 16, rows) - 1) / A.G, open = past + r0 / A.G;
-    int c0 = split * P.chunk;
-    const int c1 = min(min(P.len, c0 + P.chunk), past + j_last + 1);
-    if (SPLITW) c0 += 32 * wave;
-    constexpr int STEP = SPLITW ? 128 : 32;
-    const int *table = A.table + P.seq * (int64_t)A.max_blocks;
-    const int64_t block_stride = 2 * A.half * A.n_kv;
-    const uint8_t *head = A.data + kvh * 2 * A.half;
-    const int64_t codes = (int64_t)(D / 2) << A.shift;
-
-    f32x4 o[NG][4];
+    f32x4 o[NG][4];                                // channels 64 g + 16 i + 4 h + r in o[g][i][r]
     float vs[NG], l = 0.0f, m = -INFINITY;
     int ve = -1;                                   // the row's weights carry 2^(21 - ve)
 #pragma unroll
@@ -294,65 +751,54 @@ __global__ void __launch_bounds__(AK_WG, 2) attn_kv4_kernel(AkArgs A)
 #pragma unroll
         for (int i = 0; i < 4; i++) o[g][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    // a lane's places in an image: its chunk of K's row n, four of its tokens' 16 channels of V
+    constexpr int KV = D == 64 ? 2 : 4, VV = D == 64 ? 4 : 8;        // places that differ by more than a constant
+    int k_at[KV], v_at[VV];
+#pragma unroll
+    for (int i = 0; i < KV; i++) k_at[i] = n * D + 8 * (D == 64 ? (4 * i + h) ^ (n >> 1) : (4 * i + h) ^ n);
+#pragma unroll
+    for (int i = 0; i < VV; i++) {
+        const int t = 4 * h + (n >> 2), ch = 2 * i + ((n & 3) >> 1);
+        v_at[i] = t * D + 8 * (D == 64 ? ch ^ (t & 6) : ch ^ ((t & 7) << 1)) + 4 * (n & 1);
+    }
 
-    for (int t0 = c0; t0 < c1; t0 += STEP) {
-        // two halves of 16 tokens, each within one block
-        const uint8_t *kb[2];
-        bool there[2];
-        int off[2];
-#pragma unroll
-        for (int a = 0; a < 2; a++) {
-            const int t = t0 + 16 * a;
-            const int id = table[min(t >> A.shift, A.max_blocks - 1)];
-            there[a] = id >= 0 && id < A.n_block;
-            kb[a] = head + (there[a] ? id : 0) * block_stride;
-            off[a] = t & ((1 << A.shift) - 1);
-        }
-        uint32_t kc[2][D / 32], kdm[8][NG], vdm[8][NG], vc[8][VD];
-#pragma unroll
-        for (int a = 0; a < 2; a++) load_dwords(kb[a] + (off[a] + n) * (D / 2) + h * (D / 8), kc[a]);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int a = i >> 2, tk = off[a] + 4 * h + (i & 3);
-            load_dwords(kb[a] + codes + tk * (NG * 4), kdm[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int a = i >> 2, tk = off[a] + 4 * h + (i & 3);
-            const uint8_t *vb = kb[a] + A.half;
-            if constexpr (D == 64) vc[i][0] = *(const uint16_t *)(vb + tk * (D / 2) + n * 2);
-            else load_dwords(vb + tk * (D / 2) + n * (D / 32), vc[i]);
-            load_dwords(vb + codes + tk * (NG * 4), vdm[i]);
-        }
-
+    auto compute = [&](int t0, int b, uint32_t bad) {
         // ---- scores
         float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int a = 0; a < 2; a++)
+        for (int a = 0; a < 2; a++) {
+            uint32_t dm[4][NG];
+#pragma unroll
+            for (int r = 0; r < 4; r++) load_dwords(isc[b] + (16 * a + 4 * h + r) * (NG * 4), dm[r]);
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int st = 0; st < 2; st++) {
-                    const half8 kf = k_frag(kc[a][2 * g + st]);
+                    const int k = 2 * g + st;
+                    const half8 kf = *(const half8 *)(ik[b] + k_at[k % KV] + 128 * (k / KV) + 16 * a * D);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g][st], acc, 0, 0, 0);
                     if constexpr (NS == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g][st], acc, 0, 0, 0);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float d = step_of(kdm[4 * a + r][g]), mid = mid_of(kdm[4 * a + r][g]);
+                    const float d = step_of(dm[r][g]), mid = mid_of<RAW>(dm[r][g]);
                     s[4 * a + r] = fmaf(d, acc[r], fmaf(mid, qs[g], s[4 * a + r]));
                 }
             }
+        }
+        uint32_t vdm[8][NG];
+#pragma unroll
+        for (int i = 0; i < 8; i++) load_dwords(isc[b] + SC / 2 + (16 * (i >> 2) + 4 * h + (i & 3)) * (NG * 4), vdm[i]);
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; i++) s[i] *= rs;
-        if (!there[0] || !there[1] || t0 + 31 > open) {
+        if (bad || t0 + 31 > open) {
             // a token the row does not see has no weight, whatever the cache holds there
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int a = i >> 2, tk = t0 + 16 * a + 4 * h + (i & 3);
-                const bool seen = tk <= lim && tk < c1 && there[a];
+                const bool seen = tk <= lim && tk < mine && !((bad >> a) & 1);
                 s[i] = seen ? s[i] : -INFINITY;
 #pragma unroll
                 for (int g = 0; g < NG; g++) vdm[i][g] = seen ? vdm[i][g] : 0u;
@@ -408,182 +854,136 @@ __global__ void __launch_bounds__(AK_WG, 2) attn_kv4_kernel(AkArgs A)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = p[i] * pf * step_of(vdm[i][g]);
-                vs[g] = fmaf(p[i], mid_of(vdm[i][g]), vs[g]);
+                vs[g] = fmaf(p[i], mid_of<RAW>(vdm[i][g]), vs[g]);
             }
             half8 ph, pl;
             split8<NS>(x, &ph, &pl);
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                // byte b of group g: channels 4 n + 2 b and the next of every token
-                Frag even, odd;
+            for (int i = 0; i < 4; i++) {
+                union { s16x4 r[2]; half8 v; } vf;
+                const int part = 4 * g + i;        // of 16 channels
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int at = 2 * (g & 1) + b;
-                    const uint32_t w = __builtin_amdgcn_perm(vc[2 * k + 1][g >> 1], vc[2 * k][g >> 1],
-                                                             0x0C040C00u + 0x00010001u * (uint32_t)at);
-                    even.u[k] = even_codes(w);
-                    odd.u[k] = odd_codes(w);
-                }
-                o[g][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even.h, ph, o[g][2 * b], 0, 0, 0);
-                o[g][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd.h, ph, o[g][2 * b + 1], 0, 0, 0);
-                if constexpr (NS == 2) {
-                    o[g][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even.h, pl, o[g][2 * b], 0, 0, 0);
-                    o[g][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd.h, pl, o[g][2 * b + 1], 0, 0, 0);
-                }
+                for (int u = 0; u < 2; u++)
+                    vf.r[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) s16x4 *)(iv[b] + v_at[part % VV] + 128 * (part / VV) + 16 * u * D));
+                o[g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.v, ph, o[g][i], 0, 0, 0);
+                if constexpr (NS == 2) o[g][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.v, pl, o[g][i], 0, 0, 0);
             }
         }
+    };
+
+    arrived();
+    if (c0 + STEP < all) issue(c0 + STEP, 1);
+    else gone >>= 2;
+    if (c0 < all) unpack(0);
+    for (int t0 = c0, b = 0; t0 < all; t0 += STEP, b ^= 1) {
+        arrived();
+        // two bits each: this tile, the next, the one after it
+        const uint32_t bad = (gone >> 2) & 3;
+        if (t0 + 2 * STEP < all) issue(t0 + 2 * STEP, b);
+        else gone >>= 2;
+        if (t0 + STEP < all) unpack(b ^ 1);
+        if (t0 < mine) compute(t0, b, bad);
     }
 
-    // ---- a lane's row: channels 64 g + 4 (4 h + r) + i in o[g][i][r]
+    if (!live) return;
     l = row_sum(l);
     const float back = exp2i(max(ve, 0) - 21);
-    float y[NG][4][4];                             // [g][r][i]
-    float scale_w = 1.0f;
-    if constexpr (SPLITW) {
-        if (h == 0) {
-            join_m[wave][n] = m;
-            join_l[wave][n] = l;
-        }
-        __syncthreads();
-        float all = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; w++) all = fmaxf(all, join_m[w][n]);
-        scale_w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - all);
-        // a NaN weight leaves m at -inf: let it through
-        if (m == -INFINITY && l != 0.0f) scale_w = l;
-    }
+    const float inv = P.n_split > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    const float nan = m == -INFINITY && l != 0.0f ? l : 0.0f;       // a NaN weight leaves m at -inf
+    S *op = (S *)A.out + (P.q0 + j) * A.ot + (kvh * A.G + gh) * A.oh;
+    const int64_t at = ak_part(A, P, kvh, group, RG, wave * 16 + n) + split;
 #pragma unroll
     for (int g = 0; g < NG; g++) {
         const float add = row_sum(vs[g]);
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int i = 0; i < 4; i++) {
+            const int c = 64 * g + 16 * i + 4 * h;
+            float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                y[g][r][i] = fmaf(o[g][i][r], back, add) * scale_w;
+            for (int r = 0; r < 4; r++) y[r] = fmaf(o[g][i][r], back, add) * inv + nan;
+            if (P.n_split == 1) store4<T>(op + c, A.o_vec, y);
+            else store4<TF32>(A.part + at * D + c, true, y);
+        }
     }
-    const int64_t slot = ((int64_t)kvh * A.max_items + item) * RG;
-    if constexpr (SPLITW) {
-        float *mine = join + (wave * 16 + n) * LROW;
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                *(float4 *)(mine + 64 * g + 4 * (4 * h + r)) = make_float4(y[g][r][0], y[g][r][1], y[g][r][2], y[g][r][3]);
-        __syncthreads();
-        // 16 threads a row, four channels at a time
-        const int rr = threadIdx.x >> 4, cc = threadIdx.x & 15;
-        if (r0 + rr >= rows) return;
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) M = fmaxf(M, join_m[w][rr]);
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float mw = join_m[w][rr], lw = join_l[w][rr];
-            L += mw == -INFINITY ? (lw != 0.0f ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - M);
-        }
-        const int jj = (r0 + rr) / A.G, hh = r0 + rr - jj * A.G;
-        S *op = (S *)A.out + (P.q0 + jj) * A.ot + (kvh * A.G + hh) * A.oh;
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-        for (int c = 0; c < D; c += 64) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float4 f = *(const float4 *)(join + (w * 16 + rr) * LROW + c + 4 * cc);
-                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
-            }
-            if (P.n_split == 1) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] *= inv;
-                store4<T>(op + c + 4 * cc, A.o_vec, v);
-            } else {
-                store4<TF32>(A.part + (slot + rr) * D + c + 4 * cc, true, v);
-            }
-        }
-        if (P.n_split > 1 && cc == 0) {
-            A.ml[2 * (slot + rr)] = M;
-            A.ml[2 * (slot + rr) + 1] = L;
-        }
-    } else {
-        if (!live) return;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        S *op = (S *)A.out + (P.q0 + j) * A.ot + (kvh * A.G + gh) * A.oh;
-        const int64_t at = slot + wave * 16 + n;
-#pragma unroll
-        for (int g = 0; g < NG; g++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int c = 64 * g + 4 * (4 * h + r);
-                if (P.n_split == 1) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) y[g][r][i] *= inv;
-                    store4<T>(op + c, A.o_vec, y[g][r]);
-                } else {
-                    store4<TF32>(A.part + at * D + c, true, y[g][r]);
-                }
-            }
-        if (P.n_split > 1 && h == 0) {
-            A.ml[2 * at] = m;
-            A.ml[2 * at + 1] = l;
-        }
+    if (P.n_split > 1 && h == 0) {
+        A.ml[2 * at] = m;
+        A.ml[2 * at + 1] = l;
     }
 }
 
-// Joins the partial results of the rows whose sequence was split: a workgroup
-// for a head of a token, its waves the parts in turn.
-template <class T, int D, int RG, int STEP>
-__global__ void __launch_bounds__(AK_WG) attn_kv4_join_kernel(AkArgs A)
+// Joins the partial results of the rows whose sequence was split: a workgroup of
+// NW waves for a head of a token and CW of its channels, the waves the parts in
+// turn.  Few rows: many waves to few channels, so that a wave's parts are all
+// requested at once.
+template <class T, int D, int RG, int STEP, int NW, int CW>
+__global__ void __launch_bounds__(64 * NW) attn_kv4_join_kernel(AkArgs A)
 {
     using S = typename T::S;
-    constexpr int C = D / 64;                       // channels of a lane
-    __shared__ float sum[4][D], sl[4];
-    const int t = blockIdx.x, head = blockIdx.y, kvh = head / A.G, gh = head - kvh * A.G;
+    constexpr int C = CW / 64;                      // channels of a lane
+    __shared__ float sum[NW][CW], sl[NW];
+    const int t = blockIdx.x, head = blockIdx.y, kvh = head / A.G, gh = head - kvh * A.G, c0 = blockIdx.z * CW;
     const int wave = threadIdx.x >> 6, lane = lane_id();
     AkPlan P;
     if (!ak_find<RG, STEP>(A, t, true, &P) || P.n_split == 1) return;
     const int row = (t - P.q0) * A.G + gh;
-    const int64_t first = ((int64_t)kvh * A.max_items + P.item0 + row / RG * P.n_split) * RG + row % RG;
+    const int64_t first = ak_part(A, P, kvh, row / RG, RG, row % RG);
     float M = -INFINITY;
-    for (int i = lane; i < P.n_split; i += 64) M = fmaxf(M, A.ml[2 * (first + (int64_t)i * RG)]);
+    for (int i = lane; i < P.n_split; i += 64) M = fmaxf(M, A.ml[2 * (first + i)]);
     M = group_max<64>(M);
     float acc[C], L = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; c++) acc[c] = 0.0f;
-#pragma unroll 4
-    for (int i = wave; i < P.n_split; i += 4) {
-        const int64_t at = first + (int64_t)i * RG;
-        const float mi = A.ml[2 * at], li = A.ml[2 * at + 1];
-        const float f = mi == -INFINITY ? (li != 0.0f ? li : 0.0f) : __builtin_amdgcn_exp2f(mi - M);
-        L += mi == -INFINITY ? f : f * li;
+    constexpr int U = 8;                            // parts requested at once
+    for (int i0 = wave; i0 < P.n_split; i0 += U * NW) {
+        float mi[U], li[U], v[U][C];
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const float v = A.part[at * D + 64 * c + lane];
+        for (int u = 0; u < U; u++) {
+            const int64_t at = first + min(i0 + u * NW, P.n_split - 1);
+            const float2 x = *(const float2 *)(A.ml + 2 * at);
+            mi[u] = x.x, li[u] = x.y;
+#pragma unroll
+            for (int c = 0; c < C; c++) v[u][c] = A.part[at * D + c0 + 64 * c + lane];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const bool in = i0 + u * NW < P.n_split;
+            const float f = !in ? 0.0f : mi[u] == -INFINITY ? (li[u] != 0.0f ? li[u] : 0.0f) : __builtin_amdgcn_exp2f(mi[u] - M);
+            if (in) L += mi[u] == -INFINITY ? f : f * li[u];
             // a part without a token seen: nothing was summed there
-            acc[c] += f == 0.0f ? 0.0f : f * v;
+#pragma unroll
+            for (int c = 0; c < C; c++) acc[c] += f == 0.0f ? 0.0f : f * v[u][c];
         }
     }
 #pragma unroll
     for (int c = 0; c < C; c++) sum[wave][64 * c + lane] = acc[c];
     if (lane == 0) sl[wave] = L;
     __syncthreads();
-    L = sl[0] + sl[1] + sl[2] + sl[3];
+    L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) L += sl[w];
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    S *op = (S *)A.out + t * A.ot + head * A.oh;
-    for (int c = threadIdx.x; c < D; c += AK_WG) op[c] = T::down((sum[0][c] + sum[1][c] + sum[2][c] + sum[3][c]) * inv);
+    S *op = (S *)A.out + t * A.ot + head * A.oh + c0;
+    for (int c = threadIdx.x; c < CW; c += 64 * NW) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) v += sum[w][c];
+        op[c] = T::down(v * inv);
+    }
 }
 
-template <class T, int D, bool SPLITW>
+template <class T, int D, bool ROWS>
 static int ak_launch(AkArgs A, hipStream_t s)
 {
-    constexpr int RG = SPLITW ? 16 : 64, STEP = SPLITW ? 128 : 32;
-    // Row groups at most; two workgroups for every CU are aimed at.
+    constexpr int NW = ROWS ? 8 : 4, RG = ROWS ? 16 * NW : 16, STEP = ROWS ? 32 : 32 * NW;
+    // Row groups at most; with so many workgroups to a CU in mind chunks are cut.
     const int64_t groups = (int64_t)A.T * A.G / RG + A.n_seq;
-    const int64_t goal = 2 * (int64_t)ctx().n_cu;
+    const int64_t goal = (ROWS ? 1 : 4) * (int64_t)ctx().n_cu;
     A.target = (int)((goal + A.n_kv - 1) / A.n_kv);
     // enough row groups to fill the chip twice over: nothing is split
-    A.min_chunk = ((int64_t)A.T * A.G / RG) * A.n_kv >= 2 * goal ? 0 : 256;
+    A.min_chunk = ((int64_t)A.T * A.G / RG) * A.n_kv >= 2 * goal ? 0 : 128;
     const int64_t items = groups + (A.min_chunk ? A.target : 0);
-    if (items > INT32_MAX / AK_WG) return fail(QMAG_ERR_ARG, "attn_kv4: %lld groups of rows", (long long)items);
+    if (items >= 1 << 23) return fail(QMAG_ERR_ARG, "attn_kv4: %lld groups of rows", (long long)items);
     A.max_items = (int)items;
     if (A.min_chunk) {
         int st;
@@ -592,9 +992,16 @@ static int ak_launch(AkArgs A, hipStream_t s)
         if (st) return st;
         A.ml = A.part + rows * D;
     }
-    attn_kv4_kernel<T, D, SPLITW><<<dim3((unsigned)items, (unsigned)A.n_kv), AK_WG, 0, s>>>(A);
-    if (A.min_chunk)
-        attn_kv4_join_kernel<T, D, RG, STEP><<<dim3((unsigned)A.T, (unsigned)(A.n_kv * A.G)), AK_WG, 0, s>>>(A);
+    const dim3 grid((unsigned)items, (unsigned)A.n_kv);
+    if constexpr (ROWS) attn_kv4_rows_kernel<T, D, NW><<<grid, 64 * NW, 0, s>>>(A);
+    else attn_kv4_kernel<T, D, 2, NW><<<grid, 64 * NW, 0, s>>>(A);
+    if (A.min_chunk) {
+        const unsigned heads = (unsigned)(A.n_kv * A.G);
+        if ((int64_t)A.T * heads * (D / 64) <= ctx().n_cu)
+            attn_kv4_join_kernel<T, D, RG, STEP, 16, 64><<<dim3((unsigned)A.T, heads, D / 64), 1024, 0, s>>>(A);
+        else
+            attn_kv4_join_kernel<T, D, RG, STEP, 4, D><<<dim3((unsigned)A.T, heads), 256, 0, s>>>(A);
+    }
     return QMAG_OK;
 }
 
@@ -602,8 +1009,8 @@ template <class T, int D>
 static int ak_pick(const AkArgs &A, hipStream_t s)
 {
     // few rows to a sequence: the waves share them and split the tokens
-    if ((int64_t)A.T * A.G <= 32 * (int64_t)A.n_seq) return ak_launch<T, D, true>(A, s);
-    return ak_launch<T, D, false>(A, s);
+    if ((int64_t)A.T * A.G <= 64 * (int64_t)A.n_seq) return ak_launch<T, D, false>(A, s);
+    return ak_launch<T, D, true>(A, s);
 }
 
 }  // namespace qmag
