@@ -47,15 +47,18 @@ int with_type(int type, F f)
     return f(TBF16{});
 }
 
-// x as it is, rounded to fp32.  Before a split into two fp16 parts: without it
-// the compiler may round the product behind x to fp16 at once for the high part
-// and by way of fp32 for the low part's difference, and where the two fall to
-// different sides of a step the low part no longer fits the high one (2^-11 of
-// a value, once in some thousand values).
-__device__ __forceinline__ float rounded(float x)
+// a and b as fp16 (to nearest) in *hi, and what that leaves of them in *lo: two
+// parts of 22 bits together.  *hi is held as the packed pair it is used as: left
+// to itself the compiler converts a second time for the difference, and may then
+// round the product behind a to fp16 at once on one side and by way of fp32 on
+// the other, and where those fall to different sides of a step the parts no
+// longer fit (2^-11 of a value, once in some thousand).
+__device__ __forceinline__ void split2(float a, float b, half2v *hi, half2v *lo)
 {
-    asm("" : "+v"(x));
-    return x;
+    uint32_t h = __builtin_bit_cast(uint32_t, (half2v){(_Float16)a, (_Float16)b});
+    asm("" : "+v"(h));
+    *hi = __builtin_bit_cast(half2v, h);
+    *lo = (half2v){(_Float16)fmaf((float)(*hi)[0], -1.0f, a), (_Float16)fmaf((float)(*hi)[1], -1.0f, b)};
 }
 
 // Eight values from p; vec: p is 16-byte aligned.

@@ -179,10 +179,10 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
                 const int e = row_exp(group_max<CH>(top));
                 const float up = pow2i(14 - e);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float y = rounded(x[i] * up);
-                    hi[i] = (E)y;
-                    lo[i] = fabsf((float)hi[i]) <= 65504.0f ? (E)(y - (float)hi[i]) : (E)0.0f;
+                for (int i = 0; i < 8; i += 2) {
+                    half2v a, b;
+                    split2(x[i] * up, x[i + 1] * up, &a, &b);
+                    hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
                 }
                 *(V8 *)(row + PLANE) = lo;
                 if (c == 0) A.scale[tile * 2 * AP_KEYS + w * AP_KEYS + key] = pow2i(e - 14);
@@ -269,10 +269,10 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
             for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float y = rounded(x[k][i] * up);
-                    qh[k][i] = (E)y;
-                    ql[k][i] = (E)(y - (float)qh[k][i]);
+                for (int i = 0; i < 8; i += 2) {
+                    half2v a, b;
+                    split2(x[k][i] * up, x[k][i + 1] * up, &a, &b);
+                    qh[k][i] = a[0], qh[k][i + 1] = a[1], ql[k][i] = b[0], ql[k][i + 1] = b[1];
                 }
         } else {
 #pragma unroll
@@ -388,15 +388,20 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         const float pv = NS == 2 ? pow2i(min(7 - ve, 127)) : 1.0f;
         V8 ph[PS], pl[NS == 2 ? PS : 1];
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            float p = __builtin_amdgcn_exp2f(NS == 2 ? s[i] - m : fmaf(s[i], r, -m));
-            l += p;
+        for (int i = 0; i < NV; i += 2) {
+            float p[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                p[u] = __builtin_amdgcn_exp2f(NS == 2 ? s[i + u] - m : fmaf(s[i + u], r, -m));
+                l += p[u];
+            }
             if constexpr (NS == 2) {
-                p = rounded(p * (vp[i] * pv));
-                ph[i >> 3][i & 7] = (E)p;
-                pl[i >> 3][i & 7] = (E)(p - (float)ph[i >> 3][i & 7]);
+                half2v a, b;
+                split2(p[0] * (vp[i] * pv), p[1] * (vp[i + 1] * pv), &a, &b);
+                ph[i >> 3][i & 7] = a[0], ph[i >> 3][(i & 7) + 1] = a[1];
+                pl[i >> 3][i & 7] = b[0], pl[i >> 3][(i & 7) + 1] = b[1];
             } else {
-                ph[i >> 3][i & 7] = (E)p;
+                ph[i >> 3][i & 7] = (E)p[0], ph[i >> 3][(i & 7) + 1] = (E)p[1];
             }
         }
         // ---- output

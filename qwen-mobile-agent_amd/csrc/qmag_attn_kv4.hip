@@ -212,10 +212,14 @@ template <int NS>
 __device__ __forceinline__ void split8(const float (&x)[8], half8 *hi, half8 *lo)
 {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float v = NS == 2 ? rounded(x[i]) : x[i];
-        (*hi)[i] = (_Float16)v;
-        if constexpr (NS == 2) (*lo)[i] = (_Float16)(v - (float)(*hi)[i]);
+    for (int i = 0; i < 8; i += 2) {
+        half2v h = {(_Float16)x[i], (_Float16)x[i + 1]};
+        if constexpr (NS == 2) {
+            half2v l;
+            split2(x[i], x[i + 1], &h, &l);
+            (*lo)[i] = l[0], (*lo)[i + 1] = l[1];
+        }
+        (*hi)[i] = h[0], (*hi)[i + 1] = h[1];
     }
 }
 
