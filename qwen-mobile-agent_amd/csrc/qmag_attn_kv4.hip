@@ -6,19 +6,23 @@
 //
 // The codes go to the matrix cores as fp16 whole numbers: a nibble below the
 // exponent of 1024 (or, from the upper half of a byte, of 64) is that number plus
-// the code, and one subtraction for two values leaves code - 8.  No code is
-// rounded, and no step or minimum touches the operand.  The 8 keeps the two sums
-// below small: with codes from 0 to 15 they were each tens of times the result,
-// which cost a digit (1e-5 of the result against 1e-6).
-// bf16 calls (RAW) take the nibble alone, an fp16 subnormal (code * 2^-24, or
-// * 2^-20 in the upper half of a byte, made up for exactly): five instructions for
-// eight codes instead of nine.  The matrix cores align subnormal products as if
-// their leading zeros were digits, so the sums are 10 bits short: 3e-4 of the
-// result, a fifth of what bf16's own rounding of it takes (2^-9, 1.7e-3 in the
-// mean), but more than fp16's.
-//   scores   S = K Q^T per 64 channels on codes, then d S + (m + 8 d) sum(q) in fp32;
+// the code, and one subtraction for two values leaves it.  No code is rounded,
+// and no step or minimum touches the operand.  Three ways (Code):
+//   CENTRED  fp32 calls take code - 8, which keeps the two sums below small: with
+//            codes from 0 to 15 they were each tens of times the result, which
+//            cost a digit (1e-5 of the result against 1e-6);
+//   PLAIN    16-bit calls take the code: a digit they do not hold anyway, and the
+//            value of code 8 need not be formed;
+//   RAW      bf16 decode takes the nibble alone, an fp16 subnormal (code * 2^-24,
+//            or * 2^-20 in the upper half of a byte, made up for exactly): five
+//            instructions for eight codes instead of nine.  The matrix cores align
+//            subnormal products as if their leading zeros were digits, so the sums
+//            are 10 bits short: 3e-4 of the result, a fifth of what bf16's own
+//            rounding of it takes (1.7e-3 in the mean), but more than fp16's.
+//   scores   S = K Q^T per 64 channels on codes, then d S + mid sum(q) in fp32,
+//            mid the value of the operand 0: m, or m + 8 d;
 //   output   O^T = V^T P'^T with P' = p d: the step of a token and group is
-//            folded into the softmax weight, the rest adds sum_t p (m + 8 d).
+//            folded into the softmax weight, the rest adds sum_t p mid.
 // q and P' are fp16 after an exact scaling by a power of two; fp32 calls split
 // them into two fp16 parts (22 bits), 16-bit calls take one (11 bits, no less
 // than the type itself holds).
@@ -166,46 +170,52 @@ __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t
 
 // What turns nibbles into fp16: masks and exponents in registers of both kinds,
 // so that the two go into one instruction.
+enum Code { CENTRED, PLAIN, RAW };
 struct Nibbles {
     uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, e1024 = 0x64006400u, e64 = 0x54005400u;
-    // nibbles 0 and 4 of w (of each half dword), or 1 and 5: raw, or less 8, as fp16
     __device__ __forceinline__ Nibbles()
     {
         asm("" : "+s"(lo), "+s"(hi));
         asm("" : "+v"(e1024), "+v"(e64));
     }
-    template <bool RAW>
+    // nibbles 0 and 4 of w (of each half dword), or 1 and 5, as fp16
+    template <Code CODE>
     __device__ __forceinline__ uint32_t even(uint32_t w) const
     {
-        if (RAW) return w & lo;
-        const half2v v = __builtin_bit_cast(half2v, (w & lo) | e1024) - (half2v){(_Float16)1032.0f, (_Float16)1032.0f};
+        if (CODE == RAW) return w & lo;
+        const _Float16 z = (_Float16)(CODE == CENTRED ? 1032.0f : 1024.0f);
+        const half2v v = __builtin_bit_cast(half2v, (w & lo) | e1024) - (half2v){z, z};
         return __builtin_bit_cast(uint32_t, v);
     }
-    template <bool RAW>
+    template <Code CODE>
     __device__ __forceinline__ uint32_t odd(uint32_t w) const
     {
-        if (RAW) return w & hi;
-        const half2v v = __builtin_bit_cast(half2v, (w & hi) | e64) - (half2v){(_Float16)72.0f, (_Float16)72.0f};
+        if (CODE == RAW) return w & hi;
+        const _Float16 z = (_Float16)(CODE == CENTRED ? 72.0f : 64.0f);
+        const half2v v = __builtin_bit_cast(half2v, (w & hi) | e64) - (half2v){z, z};
         return __builtin_bit_cast(uint32_t, v);
     }
 };
 
 // Eight nibbles as eight fp16 values, in the order 0 4 1 5 2 6 3 7.
-template <bool RAW>
+template <Code CODE>
 __device__ __forceinline__ half8 k_frag(const Nibbles &N, uint32_t w)
 {
     Frag f;
-    f.u[0] = N.template even<RAW>(w);
-    f.u[1] = N.template odd<RAW>(w);
-    f.u[2] = N.template even<RAW>(w >> 8);
-    f.u[3] = N.template odd<RAW>(w >> 8);
+    f.u[0] = N.template even<CODE>(w);
+    f.u[1] = N.template odd<CODE>(w);
+    f.u[2] = N.template even<CODE>(w >> 8);
+    f.u[3] = N.template odd<CODE>(w >> 8);
     return f.h;
 }
 
-// d, and m + 8 d, the value of code 8 (RAW: m, of code 0)
+// d, and the value of the operand 0
 __device__ __forceinline__ float step_of(uint32_t dm) { return h2f(dm & 0xFFFFu); }
-template <bool RAW>
-__device__ __forceinline__ float mid_of(uint32_t dm) { return RAW ? h2f(dm >> 16) : fmaf(8.0f, h2f(dm & 0xFFFFu), h2f(dm >> 16)); }
+template <Code CODE>
+__device__ __forceinline__ float mid_of(uint32_t dm)
+{
+    return CODE == CENTRED ? fmaf(8.0f, h2f(dm & 0xFFFFu), h2f(dm >> 16)) : h2f(dm >> 16);
+}
 
 // (hi, lo) fp16 parts of eight values; NS == 1: hi alone, to nearest
 template <int NS>
@@ -255,7 +265,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 {
     using S = typename T::S;
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
-    constexpr bool RAW = std::is_same_v<T, TBF16>;
+    constexpr Code CODE = NS == 2 ? CENTRED : std::is_same_v<T, TBF16> ? RAW : PLAIN;
     constexpr int NG = D / 64;
     constexpr int RG = 16, STEP = 32 * NW;
     constexpr int VD = (D + 127) / 128;            // dwords of a lane's V codes of a token
@@ -369,7 +379,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
         // the row's largest value to 2^14 .. 2^15: exact, and undone by rs
         const int e = min(max((int)(__float_as_uint(row_max(top)) >> 23) - 127, -100), 127);
         const float up = exp2i(14 - e);
-        rs = (RAW ? exp2i(min(e, 113) - 14 + 24) : exp2i(e - 14)) * A.scale;      // (beyond 2^113 weights are 0 or 1 in any case)
+        rs = (CODE == RAW ? exp2i(min(e, 113) - 14 + 24) : exp2i(e - 14)) * A.scale;      // (beyond 2^113 weights are 0 or 1 in any case)
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             float sum = 0.0f;
@@ -380,11 +390,11 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
                 for (int i = 0; i < 8; i++) {
                     x[g][s][i] *= up;
                     sum += x[g][s][i];
-                    f[2 * (i & 3) + (i >> 2)] = x[g][s][i] * (RAW && (i & 1) ? 0.0625f : 1.0f);     // nibble i's place in a fragment
+                    f[2 * (i & 3) + (i >> 2)] = x[g][s][i] * (CODE == RAW && (i & 1) ? 0.0625f : 1.0f);     // nibble i's place in a fragment
                 }
                 split8<NS>(f, &qh[g][s], &ql[NS == 2 ? g : 0][s]);
             }
-            qs[g] = row_sum(sum) * (RAW ? 0x1p-24f : 1.0f);
+            qs[g] = row_sum(sum) * (CODE == RAW ? 0x1p-24f : 1.0f);
         }
     }
 
@@ -429,13 +439,13 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
                 f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int st = 0; st < 2; st++) {
-                    const half8 kf = k_frag<RAW>(N, kc[2 * g + st]);
+                    const half8 kf = k_frag<CODE>(N, kc[2 * g + st]);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[g][st], acc, 0, 0, 0);
                     if constexpr (NS == 2) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[g][st], acc, 0, 0, 0);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float d = step_of(dm[r][g]), mid = mid_of<RAW>(dm[r][g]);
+                    const float d = step_of(dm[r][g]), mid = mid_of<CODE>(dm[r][g]);
                     s[4 * a + r] = fmaf(d, acc[r], fmaf(mid, qs[g], s[4 * a + r]));
                 }
             }
@@ -514,7 +524,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = p[i] * pf * step_of(vdm[i][g]);
-                vs[g] = fmaf(p[i], mid_of<RAW>(vdm[i][g]), vs[g]);
+                vs[g] = fmaf(p[i], mid_of<CODE>(vdm[i][g]), vs[g]);
             }
             half8 ph, pl;
             split8<NS>(x, &ph, &pl);
@@ -527,8 +537,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
                     const int at = 2 * (g & 1) + b;
                     const uint32_t w = __builtin_amdgcn_perm(vc[2 * k + 1][g >> 1], vc[2 * k][g >> 1],
                                                              0x0C040C00u + 0x00010001u * (uint32_t)at);
-                    even.u[k] = N.template even<RAW>(w);
-                    odd.u[k] = N.template odd<RAW>(w);
+                    even.u[k] = N.template even<CODE>(w);
+                    odd.u[k] = N.template odd<CODE>(w);
                 }
                 o[g][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even.h, ph, o[g][2 * b], 0, 0, 0);
                 o[g][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd.h, ph, o[g][2 * b + 1], 0, 0, 0);
@@ -542,7 +552,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 
     // ---- the waves' shares; a lane's row: channels 64 g + 4 (4 h + r) + i in o[g][i][r]
     l = row_sum(l);
-    const float back = exp2i(max(ve, 0) - 21) * (RAW ? 0x1p24f : 1.0f), back1 = back * (RAW ? 0.0625f : 1.0f);
+    const float back = exp2i(max(ve, 0) - 21) * (CODE == RAW ? 0x1p24f : 1.0f), back1 = back * (CODE == RAW ? 0.0625f : 1.0f);
     if (h == 0) {
         join_m[wave][n] = m;
         join_l[wave][n] = l;
@@ -609,12 +619,16 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 // fp16 codes once for all the waves (K and V row by row, in the order the
 // products read them), and then serves as a tile of a prompt does; memory is two
 // tiles ahead, the codes one, and a tile costs one barrier.
+// how many of its workgroups of 8 waves the registers let a CU hold
+template <class T, int D>
+constexpr int rows_resident() { return D == 256 || (D == 128 && sizeof(typename T::S) == 4) ? 1 : 2; }
+
 template <class T, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) attn_kv4_rows_kernel(AkArgs A)
+__global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4_rows_kernel(AkArgs A)
 {
     using S = typename T::S;
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
-    constexpr bool RAW = false;                    // the codes are formed once: no need to save there
+    constexpr Code CODE = NS == 2 ? CENTRED : PLAIN;
     constexpr int NG = D / 64;
     constexpr int RG = 16 * NW, STEP = 32;
     constexpr int TILE = ak_tile<D>(), IMG = 32 * D, SC = 4 * D;   // bytes, values, bytes
@@ -686,7 +700,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_kv4_rows_kernel(AkArgs A)
                 for (int i = 0; i < 4; i++) {
                     const int hh = (d0 + i) / (D / 32), gs = (d0 + i) % (D / 32);
                     *(half8 *)(ik[b] + t * D + 8 * (D == 64 ? (4 * gs + hh) ^ ((t >> 1) & 7) : (4 * gs + hh) ^ (t & 15))) =
-                        k_frag<RAW>(N, u[i]);
+                        k_frag<CODE>(N, u[i]);
                 }
             } else if (p < 2 * D) {                // V: 16-bit word i * NG + g of a row, four channels
                 const int t = (p - D) / (D / 32), w0 = 8 * ((p - D) % (D / 32));
@@ -695,8 +709,8 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_kv4_rows_kernel(AkArgs A)
                     const uint32_t c = i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xFFFFu;
                     const int ii = (w0 + i) / NG, g = (w0 + i) % NG, ch = 8 * g + (ii >> 1);
                     union { uint32_t u[2]; s16x4 v; } y;
-                    y.u[0] = N.template even<RAW>(c | (c << 12));
-                    y.u[1] = N.template even<RAW>((c >> 8) | (c << 4));
+                    y.u[0] = N.template even<CODE>(c | (c << 12));
+                    y.u[1] = N.template even<CODE>((c >> 8) | (c << 4));
                     *(s16x4 *)(iv[b] + t * D + 8 * (D == 64 ? ch ^ (t & 6) : ch ^ ((t & 7) << 1)) + 4 * (ii & 1)) = y.v;
                 }
             } else {
@@ -786,7 +800,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_kv4_rows_kernel(AkArgs A)
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float d = step_of(dm[r][g]), mid = mid_of<RAW>(dm[r][g]);
+                    const float d = step_of(dm[r][g]), mid = mid_of<CODE>(dm[r][g]);
                     s[4 * a + r] = fmaf(d, acc[r], fmaf(mid, qs[g], s[4 * a + r]));
                 }
             }
@@ -858,7 +872,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_kv4_rows_kernel(AkArgs A)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = p[i] * pf * step_of(vdm[i][g]);
-                vs[g] = fmaf(p[i], mid_of<RAW>(vdm[i][g]), vs[g]);
+                vs[g] = fmaf(p[i], mid_of<CODE>(vdm[i][g]), vs[g]);
             }
             half8 ph, pl;
             split8<NS>(x, &ph, &pl);
@@ -916,73 +930,82 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_kv4_rows_kernel(AkArgs A)
     }
 }
 
-// Joins the partial results of the rows whose sequence was split: a workgroup of
-// NW waves for a head of a token and CW of its channels, the waves the parts in
-// turn.  Few rows: many waves to few channels, so that a wave's parts are all
-// requested at once.
+// Joins the partial results of the rows whose sequence was split: NW waves for CW
+// channels of a row, the waves the parts in turn.  Decode of a few rows has many
+// parts to a row (16 waves for 64 channels: a wave's parts are all requested at
+// once), of more rows fewer (four waves a row), many rows to a sequence a handful
+// (a wave for a row, four heads of a token to a workgroup).
 template <class T, int D, int RG, int STEP, int NW, int CW>
-__global__ void __launch_bounds__(64 * NW) attn_kv4_join_kernel(AkArgs A)
+__global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(AkArgs A)
 {
     using S = typename T::S;
-    constexpr int C = CW / 64;                      // channels of a lane
+    constexpr int C = CW / 64;                      // consecutive channels of a lane
+    constexpr int U = NW == 1 ? 4 : 8;              // parts requested at once
     __shared__ float sum[NW][CW], sl[NW];
-    const int t = blockIdx.x, head = blockIdx.y, kvh = head / A.G, gh = head - kvh * A.G, c0 = blockIdx.z * CW;
-    const int wave = threadIdx.x >> 6, lane = lane_id();
+    const int wave = NW == 1 ? 0 : threadIdx.x >> 6, lane = lane_id();
+    const int t = blockIdx.x, head = NW == 1 ? 4 * blockIdx.y + (threadIdx.x >> 6) : blockIdx.y;
+    const int kvh = head / A.G, gh = head - kvh * A.G, c0 = CW * blockIdx.z + C * lane;
     AkPlan P;
-    if (!ak_find<RG, STEP>(A, t, true, &P) || P.n_split == 1) return;
+    if (head >= A.n_kv * A.G || !ak_find<RG, STEP>(A, t, true, &P) || P.n_split == 1) return;
     const int row = (t - P.q0) * A.G + gh;
     const int64_t first = ak_part(A, P, kvh, row / RG, RG, row % RG);
     float M = -INFINITY;
     for (int i = lane; i < P.n_split; i += 64) M = fmaxf(M, A.ml[2 * (first + i)]);
     M = group_max<64>(M);
+    struct alignas(4 * C) Vec { float v[C]; };
     float acc[C], L = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; c++) acc[c] = 0.0f;
-    constexpr int U = 8;                            // parts requested at once
     for (int i0 = wave; i0 < P.n_split; i0 += U * NW) {
-        float mi[U], li[U], v[U][C];
+        float2 ml[U];
+        Vec v[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t at = first + min(i0 + u * NW, P.n_split - 1);
-            const float2 x = *(const float2 *)(A.ml + 2 * at);
-            mi[u] = x.x, li[u] = x.y;
-#pragma unroll
-            for (int c = 0; c < C; c++) v[u][c] = A.part[at * D + c0 + 64 * c + lane];
+            ml[u] = *(const float2 *)(A.ml + 2 * at);
+            v[u] = *(const Vec *)(A.part + at * D + c0);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            const float mi = ml[u].x, li = ml[u].y;
             const bool in = i0 + u * NW < P.n_split;
-            const float f = !in ? 0.0f : mi[u] == -INFINITY ? (li[u] != 0.0f ? li[u] : 0.0f) : __builtin_amdgcn_exp2f(mi[u] - M);
-            if (in) L += mi[u] == -INFINITY ? f : f * li[u];
+            const float f = !in ? 0.0f : mi == -INFINITY ? (li != 0.0f ? li : 0.0f) : __builtin_amdgcn_exp2f(mi - M);
+            if (in) L += mi == -INFINITY ? f : f * li;
             // a part without a token seen: nothing was summed there
 #pragma unroll
-            for (int c = 0; c < C; c++) acc[c] += f == 0.0f ? 0.0f : f * v[u][c];
+            for (int c = 0; c < C; c++) acc[c] += f == 0.0f ? 0.0f : f * v[u].v[c];
         }
     }
-#pragma unroll
-    for (int c = 0; c < C; c++) sum[wave][64 * c + lane] = acc[c];
-    if (lane == 0) sl[wave] = L;
-    __syncthreads();
-    L = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; w++) L += sl[w];
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     S *op = (S *)A.out + t * A.ot + head * A.oh + c0;
-    for (int c = threadIdx.x; c < CW; c += 64 * NW) {
-        float v = 0.0f;
+    if constexpr (NW > 1) {
 #pragma unroll
-        for (int w = 0; w < NW; w++) v += sum[w][c];
-        op[c] = T::down(v * inv);
+        for (int c = 0; c < C; c++) sum[wave][C * lane + c] = acc[c];
+        if (lane == 0) sl[wave] = L;
+        __syncthreads();
+        if (wave) return;
+        L = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; c++) acc[c] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            L += sl[w];
+#pragma unroll
+            for (int c = 0; c < C; c++) acc[c] += sum[w][C * lane + c];
+        }
     }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int c = 0; c < C; c++) op[c] = T::down(acc[c] * inv);
 }
 
 template <class T, int D, bool ROWS>
 static int ak_launch(AkArgs A, hipStream_t s)
 {
     constexpr int NW = ROWS ? 8 : 4, RG = ROWS ? 16 * NW : 16, STEP = ROWS ? 32 : 32 * NW;
-    // Row groups at most; with so many workgroups to a CU in mind chunks are cut.
+    // Row groups at most.  Chunks are cut for as many workgroups as the chip holds at
+    // once: of more the last ones run alone, of fewer some CUs get two and others none.
     const int64_t groups = (int64_t)A.T * A.G / RG + A.n_seq;
-    const int64_t goal = (ROWS ? 1 : 4) * (int64_t)ctx().n_cu;
+    const int64_t goal = (ROWS ? rows_resident<T, D>() : 4) * (int64_t)ctx().n_cu;
     A.target = (int)((goal + A.n_kv - 1) / A.n_kv);
     // enough row groups to fill the chip twice over: nothing is split
     A.min_chunk = ((int64_t)A.T * A.G / RG) * A.n_kv >= 2 * goal ? 0 : 128;
@@ -1000,11 +1023,13 @@ static int ak_launch(AkArgs A, hipStream_t s)
     if constexpr (ROWS) attn_kv4_rows_kernel<T, D, NW><<<grid, 64 * NW, 0, s>>>(A);
     else attn_kv4_kernel<T, D, 2, NW><<<grid, 64 * NW, 0, s>>>(A);
     if (A.min_chunk) {
-        const unsigned heads = (unsigned)(A.n_kv * A.G);
-        if ((int64_t)A.T * heads * (D / 64) <= ctx().n_cu)
-            attn_kv4_join_kernel<T, D, RG, STEP, 16, 64><<<dim3((unsigned)A.T, heads, D / 64), 1024, 0, s>>>(A);
+        const unsigned T_ = (unsigned)A.T, heads = (unsigned)(A.n_kv * A.G);
+        if constexpr (ROWS)
+            attn_kv4_join_kernel<T, D, RG, STEP, 1, D><<<dim3(T_, (heads + 3) / 4), 256, 0, s>>>(A);
+        else if ((int64_t)A.T * heads * (D / 64) <= ctx().n_cu)
+            attn_kv4_join_kernel<T, D, RG, STEP, 16, 64><<<dim3(T_, heads, D / 64), 1024, 0, s>>>(A);
         else
-            attn_kv4_join_kernel<T, D, RG, STEP, 4, D><<<dim3((unsigned)A.T, heads), 256, 0, s>>>(A);
+            attn_kv4_join_kernel<T, D, RG, STEP, 4, D><<<dim3(T_, heads), 256, 0, s>>>(A);
     }
     return QMAG_OK;
 }
