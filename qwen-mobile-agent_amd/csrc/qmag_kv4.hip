@@ -6,9 +6,11 @@
 // them.  m and d saturate at fp16's largest value; a group that holds an
 // infinity or a NaN stands for NaN throughout (d NaN).
 //
-// A thread takes 8 values of one head of one token; a group is 8 threads, its
-// minimum and maximum three lane exchanges.  Memory bound: each value is read
-// once, each code written once.
+// Append: a thread takes 8 values of one head of one token; a group is 8 threads,
+// its minimum and maximum three lane exchanges.  Read: a thread takes 4 values, so
+// that a wave writes 1 KB in one piece.  A workgroup stays with one head of K or V
+// (a division by the number of heads in every thread, and stores of every other 16
+// bytes, had cost more than the memory).
 #include "qmag_attn.h"
 
 namespace qmag {
@@ -42,14 +44,9 @@ __global__ void __launch_bounds__(KV4_WG) kv4_append_kernel(Kv4Args c, qmag_head
     constexpr int PER = D / 8;                       // threads of a head
     constexpr int ROWS = KV4_WG / PER;
     const int e = threadIdx.x % PER, g = e >> 3;
-    const int64_t rows = (int64_t)n_tok * c.n_kv * 2;
-    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < rows; r0 += (int64_t)gridDim.x * ROWS) {
-        // rows: K of every head of a token, then V
-        const int64_t row = r0 + threadIdx.x / PER;
-        if (row >= rows) continue;                   // whole groups of lanes leave together
-        const int64_t t = row / (2 * c.n_kv);
-        const int w = (int)(row - t * 2 * c.n_kv), is_v = w >= c.n_kv, head = is_v ? w - c.n_kv : w;
-        const int sl = slot[t];
+    const int is_v = (int)blockIdx.y >= c.n_kv, head = is_v ? (int)blockIdx.y - c.n_kv : (int)blockIdx.y;
+    for (int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / PER; t < n_tok; t += (int64_t)gridDim.x * ROWS) {
+        const int sl = slot[t];                      // whole groups of lanes go on together
         if (sl < 0 || sl >= c.n_slot) continue;
         const qmag_heads &H = is_v ? V : K;
         float x[8];
@@ -79,11 +76,15 @@ __global__ void __launch_bounds__(KV4_WG) kv4_append_kernel(Kv4Args c, qmag_head
         const int off = sl & ((1 << c.shift) - 1);
         uint8_t *base = c.data + (blk * c.n_kv + head) * 2 * c.half + (is_v ? c.half : 0);
         uint8_t *codes = base + off * (D / 2);
-        if (is_v) {
-            *(uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7))) = (uint16_t)dword;
-            *(uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7) + 1)) = (uint16_t)(dword >> 16);
-        } else {
+        if (!is_v) {
             *(uint32_t *)(codes + k_dword_at<D>(e)) = dword;
+        } else if constexpr (D == 64) {
+            *(uint32_t *)(codes + v_short_at<D>(0, 2 * e)) = dword;
+        } else {
+            // two groups' words of a place lie side by side: one of the two from the thread 8 on
+            const uint32_t o = (uint32_t)__shfl_xor((int)dword, 8);
+            const uint32_t both = g & 1 ? (o >> 16) | (dword & 0xFFFF0000u) : (dword & 0xFFFFu) | (o << 16);
+            *(uint32_t *)(codes + v_short_at<D>(g & ~1, 2 * (e & 7) + (g & 1))) = both;
         }
         if ((e & 7) == 0) {
             const uint32_t dm = group_ok ? (uint32_t)__builtin_bit_cast(uint16_t, d) |
@@ -97,35 +98,26 @@ __global__ void __launch_bounds__(KV4_WG) kv4_append_kernel(Kv4Args c, qmag_head
 template <int D>
 __global__ void __launch_bounds__(KV4_WG) kv4_read_kernel(Kv4Args c, const int *slot, int n_tok, float *ko, float *vo, bool vec)
 {
-    constexpr int PER = D / 8;
+    constexpr int PER = D / 4;                       // threads of a head
     constexpr int ROWS = KV4_WG / PER;
-    const int e = threadIdx.x % PER, g = e >> 3;
-    const int64_t rows = (int64_t)n_tok * c.n_kv * 2;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / PER; row < rows; row += (int64_t)gridDim.x * ROWS) {
-        const int64_t t = row / (2 * c.n_kv);
-        const int w = (int)(row - t * 2 * c.n_kv), is_v = w >= c.n_kv, head = is_v ? w - c.n_kv : w;
+    const int e = threadIdx.x % PER, g = e >> 4;
+    const int is_v = (int)blockIdx.y >= c.n_kv, head = is_v ? (int)blockIdx.y - c.n_kv : (int)blockIdx.y;
+    const int word_at = is_v ? v_short_at<D>(g, e & 15) : k_dword_at<D>(e >> 1) + 2 * (e & 1);
+    float *out = (is_v ? vo : ko) + head * D + 4 * e;
+    for (int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / PER; t < n_tok; t += (int64_t)gridDim.x * ROWS) {
         const int sl = slot[t];
-        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (sl >= 0 && sl < c.n_slot) {
             const int64_t blk = sl >> c.shift;
             const int off = sl & ((1 << c.shift) - 1);
             const uint8_t *base = c.data + (blk * c.n_kv + head) * 2 * c.half + (is_v ? c.half : 0);
-            const uint8_t *codes = base + off * (D / 2);
-            uint32_t dword;
-            if (is_v)
-                dword = *(const uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7))) |
-                        ((uint32_t)*(const uint16_t *)(codes + v_short_at<D>(g, 2 * (e & 7) + 1)) << 16);
-            else
-                dword = *(const uint32_t *)(codes + k_dword_at<D>(e));
+            const uint32_t w = *(const uint16_t *)(base + off * (D / 2) + word_at);
             const uint32_t dm = *(const uint32_t *)(base + ((int64_t)(D / 2) << c.shift) + (off * (D / KV4_GROUP) + g) * 4);
             const float d = h2f(dm & 0xFFFFu), m = h2f(dm >> 16);
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = fmaf(d, (float)((dword >> (4 * i)) & 15u), m);
+            for (int i = 0; i < 4; i++) y[i] = fmaf(d, (float)((w >> (4 * i)) & 15u), m);
         }
-        float *o = (is_v ? vo : ko) + (t * c.n_kv + head) * D + 8 * e;
-        const float a[4] = {y[0], y[1], y[2], y[3]}, b[4] = {y[4], y[5], y[6], y[7]};
-        store4<TF32>(o, vec, a);
-        store4<TF32>(o + 4, vec, b);
+        store4<TF32>(out + t * (c.n_kv * D), vec, y);
     }
 }
 
@@ -144,11 +136,11 @@ static int with_dim(int dim, F f)
     return f(std::integral_constant<int, 256>{});
 }
 
-// workgroups for `rows` heads of `dim` values, at most 16 for each CU
-static unsigned kv4_grid(int64_t rows, int dim)
+// workgroups for T tokens of every head of K and V, `per` tokens each at a time
+static dim3 kv4_grid(int T, int n_kv, int per)
 {
-    const int64_t per = KV4_WG / (dim / 8), wgs = (rows + per - 1) / per;
-    return (unsigned)(wgs < 4096 ? wgs : 4096);
+    const int64_t x = ((int64_t)T + per - 1) / per, most = 8192 / (2 * n_kv) + 1;
+    return dim3((unsigned)(x < most ? x : most), (unsigned)(2 * n_kv));
 }
 
 }  // namespace qmag
@@ -184,7 +176,7 @@ extern "C" int qmag_kv4_append_dev(const qmag_kv4 *c, int type, const qmag_heads
     DeviceScope dev;
     if (dev.st) return dev.st;
     hipStream_t s = ctx().stream;
-    const unsigned grid = kv4_grid((int64_t)T * c->n_kv * 2, c->head_dim);
+    const dim3 grid = kv4_grid(T, c->n_kv, KV4_WG / (c->head_dim / 8));
     prof_begin(PROF_KV, s);
     with_type(type, [&](auto t) {
         return with_dim(c->head_dim, [&](auto d) {
@@ -209,7 +201,7 @@ extern "C" int qmag_kv4_read_dev(const qmag_kv4 *c, const int *slot, int T, floa
     DeviceScope dev;
     if (dev.st) return dev.st;
     hipStream_t s = ctx().stream;
-    const unsigned grid = kv4_grid((int64_t)T * c->n_kv * 2, c->head_dim);
+    const dim3 grid = kv4_grid(T, c->n_kv, KV4_WG / (c->head_dim / 4));
     prof_begin(PROF_KV, s);
     with_dim(c->head_dim, [&](auto d) {
         kv4_read_kernel<decltype(d)::value><<<grid, KV4_WG, 0, s>>>(kv4_args(c), slot, T, k, v, vec);
