@@ -61,16 +61,20 @@ __device__ __forceinline__ void split2(float a, float b, half2v *hi, half2v *lo)
     *lo = (half2v){(_Float16)fmaf((float)(*hi)[0], -1.0f, a), (_Float16)fmaf((float)(*hi)[1], -1.0f, b)};
 }
 
-// Eight values from p; vec: p is 16-byte aligned.
-template <class T>
+// Eight values from p; vec: p is 16-byte aligned; ONCE: they are not kept in the
+// caches for others.
+template <class T, bool ONCE = false>
 __device__ __forceinline__ void load8(const typename T::S *p, bool vec, float (&o)[8])
 {
     constexpr int N = 16 / (int)sizeof(typename T::S);
-    struct alignas(16) Vec { typename T::S v[N]; };
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    union Vec { u32x4 u; typename T::S v[N]; };
     if (vec) {
 #pragma unroll
         for (int a = 0; a < 8; a += N) {
-            const Vec x = *reinterpret_cast<const Vec *>(p + a);
+            Vec x;
+            if constexpr (ONCE) x.u = __builtin_nontemporal_load((const u32x4 *)(p + a));
+            else x.u = *(const u32x4 *)(p + a);
 #pragma unroll
             for (int i = 0; i < N; i++) o[a + i] = T::up(x.v[i]);
         }

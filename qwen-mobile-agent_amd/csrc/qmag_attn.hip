@@ -155,46 +155,53 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
     const int kvh = blockIdx.y;
     const int64_t tile = (int64_t)kvh * A.tiles + a / AP_KEYS + seq + part;
     E *img = (E *)A.img + tile * 2 * NS * PLANE;
-    const int c = threadIdx.x % CH;
+    const int c = threadIdx.x % CH, w = blockIdx.z;                  // K's image, or V's
+    const S *base = (const S *)(w ? A.v : A.k) + kvh * (w ? A.vh : A.kh) + 8 * c;
+    const int64_t stride = w ? A.vt : A.kt;
+    constexpr int N = AP_KEYS / ROWS;
+    float x[N][8];
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        const int t = part * AP_KEYS + u * ROWS + (int)threadIdx.x / CH;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[u][i] = 0.0f;
+        if (t < n) load8<T, true>(base + (int64_t)(a + t) * stride, w ? A.v_vec : A.k_vec, x[u]);
+    }
     int odd = 0;
 #pragma unroll
-    for (int w = 0; w < 2; w++) {
-        const S *base = (const S *)(w ? A.v : A.k) + kvh * (w ? A.vh : A.kh);
-        const int64_t stride = w ? A.vt : A.kt;
-        for (int key = threadIdx.x / CH; key < AP_KEYS; key += ROWS) {
-            const int t = part * AP_KEYS + key;
-            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            if (t < n) load8<T>(base + (int64_t)(a + t) * stride + 8 * c, w ? A.v_vec : A.k_vec, x);
-            float top = 0.0f;
+    for (int u = 0; u < N; u++) {
+        const int key = u * ROWS + (int)threadIdx.x / CH;
+        float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const bool fine = fabsf(x[i]) <= 3.402823466e38f;
-                top = fmaxf(top, fine ? fabsf(x[i]) : 0.0f);
-                // V's infinities and NaN are added where they are seen, not multiplied
-                if (w && !fine) odd = 1, x[i] = 0.0f;
-            }
-            E *row = img + w * NS * PLANE + key * D + 8 * (w ? v_chunk<D, QW>(key, c) : k_chunk<D>(key, c));
-            V8 hi, lo;
-            if constexpr (NS == 2) {
-                const int e = row_exp(group_max<CH>(top));
-                const float up = pow2i(14 - e);
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    half2v a, b;
-                    split2(x[i] * up, x[i + 1] * up, &a, &b);
-                    hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
-                }
-                *(V8 *)(row + PLANE) = lo;
-                if (c == 0) A.scale[tile * 2 * AP_KEYS + w * AP_KEYS + key] = pow2i(e - 14);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) hi[i] = (E)x[i];
-            }
-            *(V8 *)row = hi;
+        for (int i = 0; i < 8; i++) {
+            const bool fine = fabsf(x[u][i]) <= 3.402823466e38f;
+            top = fmaxf(top, fine ? fabsf(x[u][i]) : 0.0f);
+            // V's infinities and NaN are added where they are seen, not multiplied
+            if (w && !fine) odd = 1, x[u][i] = 0.0f;
         }
+        E *row = img + w * NS * PLANE + key * D + 8 * (w ? v_chunk<D, QW>(key, c) : k_chunk<D>(key, c));
+        V8 hi, lo;
+        if constexpr (NS == 2) {
+            const int e = row_exp(group_max<CH>(top));
+            const float up = pow2i(14 - e);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                half2v p, q;
+                split2(x[u][i] * up, x[u][i + 1] * up, &p, &q);
+                hi[i] = p[0], hi[i + 1] = p[1], lo[i] = q[0], lo[i + 1] = q[1];
+            }
+            *(V8 *)(row + PLANE) = lo;
+            if (c == 0) A.scale[tile * 2 * AP_KEYS + w * AP_KEYS + key] = pow2i(e - 14);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) hi[i] = (E)x[u][i];
+        }
+        *(V8 *)row = hi;
     }
-    odd = __syncthreads_or(odd);
-    if (threadIdx.x == 0) A.odd[tile] = odd;
+    if (w) {
+        odd = __syncthreads_or(odd);
+        if (threadIdx.x == 0) A.odd[tile] = odd;
+    }
 }
 
 // ------------------------------------------------------------- attention ----
@@ -497,7 +504,7 @@ static int ap_run(ApArgs A, hipStream_t s)
     A.img = ws;
     A.scale = (float *)(ws + n * TILE);
     A.odd = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
-    prompt_tiles_kernel<T, D, QW><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv), AP_WG, 0, s>>>(A);
+    prompt_tiles_kernel<T, D, QW><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv, 2), AP_WG, 0, s>>>(A);
     attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
     return QMAG_OK;
 }
