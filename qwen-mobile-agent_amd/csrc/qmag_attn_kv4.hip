@@ -941,7 +941,7 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(
     using S = typename T::S;
     constexpr int C = CW / 64;                      // consecutive channels of a lane
     constexpr int U = NW == 1 ? 4 : 8;              // parts requested at once
-    __shared__ float sum[NW][CW], sl[NW];
+    __shared__ float sum[NW][CW], sl[NW], sm[NW];
     const int wave = NW == 1 ? 0 : threadIdx.x >> 6, lane = lane_id();
     const int t = blockIdx.x, head = NW == 1 ? 4 * blockIdx.y + (threadIdx.x >> 6) : blockIdx.y;
     const int kvh = head / A.G, gh = head - kvh * A.G, c0 = CW * blockIdx.z + C * lane;
@@ -949,13 +949,11 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(
     if (head >= A.n_kv * A.G || !ak_find<RG, STEP>(A, t, true, &P) || P.n_split == 1) return;
     const int row = (t - P.q0) * A.G + gh;
     const int64_t first = ak_part(A, P, kvh, row / RG, RG, row % RG);
-    float M = -INFINITY;
-    for (int i = lane; i < P.n_split; i += 64) M = fmaxf(M, A.ml[2 * (first + i)]);
-    M = group_max<64>(M);
     struct alignas(4 * C) Vec { float v[C]; };
-    float acc[C], L = 0.0f;
+    float acc[C], L = 0.0f, M = -INFINITY;
 #pragma unroll
     for (int c = 0; c < C; c++) acc[c] = 0.0f;
+    // (a part that saw no token has nothing but zeros; one with a NaN weight -inf and a NaN sum)
     for (int i0 = wave; i0 < P.n_split; i0 += U * NW) {
         float2 ml[U];
         Vec v[U];
@@ -965,13 +963,20 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(
             ml[u] = *(const float2 *)(A.ml + 2 * at);
             v[u] = *(const Vec *)(A.part + at * D + c0);
         }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; u++) top = fmaxf(top, ml[u].x);
+        const float old = M == -INFINITY ? (L == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(M - top);
+        M = top;
+        L *= old;
+#pragma unroll
+        for (int c = 0; c < C; c++) acc[c] *= old;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const float mi = ml[u].x, li = ml[u].y;
             const bool in = i0 + u * NW < P.n_split;
-            const float f = !in ? 0.0f : mi == -INFINITY ? (li != 0.0f ? li : 0.0f) : __builtin_amdgcn_exp2f(mi - M);
-            if (in) L += mi == -INFINITY ? f : f * li;
-            // a part without a token seen: nothing was summed there
+            const float f = !in ? 0.0f : mi == -INFINITY ? (li != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(mi - M);
+            L += f == 0.0f ? 0.0f : f * li;
 #pragma unroll
             for (int c = 0; c < C; c++) acc[c] += f == 0.0f ? 0.0f : f * v[u].v[c];
         }
@@ -980,17 +985,20 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(
     if constexpr (NW > 1) {
 #pragma unroll
         for (int c = 0; c < C; c++) sum[wave][C * lane + c] = acc[c];
-        if (lane == 0) sl[wave] = L;
+        if (lane == 0) sl[wave] = L, sm[wave] = M;
         __syncthreads();
         if (wave) return;
+#pragma unroll
+        for (int w = 0; w < NW; w++) M = fmaxf(M, sm[w]);
         L = 0.0f;
 #pragma unroll
         for (int c = 0; c < C; c++) acc[c] = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            L += sl[w];
+            const float f = sm[w] == -INFINITY ? (sl[w] != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(sm[w] - M);
+            L += f * sl[w];
 #pragma unroll
-            for (int c = 0; c < C; c++) acc[c] += sum[w][C * lane + c];
+            for (int c = 0; c < C; c++) acc[c] += f * sum[w][C * lane + c];
         }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
