@@ -546,8 +546,9 @@ typedef struct qmag_kv_table {
 
 /* Blocks of ended sequences go back: for each i with ended[i] != 0, in
    ascending order, table[i]'s ceil(len[i] / block_size) blocks are appended to
-   the free list and len_next[i] = 0; other lengths are copied.  len_next and
-   n_free_next are places of their own (a step may then be issued again).  With
+   the free list and len_next[i] = 0; other lengths are copied.  What is written
+   (len_next, n_free_next, status) overlaps neither the inputs nor itself (a step
+   may then be issued again).  With
    a status other than 0 nothing is given back, len_next = len and
    *n_free_next = *n_free. */
 int qmag_kv_release_dev(const qmag_kv_table *t, const int *len, const int *ended, const int *n_free, int *len_next,
@@ -560,19 +561,21 @@ int qmag_kv_release_dev(const qmag_kv_table *t, const int *len, const int *ended
    goes to slot[t] = block * block_size + place in the block.  slot and pos have T
    entries; those behind the last token get slot -1 and pos 0.  len_next[i] =
    len[i] + n_new[i].  With a status other than 0 no block is taken, every slot
-   is -1, cu is 0, and len_next and *n_free_next are as before. */
+   is -1, cu is 0, and len_next = len, *n_free_next = *n_free.  What is written
+   overlaps neither the inputs nor itself. */
 int qmag_kv_assign_dev(const qmag_kv_table *t, const int *len, const int *n_new, const int *n_free, int T, int *slot,
                        int *pos, int *cu, int *len_next, int *n_free_next, int *status);
 
 /* A cache held in 4 bits.  A block holds for each kv head [K codes | K scales |
    V codes | V scales] of its block_size tokens: per token head_dim / 2 bytes of
    codes and per 64 values a step d and a minimum m in fp16 (d first); a value is
-   d * code + m.  m = fp16(min), d = fp16((max - min) / 15), code = (x - m) / d to
-   the nearest even whole number within 0..15, each step in fp32 as written; m
-   and d saturate, and 64 values with an infinity or a NaN among them are all
-   NaN.  Codes of a token's K row: dword h * head_dim / 32 + 2 g + s holds channels
-   64 g + 32 s + 8 h .. + 7, lowest bits first; of its V row: 16-bit word
-   i * head_dim / 64 + g holds channels 64 g + 4 i .. + 3. */
+   d * code + m.  m = fp16(min), d = fp16((max - min) * (1 / 15)), code =
+   (x - m) / d to the nearest whole number within 0..15 (ties to even), each step
+   in fp32 as written and 1 / 15 the fp32 number; m and d saturate, and 64 values
+   with an infinity or a NaN among them are all NaN.  Codes of a token's K row:
+   dword h * head_dim / 32 + 2 g + s holds channels 64 g + 32 s + 8 h .. + 7,
+   lowest bits first; of its V row: 16-bit word i * head_dim / 64 + g holds
+   channels 64 g + 4 i .. + 3. */
 typedef struct qmag_kv4 {
     void *data;         /* n_block * qmag_kv4_block_bytes, 16-byte aligned */
     int n_block;

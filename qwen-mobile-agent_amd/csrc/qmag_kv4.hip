@@ -1,9 +1,12 @@
 // qmag_kv4.hip -- tokens' K and V into the 4-bit cache, and the values it holds.
 //
 // 64 consecutive values of a head share a minimum m and a step d, both fp16:
-//   m = fp16(min), d = fp16((max - min) / 15), code = clamp(rne((x - m) / d), 0, 15),
-// every step in fp32 as written, so that the codes do not depend on who forms
-// them.  m and d saturate at fp16's largest value; a group that holds an
+//   m = fp16(min), d = fp16((max - min) * (1 / 15)), code = clamp(rne((x - m) / d), 0, 15),
+// every step in fp32 as written, 1 / 15 itself rounded to fp32, so that the codes
+// do not depend on who forms them.  (The product, not the quotient, is what a
+// tensor library on this device forms for a division by a constant: for 16-bit
+// values the quotient is now and then half way between two fp16 steps, where the
+// two part.)  m and d saturate at fp16's largest value; a group that holds an
 // infinity or a NaN stands for NaN throughout (d NaN).
 //
 // Append: a thread takes 8 values of one head of one token; a group is 8 threads,
@@ -65,7 +68,7 @@ __global__ void __launch_bounds__(KV4_WG) kv4_append_kernel(Kv4Args c, qmag_head
         hi = group_max<8>(hi);
         const bool group_ok = group_min<8>(ok ? 1.0f : 0.0f) > 0.0f;
         const _Float16 m = (_Float16)fminf(fmaxf(lo, -65504.0f), 65504.0f);
-        const _Float16 d = (_Float16)fminf((hi - lo) / 15.0f, 65504.0f);
+        const _Float16 d = (_Float16)fminf((hi - lo) * (1.0f / 15.0f), 65504.0f);
         const float mf = (float)m, df = (float)d;
         uint32_t code[8];
 #pragma unroll

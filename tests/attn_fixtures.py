@@ -124,7 +124,7 @@ def quantise(x):
     g = x.reshape(*x.shape[:-1], x.shape[-1] // 64, 64)
     with np.errstate(all="ignore"):
         lo, hi = g.min(-1), g.max(-1)
-        d = np.minimum((hi - lo) / np.float32(15), np.float32(65504)).astype(np.float16)
+        d = np.minimum((hi - lo) * np.float32(1 / 15), np.float32(65504)).astype(np.float16)
         m = np.clip(lo, -65504, 65504).astype(np.float16)
         df = d.astype(np.float32)[..., None]
         c = np.where(df > 0, np.clip(np.rint((g - m.astype(np.float32)[..., None]) / df), 0, 15), 0)
