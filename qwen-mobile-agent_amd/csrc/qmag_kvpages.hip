@@ -217,6 +217,26 @@ static int check_table(const qmag_kv_table *t)
     return QMAG_OK;
 }
 
+struct Range {
+    const int *p;
+    int64_t n;
+};
+
+// The first n_out ranges are written, the others read: aligned, and none of the
+// written ones meets another.
+static int check_ranges(const char *what, const Range *r, int n_out, int n)
+{
+    for (int i = 0; i < n; i++) {
+        if ((uintptr_t)r[i].p % sizeof(int)) return fail(QMAG_ERR_ARG, "%s: a pointer is not aligned", what);
+        for (int j = 0; j < n_out && j < i; j++) {
+            const uintptr_t a = (uintptr_t)r[i].p, b = (uintptr_t)r[j].p;
+            if (a < b + (uintptr_t)r[j].n * sizeof(int) && b < a + (uintptr_t)r[i].n * sizeof(int))
+                return fail(QMAG_ERR_ARG, "%s: what is written goes to places of its own", what);
+        }
+    }
+    return QMAG_OK;
+}
+
 static int log2_of(int v)
 {
     int s = 0;
@@ -235,8 +255,9 @@ extern "C" int qmag_kv_release_dev(const qmag_kv_table *t, const int *len, const
     if (st) return st;
     if (!len || !ended || !n_free || !len_next || !n_free_next || !status)
         return fail(QMAG_ERR_ARG, "kv_release: null pointer");
-    if (len == len_next || n_free == n_free_next)
-        return fail(QMAG_ERR_ARG, "kv_release: the next lengths and free count go to places of their own");
+    const int64_t n = t->n_seq;
+    const Range r[] = {{len_next, n}, {n_free_next, 1}, {status, 1}, {len, n}, {ended, n}, {n_free, 1}};
+    if ((st = check_ranges("kv_release", r, 3, 6))) return st;
     if ((st = require_ready())) return st;
     DeviceScope dev;
     if (dev.st) return dev.st;
@@ -259,8 +280,10 @@ extern "C" int qmag_kv_assign_dev(const qmag_kv_table *t, const int *len, const 
     if (st) return st;
     if (T < 0 || !len || !n_new || !n_free || !cu || !len_next || !n_free_next || !status || (T > 0 && (!slot || !pos)))
         return fail(QMAG_ERR_ARG, "kv_assign: T=%d or a null pointer", T);
-    if (len == len_next || n_free == n_free_next || n_new == len_next)
-        return fail(QMAG_ERR_ARG, "kv_assign: the next lengths and free count go to places of their own");
+    const int64_t n = t->n_seq;
+    const Range r[] = {{len_next, n}, {n_free_next, 1}, {status, 1}, {cu, n + 1}, {slot, T},
+                       {pos, T},      {len, n},         {n_new, n},  {n_free, 1}};
+    if ((st = check_ranges("kv_assign", r, 6, 9))) return st;
     if ((st = require_ready())) return st;
     DeviceScope dev;
     if (dev.st) return dev.st;

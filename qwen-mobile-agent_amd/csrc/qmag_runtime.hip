@@ -73,6 +73,7 @@ void *workspace(int slot, size_t bytes, int *status)
     void *p = nullptr;
     hipError_t e = hipMalloc(&p, cap);
     if (e != hipSuccess) {
+        (void)hipGetLastError();               // reported here, not by the next launch too
         *status = hip_fail(e, "workspace hipMalloc", __FILE__, __LINE__);
         return nullptr;
     }

@@ -134,6 +134,24 @@ def test_bookkeeping_pointers(lib):
     assert L.qmag_kv_assign_dev(C.byref(t), p[0], p[1], p[2], 0, None, None, *p[5:9]) == NODEV
 
 
+def test_bookkeeping_results_over_inputs(lib):
+    """What is written meets neither an input nor another result, by a part of it either."""
+    L, t = lib.lib(), table(lib, n_seq=10)
+    p = [A + 4096 * i for i in range(10)]
+    ok = dict(zip(("len", "ended", "n_free", "len_next", "n_free_next", "status"), p))
+    rel = lambda **k: L.qmag_kv_release_dev(C.byref(t), *dict(ok, **k).values())  # noqa: E731
+    assert rel() == NODEV and rel(ended=p[0]) == NODEV and rel(len_next=p[0] + 40) == NODEV
+    for k in (dict(len_next=p[0] + 36), dict(len_next=p[1]), dict(status=p[0] + 4), dict(status=p[2]), dict(status=p[4]),
+              dict(n_free_next=p[3] + 36), dict(len=p[0] + 2), dict(status=p[5] + 1)):
+        assert rel(**k) == ARG, k
+    ok = dict(zip(("len", "new", "n_free"), p), T=20, slot=p[3], pos=p[4], cu=p[5], len_next=p[6], n_free_next=p[7], status=p[8])
+    assign = lambda **k: L.qmag_kv_assign_dev(C.byref(t), *dict(ok, **k).values())  # noqa: E731
+    assert assign() == NODEV and assign(pos=p[3] + 80) == NODEV and assign(len_next=p[5] + 44) == NODEV
+    for k in (dict(pos=p[3]), dict(pos=p[3] + 76), dict(len_next=p[5] + 40), dict(cu=p[1]), dict(len_next=p[1] - 36),
+              dict(status=p[2]), dict(n_free_next=p[8]), dict(slot=p[0] + 4), dict(cu=p[5] + 2)):
+        assert assign(**k) == ARG, k
+
+
 @pytest.mark.parametrize("bad", [dict(T=-1), dict(T=(1 << 22) + 1), dict(n_seq=5000), dict(cu=None), dict(cu=A + 1), dict(len=None),
                                  dict(len=A + 2), dict(table=None), dict(max_blocks=0), dict(max_blocks=1 << 27), dict(n_block=63),
                                  dict(tbs=32), dict(q=(A, 3, 384, 128)), dict(out=(A << 4, 8, 1024, 128)), dict(q=(A, 0, 0, 0)),
