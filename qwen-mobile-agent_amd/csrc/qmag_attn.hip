@@ -256,12 +256,13 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     };
     load(0, 0);
 
-    // ---- queries; a negative scale turns their sign
+    // ---- queries; a negative scale turns their sign, none makes them zero (the
+    // scores are multiplied behind the mask, whose -inf has to stay)
     V8 qh[KS], ql[NS == 2 ? KS : 1];
-    float rs = fabsf(A.sc);
+    float rs = A.sc == 0.0f ? 1.0f : fabsf(A.sc);
     {
         const S *qp = (const S *)A.q + (int64_t)(a + min(qi, len - 1)) * A.qt + head * A.qh;
-        const float sign = A.sc < 0.0f ? -1.0f : 1.0f;
+        const float sign = A.sc == 0.0f ? 0.0f : A.sc < 0.0f ? -1.0f : 1.0f;
         if constexpr (NS == 2) {
             float x[KS][8], top = 0.0f;
 #pragma unroll
@@ -383,7 +384,8 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             }
         }
         if (__any(move)) {
-            const float mn = fmaxf(m, top), g = __builtin_amdgcn_exp2f(m - mn);
+            // (a query that need not move stays: what others see has no part in its rounding)
+            const float mn = move ? fmaxf(m, top) : m, g = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= g;
             f *= g;

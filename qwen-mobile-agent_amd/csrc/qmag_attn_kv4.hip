@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 {
     using S = typename T::S;
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
-    constexpr Code CODE = NS == 2 ? CENTRED : std::is_same_v<T, TBF16> ? RAW : PLAIN;
+    constexpr Code CODE = std::is_same_v<T, TBF16> ? RAW : CENTRED;
     constexpr int NG = D / 64;
     constexpr int RG = 16, STEP = 32 * NW;
     constexpr int VD = (D + 127) / 128;            // dwords of a lane's V codes of a token
@@ -473,7 +473,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 
         // ---- running maximum: moved only when a weight would pass 2^8
         if (__any(top > m + 8.0f)) {
-            const float mn = fmaxf(m, top);
+            // (a row that need not move stays: what others see has no part in its rounding)
+            const float mn = top > m + 8.0f ? fmaxf(m, top) : m;
             const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= f;
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
 {
     using S = typename T::S;
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
-    constexpr Code CODE = NS == 2 ? CENTRED : PLAIN;
+    constexpr Code CODE = std::is_same_v<T, TBF16> ? PLAIN : CENTRED;
     constexpr int NG = D / 64;
     constexpr int RG = 16 * NW, STEP = 32;
     constexpr int TILE = ak_tile<D>(), IMG = 32 * D, SC = 4 * D;   // bytes, values, bytes
@@ -828,7 +829,8 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
 
         // ---- running maximum: moved only when a weight would pass 2^8
         if (__any(top > m + 8.0f)) {
-            const float mn = fmaxf(m, top);
+            // (a row that need not move stays: what others see has no part in its rounding)
+            const float mn = top > m + 8.0f ? fmaxf(m, top) : m;
             const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= f;
@@ -1012,7 +1014,7 @@ static int ak_launch(AkArgs A, hipStream_t s)
     constexpr int NW = ROWS ? 8 : 4, RG = ROWS ? 16 * NW : 16, STEP = ROWS ? 32 : 32 * NW;
     // Row groups at most.  Chunks are cut for as many workgroups as the chip holds at
     // once: of more the last ones run alone, of fewer some CUs get two and others none.
-    const int64_t groups = (int64_t)A.T * A.G / RG + A.n_seq;
+    const int64_t groups = (int64_t)A.T * A.G / RG + (A.T < A.n_seq ? A.T : A.n_seq);
     const int64_t goal = (ROWS ? rows_resident<T, D>() : 4) * (int64_t)ctx().n_cu;
     A.target = (int)((goal + A.n_kv - 1) / A.n_kv);
     // enough row groups to fill the chip twice over: nothing is split
