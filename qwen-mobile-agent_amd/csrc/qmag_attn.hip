@@ -456,8 +456,6 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             else if (kt == mine) tile(lds[b] + i * TILE, sc, std::true_type{});
         }
     }
-    if (qi >= len) return;
-
     // ---- infinities and NaN of V, to the rows that see them: whatever else a
     // row sums, they decide its result, so they are added to it at the end
     const float inv = 1.0f / query_sum<QW>(l);          // every row sees itself
@@ -466,19 +464,23 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < R; i++) o[d][i] *= inv;
-    for (int t = 0; t <= mine; t++) {
-        if (!A.odd[tile0 + t]) continue;
-        for (int k = t * AP_KEYS; k < min(t * AP_KEYS + AP_KEYS, qi + 1); k++) {
-            const S *vr = (const S *)A.v + (int64_t)(a + k) * A.vt + kvh * A.vh;
+    for (int t0 = 0; t0 <= mine; t0 += 64) {       // (64 flags to a load: one after the other they took longer than a tile)
+        unsigned long long odd = __ballot(t0 + lane <= mine && A.odd[tile0 + t0 + lane] != 0);
+        for (; odd; odd &= odd - 1) {
+            const int k0 = (t0 + __ffsll(odd) - 1) * AP_KEYS, k1 = min(min(k0 + AP_KEYS, qi + 1), len);
+            for (int k = k0; k < k1; k++) {
+                const S *vr = (const S *)A.v + (int64_t)(a + k) * A.vt + kvh * A.vh;
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+                for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < R; i++) {
-                    const float x = T::up(vr[QW * d + CG * (i >> 2) + 4 * h + (i & 3)]);
-                    o[d][i] += fabsf(x) <= 3.402823466e38f ? 0.0f : x;
-                }
+                    for (int i = 0; i < R; i++) {
+                        const float x = T::up(vr[QW * d + CG * (i >> 2) + 4 * h + (i & 3)]);
+                        o[d][i] += fabsf(x) <= 3.402823466e38f ? 0.0f : x;
+                    }
+            }
         }
     }
+    if (qi >= len) return;
     S *op = (S *)A.out + (int64_t)(a + qi) * A.ot + head * A.oh;
 #pragma unroll
     for (int d = 0; d < DT; d++)
