@@ -34,7 +34,8 @@ struct ApArgs {
     const int *cu;
     uint8_t *img;                         // [n_kv][tiles][K image | V image]
     float *scale;                         // [n_kv][tiles][32 of K | 32 of V], fp32 calls
-    int *odd;                             // [n_kv][tiles]: V holds an infinity or a NaN
+    int *flags;                           // [n_kv][tiles]: bit 0 V holds an infinity or a NaN; fp32 calls: 2 (128 + its
+                                          // largest power of two's exponent)
     int n_seq, T, tiles, n_kv, G;
     float sc;                             // scale * log2 e
     int q_vec, k_vec, v_vec, o_vec;
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
         for (int i = 0; i < 8; i++) x[u][i] = 0.0f;
         if (t < n) load8<T, true>(base + (int64_t)(a + t) * stride, w ? A.v_vec : A.k_vec, x[u]);
     }
-    int odd = 0;
+    int odd = 0, most = -126;
 #pragma unroll
     for (int u = 0; u < N; u++) {
         const int key = u * ROWS + (int)threadIdx.x / CH;
@@ -192,6 +193,7 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
             }
             *(V8 *)(row + PLANE) = lo;
             if (c == 0) A.scale[tile * 2 * AP_KEYS + w * AP_KEYS + key] = pow2i(e - 14);
+            most = max(most, e - 14);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) hi[i] = (E)x[u][i];
@@ -199,8 +201,17 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
         *(V8 *)row = hi;
     }
     if (w) {
-        odd = __syncthreads_or(odd);
-        if (threadIdx.x == 0) A.odd[tile] = odd;
+        if constexpr (NS == 2) {
+            __shared__ int wave_most[AP_WG / 64];
+#pragma unroll
+            for (int d = CH; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
+            if (lane_id() == 0) wave_most[threadIdx.x >> 6] = most;
+            odd = __syncthreads_or(odd);
+            for (int i = 0; i < AP_WG / 64; i++) most = max(most, wave_most[i]);
+        } else {
+            odd = __syncthreads_or(odd);
+        }
+        if (threadIdx.x == 0) A.flags[tile] = (odd ? 1 : 0) | 2 * (128 + most);
     }
 }
 
@@ -250,11 +261,17 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (int64_t)step * PIECES + at + lane),
                                              (__attribute__((address_space(3))) void *)((uint4 *)lds[b] + at), 16, 0, 0);
         }
+        // their powers of two, a wave for a tile's 64, the same way (through a register the
+        // wave waited here for the whole step)
         if constexpr (NS == 2)
-            if (threadIdx.x < KT * 2 * AP_KEYS)
-                lsc[b][threadIdx.x] = A.scale[(tile0 + (int64_t)step * KT) * 2 * AP_KEYS + threadIdx.x];
+            if (wave < KT)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void *)(A.scale + ((tile0 + (int64_t)step * KT + wave) * 64 + lane)),
+                    (__attribute__((address_space(3))) void *)(lsc[b] + wave * 64), 4, 0, 0);
     };
     load(0, 0);
+    // (as constants: scalar loads, which wait for no step)
+    const __attribute__((address_space(4))) int *flags = (const __attribute__((address_space(4))) int *)(uintptr_t)(A.flags + tile0);
 
     // ---- queries; a negative scale turns their sign, none makes them zero (the
     // scores are multiplied behind the mask, whose -inf has to stay)
@@ -314,7 +331,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     }
 
     // One tile of 32 keys; EDGE: the one that holds the wave's own tokens.
-    auto tile = [&](const E *K, const float *sc, auto EDGE) {
+    auto tile = [&](const E *K, const float *sc, int flag, auto EDGE) {
         // ---- scores
         Acc sa[NA];
 #pragma unroll
@@ -346,14 +363,12 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
         for (int i = 0; i < NV; i++) s[i] = sa[i / R][i % R];
         constexpr int KG = QW == 32 ? 8 : 16;      // a lane's keys: KG g + 4 h + 0 .. 3
-        float vp[NS == 2 ? NV : 1];                // V's powers of two
         if constexpr (NS == 2) {
 #pragma unroll
             for (int g = 0; g < NV / 4; g++) {
-                const float4 ks = *(const float4 *)(sc + KG * g + 4 * h), vs = *(const float4 *)(sc + AP_KEYS + KG * g + 4 * h);
+                const float4 ks = *(const float4 *)(sc + KG * g + 4 * h);
                 s[4 * g] *= rs * ks.x, s[4 * g + 1] *= rs * ks.y;
                 s[4 * g + 2] *= rs * ks.z, s[4 * g + 3] *= rs * ks.w;
-                vp[4 * g] = vs.x, vp[4 * g + 1] = vs.y, vp[4 * g + 2] = vs.z, vp[4 * g + 3] = vs.w;
             }
         }
         if constexpr (EDGE.value) {                // (keys behind the end are behind every query)
@@ -361,31 +376,44 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             for (int i = 0; i < NV; i++) {
                 const bool seen = KG * (i >> 2) + 4 * h + (i & 3) <= qi % AP_KEYS;
                 s[i] = seen ? s[i] : -INFINITY;
-                if constexpr (NS == 2) vp[i] = seen ? vp[i] : 0.0f;
             }
         }
-        // ---- running maximum: moved only when a weight would pass 2^8
+        // ---- weights, by the maximum so far.  Whether it has to move is seen from
+        // their sum, which is needed in any case: past 2^8, an infinity included.
         const float r = NS == 2 ? 1.0f : rs;
-        float top = s[0];
+        float p[NV], sum = 0.0f;
+        auto weigh = [&] {
+            sum = 0.0f;
 #pragma unroll
-        for (int i = 1; i < NV; i++) top = fmaxf(top, s[i]);
-        top = query_max<QW>(top) * r;
-        float f = 1.0f;
-        bool move = top > m + 8.0f;
-        if constexpr (NS == 2) {
-            float vt = vp[0];
-#pragma unroll
-            for (int i = 1; i < NV; i++) vt = fmaxf(vt, vp[i]);
-            const int e = max((int)(__float_as_uint(query_max<QW>(vt)) >> 23) - 127, -126);
-            if (e > ve) {
-                f = ve == -127 ? 0.0f : pow2i(max(ve - e, -126));
-                ve = e;
-                move = true;
+            for (int i = 0; i < NV; i++) {
+                p[i] = __builtin_amdgcn_exp2f(NS == 2 ? s[i] - m : fmaf(s[i], r, -m));
+                sum += p[i];
             }
+        };
+        weigh();
+        bool move = sum > 256.0f;
+        int e = (flag >> 1) - 128;                 // of the largest V that the row sees here
+        if constexpr (NS == 2) {
+            if constexpr (EDGE.value) {
+                float vt = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NV; i++) vt = fmaxf(vt, s[i] == -INFINITY ? 0.0f : sc[AP_KEYS + KG * (i >> 2) + 4 * h + (i & 3)]);
+                e = max((int)(__float_as_uint(query_max<QW>(vt)) >> 23) - 127, -126);
+            }
+            move = move || e > ve;
         }
         if (__any(move)) {
+            float top = s[0], f = 1.0f;
+#pragma unroll
+            for (int i = 1; i < NV; i++) top = fmaxf(top, s[i]);
+            top = query_max<QW>(top) * r;
             // (a query that need not move stays: what others see has no part in its rounding)
-            const float mn = move ? fmaxf(m, top) : m, g = __builtin_amdgcn_exp2f(m - mn);
+            const float mn = query_max<QW>(sum) > 256.0f ? fmaxf(m, top) : m;
+            if (NS == 2 && e > ve) {
+                f = ve == -127 ? 0.0f : pow2i(max(ve - e, -126));
+                ve = e;
+            }
+            const float g = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= g;
             f *= g;
@@ -393,24 +421,23 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int i = 0; i < R; i++) o[d][i] *= f;
+            weigh();
         }
+        l += sum;
         const float pv = NS == 2 ? pow2i(min(7 - ve, 127)) : 1.0f;
         V8 ph[PS], pl[NS == 2 ? PS : 1];
 #pragma unroll
         for (int i = 0; i < NV; i += 2) {
-            float p[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                p[u] = __builtin_amdgcn_exp2f(NS == 2 ? s[i + u] - m : fmaf(s[i + u], r, -m));
-                l += p[u];
-            }
             if constexpr (NS == 2) {
                 half2v a, b;
-                split2(p[0] * (vp[i] * pv), p[1] * (vp[i + 1] * pv), &a, &b);
+                float2 vp = *(const float2 *)(sc + AP_KEYS + KG * (i >> 2) + 4 * h + (i & 3));
+                vp.x *= pv, vp.y *= pv;                // up to 2^7; of keys not seen to infinity
+                if constexpr (EDGE.value) vp.x = fminf(vp.x, 128.0f), vp.y = fminf(vp.y, 128.0f);
+                split2(p[i] * vp.x, p[i + 1] * vp.y, &a, &b);
                 ph[i >> 3][i & 7] = a[0], ph[i >> 3][(i & 7) + 1] = a[1];
                 pl[i >> 3][i & 7] = b[0], pl[i >> 3][(i & 7) + 1] = b[1];
             } else {
-                ph[i >> 3][i & 7] = (E)p[0], ph[i >> 3][(i & 7) + 1] = (E)p[1];
+                ph[i >> 3][i & 7] = (E)p[i], ph[i >> 3][(i & 7) + 1] = (E)p[i + 1];
             }
         }
         // ---- output
@@ -443,18 +470,26 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 
     const int mine = q0 < len ? q0 / AP_KEYS : -1;           // the wave's last tile
     const int steps = (tiles + KT - 1) / KT;
+    int flag[KT];
+#pragma unroll
+    for (int i = 0; i < KT; i++) flag[i] = NS == 2 ? flags[i] : 0;
     for (int step = 0; step < steps; step++) {
         const int b = step & 1;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __syncthreads();
+        int next[KT];
+#pragma unroll
+        for (int i = 0; i < KT; i++) next[i] = NS == 2 ? flags[(step + 1) * KT + i] : 0;
         if (step + 1 < steps) load(step + 1, b ^ 1);
 #pragma unroll
         for (int i = 0; i < KT; i++) {
             const int kt = step * KT + i;
             const float *sc = lsc[b] + (NS == 2 ? i * 2 * AP_KEYS : 0);
-            if (kt < mine) tile(lds[b] + i * TILE, sc, std::false_type{});
-            else if (kt == mine) tile(lds[b] + i * TILE, sc, std::true_type{});
+            if (kt < mine) tile(lds[b] + i * TILE, sc, flag[i], std::false_type{});
+            else if (kt == mine) tile(lds[b] + i * TILE, sc, 0, std::true_type{});
         }
+#pragma unroll
+        for (int i = 0; i < KT; i++) flag[i] = next[i];
     }
     // ---- infinities and NaN of V, to the rows that see them: whatever else a
     // row sums, they decide its result, so they are added to it at the end
@@ -465,7 +500,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
         for (int i = 0; i < R; i++) o[d][i] *= inv;
     for (int t0 = 0; t0 <= mine; t0 += 64) {       // (64 flags to a load: one after the other they took longer than a tile)
-        unsigned long long odd = __ballot(t0 + lane <= mine && A.odd[tile0 + t0 + lane] != 0);
+        unsigned long long odd = __ballot(t0 + lane <= mine && A.flags[tile0 + t0 + lane] & 1);
         for (; odd; odd &= odd - 1) {
             const int k0 = (t0 + __ffsll(odd) - 1) * AP_KEYS, k1 = min(min(k0 + AP_KEYS, qi + 1), len);
             for (int k = k0; k < k1; k++) {
@@ -507,7 +542,7 @@ static int ap_run(ApArgs A, hipStream_t s)
     if (st) return st;
     A.img = ws;
     A.scale = (float *)(ws + n * TILE);
-    A.odd = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
+    A.flags = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
     prompt_tiles_kernel<T, D, QW><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv, 2), AP_WG, 0, s>>>(A);
     attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
     return QMAG_OK;
@@ -520,7 +555,7 @@ static int ap_launch(const ApArgs &A, hipStream_t s)
     const int64_t wgs = ((int64_t)A.T / 128 + A.n_seq) * A.n_kv * A.G;
     if (wgs < (F32 && D == 256 ? 1 : 4) * (int64_t)ctx().n_cu) return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);
     if constexpr (F32 || D == 256) return ap_run<T, D, 8, 16, D == 64 ? 2 : 1, F32 && D == 128 ? 2 : 3, F32 && D == 128 ? 4 : 2>(A, s);
-    else return ap_run<T, D, 4, 32, D == 64 ? 2 : 1, 3, 2>(A, s);
+    else return ap_run<T, D, 4, 32, D == 64 ? 2 : 1, 3, D == 64 ? 4 : 3>(A, s);
 }
 
 }  // namespace qmag
