@@ -100,6 +100,19 @@ __device__ __forceinline__ void store4(typename T::S *p, bool vec, const float (
     }
 }
 
+// Inclusive sums over the wave, all lanes active: within rows of 16 lanes, then a
+// row's last to the row behind it, then the lower half's to the upper.
+__device__ __forceinline__ int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
 // ------------------------------------------------------------- host side --
 // The device of the library current for the life of a call, whichever one the
 // calling thread had.

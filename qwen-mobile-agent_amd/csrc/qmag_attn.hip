@@ -50,44 +50,40 @@ __device__ __forceinline__ void ap_seq(const ApArgs &A, int i, int *a, int *n)
 }
 
 // The sequence and part of it that hold unit `want` of `per` rows each; last:
-// counted from the end.  Found by the calling wave alone.
+// counted from the end.  Found by the calling wave alone.  (At most 2^22 / 32
+// units a sequence, whatever the lengths: the sums stay below 2^30.)
 __device__ __forceinline__ bool ap_find(const ApArgs &A, int want, int per, bool last, int *seq, int *part, int *a, int *n)
 {
     const int lane = lane_id();
-    int x, len;
+    int x = 0, len = 0;
+    if (lane < A.n_seq) ap_seq(A, lane, &x, &len);
     if (last) {
-        long long all = 0;
-        for (int i = lane; i < A.n_seq; i += 64) {
-            ap_seq(A, i, &x, &len);
-            all += (len + per - 1) / per;
+        int all = (len + per - 1) / per, y, m;
+        for (int i = 64 + lane; i < A.n_seq; i += 64) {
+            ap_seq(A, i, &y, &m);
+            all += (m + per - 1) / per;
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+        all = group_sum_i<64>(all);
         if (want >= all) return false;
-        want = (int)min(all - 1 - want, (long long)INT32_MAX);
+        want = all - 1 - want;
     }
-    long long before = 0;
+    int before = 0;
     for (int base = 0; base < A.n_seq; base += 64) {
-        const int i = base + lane;
-        x = len = 0;
-        if (i < A.n_seq) ap_seq(A, i, &x, &len);
-        const int mine = (len + per - 1) / per;
-        long long incl = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const long long v = __shfl_up(incl, d);
-            if (lane >= d) incl += v;
+        if (base) {
+            x = len = 0;
+            if (base + lane < A.n_seq) ap_seq(A, base + lane, &x, &len);
         }
+        const int mine = (len + per - 1) / per, incl = wave_scan(mine);
         const unsigned long long hit = __ballot(want < before + incl);
         if (hit) {
-            const int at = __ffsll(hit) - 1;
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll(hit) - 1);
             *seq = base + at;
             *a = __builtin_amdgcn_readlane(x, at);
             *n = __builtin_amdgcn_readlane(len, at);
-            *part = (int)(want - before - __shfl(incl - mine, at));
+            *part = want - before - __builtin_amdgcn_readlane(incl - mine, at);
             return true;
         }
-        before += __shfl(incl, 63);
+        before += __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
 }
@@ -142,69 +138,89 @@ __device__ __forceinline__ f32x4 mfma(bf168 a, bf168 b, f32x4 c) { return __buil
 __device__ __forceinline__ f32x16 mfma(bf168 a, bf168 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 // ---------------------------------------------------------------- tiles ----
-template <class T, int D, int QW>
-__global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
-{
+// A thread's part of a tile of K or V, NT threads: 8 channels of every ROWSth of
+// its 32 rows.
+template <class T, int D, int QW, int NT>
+struct ApRows {
     using S = typename T::S;
     using E = typename ApOperand<T>::E;
     using V8 = typename ApOperand<T>::V;
-    constexpr int NS = sizeof(S) == 4 ? 2 : 1;
-    constexpr int CH = D / 8, ROWS = AP_WG / CH;
-    constexpr int PLANE = AP_KEYS * D;
+    static constexpr int NS = sizeof(S) == 4 ? 2 : 1;
+    static constexpr int CH = D / 8, ROWS = NT / CH, N = AP_KEYS / ROWS, PLANE = AP_KEYS * D;
+    float x[N][8];
+
+    // rows t0 .. t0 + 31 of a sequence of n, which begins at row a; zero behind its end
+    template <bool ONCE>
+    __device__ __forceinline__ void fetch(const ApArgs &A, bool v, int kvh, int a, int n, int t0)
+    {
+        const int c = threadIdx.x % CH;
+        const S *base = (const S *)(v ? A.v : A.k) + kvh * (v ? A.vh : A.kh) + 8 * c;
+        const int64_t stride = v ? A.vt : A.kt;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            const int t = t0 + u * ROWS + (int)threadIdx.x / CH;
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[u][i] = 0.0f;
+            if (t < n) load8<T, ONCE>(base + (int64_t)(a + t) * stride, v ? A.v_vec : A.k_vec, x[u]);
+        }
+    }
+
+    // into a tile's image and powers of two; odd: V had an infinity or a NaN (added
+    // where it is seen, not multiplied); most: the largest power's exponent
+    __device__ __forceinline__ void lay(bool v, E *img, float *scale, int *odd, int *most)
+    {
+        const int c = threadIdx.x % CH;
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            const int key = u * ROWS + (int)threadIdx.x / CH;
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool fine = fabsf(x[u][i]) <= 3.402823466e38f;
+                top = fmaxf(top, fine ? fabsf(x[u][i]) : 0.0f);
+                if (v && !fine) *odd = 1, x[u][i] = 0.0f;
+            }
+            E *row = img + (v ? NS * PLANE : 0) + key * D + 8 * (v ? v_chunk<D, QW>(key, c) : k_chunk<D>(key, c));
+            V8 hi, lo;
+            if constexpr (NS == 2) {
+                const int e = row_exp(group_max<CH>(top));
+                const float up = pow2i(14 - e);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    half2v p, q;
+                    split2(x[u][i] * up, x[u][i + 1] * up, &p, &q);
+                    hi[i] = p[0], hi[i + 1] = p[1], lo[i] = q[0], lo[i + 1] = q[1];
+                }
+                *(V8 *)(row + PLANE) = lo;
+                if (c == 0) scale[(v ? AP_KEYS : 0) + key] = pow2i(e - 14);
+                *most = max(*most, e - 14);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) hi[i] = (E)x[u][i];
+            }
+            *(V8 *)row = hi;
+        }
+    }
+};
+
+template <class T, int D, int QW>
+__global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
+{
+    using R = ApRows<T, D, QW, AP_WG>;
     int seq, part, a, n;
     if (!ap_find(A, blockIdx.x, AP_KEYS, false, &seq, &part, &a, &n)) return;
     const int kvh = blockIdx.y;
     const int64_t tile = (int64_t)kvh * A.tiles + a / AP_KEYS + seq + part;
-    E *img = (E *)A.img + tile * 2 * NS * PLANE;
-    const int c = threadIdx.x % CH, w = blockIdx.z;                  // K's image, or V's
-    const S *base = (const S *)(w ? A.v : A.k) + kvh * (w ? A.vh : A.kh) + 8 * c;
-    const int64_t stride = w ? A.vt : A.kt;
-    constexpr int N = AP_KEYS / ROWS;
-    float x[N][8];
-#pragma unroll
-    for (int u = 0; u < N; u++) {
-        const int t = part * AP_KEYS + u * ROWS + (int)threadIdx.x / CH;
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[u][i] = 0.0f;
-        if (t < n) load8<T, true>(base + (int64_t)(a + t) * stride, w ? A.v_vec : A.k_vec, x[u]);
-    }
+    const bool v = blockIdx.z;                     // K's image, or V's
     int odd = 0, most = -126;
-#pragma unroll
-    for (int u = 0; u < N; u++) {
-        const int key = u * ROWS + (int)threadIdx.x / CH;
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const bool fine = fabsf(x[u][i]) <= 3.402823466e38f;
-            top = fmaxf(top, fine ? fabsf(x[u][i]) : 0.0f);
-            // V's infinities and NaN are added where they are seen, not multiplied
-            if (w && !fine) odd = 1, x[u][i] = 0.0f;
-        }
-        E *row = img + w * NS * PLANE + key * D + 8 * (w ? v_chunk<D, QW>(key, c) : k_chunk<D>(key, c));
-        V8 hi, lo;
-        if constexpr (NS == 2) {
-            const int e = row_exp(group_max<CH>(top));
-            const float up = pow2i(14 - e);
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                half2v p, q;
-                split2(x[u][i] * up, x[u][i + 1] * up, &p, &q);
-                hi[i] = p[0], hi[i + 1] = p[1], lo[i] = q[0], lo[i + 1] = q[1];
-            }
-            *(V8 *)(row + PLANE) = lo;
-            if (c == 0) A.scale[tile * 2 * AP_KEYS + w * AP_KEYS + key] = pow2i(e - 14);
-            most = max(most, e - 14);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) hi[i] = (E)x[u][i];
-        }
-        *(V8 *)row = hi;
-    }
-    if (w) {
-        if constexpr (NS == 2) {
+    R rows;
+    rows.template fetch<true>(A, v, kvh, a, n, part * AP_KEYS);
+    rows.lay(v, (typename R::E *)A.img + tile * 2 * R::NS * R::PLANE, A.scale + tile * 2 * AP_KEYS, &odd, &most);
+    if (v) {
+        if constexpr (R::NS == 2) {
             __shared__ int wave_most[AP_WG / 64];
 #pragma unroll
-            for (int d = CH; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
+            for (int d = R::CH; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
             if (lane_id() == 0) wave_most[threadIdx.x >> 6] = most;
             odd = __syncthreads_or(odd);
             for (int i = 0; i < AP_WG / 64; i++) most = max(most, wave_most[i]);
@@ -217,8 +233,9 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
 
 // ------------------------------------------------------------- attention ----
 // NW waves of QW queries; KT tiles of keys to a barrier; LDS read AHEAD steps
-// ahead of the products; WE waves to a SIMD.
-template <class T, int D, int NW, int QW, int KT, int AHEAD, int WE>
+// ahead of the products; WE waves to a SIMD.  DIRECT: no tiles were laid out; the
+// workgroup takes K and V as they are and lays each tile out in LDS itself.
+template <class T, int D, int NW, int QW, int KT, int AHEAD, int WE, bool DIRECT>
 __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 {
     using S = typename T::S;
@@ -235,6 +252,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     constexpr int DT = D / QW;                    // QW-channel parts of the output
     constexpr int PK = KW, PS = 32 / PK;
     constexpr int ROWS = QW * NW;
+    static_assert(!DIRECT || KT == 1, "tiles are laid out one at a time");
     __shared__ __attribute__((aligned(16))) E lds[2][KT * TILE];
     __shared__ __attribute__((aligned(16))) float lsc[2][NS == 2 ? KT * 2 * AP_KEYS : 4];
 
@@ -269,7 +287,13 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
                     (const __attribute__((address_space(1))) void *)(A.scale + ((tile0 + (int64_t)step * KT + wave) * 64 + lane)),
                     (__attribute__((address_space(3))) void *)(lsc[b] + wave * 64), 4, 0, 0);
     };
-    load(0, 0);
+    ApRows<T, D, QW, 64 * NW> kr, vr;
+    if constexpr (DIRECT) {
+        kr.template fetch<false>(A, false, kvh, a, len, 0);
+        vr.template fetch<false>(A, true, kvh, a, len, 0);
+    } else {
+        load(0, 0);
+    }
     // (as constants: scalar loads, which wait for no step)
     const __attribute__((address_space(4))) int *flags = (const __attribute__((address_space(4))) int *)(uintptr_t)(A.flags + tile0);
 
@@ -394,7 +418,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         bool move = sum > 256.0f;
         int e = (flag >> 1) - 128;                 // of the largest V that the row sees here
         if constexpr (NS == 2) {
-            if constexpr (EDGE.value) {
+            if constexpr (EDGE.value || DIRECT) {
                 float vt = 0.0f;
 #pragma unroll
                 for (int i = 0; i < NV; i++) vt = fmaxf(vt, s[i] == -INFINITY ? 0.0f : sc[AP_KEYS + KG * (i >> 2) + 4 * h + (i & 3)]);
@@ -472,15 +496,27 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     const int steps = (tiles + KT - 1) / KT;
     int flag[KT];
 #pragma unroll
-    for (int i = 0; i < KT; i++) flag[i] = NS == 2 ? flags[i] : 0;
+    for (int i = 0; i < KT; i++) flag[i] = NS == 2 && !DIRECT ? flags[i] : 0;
+    unsigned long long odd = 0;                    // DIRECT: tiles whose V holds an infinity or a NaN
     for (int step = 0; step < steps; step++) {
         const int b = step & 1;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __syncthreads();
-        int next[KT];
+        int next[KT] = {};
+        if constexpr (DIRECT) {
+            int here = 0, most = 0;
+            kr.lay(false, lds[b], lsc[b], &here, &most);
+            vr.lay(true, lds[b], lsc[b], &here, &most);
+            if (__syncthreads_or(here)) odd |= 1ull << step;
+            if (step + 1 < steps) {
+                kr.template fetch<false>(A, false, kvh, a, len, (step + 1) * AP_KEYS);
+                vr.template fetch<false>(A, true, kvh, a, len, (step + 1) * AP_KEYS);
+            }
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < KT; i++) next[i] = NS == 2 ? flags[(step + 1) * KT + i] : 0;
-        if (step + 1 < steps) load(step + 1, b ^ 1);
+            for (int i = 0; i < KT; i++) next[i] = NS == 2 ? flags[(step + 1) * KT + i] : 0;
+            if (step + 1 < steps) load(step + 1, b ^ 1);
+        }
 #pragma unroll
         for (int i = 0; i < KT; i++) {
             const int kt = step * KT + i;
@@ -500,7 +536,8 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
         for (int i = 0; i < R; i++) o[d][i] *= inv;
     for (int t0 = 0; t0 <= mine; t0 += 64) {       // (64 flags to a load: one after the other they took longer than a tile)
-        unsigned long long odd = __ballot(t0 + lane <= mine && A.flags[tile0 + t0 + lane] & 1);
+        if constexpr (DIRECT) odd = mine < 0 ? 0 : odd & (~0ull >> (63 - mine));
+        else odd = __ballot(t0 + lane <= mine && A.flags[tile0 + t0 + lane] & 1);
         for (; odd; odd &= odd - 1) {
             const int k0 = (t0 + __ffsll(odd) - 1) * AP_KEYS, k1 = min(min(k0 + AP_KEYS, qi + 1), len);
             for (int k = k0; k < k1; k++) {
@@ -528,7 +565,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         }
 }
 
-template <class T, int D, int NW, int QW, int KT, int AHEAD, int WE>
+template <class T, int D, int NW, int QW, int KT, int AHEAD, int WE, bool DIRECT = false>
 static int ap_run(ApArgs A, hipStream_t s)
 {
     constexpr int NS = sizeof(typename T::S) == 4 ? 2 : 1;
@@ -537,6 +574,10 @@ static int ap_run(ApArgs A, hipStream_t s)
     const size_t n = (size_t)A.tiles * A.n_kv + 8;         // a barrier's tiles may reach past the last one
     const int64_t wgs = (((int64_t)A.T / (QW * NW) + A.n_seq + 7) / 8 * 8) * A.n_kv * A.G;
     if (wgs > UINT32_MAX / (64 * NW)) return fail(QMAG_ERR_ARG, "attn_prompt: %lld workgroups", (long long)wgs);
+    if constexpr (DIRECT) {
+        attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE, true><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
+        return QMAG_OK;
+    }
     int st;
     uint8_t *ws = (uint8_t *)workspace(WS_ATTN, n * (TILE + (NS == 2 ? 2 * AP_KEYS * sizeof(float) : 0) + sizeof(int)), &st);
     if (st) return st;
@@ -544,7 +585,7 @@ static int ap_run(ApArgs A, hipStream_t s)
     A.scale = (float *)(ws + n * TILE);
     A.flags = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
     prompt_tiles_kernel<T, D, QW><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv, 2), AP_WG, 0, s>>>(A);
-    attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
+    attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE, false><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
     return QMAG_OK;
 }
 
@@ -553,6 +594,7 @@ static int ap_launch(const ApArgs &A, hipStream_t s)
 {
     constexpr bool F32 = sizeof(typename T::S) == 4;
     const int64_t wgs = ((int64_t)A.T / 128 + A.n_seq) * A.n_kv * A.G;
+    if (A.T <= (D == 64 ? 128 : D == 128 ? 96 : 64) * (A.n_seq > 1 ? 3 : 2) / 2) return ap_run<T, D, F32 && D == 256 ? 8 : 4, 16, 1, 3, 2, true>(A, s);
     if (wgs < (F32 && D == 256 ? 1 : 4) * (int64_t)ctx().n_cu) return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);
     if constexpr (F32 || D == 256) return ap_run<T, D, 8, 16, D == 64 ? 2 : 1, F32 && D == 128 ? 2 : 3, F32 && D == 128 ? 4 : 2>(A, s);
     else return ap_run<T, D, 4, 32, D == 64 ? 2 : 1, 3, D == 64 ? 4 : 3>(A, s);

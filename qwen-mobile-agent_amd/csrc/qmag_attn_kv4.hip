@@ -105,12 +105,7 @@ __device__ __forceinline__ bool ak_find(const AkArgs &A, int want, bool by_token
         }
         const int split = max(1, (int)(((unsigned)len + (unsigned)P->chunk - 1u) / (unsigned)P->chunk));
         const int mine = (int)min((long long)ak_groups(A, nq, RG) * split, 1ll << 23);
-        int incl = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(incl, d);
-            if (lane >= d) incl += v;
-        }
+        const int incl = wave_scan(mine);
         const bool here = by_token ? want >= q0 && want < q0 + nq : want < items + incl;
         const unsigned long long hit = __ballot(here);
         if (hit) {
