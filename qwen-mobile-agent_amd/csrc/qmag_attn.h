@@ -102,14 +102,23 @@ __device__ __forceinline__ void store4(typename T::S *p, bool vec, const float (
 
 // Inclusive sums over the wave, all lanes active: within rows of 16 lanes, then a
 // row's last to the row behind it, then the lower half's to the upper.
-__device__ __forceinline__ int wave_scan(int v)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_move(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long long scan_move(long long v)
 {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    const uint32_t lo = (uint32_t)scan_move<CTRL, ROWS>((int)v);
+    return (long long)((unsigned long long)(uint32_t)scan_move<CTRL, ROWS>((int)(v >> 32)) << 32 | lo);
+}
+template <class I>
+__device__ __forceinline__ I wave_scan(I v)
+{
+    v += scan_move<0x111, 0xf>(v);
+    v += scan_move<0x112, 0xf>(v);
+    v += scan_move<0x114, 0xf>(v);
+    v += scan_move<0x118, 0xf>(v);
+    v += scan_move<0x142, 0xa>(v);
+    v += scan_move<0x143, 0xc>(v);
     return v;
 }
 

@@ -594,7 +594,7 @@ static int ap_launch(const ApArgs &A, hipStream_t s)
 {
     constexpr bool F32 = sizeof(typename T::S) == 4;
     const int64_t wgs = ((int64_t)A.T / 128 + A.n_seq) * A.n_kv * A.G;
-    if (A.T <= (D == 64 ? 128 : D == 128 ? 96 : 64) * (A.n_seq > 1 ? 3 : 2) / 2) return ap_run<T, D, F32 && D == 256 ? 8 : 4, 16, 1, 3, 2, true>(A, s);
+    if (A.T <= (D == 64 ? 128 : D == 128 ? 96 : 64) * (A.n_seq > 1 ? 3 : 2) / 2) return ap_run<T, D, D == 256 ? 8 : 4, 16, 1, 3, 2, true>(A, s);
     if (wgs < (F32 && D == 256 ? 1 : 4) * (int64_t)ctx().n_cu) return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);
     if constexpr (F32 || D == 256) return ap_run<T, D, 8, 16, D == 64 ? 2 : 1, F32 && D == 128 ? 2 : 3, F32 && D == 128 ? 4 : 2>(A, s);
     else return ap_run<T, D, 4, 32, D == 64 ? 2 : 1, 3, D == 64 ? 4 : 3>(A, s);

@@ -20,23 +20,15 @@ constexpr int PG_TOK = 4;                  // consecutive tokens of a thread and
 // come back too.  In 64 bits: lengths are the caller's data.
 struct PgScan {
     long long tok, blk;
+    int bad;                               // bits of any thread
 };
 __device__ __forceinline__ PgScan pg_scan(PgScan v, PgScan *total, PgScan *wave_sum)
 {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    PgScan in = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long t = __shfl_up(in.tok, d);
-        const long long b = __shfl_up(in.blk, d);
-        if (lane >= d) {
-            in.tok += t;
-            in.blk += b;
-        }
-    }
+    const PgScan in = {wave_scan(v.tok), wave_scan(v.blk), (__any(v.bad & 1) ? 1 : 0) | (__any(v.bad & 2) ? 2 : 0)};
     if (lane == 63) wave_sum[w] = in;
     __syncthreads();
-    PgScan base = {0, 0}, all = {0, 0};
+    PgScan base = {0, 0, 0}, all = {0, 0, 0};
 #pragma unroll
     for (int i = 0; i < PG_WG / 64; i++) {
         if (i < w) {
@@ -45,9 +37,10 @@ __device__ __forceinline__ PgScan pg_scan(PgScan v, PgScan *total, PgScan *wave_
         }
         all.tok += wave_sum[i].tok;
         all.blk += wave_sum[i].blk;
+        all.bad |= wave_sum[i].bad;
     }
     *total = all;
-    return {base.tok + in.tok - v.tok, base.blk + in.blk - v.blk};
+    return {base.tok + in.tok - v.tok, base.blk + in.blk - v.blk, 0};
 }
 
 // the last i in [0, n) with off[i] <= k (off ascending, off[0] = 0, k < off[n])
@@ -73,13 +66,13 @@ struct PgArgs {
 __device__ __forceinline__ int pg_blocks(int n, int shift) { return (int)(((unsigned)n + (1u << shift) - 1u) >> shift); }
 
 // What both kernels begin with.  ASSIGN: tok[i] and blk[i] become the tokens and
-// blocks of the sequences before i; otherwise blk[i] the blocks given back
+// blocks of the sequences before i, held[i] its length; otherwise blk[i] the blocks given back
 // before i.  Returns the status every workgroup agrees on.
 template <bool ASSIGN>
-__device__ __forceinline__ int pg_plan(const PgArgs &A, int *tok, int *blk, PgScan *wave_sum, int n_free, PgScan *total)
+__device__ __forceinline__ int pg_plan(const PgArgs &A, int *tok, int *blk, int *held, PgScan *wave_sum, int n_free, PgScan *total)
 {
     const int per = (A.n_seq + PG_WG - 1) / PG_WG, a = min(A.n_seq, (int)threadIdx.x * per), b = min(A.n_seq, a + per);
-    PgScan mine = {0, 0};
+    PgScan mine = {0, 0, 0};
     int bad = 0;
     for (int i = a; i < b; i++) {
         const int len = A.len[i], w = A.what[i];
@@ -97,15 +90,15 @@ __device__ __forceinline__ int pg_plan(const PgArgs &A, int *tok, int *blk, PgSc
             else if ((n = pg_blocks(len, A.shift)) > A.max_blocks) bad |= 2;
         }
         if (bad) n = t = 0;
-        if (ASSIGN) tok[i] = t;
+        if (ASSIGN) tok[i] = t, held[i] = len;
         blk[i] = n;
         mine.tok += t;
         mine.blk += n;
     }
-    const int any1 = __syncthreads_or(bad & 1), any2 = __syncthreads_or(bad & 2);
+    mine.bad = bad;
     PgScan at = pg_scan(mine, total, wave_sum);
-    if (any1 || total->tok > (ASSIGN ? A.T : 0)) return QMAG_KV_LENGTH;
-    if (any2) return QMAG_KV_ROW;
+    if ((total->bad & 1) || total->tok > (ASSIGN ? A.T : 0)) return QMAG_KV_LENGTH;
+    if (total->bad & 2) return QMAG_KV_ROW;
     if (n_free < 0 || n_free > A.n_block) return QMAG_KV_LIST;
     if (ASSIGN ? total->blk > n_free : total->blk > A.n_block - n_free) return ASSIGN ? QMAG_KV_FULL : QMAG_KV_LIST;
     for (int i = a; i < b; i++) {
@@ -128,16 +121,16 @@ __device__ __forceinline__ int pg_plan(const PgArgs &A, int *tok, int *blk, PgSc
 
 __global__ void __launch_bounds__(PG_WG) kv_assign_kernel(PgArgs A)
 {
-    __shared__ int tok[QMAG_KV_MAX_SEQ + 1], blk[QMAG_KV_MAX_SEQ + 1];
+    __shared__ int tok[QMAG_KV_MAX_SEQ + 1], blk[QMAG_KV_MAX_SEQ + 1], held[QMAG_KV_MAX_SEQ];
     __shared__ PgScan wave_sum[PG_WG / 64];
     const int n_free = *A.n_free;
     PgScan total;
-    const int st = pg_plan<true>(A, tok, blk, wave_sum, n_free, &total);
+    const int st = pg_plan<true>(A, tok, blk, held, wave_sum, n_free, &total);
     const int tid = threadIdx.x;
     if (blockIdx.x == 0) {
         for (int i = tid; i < A.n_seq; i += PG_WG) {
             A.cu[i] = st ? 0 : tok[i];
-            A.len_next[i] = A.len[i] + (st ? 0 : A.what[i]);
+            A.len_next[i] = held[i] + (st ? 0 : A.what[i]);
         }
         if (tid == 0) {
             A.cu[A.n_seq] = st ? 0 : tok[A.n_seq];
@@ -150,7 +143,7 @@ __global__ void __launch_bounds__(PG_WG) kv_assign_kernel(PgArgs A)
     if (!st)
         for (int k = (int)blockIdx.x * PG_WG + tid; k < total.blk; k += step) {
             const int i = pg_find(blk, A.n_seq, k);
-            const int64_t col = pg_blocks(A.len[i], A.shift) + k - blk[i];
+            const int64_t col = pg_blocks(held[i], A.shift) + k - blk[i];
             A.table[i * (int64_t)A.max_blocks + col] = A.free_list[n_free - 1 - k];
         }
     const bool vec = ((uintptr_t)A.slot | (uintptr_t)A.pos) % 16 == 0;
@@ -164,7 +157,7 @@ __global__ void __launch_bounds__(PG_WG) kv_assign_kernel(PgArgs A)
             ps[j] = 0;
             if (t0 + j >= n_tok) continue;
             while (tok[i + 1] <= t) i++;
-            const int len = A.len[i], had = pg_blocks(len, A.shift);
+            const int len = held[i], had = pg_blocks(len, A.shift);
             const int p = len + t - tok[i], col = p >> A.shift;
             const int id = col < had ? A.table[i * (int64_t)A.max_blocks + col]
                                      : A.free_list[n_free - 1 - (blk[i] + col - had)];
@@ -189,7 +182,7 @@ __global__ void __launch_bounds__(PG_WG) kv_release_kernel(PgArgs A)
     __shared__ PgScan wave_sum[PG_WG / 64];
     const int n_free = *A.n_free;
     PgScan total;
-    const int st = pg_plan<false>(A, nullptr, blk, wave_sum, n_free, &total);
+    const int st = pg_plan<false>(A, nullptr, blk, nullptr, wave_sum, n_free, &total);
     const int tid = threadIdx.x;
     if (blockIdx.x == 0) {
         for (int i = tid; i < A.n_seq; i += PG_WG) A.len_next[i] = !st && A.what[i] ? 0 : A.len[i];
