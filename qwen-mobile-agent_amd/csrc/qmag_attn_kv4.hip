@@ -124,6 +124,18 @@ __device__ __forceinline__ bool ak_find(const AkArgs &A, int want, bool by_token
     return false;
 }
 
+// The workgroup's kv head and item.  Items in order, all heads of each, so that
+// those that have no work are the last to start: with the heads one behind
+// another the idle ones between them left some CUs two busy workgroups and others
+// none (32 sequences in bf16 52.4 us so, 48.3 in order; one of 32,768 tokens 22.1
+// and 19.7).
+__device__ __forceinline__ void ak_item(const AkArgs &A, int *item, int *kvh)
+{
+    const unsigned i = blockIdx.x / (unsigned)A.n_kv;
+    *item = (int)i;
+    *kvh = (int)(blockIdx.x - i * (unsigned)A.n_kv);
+}
+
 // Where row r of a group of RG rows has its partial results: a row's parts one
 // behind another (16 KB apart, as the workgroups write them, they would all lie
 // in one memory channel: joining 256 of them took 14 us against 3).
@@ -270,7 +282,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
     __shared__ float join_m[NW][16], join_l[NW][16];
 
-    const int kvh = blockIdx.y, item = blockIdx.x;
+    int item, kvh;
+    ak_item(A, &item, &kvh);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, h = lane >> 4;
     AkPlan P;
     if (!ak_find<RG, STEP>(A, item, false, &P)) return;
@@ -632,7 +645,8 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
     __shared__ __attribute__((aligned(16))) _Float16 ik[2][IMG], iv[2][IMG];
     __shared__ __attribute__((aligned(16))) uint8_t isc[2][SC];    // scales of K, then of V: [32][NG] each
 
-    const int kvh = blockIdx.y, item = blockIdx.x;
+    int item, kvh;
+    ak_item(A, &item, &kvh);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), n = lane & 15, h = lane >> 4;
     AkPlan P;
     if (!ak_find<RG, STEP>(A, item, false, &P)) return;
@@ -1009,13 +1023,16 @@ static int ak_launch(AkArgs A, hipStream_t s)
     constexpr int NW = ROWS ? 8 : 4, RG = ROWS ? 16 * NW : 16, STEP = ROWS ? 32 : 32 * NW;
     // Row groups at most.  Chunks are cut for as many workgroups as the chip holds at
     // once: of more the last ones run alone, of fewer some CUs get two and others none.
+    // (Heads of 256 for 4 of a CU instead of the 2 that its LDS holds: 41.2 us against
+    // 37.2 for 131,072 tokens, 31.4 against 27.6 for four sequences of up to 8192.)
     const int64_t groups = (int64_t)A.T * A.G / RG + (A.T < A.n_seq ? A.T : A.n_seq);
-    const int64_t goal = (ROWS ? rows_resident<T, D>() : 4) * (int64_t)ctx().n_cu;
+    const int64_t goal = (ROWS ? rows_resident<T, D>() : D == 256 ? 2 : 4) * (int64_t)ctx().n_cu;
     A.target = (int)((goal + A.n_kv - 1) / A.n_kv);
     // enough row groups to fill the chip twice over: nothing is split
     A.min_chunk = ((int64_t)A.T * A.G / RG) * A.n_kv >= 2 * goal ? 0 : 128;
-    const int64_t items = groups + (A.min_chunk ? A.target : 0);
-    if (items >= 1 << 23) return fail(QMAG_ERR_ARG, "attn_kv4: %lld groups of rows", (long long)items);
+    const int64_t parts = (((int64_t)A.max_blocks << A.shift) + 127) / 128;       // of a sequence at most
+    const int64_t items = !A.min_chunk ? groups : groups * parts < groups + A.target ? groups * parts : groups + A.target;
+    if (items * A.n_kv >= 1 << 23) return fail(QMAG_ERR_ARG, "attn_kv4: %lld groups of rows", (long long)items);
     A.max_items = (int)items;
     if (A.min_chunk) {
         int st;
@@ -1024,14 +1041,14 @@ static int ak_launch(AkArgs A, hipStream_t s)
         if (st) return st;
         A.ml = A.part + rows * D;
     }
-    const dim3 grid((unsigned)items, (unsigned)A.n_kv);
+    const dim3 grid((unsigned)(items * A.n_kv));
     if constexpr (ROWS) attn_kv4_rows_kernel<T, D, NW><<<grid, 64 * NW, 0, s>>>(A);
     else attn_kv4_kernel<T, D, 2, NW><<<grid, 64 * NW, 0, s>>>(A);
     if (A.min_chunk) {
         const unsigned T_ = (unsigned)A.T, heads = (unsigned)(A.n_kv * A.G);
         if constexpr (ROWS)
             attn_kv4_join_kernel<T, D, RG, STEP, 1, D><<<dim3(T_, (heads + 3) / 4), 256, 0, s>>>(A);
-        else if ((int64_t)A.T * heads * (D / 64) <= ctx().n_cu)
+        else if ((int64_t)A.T * heads * (D / 64) <= ctx().n_cu && (parts < A.target ? parts : A.target) > 48)
             attn_kv4_join_kernel<T, D, RG, STEP, 16, 64><<<dim3(T_, heads, D / 64), 1024, 0, s>>>(A);
         else
             attn_kv4_join_kernel<T, D, RG, STEP, 4, D><<<dim3(T_, heads), 256, 0, s>>>(A);
@@ -1042,8 +1059,12 @@ static int ak_launch(AkArgs A, hipStream_t s)
 template <class T, int D>
 static int ak_pick(const AkArgs &A, hipStream_t s)
 {
-    // few rows to a sequence: the waves share them and split the tokens
-    if ((int64_t)A.T * A.G <= 64 * (int64_t)A.n_seq) return ak_launch<T, D, false>(A, s);
+    // Few rows to a sequence: the waves share them and split the tokens, and every 16
+    // rows read the cache again; of more the codes are formed once for 128.  With / without
+    // that, 256 rows: 25.9 / 22.4 us over 2000 tokens, 99 / 97 over 32,768 (bf16, 32 heads of
+    // 128), 37 / 21 and 89 / 80 (fp32, 16 heads of 256); 512 rows: 35 / 32, 175 / 182, 40 / 26
+    // and 137 / 138.
+    if ((int64_t)A.T * A.G <= 256 * (int64_t)A.n_seq) return ak_launch<T, D, false>(A, s);
     return ak_launch<T, D, true>(A, s);
 }
 

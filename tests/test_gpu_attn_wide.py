@@ -50,7 +50,7 @@ def error(got, want):
     return np.linalg.norm(got - want) / np.linalg.norm(want)
 
 
-@pytest.mark.parametrize("rows", [1, 60])
+@pytest.mark.parametrize("rows", [1, 60, 70])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("typ", TYPES)
 def test_attn_kv4_error(qm, typ, D, rows):
@@ -181,6 +181,18 @@ def test_attn_kv4_many_rows_do_not_see_later_tokens(qm, typ):
             assert not np.isfinite(got[n - 30:]).all()
 
 
+@pytest.mark.parametrize("D,layout", [(64, "odd"), (128, "packed"), (256, "gap")])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_kv4_many_rows(qm, typ, D, layout):
+    """Ragged lengths, more rows than tokens, sequences that ask nothing or have nothing."""
+    t = TYPES[typ]
+    r = rng_of(D, 31, 7)
+    lens, ask = [300, 40, 0, 500, 33, 64], [290, 60, 3, 129, 0, 64]
+    case = CacheCase(qm, r, lens, 2, D, 16)
+    q = to_type(r.randn(sum(ask) + 2, 8, D), t)
+    check_kv4(case, q, ask, t, run_kv4(qm, case, q, ask, t, layout))
+
+
 @pytest.mark.parametrize("typ", TYPES)
 @pytest.mark.parametrize("rows", [1, 80])
 def test_attn_kv4_bad_pages_anywhere(qm, typ, rows):
@@ -223,7 +235,7 @@ def test_scales(qm, typ, scale):
     r = rng_of(int(10 * abs(scale)), 6)
     D, H, KV, L = 64, 4, 2, 200
     case = CacheCase(qm, r, [L], KV, D, 16)
-    for rows in (1, 50):
+    for rows in (1, 50, 150):
         q = to_type(r.randn(rows, H, D), t)
         check_kv4(case, q, [rows], t, run_kv4(qm, case, q, [rows], t, scale=scale, pad=0), scale)
     q, k, v = (to_type(r.randn(L, n, D), t) for n in (H, KV, KV))
@@ -238,7 +250,7 @@ def test_a_row_of_nan_stays_alone(qm, typ):
     D, H, KV, L = 128, 8, 2, 180
     k, v = (r.randn(L, KV, D).astype(np.float32) for _ in range(2))
     case = CacheCase(qm, r, [L], KV, D, 16, [k], [v])
-    for rows in (3, 60, L):                        # the last: a prompt
+    for rows in (3, 60, 90, L):                      # the last: a prompt
         q = r.randn(rows, H, D)
         run = ((lambda x: run_prompt(qm, x, to_type(k, t), to_type(v, t), [L], t)) if rows == L else
                (lambda x: run_kv4(qm, case, x, [rows], t, pad=0)))
@@ -297,7 +309,7 @@ def test_cache_beyond_4_gib(qm):
     assert np.array_equal(ko.download(np.float32).reshape(k.shape), hk) and np.array_equal(vo.download(np.float32).reshape(v.shape), hv)
     table, len_d = ints(qm, pages), ints(qm, lens)
     t = qm.KvTable(2, 2, bs, n_block, table.ptr, None)
-    for ask in ([1, 1], [70, 40]):
+    for ask in ([1, 1], [70, 40], [300, 40]):
         n = sum(ask)
         q = r.randn(n, 16, D).astype(np.float32)
         qd, od = View(qm, q, F32), View(qm, np.zeros_like(q), F32)
