@@ -6,8 +6,10 @@
 //
 // Two launches.  The first lays K and V out in tiles of 32 keys of one sequence
 // and kv head, in the order the second's LDS wants them, rows behind a
-// sequence's end zero.  The second takes 128 queries of a head per workgroup,
-// 32 to a wave, and passes over the tiles once with a running maximum and sum.
+// sequence's end zero: split or converted once instead of by every head and
+// group of queries that reads them.  In the second a workgroup takes 64 or 128
+// queries of a head, 16 or 32 to a wave, and passes over the tiles once with a
+// running maximum and sum.  Calls of few tokens are one launch (DIRECT).
 //
 // 16-bit calls multiply in their own type.  fp32 calls are carried by the fp16
 // matrix cores, 16 times the fp32 ones' rate: every row of Q, K and V is scaled
@@ -15,9 +17,18 @@
 // bits, and a product is hi hi + hi lo + lo hi.
 //
 // S^T = K Q^T by v_mfma_f32_32x32x16 leaves a lane with one query (n = lane % 32)
-// and keys 8 (r / 4) + 4 (lane / 32) + r % 4 of a tile; O^T = V^T P^T takes the
+// and keys 8 (r / 4) + 4 (lane / 32) + r % 4 of a tile, by v_mfma_f32_16x16x32
+// (n = lane % 16) with keys 4 (lane / 16) + r of each 16; O^T = V^T P^T takes the
 // weights as they are when V's keys are read in that order, so they never leave
 // their lane.  V^T comes from row-major LDS by transposing reads.
+//
+// Bound by the matrix and vector units in turn: a tile of 32 x 32 scores of heads
+// of 128 is 512 cycles of products and about 500 of vector instructions, half of
+// them exponentials (a quarter rate), on a SIMD that three waves share.  Measured,
+// both launches: bf16, 8192 tokens in five prompts, 32 heads of 128 over 8: 371 us,
+// 826 TFLOP/s (a large bf16 product in the library: 1223); fp32, 4096 tokens, 16
+// heads of 256 over 2: 424 us, 324 TFLOP/s, or 972 of fp16 products (library: 1179;
+// its fp32 ones 153).  The first launch is 16 and 11 us of these.
 #include <type_traits>
 
 #include "qmag_attn.h"
@@ -593,9 +604,21 @@ template <class T, int D>
 static int ap_launch(const ApArgs &A, hipStream_t s)
 {
     constexpr bool F32 = sizeof(typename T::S) == 4;
+    // Few tokens: one launch, every workgroup lays its tiles out itself.  With / without:
+    // one token 8.6 / 11.7 us (fp32, 16 heads of 256) and 4.9 / 8.0 (bf16, 32 of 128), 64
+    // tokens 14.8 / 16.8 and 8.9 / 10.3, 128 tokens 27 / 22 and 12.1 / 11.3.  (The lengths
+    // are the device's: of several prompts none is taken to have all tokens.)
+    if (A.T <= (D == 64 ? 128 : D == 128 ? 96 : 64) * (A.n_seq > 1 ? 3 : 2) / 2)
+        return ap_run<T, D, D == 256 ? 8 : 4, 16, 1, 3, 2, true>(A, s);
+    // Few workgroups of 128 queries: 64 to a workgroup, which leaves twice as many.  With /
+    // without, at these counts of the large ones: fp32, heads of 256: 208 129 / 132 us, 256
+    // 196 / 162; of 128: 416 91 / 95, 512 133 / 128; of 64: 800 130 / 135, 960 175 / 176; 16
+    // bits, of 256: 384 119 / 129, 640 279 / 273; of 128: 640 88 / 91, 768 123 / 114; of 64:
+    // 960 81 / 88, 1600 184 / 181.
     const int64_t wgs = ((int64_t)A.T / 128 + A.n_seq) * A.n_kv * A.G;
-    if (A.T <= (D == 64 ? 128 : D == 128 ? 96 : 64) * (A.n_seq > 1 ? 3 : 2) / 2) return ap_run<T, D, D == 256 ? 8 : 4, 16, 1, 3, 2, true>(A, s);
-    if (wgs < (F32 && D == 256 ? 1 : 4) * (int64_t)ctx().n_cu) return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);
+    if (wgs < (int64_t)ctx().n_cu * (F32 ? 1024 / D : D == 64 ? 16 : 11) / 4)
+        return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);
+    // Where 32 queries to a wave need more registers than three waves to a SIMD have: 16, and 8 waves
     if constexpr (F32 || D == 256) return ap_run<T, D, 8, 16, D == 64 ? 2 : 1, F32 && D == 128 ? 2 : 3, F32 && D == 128 ? 4 : 2>(A, s);
     else return ap_run<T, D, 4, 32, D == 64 ? 2 : 1, 3, D == 64 ? 4 : 3>(A, s);
 }

@@ -8,11 +8,12 @@
 // exponent of 1024 (or, from the upper half of a byte, of 64) is that number plus
 // the code, and one subtraction for two values leaves it.  No code is rounded,
 // and no step or minimum touches the operand.  Three ways (Code):
-//   CENTRED  fp32 calls take code - 8, which keeps the two sums below small: with
-//            codes from 0 to 15 they were each tens of times the result, which
-//            cost a digit (1e-5 of the result against 1e-6);
-//   PLAIN    16-bit calls take the code: a digit they do not hold anyway, and the
-//            value of code 8 need not be formed;
+//   CENTRED  fp32 and fp16 calls take code - 8, which keeps the two sums below
+//            small: with codes from 0 to 15 they were each tens of times the
+//            result, which cost a digit (fp32: 1e-5 of the result against 1e-6;
+//            fp16: 3.6e-4 against 2.4e-4, of which its rounding is 2.0e-4);
+//   PLAIN    bf16 calls of many rows take the code: a digit they do not hold
+//            anyway, and the value of code 8 need not be formed;
 //   RAW      bf16 decode takes the nibble alone, an fp16 subnormal (code * 2^-24,
 //            or * 2^-20 in the upper half of a byte, made up for exactly): five
 //            instructions for eight codes instead of nine.  The matrix cores align
@@ -30,13 +31,14 @@
 // S^T comes out of v_mfma_f32_16x16x32_f16 with a lane holding one query row and
 // the tokens 4 h .. 4 h + 3 of each 16 (h = lane / 16), which is just what the
 // second product wants as its operand when V's tokens are taken in that order:
-// neither scores nor weights ever cross lanes, and the loop uses no LDS.
+// neither scores nor weights ever cross lanes.
 //
 // Rows are the queries of the heads that share a kv head.  The work is (kv head,
 // sequence, group of rows, chunk of the cache); every workgroup finds its own
 // from the lengths on the device.  The chunk is the same for all sequences, so
 // that a long one among short ones is spread over the chip; partial results of
-// split sequences are joined by a second launch.
+// split sequences are joined by a second launch.  Two kernels: up to 256 rows to a
+// sequence, and more (ak_pick).
 #include <type_traits>
 
 #include "qmag_attn.h"
@@ -267,6 +269,13 @@ constexpr int ak_tile() { return 36 * D; }
 // of 32 tokens in turn and join at the end.  Each wave keeps its next tiles in
 // flight from memory to its own part of LDS (NB tiles, no registers, no
 // barriers); a lane later reads back little more than what it asked for itself.
+//
+// A step of one sequence is bound by a chain of round trips: of 14 us for 32,768
+// tokens (fp32, 16 heads of 256; 18.9 MB, 4 us at a large copy's rate) 0.8 are the
+// plan, 1.2 the table and the first tiles' requests, 1.2 the queries, 3.3 the tiles,
+// 2 the join of the waves, the rest the launch.  A batch is bound by the vector
+// instructions that turn codes into operands and by memory together: 32 sequences
+// of up to 16,384 tokens (bf16, 32 heads of 128; 163 MB) 42 us, 3.9 TB/s.
 template <class T, int D, int NB, int NW>
 __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typename T::S) == 4 ? 3 : 4) attn_kv4_kernel(AkArgs A)
 {
@@ -628,6 +637,14 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 // fp16 codes once for all the waves (K and V row by row, in the order the
 // products read them), and then serves as a tile of a prompt does; memory is two
 // tiles ahead, the codes one, and a tile costs one barrier.
+//
+// Bound by what a tile costs a wave besides its 64 products (fp32, heads of 256:
+// 1024 cycles): about 400 vector instructions, a quarter of them for steps and
+// minima, and as many cycles of LDS reads, which 8 waves share.  512 rows of 8 heads
+// each at 12,001 tokens: 327 us with the join, 294 TFLOP/s, or 588 of fp16 products.
+// (With 4 waves of it 544 us against 349; 64 rows that formed their codes themselves
+// 457; a step's exponent found once for a tile 332 against 334, not kept.)
+
 // how many of its workgroups of 8 waves the registers let a CU hold
 template <class T, int D>
 constexpr int rows_resident() { return D == 256 || (D == 128 && sizeof(typename T::S) == 4) ? 1 : 2; }
@@ -945,7 +962,9 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
 // channels of a row, the waves the parts in turn.  Decode of a few rows has many
 // parts to a row (16 waves for 64 channels: a wave's parts are all requested at
 // once), of more rows fewer (four waves a row), many rows to a sequence a handful
-// (a wave for a row, four heads of a token to a workgroup).
+// (a wave for a row, four heads of a token to a workgroup).  4.9 us for 16 rows of 128
+// parts, of which 2 are the launch; with 4 waves a row 7.2.  Of 16 parts 4 waves are
+// 1.2 us faster than 16.
 template <class T, int D, int RG, int STEP, int NW, int CW>
 __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(AkArgs A)
 {

@@ -7,8 +7,9 @@
 // blocks) for itself in LDS and then writes its share of the tokens and of the
 // table: no workgroup waits for another, and a step is one launch.  The k-th
 // block taken in a call is free_list[n_free - 1 - k], so a token's slot does
-// not need the table entry another workgroup writes.  A few microseconds up to
-// some 10^5 tokens: the launch and the sums.
+// not need the table entry another workgroup writes.  Bound by the launch and the
+// chain lengths - sums - search - table: 48 sequences, one token each, 3.5 us given
+// back and 4.7 assigned; 509 sequences and 262,144 tokens 5.0 and 6.6.
 #include "qmag_attn.h"
 
 namespace qmag {

@@ -8,7 +8,8 @@
 //
 // A workgroup takes one token and some of its heads: the token's cosines and
 // sines go to LDS once, then each thread turns 16 bytes of pairs.  Memory
-// bound beyond a few hundred tokens; one token is a launch.
+// bound beyond a few hundred tokens: 4096 of 32 + 8 heads of 128 in bf16 15.1 us, 5.6
+// TB/s (84 MB, part of which stays in the caches); one token is a launch, 3.4 us.
 #include <math.h>
 
 #include "qmag_attn.h"
