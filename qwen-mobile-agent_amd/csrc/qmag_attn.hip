@@ -582,8 +582,9 @@ static int ap_run(ApArgs A, hipStream_t s)
     constexpr int NS = sizeof(typename T::S) == 4 ? 2 : 1;
     constexpr size_t TILE = 2 * NS * AP_KEYS * D * 2;
     A.tiles = A.T / AP_KEYS + A.n_seq;
+    const int filled = A.T < A.n_seq ? A.T : A.n_seq;      // sequences that can hold a token
     const size_t n = (size_t)A.tiles * A.n_kv + 8;         // a barrier's tiles may reach past the last one
-    const int64_t wgs = (((int64_t)A.T / (QW * NW) + A.n_seq + 7) / 8 * 8) * A.n_kv * A.G;
+    const int64_t wgs = (((int64_t)A.T / (QW * NW) + filled + 7) / 8 * 8) * A.n_kv * A.G;
     if (wgs > UINT32_MAX / (64 * NW)) return fail(QMAG_ERR_ARG, "attn_prompt: %lld workgroups", (long long)wgs);
     if constexpr (DIRECT) {
         attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE, true><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
@@ -595,7 +596,7 @@ static int ap_run(ApArgs A, hipStream_t s)
     A.img = ws;
     A.scale = (float *)(ws + n * TILE);
     A.flags = (int *)(A.scale + (NS == 2 ? n * 2 * AP_KEYS : 0));
-    prompt_tiles_kernel<T, D, QW><<<dim3((unsigned)A.tiles, (unsigned)A.n_kv, 2), AP_WG, 0, s>>>(A);
+    prompt_tiles_kernel<T, D, QW><<<dim3((unsigned)(A.T / AP_KEYS + filled), (unsigned)A.n_kv, 2), AP_WG, 0, s>>>(A);
     attn_prompt_kernel<T, D, NW, QW, KT, AHEAD, WE, false><<<dim3((unsigned)wgs), 64 * NW, 0, s>>>(A);
     return QMAG_OK;
 }
@@ -615,7 +616,7 @@ static int ap_launch(const ApArgs &A, hipStream_t s)
     // 196 / 162; of 128: 416 91 / 95, 512 133 / 128; of 64: 800 130 / 135, 960 175 / 176; 16
     // bits, of 256: 384 119 / 129, 640 279 / 273; of 128: 640 88 / 91, 768 123 / 114; of 64:
     // 960 81 / 88, 1600 184 / 181.
-    const int64_t wgs = ((int64_t)A.T / 128 + A.n_seq) * A.n_kv * A.G;
+    const int64_t wgs = ((int64_t)A.T / 128 + (A.T < A.n_seq ? A.T : A.n_seq)) * A.n_kv * A.G;
     if (wgs < (int64_t)ctx().n_cu * (F32 ? 1024 / D : D == 64 ? 16 : 11) / 4)
         return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);
     // Where 32 queries to a wave need more registers than three waves to a SIMD have: 16, and 8 waves

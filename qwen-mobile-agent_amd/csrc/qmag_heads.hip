@@ -34,8 +34,9 @@ int check_heads(const char *what, const qmag_heads *h, int type, int dim, int64_
     if (h->n_head == 0 || n_tok == 0) return QMAG_OK;
     if (!h->ptr) return fail(QMAG_ERR_ARG, "%s: null pointer", what);
     if ((uintptr_t)h->ptr % (unsigned)size) return fail(QMAG_ERR_ARG, "%s: not aligned to its values", what);
-    // 2^40 values: no product of these with a token or head number leaves 64 bits
-    if (h->token_stride < 0 || h->head_stride < 0 || h->token_stride > (int64_t)1 << 40 || h->head_stride > (int64_t)1 << 40)
+    // 2^59 values at most: no place, in bytes either, leaves 64 bits
+    const int64_t most = (int64_t)1 << 58;
+    if (h->token_stride < 0 || h->head_stride < 0 || h->token_stride > most / n_tok || h->head_stride > most / h->n_head)
         return fail(QMAG_ERR_ARG, "%s: strides %lld, %lld", what, (long long)h->token_stride, (long long)h->head_stride);
     if (!written) return QMAG_OK;
     const int64_t ts = h->token_stride, hs = h->head_stride;

@@ -43,6 +43,7 @@ def rope_call(qm, **k):
     dict(theta=float("nan")), dict(theta=float("inf")),
     dict(src=((None, 4, 512, 128),)), dict(src=((A + 2, 4, 512, 128),)), dict(src=((A, -1, 512, 128),)),
     dict(src=((A, 5000, 512, 128),)), dict(src=((A, 4, -512, 128),)),
+    dict(src=((A, 4, 1 << 40, 128),), T=2 ** 31 - 1), dict(src=((A, 4, 128, 1 << 57),)),   # places beyond 64 bits
     dict(src=((A, 4, 512, 64),)),                                             # heads on one another, written
     dict(src=((A, 4, 500, 128),)),                                            # tokens on one another
     dict(src=((A, 4, 512, 128),), dst=((A + 4, 4, 512, 128),)),               # over its source, shifted

@@ -161,6 +161,18 @@ def test_attn_prompt_large_bad_lengths(qm, cu):
         assert out.read()[1]
 
 
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n_seq,T,D", [(700, 40, 64), (4096, 300, 128)])
+def test_attn_prompt_mostly_empty(qm, typ, n_seq, T, D):
+    """Far more prompts than tokens: all but a few are empty."""
+    t = TYPES[typ]
+    r = rng_of(n_seq, T)
+    lens = np.zeros(n_seq, int)
+    lens[r.choice(n_seq, 7, replace=False)] = np.diff(np.concatenate([[0], np.sort(r.choice(np.arange(1, T), 6, replace=False)), [T]]))
+    q, k, v = (to_type(r.randn(T, n, D), t) for n in (4, 2, 2))
+    check_prompt(q, k, v, lens, t, run_prompt(qm, q, k, v, lens, t))
+
+
 # ------------------------------------------------------- the cache, many rows --
 
 @pytest.mark.parametrize("typ", TYPES)
