@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 // Bound by what a tile costs a wave besides its 64 products (fp32, heads of 256:
 // 1024 cycles): about 400 vector instructions, a quarter of them for steps and
 // minima, and as many cycles of LDS reads, which 8 waves share.  512 rows of 8 heads
-// each at 12,001 tokens: 327 us with the join, 294 TFLOP/s, or 588 of fp16 products.
+// each at 12,001 tokens: 316 us with the join, 312 TFLOP/s, or 623 of fp16 products.
 // (With 4 waves of it 544 us against 349; 64 rows that formed their codes themselves
 // 457; a step's exponent found once for a tile 332 against 334, not kept.)
 
@@ -893,6 +893,10 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
             l += p[i];
         }
 
+        // the next tile's codes, between the two products: its LDS reads and vector work run while
+        // the other waves multiply (ahead of the scores 334 us, behind the output 323, here 316)
+        if (t0 + STEP < all) unpack(b ^ 1);
+
         // ---- output
 #pragma unroll
         for (int g = 0; g < NG; g++) {
@@ -928,8 +932,8 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
         const uint32_t bad = (gone >> 2) & 3;
         if (t0 + 2 * STEP < all) issue(t0 + 2 * STEP, b);
         else gone >>= 2;
-        if (t0 + STEP < all) unpack(b ^ 1);
         if (t0 < mine) compute(t0, b, bad);
+        else if (t0 + STEP < all) unpack(b ^ 1);
     }
 
     if (!live) return;
