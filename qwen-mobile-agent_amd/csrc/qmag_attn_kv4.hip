@@ -275,7 +275,7 @@ constexpr int ak_tile() { return 36 * D; }
 // plan, 1.2 the table and the first tiles' requests, 1.2 the queries, 3.3 the tiles,
 // 2 the join of the waves, the rest the launch.  A batch is bound by the vector
 // instructions that turn codes into operands and by memory together: 32 sequences
-// of up to 16,384 tokens (bf16, 32 heads of 128; 163 MB) 42 us, 3.9 TB/s.
+// of up to 16,384 tokens (bf16, 32 heads of 128; 163 MB) 41 us, 4.0 TB/s.
 template <class T, int D, int NB, int NW>
 __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typename T::S) == 4 ? 3 : 4) attn_kv4_kernel(AkArgs A)
 {
@@ -1047,9 +1047,10 @@ static int ak_launch(AkArgs A, hipStream_t s)
     // Row groups at most.  Chunks are cut for as many workgroups as the chip holds at
     // once: of more the last ones run alone, of fewer some CUs get two and others none.
     // (Heads of 256 for 4 of a CU instead of the 2 that its LDS holds: 41.2 us against
-    // 37.2 for 131,072 tokens, 31.4 against 27.6 for four sequences of up to 8192.)
+    // 37.2 for 131,072 tokens, 31.4 against 27.6 for four sequences of up to 8192; of 128
+    // for 4 instead of 3: 48.5 against 47.5 for 32 sequences, 35.4 against 34.8 for 8.)
     const int64_t groups = (int64_t)A.T * A.G / RG + (A.T < A.n_seq ? A.T : A.n_seq);
-    const int64_t goal = (ROWS ? rows_resident<T, D>() : D == 256 ? 2 : 4) * (int64_t)ctx().n_cu;
+    const int64_t goal = (ROWS ? rows_resident<T, D>() : D == 256 ? 2 : 3) * (int64_t)ctx().n_cu;
     A.target = (int)((goal + A.n_kv - 1) / A.n_kv);
     // enough row groups to fill the chip twice over: nothing is split
     A.min_chunk = ((int64_t)A.T * A.G / RG) * A.n_kv >= 2 * goal ? 0 : 128;
