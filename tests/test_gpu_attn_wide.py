@@ -115,11 +115,13 @@ def test_attn_prompt_large(qm, typ, D, layout):
                 close(values(got[s, a:a + 1], t), want, prompt_tol(t, D, n, want, mag, es), (n, a))
 
 
+@pytest.mark.parametrize("few", [False, True])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("typ", TYPES)
-def test_attn_prompt_large_is_not_reached_by_what_it_does_not_see(qm, typ, D):
+def test_attn_prompt_large_is_not_reached_by_what_it_does_not_see(qm, typ, D, few):
+    """With many query heads, and with so few that a workgroup takes fewer queries."""
     t = TYPES[typ]
-    H, KV, lens, T, at = many(t, D), 4, [150, 0, 40, 140, 1], 335, 70
+    H, KV, lens, T, at = 4 if few else many(t, D), 4, [150, 0, 40, 140, 1], 335, 70
     r = rng_of(D, 41)
     q, k, v = r.randn(T, H, D), kv_values(r, (T, KV, D)), r.randn(T, KV, D)
     want = values(run_prompt(qm, *(to_type(x, t) for x in (q, k, v)), lens, t), t)
@@ -135,11 +137,12 @@ def test_attn_prompt_large_is_not_reached_by_what_it_does_not_see(qm, typ, D):
             assert not np.isfinite(got[seen]).all()
 
 
+@pytest.mark.parametrize("n,H", [(130, 600), (300, 2)])
 @pytest.mark.parametrize("typ", TYPES)
-def test_attn_prompt_large_infinite_values(qm, typ):
+def test_attn_prompt_large_infinite_values(qm, typ, n, H):
     """V's infinities keep their sign."""
     t = TYPES[typ]
-    n, H, KV, D = 130, 600, 1, 64
+    KV, D = 1, 64
     r = rng_of(9, 9)
     q, k, v = 0.1 * r.randn(n, H, D), 0.1 * r.randn(n, KV, D), r.randn(n, KV, D)
     v[65, 0, 2], v[100, 0, 2], v[70, 0, 63] = -np.inf, np.inf, np.inf
