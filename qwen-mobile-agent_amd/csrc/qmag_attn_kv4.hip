@@ -266,8 +266,8 @@ template <int D>
 constexpr int ak_tile() { return 36 * D; }
 
 // A group of 16 rows against a chunk of the cache: the NW waves take its tiles
-// of 32 tokens in turn and join at the end.  Each wave keeps its next tiles in
-// flight from memory to its own part of LDS (NB tiles, no registers, no
+// of 32 tokens in turn and join at the end.  Each wave keeps its next tile in
+// flight from memory to its own part of LDS (two tiles, no registers, no
 // barriers); a lane later reads back little more than what it asked for itself.
 //
 // A step of one sequence is bound by a chain of round trips: of 14 us for 32,768
@@ -276,7 +276,7 @@ constexpr int ak_tile() { return 36 * D; }
 // 2 the join of the waves, the rest the launch.  A batch is bound by the vector
 // instructions that turn codes into operands and by memory together: 32 sequences
 // of up to 16,384 tokens (bf16, 32 heads of 128; 163 MB) 41 us, 4.0 TB/s.
-template <class T, int D, int NB, int NW>
+template <class T, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typename T::S) == 4 ? 3 : 4) attn_kv4_kernel(AkArgs A)
 {
     using S = typename T::S;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
     constexpr int VD = (D + 127) / 128;            // dwords of a lane's V codes of a token
     constexpr int TILE = ak_tile<D>();
     constexpr int LROW = D + 4;                    // row of the join
-    constexpr int LDS = NW * NB * TILE > NW * 16 * LROW * 4 ? NW * NB * TILE : NW * 16 * LROW * 4;
+    constexpr int LDS = NW * 2 * TILE > NW * 16 * LROW * 4 ? NW * 2 * TILE : NW * 16 * LROW * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
     __shared__ float join_m[NW][16], join_l[NW][16];
 
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
     const int64_t block_stride = 2 * A.half * A.n_kv;
     const uint8_t *head = A.data + kvh * 2 * A.half;
     const int64_t codes = (int64_t)(D / 2) << A.shift;
-    uint8_t *ring = lds + wave * NB * TILE;
+    uint8_t *ring = lds + wave * 2 * TILE;
 
     // ---- tiles from memory: where in a half (16 tokens, within a block) a lane's pieces lie
     int k_from, v_from, s_from;
@@ -333,7 +333,6 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
         s_up = c >= 4 * NG;
         s_from = (w ? (int)A.half : 0) + (int)codes + (c % (4 * NG)) * 16;
     }
-    constexpr int LOADS = (D == 256 ? 8 : D == 128 ? 4 : 2) + 1;
     uint32_t gone = 0;                             // two bits a tile in flight: a half whose block is none
     auto dma = [&](const uint8_t *from, uint8_t *to) {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
@@ -352,7 +351,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
             kb[a] = head + (there ? id : 0) * block_stride;
             off[a] = t & ((1 << A.shift) - 1);
         }
-        gone = (gone >> 2) | (bad << (2 * (NB - 1)));
+        gone = (gone >> 2) | (bad << 2);
         uint8_t *to = ring + slot * TILE;
         const uint8_t *k[2] = {kb[0] + off[0] * (D / 2), kb[1] + off[1] * (D / 2)};
         if constexpr (D == 64) {
@@ -376,10 +375,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 #pragma unroll
             for (int s = 0; s < 2; s++) load8<T>(qp + g * 64 + s * 32 + h * 8, A.q_vec, x[g][s]);
     }
-#pragma unroll
-    for (int i = 0; i < NB - 1; i++)
-        if (c0 + i * STEP < c1) issue(c0 + i * STEP, i);
-        else gone >>= 2;
+    if (c0 < c1) issue(c0, 0);
 
     const Nibbles N;
     // ---- queries
@@ -427,14 +423,13 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 
     int slot = 0;
     for (int t0 = c0; t0 < c1; t0 += STEP) {
-        // this tile's pieces are in once no more than the next ones' are under way
-        if (NB > 2 && t0 + STEP < c1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * LOADS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (t0 + (NB - 1) * STEP < c1) issue(t0 + (NB - 1) * STEP, slot == 0 ? NB - 1 : slot - 1);
+        // this tile's pieces are in; the next ones' go out
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (t0 + STEP < c1) issue(t0 + STEP, slot ^ 1);
         else gone >>= 2;
         const uint32_t bad = gone & 3;
         const uint8_t *tile = ring + slot * TILE;
-        slot = slot + 1 == NB ? 0 : slot + 1;
+        slot ^= 1;
 
         // ---- scores
         float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -1067,7 +1062,7 @@ static int ak_launch(AkArgs A, hipStream_t s)
     }
     const dim3 grid((unsigned)(items * A.n_kv));
     if constexpr (ROWS) attn_kv4_rows_kernel<T, D, NW><<<grid, 64 * NW, 0, s>>>(A);
-    else attn_kv4_kernel<T, D, 2, NW><<<grid, 64 * NW, 0, s>>>(A);
+    else attn_kv4_kernel<T, D, NW><<<grid, 64 * NW, 0, s>>>(A);
     if (A.min_chunk) {
         const unsigned T_ = (unsigned)A.T, heads = (unsigned)(A.n_kv * A.G);
         if constexpr (ROWS)
