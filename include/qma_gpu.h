@@ -599,7 +599,9 @@ int qmag_kv4_read_dev(const qmag_kv4 *c, const int *slot, int T, float *k, float
    len[i] - n + j and sees the tokens up to itself.  T: rows of q and out; heads
    of q share kv heads in runs of q->n_head / n_kv.  A row that sees nothing is
    zero, and so a row ahead of its sequence; rows behind cu[n_seq] are left as
-   they were.  A table entry outside the cache stands for tokens that are not
+   they were.  cu ascends within 0 .. T and a length is at most the table row's
+   max_blocks * block_size: of others the results are not defined (some rows may
+   be left as they were), and nothing but rows of out is written.  A table entry outside the cache stands for tokens that are not
    there.  What the cache holds where a row does not see has no effect on it.
    t->n_block and block_size are the cache's; max_blocks * block_size <= 2^30.
    Sequences are split over the chip by their lengths and joined in a fixed

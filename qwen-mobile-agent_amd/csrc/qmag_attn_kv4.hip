@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "qmag_attn.h"
+#include "qmag_attn_plan.h"
 
 namespace qmag {
 
@@ -68,36 +69,28 @@ struct AkPlan {
 
 __device__ __forceinline__ void ak_seq(const AkArgs &A, int i, int *q0, int *nq, int *len)
 {
-    const int a = min(max(A.cu[i], 0), A.T), b = min(max(A.cu[i + 1], 0), A.T);
-    *q0 = a;
-    *nq = max(b - a, 0);
-    *len = min(max(A.len[i], 0), A.max_blocks << A.shift);
-}
-
-__device__ __forceinline__ int ak_groups(const AkArgs &A, int nq, int RG)
-{
-    return (int)(((int64_t)nq * A.G + RG - 1) / RG);
+    *q0 = ak_row(A.cu[i], A.T);
+    *nq = max(ak_row(A.cu[i + 1], A.T) - *q0, 0);
+    *len = ak_len(A.len[i], A.max_blocks, A.shift);
 }
 
 // The sequence of item `want` (by_token: of row `want` of q), found by the
-// calling wave alone.  False if there is none.  (The caps only meet lengths that
-// are none, and keep their sums in range; the host refuses 2^23 groups.)
+// calling wave alone.  False if there is none, or none that has room.
 template <int RG, int STEP>
 __device__ __forceinline__ bool ak_find(const AkArgs &A, int want, bool by_token, AkPlan *P)
 {
     const int lane = lane_id();
     int q0 = 0, nq = 0, len = 0;
     if (lane < A.n_seq) ak_seq(A, lane, &q0, &nq, &len);
-    P->chunk = 1 << 30;                            // no sequence is longer
+    P->chunk = AK_UNSPLIT;
     if (A.min_chunk) {
-        float cost = (float)ak_groups(A, nq, RG) * (float)len;       // the same for whoever forms it
+        float cost = ak_cost(ak_groups(nq, A.G, RG), len);       // the same for whoever forms it
         for (int i = 64 + lane; i < A.n_seq; i += 64) {
             int x, n, l;
             ak_seq(A, i, &x, &n, &l);
-            cost += (float)ak_groups(A, n, RG) * (float)l;
+            cost += ak_cost(ak_groups(n, A.G, RG), l);
         }
-        const float c = fminf(group_sum<64>(cost) / (float)A.target, 1073741824.0f);
-        P->chunk = __builtin_amdgcn_readfirstlane(max((int)c / STEP * STEP + STEP, A.min_chunk));
+        P->chunk = __builtin_amdgcn_readfirstlane(ak_chunk(group_sum<64>(cost), A.target, STEP, A.min_chunk));
     }
     int items = 0;
     for (int base = 0; base < A.n_seq; base += 64) {
@@ -105,8 +98,7 @@ __device__ __forceinline__ bool ak_find(const AkArgs &A, int want, bool by_token
             q0 = nq = len = 0;
             if (base + lane < A.n_seq) ak_seq(A, base + lane, &q0, &nq, &len);
         }
-        const int split = max(1, (int)(((unsigned)len + (unsigned)P->chunk - 1u) / (unsigned)P->chunk));
-        const int mine = (int)min((long long)ak_groups(A, nq, RG) * split, 1ll << 23);
+        const int split = ak_split(len, P->chunk), mine = ak_items(ak_groups(nq, A.G, RG), split);
         const int incl = wave_scan(mine);
         const bool here = by_token ? want >= q0 && want < q0 + nq : want < items + incl;
         const unsigned long long hit = __ballot(here);
@@ -118,8 +110,7 @@ __device__ __forceinline__ bool ak_find(const AkArgs &A, int want, bool by_token
             P->len = __builtin_amdgcn_readlane(len, at);
             P->n_split = __builtin_amdgcn_readlane(split, at);
             P->item0 = items + __builtin_amdgcn_readlane(incl - mine, at);
-            // lengths that overlap make more items than there are workgroups
-            return !by_token || items + __builtin_amdgcn_readlane(incl, at) <= A.max_items;
+            return ak_room(P->item0, __builtin_amdgcn_readlane(mine, at), A.max_items);
         }
         items = min(items + __builtin_amdgcn_readlane(incl, 63), 1 << 30);
     }
@@ -143,7 +134,7 @@ __device__ __forceinline__ void ak_item(const AkArgs &A, int *item, int *kvh)
 // in one memory channel: joining 256 of them took 14 us against 3).
 __device__ __forceinline__ int64_t ak_part(const AkArgs &A, const AkPlan &P, int kvh, int group, int RG, int r)
 {
-    return ((int64_t)kvh * A.max_items + P.item0 + (int64_t)group * P.n_split) * RG + (int64_t)r * P.n_split;
+    return ak_part_row(kvh, A.max_items, P.item0, group, P.n_split, RG, r);
 }
 
 // max and sum over the four lanes that hold a row
@@ -1044,13 +1035,13 @@ static int ak_launch(AkArgs A, hipStream_t s)
     // (Heads of 256 for 4 of a CU instead of the 2 that its LDS holds: 41.2 us against
     // 37.2 for 131,072 tokens, 31.4 against 27.6 for four sequences of up to 8192; of 128
     // for 4 instead of 3: 48.5 against 47.5 for 32 sequences, 35.4 against 34.8 for 8.)
-    const int64_t groups = (int64_t)A.T * A.G / RG + (A.T < A.n_seq ? A.T : A.n_seq);
+    const int64_t groups = ak_most_groups(A.T, A.G, RG, A.n_seq);
     const int64_t goal = (ROWS ? rows_resident<T, D>() : D == 256 ? 2 : 3) * (int64_t)ctx().n_cu;
     A.target = (int)((goal + A.n_kv - 1) / A.n_kv);
     // enough row groups to fill the chip twice over: nothing is split
     A.min_chunk = ((int64_t)A.T * A.G / RG) * A.n_kv >= 2 * goal ? 0 : 128;
     const int64_t parts = (((int64_t)A.max_blocks << A.shift) + 127) / 128;       // of a sequence at most
-    const int64_t items = !A.min_chunk ? groups : groups * parts < groups + A.target ? groups * parts : groups + A.target;
+    const int64_t items = A.min_chunk ? ak_most_items(groups, A.target, parts) : groups;
     if (items * A.n_kv >= 1 << 23) return fail(QMAG_ERR_ARG, "attn_kv4: %lld groups of rows", (long long)items);
     A.max_items = (int)items;
     if (A.min_chunk) {

@@ -1,0 +1,127 @@
+"""CPU check of how attention over the cache is cut into workgroups: the plan's
+arithmetic (qmag_attn_plan.h) is compiled for the host and walked through for every
+item that runs.  All partial results lie in what the host allots, no two in one
+place, whatever the lengths; and ascending lengths get all their items."""
+import os
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+WALK = r"""
+#include <stdio.h>
+#include <vector>
+#include "qmag_attn_plan.h"
+using namespace qmag;
+
+// stdin: calls of RG STEP n_kv G T target min_chunk max_blocks shift n_seq, then cu and len
+int main()
+{
+    int RG, step, n_kv, G, T, target, min_chunk, max_blocks, shift, n;
+    for (int call = 0; scanf("%d%d%d%d%d%d%d%d%d%d", &RG, &step, &n_kv, &G, &T, &target, &min_chunk, &max_blocks, &shift, &n) == 10; call++) {
+        std::vector<int> cu(n + 1), len(n);
+        for (int &v : cu) if (scanf("%d", &v) != 1) return 1;
+        for (int &v : len) if (scanf("%d", &v) != 1) return 1;
+        const int64_t groups = ak_most_groups(T, G, RG, n), parts = (((int64_t)max_blocks << shift) + 127) / 128;
+        const int64_t most = min_chunk ? ak_most_items(groups, target, parts) : groups, rows = n_kv * most * RG;
+        bool ascending = cu[0] >= 0 && cu[n] <= T;
+        for (int i = 0; i < n; i++) ascending = ascending && cu[i] <= cu[i + 1];
+        // the kernels form this sum by lanes, sequences 64 apart, then over the lanes
+        float cost = 0, lane[64] = {};
+        for (int i = 0; i < n; i++) {
+            const int nq = ak_row(cu[i + 1], T) - ak_row(cu[i], T);
+            lane[i % 64] += ak_cost(ak_groups(nq > 0 ? nq : 0, G, RG), ak_len(len[i], max_blocks, shift));
+        }
+        for (float v : lane) cost += v;
+        const int chunk = min_chunk ? ak_chunk(cost, target, step, min_chunk) : AK_UNSPLIT;
+        std::vector<bool> taken(rows);
+        int64_t items = 0, bad = 0;
+        for (int i = 0; i < n; i++) {
+            const int q0 = ak_row(cu[i], T), q1 = ak_row(cu[i + 1], T), nq = q1 > q0 ? q1 - q0 : 0;
+            const int L = ak_len(len[i], max_blocks, shift), g = ak_groups(nq, G, RG), split = ak_split(L, chunk), mine = ak_items(g, split);
+            if (ascending && !ak_room((int)items, mine, (int)most) && !bad++)
+                printf("call %d: sequence %d of ascending lengths has no room, items %ld + %d of %ld\n", call, i, (long)items, mine, (long)most);
+            for (int it = 0; it < mine && items + it < most && ak_room((int)items, mine, (int)most); it++)
+                for (int k = 0; k < n_kv; k++)
+                    for (int r = 0; r < RG && (it / split) * (int64_t)RG + r < (int64_t)nq * G; r++) {
+                        const int64_t at = ak_part_row(k, (int)most, (int)items, it / split, split, RG, r) + it % split;
+                        if (split == 1) continue;          // written to the output
+                        if ((at < 0 || at >= rows || taken[at]) && !bad++)
+                            printf("call %d: sequence %d (item %ld, %d parts) row %d at %ld of %ld%s\n", call, i, (long)items + it, split, r,
+                                   (long)at, (long)rows, at >= 0 && at < rows ? ", taken" : "");
+                        if (at >= 0 && at < rows) taken[at] = true;
+                    }
+            items += mine;
+            if (items > 1 << 30) items = 1 << 30;
+        }
+        if (bad) return 1;
+    }
+    puts("all in place");
+    return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def walk(tmp_path_factory):
+    cxx = shutil.which("g++")
+    if not cxx:
+        pytest.skip("no host compiler")
+    d = tmp_path_factory.mktemp("plan")
+    src, exe = d / "walk.cpp", d / "walk"
+    src.write_text(WALK)
+    subprocess.run([cxx, "-std=c++17", "-O2", "-Wall", "-Werror", "-I", os.path.join(ROOT, "qwen-mobile-agent_amd", "csrc"),
+                    str(src), "-o", str(exe)], check=True)
+
+    def run(calls):
+        text = "\n".join(" ".join(str(int(v)) for v in [*c[0], len(c[2]), *c[1], *c[2]]) for c in calls)
+        r = subprocess.run([str(exe)], input=text, capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0 and "all in place" in r.stdout, r.stdout
+    return run
+
+
+def call(cu, lens, T, n_kv=1, G=1, rg=16, goal=512, blocks=1 << 16, shift=4, min_chunk=128):
+    return (rg, 128 if rg == 16 else 32, n_kv, G, T, -(-goal // n_kv), min_chunk, blocks, shift), cu, lens
+
+
+def test_lengths_that_lap_over(walk):
+    """cu up and down over sequences, the last of many long: its parts once lay 7 MB behind the end."""
+    n = 1031
+    cu = [16 * (i % 2) for i in range(n + 1)]
+    lens = [1] * n
+    lens[2 * 514] = 1 << 20
+    walk([call(cu, lens, 16)])
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_any_lengths(walk, seed):
+    r = np.random.RandomState(seed)
+    calls = []
+    for _ in range(60):
+        n, T, n_kv = int(r.choice([1, 2, 5, 64, 65, 130, 700])), int(r.choice([1, 3, 16, 100, 900])), int(r.choice([1, 2, 8]))
+        blocks, shift = int(r.choice([1, 7, 100, 3000])), int(r.choice([4, 6]))
+        cu = r.randint(-3, T + 4, n + 1) if r.rand() < 0.7 else r.choice([0, T, -2 ** 31, 2 ** 31 - 1, T // 2], n + 1)
+        lens = np.where(r.rand(n) < 0.2, r.choice([0, 2 ** 31 - 1, -2 ** 31, blocks << shift], n), r.randint(0, (blocks << shift) + 9, n))
+        calls.append(call(cu, lens, T, n_kv, int(r.choice([1, 3, 8])), int(r.choice([16, 128])), int(r.choice([256, 512, 768])),
+                          blocks, shift, int(r.choice([128, 128, 128, 0]))))
+    walk(calls)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_ascending_lengths_have_room(walk, seed):
+    """Every sequence of a call that is one gets all its items, at the largest lengths too."""
+    r = np.random.RandomState(100 + seed)
+    calls = []
+    for _ in range(60):
+        n, T, n_kv = int(r.choice([1, 2, 33, 64, 200, 1000])), int(r.choice([1, 3, 16, 100, 900])), int(r.choice([1, 2, 4]))
+        blocks, shift = int(r.choice([1, 7, 100, 3000, 1 << 22])), int(r.choice([4, 8]))
+        cu = np.sort(r.randint(0, T + 1, n + 1))
+        cap = blocks << shift
+        lens = r.choice([np.full(n, cap), r.randint(0, cap + 1, n), np.where(np.arange(n) == n // 2, cap, min(cap, 5)),
+                         np.exp(r.uniform(0, np.log(cap + 1), n)).astype(np.int64).clip(0, cap)][r.randint(4)], n)
+        calls.append(call(cu, lens, T, n_kv, int(r.choice([1, 3, 8])), int(r.choice([16, 128])), int(r.choice([256, 512, 768])),
+                          blocks, shift, int(r.choice([128, 128, 0]))))
+    walk(calls)
