@@ -498,7 +498,8 @@ int qmag_sampler_sample_dev(int n_vocab, const float *logits, qmag_sampler *s, i
    engine's attention layer, which lies beside its gate: {d_q, N_HEAD,
    2 * N_HEAD * N_EMBD_HEAD, 2 * N_EMBD_HEAD}.  Any strides; ptr and strides of
    whole 16 bytes are the fast form.  Views that are written hold each value
-   once and overlap no view that is read, except where said. */
+   once and overlap nothing else that a call reads or writes (its integers and the
+   cache among them), except where said. */
 #define QMAG_MAX_HEADS 4096
 typedef struct qmag_heads {
     void *ptr;
@@ -547,8 +548,8 @@ typedef struct qmag_kv_table {
 /* Blocks of ended sequences go back: for each i with ended[i] != 0, in
    ascending order, table[i]'s ceil(len[i] / block_size) blocks are appended to
    the free list and len_next[i] = 0; other lengths are copied.  What is written
-   (len_next, n_free_next, status) overlaps neither the inputs nor itself (a step
-   may then be issued again).  With
+   (len_next, n_free_next, status, the free list) overlaps neither the inputs, the
+   table among them, nor itself (a step may then be issued again).  With
    a status other than 0 nothing is given back, len_next = len and
    *n_free_next = *n_free. */
 int qmag_kv_release_dev(const qmag_kv_table *t, const int *len, const int *ended, const int *n_free, int *len_next,
@@ -561,8 +562,9 @@ int qmag_kv_release_dev(const qmag_kv_table *t, const int *len, const int *ended
    goes to slot[t] = block * block_size + place in the block.  slot and pos have T
    entries; those behind the last token get slot -1 and pos 0.  len_next[i] =
    len[i] + n_new[i].  With a status other than 0 no block is taken, every slot
-   is -1, cu is 0, and len_next = len, *n_free_next = *n_free.  What is written
-   overlaps neither the inputs nor itself. */
+   is -1, cu is 0, and len_next = len, *n_free_next = *n_free.  What is written,
+   the table among it, overlaps neither the inputs, the free list among them, nor
+   itself. */
 int qmag_kv_assign_dev(const qmag_kv_table *t, const int *len, const int *n_new, const int *n_free, int T, int *slot,
                        int *pos, int *cu, int *len_next, int *n_free_next, int *status);
 
@@ -587,10 +589,10 @@ typedef struct qmag_kv4 {
 int qmag_kv4_block_bytes(const qmag_kv4 *c, size_t *bytes);
 /* K and V of T tokens (n_kv heads each) into their slots; a token whose slot is
    outside the cache (-1: a padded one) is left out.  A slot named twice holds
-   one of the tokens, or parts of both. */
+   one of the tokens, or parts of both.  k, v and slot lie outside the cache. */
 int qmag_kv4_append_dev(const qmag_kv4 *c, int type, const qmag_heads *k, const qmag_heads *v, const int *slot, int T);
 /* The values the cache holds for T slots, f32 [T][n_kv][head_dim] each; zeros
-   for a slot outside it. */
+   for a slot outside it.  k and v overlap neither one another nor what is read. */
 int qmag_kv4_read_dev(const qmag_kv4 *c, const int *slot, int T, float *k, float *v);
 
 /* Attention of the newest tokens over the cache (attn_worker over its 4-bit

@@ -139,6 +139,8 @@ int check_heads(const char *what, const qmag_heads *h, int type, int dim, int64_
 // whether the two may share a byte: false when their ranges are apart, or when
 // they lie side by side within the tokens, or the heads, of one buffer
 bool heads_overlap(const qmag_heads *a, const qmag_heads *b, int size, int dim, int64_t n_tok);
+// whether any of h's values lies in the `bytes` bytes from p
+bool heads_meet(const qmag_heads *h, int size, int dim, int64_t n_tok, const void *p, size_t bytes);
 // every head's first value 16-byte aligned
 bool heads_aligned(const qmag_heads *h, int type);
 
@@ -149,6 +151,10 @@ constexpr int KV4_GROUP = 64;
 __host__ __device__ __forceinline__ constexpr int64_t kv4_half_bytes(int block, int dim)
 {
     return (int64_t)block * (dim / 2 + dim / KV4_GROUP * 4);
+}
+inline size_t kv4_bytes(const qmag_kv4 *c)
+{
+    return (size_t)c->n_block * (size_t)c->n_kv * (size_t)(2 * kv4_half_bytes(c->block_size, c->head_dim));
 }
 int check_kv4(const qmag_kv4 *c);
 

@@ -649,6 +649,8 @@ extern "C" int qmag_attn_prompt_dev(int type, int head_dim, const qmag_heads *q,
     if (heads_overlap(q, out, size, head_dim, T) || heads_overlap(k, out, size, head_dim, T) ||
         heads_overlap(v, out, size, head_dim, T))
         return fail(QMAG_ERR_ARG, "attn_prompt: the output overlaps an input");
+    if (T > 0 && n_seq > 0 && heads_meet(out, size, head_dim, T, cu, sizeof(int) * (size_t)(n_seq + 1)))
+        return fail(QMAG_ERR_ARG, "attn_prompt: the output overlaps cu");
     if ((st = require_ready())) return st;
     if (T == 0 || n_seq == 0) return QMAG_OK;
     DeviceScope dev;

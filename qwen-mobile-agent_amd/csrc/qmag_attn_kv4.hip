@@ -1103,6 +1103,12 @@ extern "C" int qmag_attn_kv4_dev(const qmag_kv4 *c, const qmag_kv_table *t, int 
         return fail(QMAG_ERR_ARG, "attn_kv4: a null or unaligned pointer");
     if (heads_overlap(q, out, attn_type_size(type), c->head_dim, T))
         return fail(QMAG_ERR_ARG, "attn_kv4: the output overlaps the queries");
+    if (T > 0 && t->n_seq > 0) {
+        auto meets = [&](const void *p, size_t bytes) { return heads_meet(out, attn_type_size(type), c->head_dim, T, p, bytes); };
+        if (meets(cu, sizeof(int) * (size_t)(t->n_seq + 1)) || meets(len, sizeof(int) * (size_t)t->n_seq) ||
+            meets(t->table, sizeof(int) * (size_t)t->n_seq * (size_t)t->max_blocks) || meets(c->data, kv4_bytes(c)))
+            return fail(QMAG_ERR_ARG, "attn_kv4: the output overlaps the lengths, the table or the cache");
+    }
     if ((st = require_ready())) return st;
     if (T == 0 || t->n_seq == 0) return QMAG_OK;
     DeviceScope dev;

@@ -82,6 +82,30 @@ bool heads_overlap(const qmag_heads *a, const qmag_heads *b, int size, int dim, 
     return true;
 }
 
+bool heads_meet(const qmag_heads *h, int size, int dim, int64_t n_tok, const void *p, size_t bytes)
+{
+    const int64_t all = extent(h, dim, n_tok);
+    const uintptr_t a = (uintptr_t)h->ptr, b = (uintptr_t)p;
+    if (all == 0 || bytes == 0 || a + (uintptr_t)(all * size) <= b || b + bytes <= a) return false;
+    // bytes from h's first value: rows of `row` bytes, inner ones within outer ones
+    const int64_t row = (int64_t)dim * size, lo = (int64_t)(b - a), hi = lo + (int64_t)bytes;
+    int64_t so = h->token_stride * size, si = h->head_stride * size, no = n_tok, ni = h->n_head;
+    if (so < si) {
+        const int64_t s = so, n = no;
+        so = si, no = ni, si = s, ni = n;
+    }
+    if (so == 0) return true;                      // a single row, and it lies there
+    if (si == 0) ni = 1;
+    // the first outer one that begins at or behind lo, then those before it that reach behind lo
+    const int64_t first = lo <= 0 ? 0 : (lo + so - 1) / so;
+    if (first < no && first * so < hi) return true;
+    for (int64_t o = (first < no ? first : no) - 1; o >= 0 && o * so + (ni - 1) * si + row > lo; o--) {
+        const int64_t d = lo - row - o * so, j = d < 0 || si == 0 ? 0 : d / si + 1;      // the first inner row that ends behind lo
+        if (j < ni && o * so + j * si + row > lo && o * so + j * si < hi) return true;
+    }
+    return false;
+}
+
 int check_kv4(const qmag_kv4 *c)
 {
     if (!c) return fail(QMAG_ERR_ARG, "kv4: null cache");

@@ -214,6 +214,12 @@ extern "C" int qmag_kv4_read_dev(const qmag_kv4 *c, const int *slot, int T, floa
     if (st) return st;
     if (T < 0 || (T > 0 && (!slot || !k || !v || ((uintptr_t)slot | (uintptr_t)k | (uintptr_t)v) % 4)))
         return fail(QMAG_ERR_ARG, "kv4_read: T=%d or a null or unaligned pointer", T);
+    const qmag_heads ko = {k, c->n_kv, (int64_t)c->n_kv * c->head_dim, c->head_dim}, vo = {v, ko.n_head, ko.token_stride, ko.head_stride};
+    if (heads_overlap(&ko, &vo, 4, c->head_dim, T)) return fail(QMAG_ERR_ARG, "kv4_read: k and v overlap");
+    for (const qmag_heads &o : {ko, vo})
+        if (heads_meet(&o, 4, c->head_dim, T, slot, sizeof(int) * (size_t)T) ||
+            heads_meet(&o, 4, c->head_dim, T, c->data, kv4_bytes(c)))
+            return fail(QMAG_ERR_ARG, "kv4_read: k or v overlaps the slots or the cache");
     if ((st = require_ready())) return st;
     if (T == 0) return QMAG_OK;
     const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0;

@@ -216,18 +216,37 @@ struct Range {
     int64_t n;
 };
 
+static bool ranges_meet(const Range &x, const Range &y)
+{
+    const uintptr_t a = (uintptr_t)x.p, b = (uintptr_t)y.p;
+    return x.n > 0 && y.n > 0 && a < b + (uintptr_t)y.n * sizeof(int) && b < a + (uintptr_t)x.n * sizeof(int);
+}
+
 // The first n_out ranges are written, the others read: aligned, and none of the
 // written ones meets another.
 static int check_ranges(const char *what, const Range *r, int n_out, int n)
 {
     for (int i = 0; i < n; i++) {
         if ((uintptr_t)r[i].p % sizeof(int)) return fail(QMAG_ERR_ARG, "%s: a pointer is not aligned", what);
-        for (int j = 0; j < n_out && j < i; j++) {
-            const uintptr_t a = (uintptr_t)r[i].p, b = (uintptr_t)r[j].p;
-            if (a < b + (uintptr_t)r[j].n * sizeof(int) && b < a + (uintptr_t)r[i].n * sizeof(int))
-                return fail(QMAG_ERR_ARG, "%s: what is written goes to places of its own", what);
-        }
+        for (int j = 0; j < n_out && j < i; j++)
+            if (ranges_meet(r[i], r[j])) return fail(QMAG_ERR_ARG, "%s: what is written goes to places of its own", what);
     }
+    return QMAG_OK;
+}
+
+// The table and the free list, of which a call writes one, against what else it
+// takes.  (A descriptor with the two in one place holds no blocks yet and is not
+// looked into.)
+static int check_lists(const char *what, const qmag_kv_table *t, bool table_written, const Range *r, int n_out, int n)
+{
+    const Range table = {t->table, (int64_t)t->n_seq * t->max_blocks}, list = {t->free_list, t->n_block};
+    if ((uintptr_t)table.p % sizeof(int) || (uintptr_t)list.p % sizeof(int))
+        return fail(QMAG_ERR_ARG, "%s: the table or the free list is not aligned", what);
+    if (table.p == list.p) return QMAG_OK;
+    if (ranges_meet(table, list)) return fail(QMAG_ERR_ARG, "%s: the table and the free list overlap", what);
+    for (int i = 0; i < n; i++)
+        if (i < n_out ? ranges_meet(r[i], table) || ranges_meet(r[i], list) : ranges_meet(r[i], table_written ? table : list))
+            return fail(QMAG_ERR_ARG, "%s: the table or the free list overlaps another argument", what);
     return QMAG_OK;
 }
 
@@ -252,6 +271,7 @@ extern "C" int qmag_kv_release_dev(const qmag_kv_table *t, const int *len, const
     const int64_t n = t->n_seq;
     const Range r[] = {{len_next, n}, {n_free_next, 1}, {status, 1}, {len, n}, {ended, n}, {n_free, 1}};
     if ((st = check_ranges("kv_release", r, 3, 6))) return st;
+    if ((st = check_lists("kv_release", t, false, r, 3, 6))) return st;
     if ((st = require_ready())) return st;
     DeviceScope dev;
     if (dev.st) return dev.st;
@@ -278,6 +298,7 @@ extern "C" int qmag_kv_assign_dev(const qmag_kv_table *t, const int *len, const 
     const Range r[] = {{len_next, n}, {n_free_next, 1}, {status, 1}, {cu, n + 1}, {slot, T},
                        {pos, T},      {len, n},         {n_new, n},  {n_free, 1}};
     if ((st = check_ranges("kv_assign", r, 6, 9))) return st;
+    if ((st = check_lists("kv_assign", t, true, r, 6, 9))) return st;
     if ((st = require_ready())) return st;
     DeviceScope dev;
     if (dev.st) return dev.st;

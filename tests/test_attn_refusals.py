@@ -180,3 +180,75 @@ def test_attn_prompt_refusals(lib, bad):
                                               k.get("T", 5), 1.0)
     assert call() == NODEV and call(T=0, cu=None) == NODEV and call(type=30) == NODEV
     assert call(**bad) == ARG, lib.lib().qmag_last_error()
+
+
+def test_bookkeeping_results_over_the_lists(lib):
+    """The table and the free list, which the workgroups of a call read and write, meet neither one
+    another nor a result; the one that is written meets no input."""
+    L = lib.lib()
+    p = [A + 4096 * i for i in range(10)]
+    T, F = A + (1 << 16), A + (1 << 17)                     # 10 x 4 and 64 words
+
+    def rel(table=T, free=F, **k):
+        t = lib.KvTable(10, 4, 16, 64, table, free)
+        ok = dict(zip(("len", "ended", "n_free", "len_next", "n_free_next", "status"), p))
+        return L.qmag_kv_release_dev(C.byref(t), *dict(ok, **k).values())
+
+    def assign(table=T, free=F, **k):
+        t = lib.KvTable(10, 4, 16, 64, table, free)
+        ok = dict(zip(("len", "new", "n_free"), p), T=20, slot=p[3], pos=p[4], cu=p[5], len_next=p[6], n_free_next=p[7], status=p[8])
+        return L.qmag_kv_assign_dev(C.byref(t), *dict(ok, **k).values())
+
+    assert rel() == NODEV and assign() == NODEV
+    assert rel(table=F - 160) == NODEV and rel(table=F - 156) == ARG and assign(free=T - 252) == ARG and assign(free=T - 256) == NODEV
+    assert rel(table=T + 2) == ARG and assign(free=F + 1) == ARG
+    for name in ("len_next", "n_free_next", "status"):
+        assert rel(**{name: T + 156}) == ARG and rel(**{name: F + 252}) == ARG and rel(**{name: F + 256}) == NODEV, name
+    for name in ("len", "ended", "n_free"):                 # the free list is written, the table is not
+        assert rel(**{name: F + 4}) == ARG and rel(**{name: T}) == NODEV, name
+    for name in ("slot", "pos", "cu", "len_next", "n_free_next", "status"):
+        assert assign(**{name: T + 156}) == ARG and assign(**{name: F}) == ARG and assign(**{name: T + 160}) == NODEV, name
+    for name in ("len", "new", "n_free"):                   # the table is written
+        assert assign(**{name: T}) == ARG and assign(**{name: F}) == NODEV, name
+    assert assign(T=0, slot=T, pos=F) == NODEV              # nothing of them is written
+
+
+def test_attention_output_over_what_it_reads(lib):
+    """The output meets neither lengths, table nor cache; beside them, between its own heads or tokens, it may lie."""
+    L, out = lib.lib(), A << 4
+    size = 64 * 16 * 2 * 2 * (64 + 8)
+
+    def kv4_call(layout=(out, 4, 640, 160), **k):           # heads of 128 values of 4 bytes, 32 values between them
+        c = kv4(lib, data=k.get("data", A))
+        t = lib.KvTable(3, 4, 16, 64, k.get("table", A), None)
+        q, o = lib.heads((A, 4, 512, 128)), lib.heads(layout)
+        return L.qmag_attn_kv4_dev(C.byref(c), C.byref(t), 0, q, o, k.get("cu", A), k.get("len", A), 5, 1.0)
+
+    assert kv4_call() == NODEV
+    end = out + 4 * (4 * 640 + 3 * 160 + 128)
+    for name, n in (("cu", 16), ("len", 12), ("table", 48)):
+        for at in (out, out + 4 * 640, end - 4, out - n + 4, out + 4 * 100, out + 4 * (640 + 128) - 4):
+            assert kv4_call(**{name: at}) == ARG, (name, at - out)
+        for at in (out - n, end, out + 4 * 128, out + 4 * (2 * 640 + 160 + 128)):
+            assert kv4_call(**{name: at}) == NODEV, (name, at - out)
+        # heads one behind another: a token's values lie among them
+        heads_major = (out, 4, 160, 1000)
+        assert kv4_call(heads_major, **{name: out + 4 * (2 * 1000 + 160)}) == ARG
+        assert kv4_call(heads_major, **{name: out + 4 * (1000 + 3 * 160 + 128)}) == NODEV
+    assert kv4_call(data=out + 16) == ARG and kv4_call(data=out - size + 16) == ARG and kv4_call(data=out - size) == NODEV
+
+    def prompt(cu):
+        h = [lib.heads((a, n, n * 128, 128)) for a, n in ((A, 4), (A << 1, 2), (A << 2, 2), (A << 3, 4))]
+        return L.qmag_attn_prompt_dev(0, 128, *h, cu, 2, 5, 1.0)
+    assert prompt(A << 3) == ARG and prompt((A << 3) + 4 * 5 * 512 - 4) == ARG and prompt((A << 3) - 8) == ARG
+    assert prompt((A << 3) + 4 * 5 * 512) == NODEV and prompt((A << 3) - 12) == NODEV
+
+
+def test_read_results_over_what_it_reads(lib):
+    L, c = lib.lib(), kv4(lib)
+    k, v, s, n = A << 2, A << 3, A << 4, 4 * 2 * 128 * 4    # four tokens of two heads
+    size = 64 * 16 * 2 * 2 * (64 + 8)
+    read = lambda slot, k, v: L.qmag_kv4_read_dev(C.byref(c), slot, 4, k, v)  # noqa: E731
+    assert read(s, k, v) == NODEV and read(s, k, k + n) == NODEV and read(s, k, k + n - 4) == ARG and read(s, k, k) == ARG
+    assert read(k + n - 4, k, v) == ARG and read(v - 12, k, v) == ARG and read(k + n, k, v) == NODEV
+    assert read(s, A, v) == ARG and read(s, k, A + size - 16) == ARG and read(s, k, A + size) == NODEV
