@@ -7,19 +7,17 @@
 // The codes go to the matrix cores as fp16 whole numbers: a nibble below the
 // exponent of 1024 (or, from the upper half of a byte, of 64) is that number plus
 // the code, and one subtraction for two values leaves it.  No code is rounded,
-// and no step or minimum touches the operand.  Three ways (Code):
+// and no step or minimum touches the operand.  Two ways (Code):
 //   CENTRED  fp32 and fp16 calls take code - 8, which keeps the two sums below
 //            small: with codes from 0 to 15 they were each tens of times the
 //            result, which cost a digit (fp32: 1e-5 of the result against 1e-6;
 //            fp16: 3.6e-4 against 2.4e-4, of which its rounding is 2.0e-4);
-//   PLAIN    bf16 calls of many rows take the code: a digit they do not hold
-//            anyway, and the value of code 8 need not be formed;
-//   RAW      bf16 decode takes the nibble alone, an fp16 subnormal (code * 2^-24,
-//            or * 2^-20 in the upper half of a byte, made up for exactly): five
-//            instructions for eight codes instead of nine.  The matrix cores align
-//            subnormal products as if their leading zeros were digits, so the sums
-//            are 10 bits short: 3e-4 of the result, a fifth of what bf16's own
-//            rounding of it takes (1.7e-3 in the mean), but more than fp16's.
+//   PLAIN    bf16 calls take the code: a digit they do not hold anyway, and the
+//            value of code 8 need not be formed.
+// (The nibble alone, an fp16 subnormal, would be four instructions fewer for eight
+// codes.  But the matrix cores align subnormal products as if their leading zeros
+// were digits, which leaves sums of 14 bits: with a few query channels some thousand
+// times the others the weights were wrong altogether.)
 //   scores   S = K Q^T per 64 channels on codes, then d S + mid sum(q) in fp32,
 //            mid the value of the operand 0: m, or m + 8 d;
 //   output   O^T = V^T P'^T with P' = p d: the step of a token and group is
@@ -170,7 +168,7 @@ __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t
 
 // What turns nibbles into fp16: masks and exponents in registers of both kinds,
 // so that the two go into one instruction.
-enum Code { CENTRED, PLAIN, RAW };
+enum Code { CENTRED, PLAIN };
 struct Nibbles {
     uint32_t lo = 0x000F000Fu, hi = 0x00F000F0u, e1024 = 0x64006400u, e64 = 0x54005400u;
     __device__ __forceinline__ Nibbles()
@@ -182,7 +180,6 @@ struct Nibbles {
     template <Code CODE>
     __device__ __forceinline__ uint32_t even(uint32_t w) const
     {
-        if (CODE == RAW) return w & lo;
         const _Float16 z = (_Float16)(CODE == CENTRED ? 1032.0f : 1024.0f);
         const half2v v = __builtin_bit_cast(half2v, (w & lo) | e1024) - (half2v){z, z};
         return __builtin_bit_cast(uint32_t, v);
@@ -190,7 +187,6 @@ struct Nibbles {
     template <Code CODE>
     __device__ __forceinline__ uint32_t odd(uint32_t w) const
     {
-        if (CODE == RAW) return w & hi;
         const _Float16 z = (_Float16)(CODE == CENTRED ? 72.0f : 64.0f);
         const half2v v = __builtin_bit_cast(half2v, (w & hi) | e64) - (half2v){z, z};
         return __builtin_bit_cast(uint32_t, v);
@@ -272,7 +268,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 {
     using S = typename T::S;
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
-    constexpr Code CODE = std::is_same_v<T, TBF16> ? RAW : CENTRED;
+    constexpr Code CODE = std::is_same_v<T, TBF16> ? PLAIN : CENTRED;
     constexpr int NG = D / 64;
     constexpr int RG = 16, STEP = 32 * NW;
     constexpr int VD = (D + 127) / 128;            // dwords of a lane's V codes of a token
@@ -383,7 +379,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
         // the row's largest value to 2^14 .. 2^15: exact, and undone by rs
         const int e = min(max((int)(__float_as_uint(row_max(top)) >> 23) - 127, -100), 127);
         const float up = exp2i(14 - e);
-        rs = (CODE == RAW ? exp2i(min(e, 113) - 14 + 24) : exp2i(e - 14)) * A.scale;      // (beyond 2^113 weights are 0 or 1 in any case)
+        rs = exp2i(e - 14) * A.scale;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             float sum = 0.0f;
@@ -394,11 +390,11 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
                 for (int i = 0; i < 8; i++) {
                     x[g][s][i] *= up;
                     sum += x[g][s][i];
-                    f[2 * (i & 3) + (i >> 2)] = x[g][s][i] * (CODE == RAW && (i & 1) ? 0.0625f : 1.0f);     // nibble i's place in a fragment
+                    f[2 * (i & 3) + (i >> 2)] = x[g][s][i];         // nibble i's place in a fragment
                 }
                 split8<NS>(f, &qh[g][s], &ql[NS == 2 ? g : 0][s]);
             }
-            qs[g] = row_sum(sum) * (CODE == RAW ? 0x1p-24f : 1.0f);
+            qs[g] = row_sum(sum);
         }
     }
 
@@ -556,7 +552,7 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 
     // ---- the waves' shares; a lane's row: channels 64 g + 4 (4 h + r) + i in o[g][i][r]
     l = row_sum(l);
-    const float back = exp2i(max(ve, 0) - 21) * (CODE == RAW ? 0x1p24f : 1.0f), back1 = back * (CODE == RAW ? 0.0625f : 1.0f);
+    const float back = exp2i(max(ve, 0) - 21);
     if (h == 0) {
         join_m[wave][n] = m;
         join_l[wave][n] = l;
@@ -574,8 +570,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 #pragma unroll
         for (int r = 0; r < 4; r++)
             *(float4 *)(mine + 64 * g + 4 * (4 * h + r)) =
-                make_float4(fmaf(o[g][0][r], back, add) * share, fmaf(o[g][1][r], back1, add) * share,
-                            fmaf(o[g][2][r], back, add) * share, fmaf(o[g][3][r], back1, add) * share);
+                make_float4(fmaf(o[g][0][r], back, add) * share, fmaf(o[g][1][r], back, add) * share,
+                            fmaf(o[g][2][r], back, add) * share, fmaf(o[g][3][r], back, add) * share);
     }
     __syncthreads();
     // 4 NW threads a row, four channels at a time

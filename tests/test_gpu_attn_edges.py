@@ -3,7 +3,7 @@ none, values far apart in size, infinite keys, the forms that only large calls t
 import numpy as np
 import pytest
 
-from attn_fixtures import BF16, F16, F32, TYPES, View, attention, held, ints, to_type, values
+from attn_fixtures import BF16, F16, F32, HALF, TYPES, View, attention, held, ints, to_type, values
 from test_gpu_attn import CacheCase, check_kv4, close, kv4_tol, kv_values, rng_of, run_kv4, run_prompt
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +28,65 @@ def test_attn_kv4_lengths_that_lap_over(qm, typ, rows, n):
     qm.attn_kv4_dev(case.c, c, t, q.heads, out.heads, cu.ptr, lens.ptr, rows, 0.125)
     got, rest = out.read()
     assert rest and np.isfinite(values(got, t)).all()
+
+
+# ------------------------------------------------------------------ sums of scores --
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_kv4_scores_that_nearly_cancel(qm, typ, D, rows):
+    """Keys of whole numbers from -8 to 7, queries of 1 to 1 + 15 / 128: the sums of products of codes
+    are hundreds to thousands, need up to 20 bits, and the minima take most of them off again.  A
+    value of V for each token, so that a channel is one token's weight.
+
+    The sums are exact in fp32.  A score of up to 256 log2(e) is rounded when scaled and when the
+    maximum is taken off: 2 x 370 x 2^-24 of an exponent, numerator and sum each: under 1e-4 of a
+    weight.  Weights to 2^-11 (fp32 calls 2^-21), and where codes are taken less 8, as much of 8.
+    The largest weight enters the product as 2^6 at least (a step of 1), where fp16's smallest half
+    step is 2^-25: 15 x 2^-31 of a value."""
+    t = TYPES[typ]
+    r = rng_of(D, rows, 5)
+    L, H, KV = 60, 8, 2
+    k = r.randint(-8, 8, (L, KV, D)).astype(np.float32)
+    k[..., ::64], k[..., 1::64] = -8, 7
+    v = np.zeros((L, KV, D), np.float32)
+    v[np.arange(L), :, np.arange(L)] = 15
+    q = to_type(1 + r.randint(0, 16, (rows, H, D)) / 128.0, t)
+    case = CacheCase(qm, r, [L + rows - 1], KV, D, 16, [np.concatenate([k, np.repeat(k[:1], rows - 1, 0)])],
+                     [np.concatenate([v, np.zeros((rows - 1, KV, D), np.float32)])])
+    got = values(run_kv4(qm, case, q, [rows], t, scale=1.0, pad=0), t)[..., :L]
+    want = attention(values(q, t), case.k[0], case.v[0], L - 1 + np.arange(rows), 1.0)[0][..., :L]
+    part = 2.0 ** -21 if t == F32 else 2.0 ** -11
+    close(got, want, (HALF[t] + part + 1e-4) * want + 8 * part * (t != BF16) + 2.0 ** -27 + 2.0 ** -25 * (t == F16))
+
+
+@pytest.mark.parametrize("large", [0, 128, 4096])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_kv4_scores_close_to_one_another(qm, typ, D, rows, large):
+    """As above, with keys that hold the same numbers in another order; and with queries of 128 or
+    4096 in every fourth channel, where all keys are 0, the others 1 to 1 + 15 / 16: products of up to
+    2^15 beside such of 2^-4, all of whose sums are whole multiples of 2^-4 below 2^20, so exact in fp32.
+
+    Where codes are taken less 8, what the other tokens leave of 8 is rounded by the sums too: up to
+    130 tokens in 5 tiles, two products each, and 40 additions of minima, each to 2^-24 of 8."""
+    t = TYPES[typ]
+    r = rng_of(D, rows, 6)
+    L, H, KV = 60, 8, 2
+    one = r.randint(-8, 8, 64)
+    one[:2] = -8, 7
+    k = np.stack([np.concatenate([r.permutation(one) for _ in range(KV * D // 64)]).reshape(KV, D) for _ in range(L)]).astype(np.float32)
+    v = np.zeros((L, KV, D), np.float32)
+    v[np.arange(L), :, np.arange(L)] = 15
+    q = 1 + r.randint(0, 16, (rows, H, D)) / (16.0 if large else 128.0)
+    if large:
+        k[..., 2::4], k[..., 0::64], k[..., 1::64], q[..., 2::4] = 0, -8, 7, large
+    q = to_type(q, t)
+    case = CacheCase(qm, r, [L + rows - 1], KV, D, 16, [np.concatenate([k, np.repeat(k[:1], rows - 1, 0)])],
+                     [np.concatenate([v, np.zeros((rows - 1, KV, D), np.float32)])])
+    got = values(run_kv4(qm, case, q, [rows], t, scale=1.0, pad=0), t)[..., :L]
+    want = attention(values(q, t), case.k[0], case.v[0], L - 1 + np.arange(rows), 1.0)[0][..., :L]
+    part = 2.0 ** -21 if t == F32 else 2.0 ** -11
+    close(got, want, (HALF[t] + part + 1e-4) * want + 8 * (part + 52 * 2.0 ** -24) * (t != BF16) + 2.0 ** -27)
