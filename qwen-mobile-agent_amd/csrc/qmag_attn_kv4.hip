@@ -143,13 +143,6 @@ __device__ __forceinline__ float row_max(float v)
     p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
 }
-__device__ __forceinline__ int row_max_i(int v)
-{
-    auto p = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
-    v = max((int)p[0], (int)p[1]);
-    p = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
-    return max((int)p[0], (int)p[1]);
-}
 __device__ __forceinline__ float row_sum(float v)
 {
     auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -162,6 +155,10 @@ union Frag {
     uint32_t u[4];
     half8 h;
 };
+
+// The maximum of a row that has seen nothing: below any score, and finite, so that
+// differences from it are numbers.
+constexpr float AK_NONE = -3e38f;
 
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -246,6 +243,73 @@ __device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&o)[N])
 #pragma unroll
         for (int i = 0; i < N; i++) o[i] = *(const uint32_t *)(p + 4 * i);
     }
+}
+
+// The size of a step d (bits 0 .. 15, not negative): its exponent and first two digits, an
+// e with d < 2^(e - 14.5), and of a normal d at least 2^(e - 15).  NaN and infinity have 31
+// and more.
+__device__ __forceinline__ float ak_size(uint32_t d) { return 0.25f * (float)(d >> 8 & 255u); }
+
+// The weights p of a lane's eight scores (of what its row does not see -inf), by the
+// maximum m so far, and their sum into l.  o and vs are the sums of p d code and p mid,
+// o times 2^(7 - ve): the products' operands p d 2^(7 - ve) have to stay below 2^16, and
+// near there to keep their bits.  Maximum and power of two move only where a weight
+// would pass 2^8 or an operand 2^15.  The power follows the largest p d, not the largest
+// d: a token of large values and no weight takes no bits from the others (300 tokens,
+// one with a step 2^20 times theirs and a weight of e^-60: fp32 calls were off by 1e-3).
+// size(i): of a token's largest step, or more; exact(far): the largest score + size of
+// the lane, which is far where size gives no more.
+// (Arrays by reference: as members of a struct the compiler copied all of o in every tile.)
+template <int NG, class Size, class Exact>
+__device__ __forceinline__ void ak_weigh(const float (&s)[8], float (&p)[8], float &m, float &l, int &ve, float (&vs)[NG],
+                                         f32x4 (&o)[NG][4], Size size, Exact exact)
+{
+    float top = s[0], far = s[0] + size(0);
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        top = fmaxf(top, s[i]);
+        far = fmaxf(far, s[i] + size(i));
+    }
+    if (__any(top > m + 8.0f || far > m + ((float)ve + 22.5f))) {
+        // (a row that need not move stays: what others see has no part in its rounding)
+        top = row_max(top);
+        far = row_max(exact(far));
+        const float was = m;
+        const bool wide = far > m + ((float)ve + 22.5f);
+        m = top > m + 8.0f ? top : m;
+        // what is summed so far shrinks with the maximum's move, and its power of two with it
+        const int sunk = ve - (int)fminf(m - was, 200.0f), here = (int)ceilf(fminf(fmaxf(far - m - 14.5f, -60.0f), 40.0f));
+        const int e = wide || m != was ? max(max(here, sunk), -60) : ve;
+        const float f = __builtin_amdgcn_exp2f(was - m), fo = __builtin_amdgcn_exp2f(was - m + (float)(ve - e));
+        ve = e;
+        l *= f;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            vs[g] *= f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[g][i] *= fo;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        p[i] = __builtin_amdgcn_exp2f(s[i] - m);
+        l += p[i];
+    }
+}
+
+// p[i] d[i] 2^(7 - ve) in fp16 parts, for group g
+template <Code CODE, int NS, int NG>
+__device__ __forceinline__ void ak_operand(const float (&p)[8], const uint32_t (&vdm)[8][NG], int ve, float (&vs)[NG], int g,
+                                           half8 *ph, half8 *pl)
+{
+    const float up = exp2i(7 - ve);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        x[i] = p[i] * up * step_of(vdm[i][g]);
+        vs[g] = fmaf(p[i], mid_of<CODE>(vdm[i][g]), vs[g]);
+    }
+    split8<NS>(x, ph, pl);
 }
 
 // Bytes of a wave's tile of 32 tokens in LDS: K codes, V codes, scales of both.
@@ -399,15 +463,14 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
     }
 
     f32x4 o[NG][4];
-    float vs[NG], l = 0.0f, m = -INFINITY;
-    int ve = -1;                                   // the row's weights carry 2^(21 - ve)
+    float vs[NG], l = 0.0f, m = AK_NONE;
+    int ve = -60;                                  // o carries 2^(7 - ve)
 #pragma unroll
     for (int g = 0; g < NG; g++) {
         vs[g] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) o[g][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-
     int slot = 0;
     for (int t0 = c0; t0 < c1; t0 += STEP) {
         // this tile's pieces are in; the next ones' go out
@@ -452,7 +515,6 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
         uint32_t vdm[8][NG];
 #pragma unroll
         for (int i = 0; i < 8; i++) load_dwords(tile + 32 * D + 128 * NG + (16 * (i >> 2) + 4 * h + (i & 3)) * (NG * 4), vdm[i]);
-        float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; i++) s[i] *= rs;
         if (bad || t0 + 31 > open) {
@@ -466,49 +528,27 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
                 for (int g = 0; g < NG; g++) vdm[i][g] = seen ? vdm[i][g] : 0u;
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, s[i]);
-        top = row_max(top);
-
-        // ---- running maximum: moved only when a weight would pass 2^8
-        if (__any(top > m + 8.0f)) {
-            // (a row that need not move stays: what others see has no part in its rounding)
-            const float mn = top > m + 8.0f ? fmaxf(m, top) : m;
-            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= f;
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                vs[g] *= f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[g][i] *= f;
-            }
-        }
-        const float ms = m == -INFINITY ? 0.0f : m;
-        // ---- the largest step the row has seen sets the power of two of its weights
-        typedef short s16x2 __attribute__((ext_vector_type(2)));
-        s16x2 dt = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int g = 0; g < NG; g++) dt = __builtin_elementwise_max(dt, __builtin_bit_cast(s16x2, vdm[i][g]));
-        const int de = row_max_i(min((int)dt[0] >> 10, 30));
-        if (__any(de > ve)) {
-            const int en = max(de, ve);
-            const float f = ve < 0 ? 0.0f : exp2i(ve - en);
-            ve = en;
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[g][i] *= f;
-        }
-        const float pf = exp2i(21 - ve);
         float p[8];
+        ak_weigh<NG>(
+            s, p, m, l, ve, vs, o,
+            [&](int i) {
+                typedef short s16x2 __attribute__((ext_vector_type(2)));
+                s16x2 d = __builtin_bit_cast(s16x2, vdm[i][0]);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            p[i] = __builtin_amdgcn_exp2f(s[i] - ms);
-            l += p[i];
-        }
+                for (int g = 1; g < NG; g++) d = __builtin_elementwise_max(d, __builtin_bit_cast(s16x2, vdm[i][g]));
+                return ak_size(__builtin_bit_cast(uint32_t, d));
+            },
+            [&](float) {
+                float far = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        const float e = ak_size(vdm[i][g]);
+                        far = fmaxf(far, e < 31.0f ? s[i] + e : -INFINITY);        // (NaN has no part in it)
+                    }
+                return far;
+            });
 
         // ---- output
         uint32_t vc[8][VD];
@@ -520,14 +560,8 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
         }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[i] = p[i] * pf * step_of(vdm[i][g]);
-                vs[g] = fmaf(p[i], mid_of<CODE>(vdm[i][g]), vs[g]);
-            }
             half8 ph, pl;
-            split8<NS>(x, &ph, &pl);
+            ak_operand<CODE, NS>(p, vdm, ve, vs, g, &ph, &pl);
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 // byte b of group g: channels 4 n + 2 b and the next of every token
@@ -552,17 +586,16 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
 
     // ---- the waves' shares; a lane's row: channels 64 g + 4 (4 h + r) + i in o[g][i][r]
     l = row_sum(l);
-    const float back = exp2i(max(ve, 0) - 21);
+    const float back = exp2i(ve - 7);
     if (h == 0) {
         join_m[wave][n] = m;
         join_l[wave][n] = l;
     }
     __syncthreads();                               // no wave reads its tiles any more either
-    float all = -INFINITY;
+    float all = AK_NONE;
 #pragma unroll
     for (int w = 0; w < NW; w++) all = fmaxf(all, join_m[w][n]);
-    float share = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - all);
-    if (m == -INFINITY && l != 0.0f) share = l;    // a NaN weight leaves m at -inf: let it through
+    const float share = __builtin_amdgcn_exp2f(m - all);      // (nothing seen: sums of zero; a NaN stays one)
     float *join = (float *)lds, *mine = join + (wave * 16 + n) * LROW;
 #pragma unroll
     for (int g = 0; g < NG; g++) {
@@ -578,14 +611,11 @@ __global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typ
     constexpr int PER = 4 * NW, CP = D / (4 * PER) > 0 ? D / (4 * PER) : 1;
     const int rr = threadIdx.x / PER, cc = threadIdx.x % PER;
     if (r0 + rr >= rows) return;
-    float M = -INFINITY, L = 0.0f;
+    float M = AK_NONE, L = 0.0f;
 #pragma unroll
     for (int w = 0; w < NW; w++) M = fmaxf(M, join_m[w][rr]);
 #pragma unroll
-    for (int w = 0; w < NW; w++) {
-        const float mw = join_m[w][rr], lw = join_l[w][rr];
-        L += mw == -INFINITY ? (lw != 0.0f ? lw : 0.0f) : lw * __builtin_amdgcn_exp2f(mw - M);
-    }
+    for (int w = 0; w < NW; w++) L += join_l[w][rr] * __builtin_amdgcn_exp2f(join_m[w][rr] - M);
     const int jj = (r0 + rr) / A.G, hh = r0 + rr - jj * A.G;
     S *op = (S *)A.out + (P.q0 + jj) * A.ot + (kvh * A.G + hh) * A.oh;
     const int64_t at = ak_part(A, P, kvh, group, RG, rr) + split;
@@ -643,6 +673,7 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
     __shared__ __attribute__((aligned(16))) uint8_t raw[2][TILE];
     __shared__ __attribute__((aligned(16))) _Float16 ik[2][IMG], iv[2][IMG];
     __shared__ __attribute__((aligned(16))) uint8_t isc[2][SC];    // scales of K, then of V: [32][NG] each
+    __shared__ __attribute__((aligned(16))) float isize[2][32];    // ak_size of a token's largest step of V
 
     int item, kvh;
     ak_item(A, &item, &kvh);
@@ -724,6 +755,15 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
                 }
             } else {
                 *(uint4 *)(isc[b] + 16 * (p - 2 * D)) = x;
+                const int w0 = 4 * (p - 2 * D) - 32 * NG;          // V's, from this piece on
+                if (w0 >= 0)
+#pragma unroll
+                    for (int i = 0; i < 4; i += NG) {
+                        float e = 0.0f;            // (NaN has no part in it)
+#pragma unroll
+                        for (int g = 0; g < NG; g++) e = fmaxf(e, ak_size(u[i + g]) < 31.0f ? ak_size(u[i + g]) : 0.0f);
+                        isize[b][w0 / NG + i / NG] = e;
+                    }
             }
         }
     };
@@ -770,8 +810,8 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
     }
 
     f32x4 o[NG][4];                                // channels 64 g + 16 i + 4 h + r in o[g][i][r]
-    float vs[NG], l = 0.0f, m = -INFINITY;
-    int ve = -1;                                   // the row's weights carry 2^(21 - ve)
+    float vs[NG], l = 0.0f, m = AK_NONE;
+    int ve = -60;                                  // o carries 2^(7 - ve)
 #pragma unroll
     for (int g = 0; g < NG; g++) {
         vs[g] = 0.0f;
@@ -817,7 +857,6 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
         uint32_t vdm[8][NG];
 #pragma unroll
         for (int i = 0; i < 8; i++) load_dwords(isc[b] + SC / 2 + (16 * (i >> 2) + 4 * h + (i & 3)) * (NG * 4), vdm[i]);
-        float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; i++) s[i] *= rs;
         if (bad || t0 + 31 > open) {
@@ -831,49 +870,9 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
                 for (int g = 0; g < NG; g++) vdm[i][g] = seen ? vdm[i][g] : 0u;
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, s[i]);
-        top = row_max(top);
-
-        // ---- running maximum: moved only when a weight would pass 2^8
-        if (__any(top > m + 8.0f)) {
-            // (a row that need not move stays: what others see has no part in its rounding)
-            const float mn = top > m + 8.0f ? fmaxf(m, top) : m;
-            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= f;
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                vs[g] *= f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[g][i] *= f;
-            }
-        }
-        const float ms = m == -INFINITY ? 0.0f : m;
-        // ---- the largest step the row has seen sets the power of two of its weights
-        typedef short s16x2 __attribute__((ext_vector_type(2)));
-        s16x2 dt = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int g = 0; g < NG; g++) dt = __builtin_elementwise_max(dt, __builtin_bit_cast(s16x2, vdm[i][g]));
-        const int de = row_max_i(min((int)dt[0] >> 10, 30));
-        if (__any(de > ve)) {
-            const int en = max(de, ve);
-            const float f = ve < 0 ? 0.0f : exp2i(ve - en);
-            ve = en;
-#pragma unroll
-            for (int g = 0; g < NG; g++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[g][i] *= f;
-        }
-        const float pf = exp2i(21 - ve);
         float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            p[i] = __builtin_amdgcn_exp2f(s[i] - ms);
-            l += p[i];
-        }
+        const f32x4 size[2] = {*(const f32x4 *)(isize[b] + 4 * h), *(const f32x4 *)(isize[b] + 16 + 4 * h)};
+        ak_weigh<NG>(s, p, m, l, ve, vs, o, [&](int i) { return size[i >> 2][i & 3]; }, [](float far) { return far; });
 
         // the next tile's codes, between the two products: its LDS reads and vector work run while
         // the other waves multiply (ahead of the scores 334 us, behind the output 323, here 316)
@@ -882,14 +881,8 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
         // ---- output
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[i] = p[i] * pf * step_of(vdm[i][g]);
-                vs[g] = fmaf(p[i], mid_of<CODE>(vdm[i][g]), vs[g]);
-            }
             half8 ph, pl;
-            split8<NS>(x, &ph, &pl);
+            ak_operand<CODE, NS>(p, vdm, ve, vs, g, &ph, &pl);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 union { s16x4 r[2]; half8 v; } vf;
@@ -920,9 +913,8 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
 
     if (!live) return;
     l = row_sum(l);
-    const float back = exp2i(max(ve, 0) - 21);
+    const float back = exp2i(ve - 7);
     const float inv = P.n_split > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    const float nan = m == -INFINITY && l != 0.0f ? l : 0.0f;       // a NaN weight leaves m at -inf
     S *op = (S *)A.out + (P.q0 + j) * A.ot + (kvh * A.G + gh) * A.oh;
     const int64_t at = ak_part(A, P, kvh, group, RG, wave * 16 + n) + split;
 #pragma unroll
@@ -933,7 +925,7 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
             const int c = 64 * g + 16 * i + 4 * h;
             float y[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = fmaf(o[g][i][r], back, add) * inv + nan;
+            for (int r = 0; r < 4; r++) y[r] = fmaf(o[g][i][r], back, add) * inv;
             if (P.n_split == 1) store4<T>(op + c, A.o_vec, y);
             else store4<TF32>(A.part + at * D + c, true, y);
         }
@@ -966,10 +958,10 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(
     const int row = (t - P.q0) * A.G + gh;
     const int64_t first = ak_part(A, P, kvh, row / RG, RG, row % RG);
     struct alignas(4 * C) Vec { float v[C]; };
-    float acc[C], L = 0.0f, M = -INFINITY;
+    float acc[C], L = 0.0f, M = AK_NONE;
 #pragma unroll
     for (int c = 0; c < C; c++) acc[c] = 0.0f;
-    // (a part that saw no token has nothing but zeros; one with a NaN weight -inf and a NaN sum)
+    // (a part that saw no token has nothing but zeros)
     for (int i0 = wave; i0 < P.n_split; i0 += U * NW) {
         float2 ml[U];
         Vec v[U];
@@ -982,19 +974,17 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(
         float top = M;
 #pragma unroll
         for (int u = 0; u < U; u++) top = fmaxf(top, ml[u].x);
-        const float old = M == -INFINITY ? (L == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(M - top);
+        const float old = __builtin_amdgcn_exp2f(M - top);
         M = top;
         L *= old;
 #pragma unroll
         for (int c = 0; c < C; c++) acc[c] *= old;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const float mi = ml[u].x, li = ml[u].y;
-            const bool in = i0 + u * NW < P.n_split;
-            const float f = !in ? 0.0f : mi == -INFINITY ? (li != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(mi - M);
-            L += f == 0.0f ? 0.0f : f * li;
+            const float f = i0 + u * NW < P.n_split ? __builtin_amdgcn_exp2f(ml[u].x - M) : 0.0f;
+            L = fmaf(f, ml[u].y, L);
 #pragma unroll
-            for (int c = 0; c < C; c++) acc[c] += f == 0.0f ? 0.0f : f * v[u].v[c];
+            for (int c = 0; c < C; c++) acc[c] = fmaf(f, v[u].v[c], acc[c]);
         }
     }
     S *op = (S *)A.out + t * A.ot + head * A.oh + c0;
@@ -1011,7 +1001,7 @@ __global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) attn_kv4_join_kernel(
         for (int c = 0; c < C; c++) acc[c] = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const float f = sm[w] == -INFINITY ? (sl[w] != 0.0f ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(sm[w] - M);
+            const float f = __builtin_amdgcn_exp2f(sm[w] - M);
             L += f * sl[w];
 #pragma unroll
             for (int c = 0; c < C; c++) acc[c] += f * sum[w][C * lane + c];

@@ -5,6 +5,7 @@ import pytest
 
 from attn_fixtures import BF16, F16, F32, HALF, TYPES, View, attention, held, ints, to_type, values
 from test_gpu_attn import CacheCase, check_kv4, close, kv4_tol, kv_values, rng_of, run_kv4, run_prompt
+from test_gpu_attn_wide import kv4_bound, prompt_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +91,82 @@ def test_attn_kv4_scores_close_to_one_another(qm, typ, D, rows, large):
     want = attention(values(q, t), case.k[0], case.v[0], L - 1 + np.arange(rows), 1.0)[0][..., :L]
     part = 2.0 ** -21 if t == F32 else 2.0 ** -11
     close(got, want, (HALF[t] + part + 1e-4) * want + 8 * (part + 52 * 2.0 ** -24) * (t != BF16) + 2.0 ** -27)
+
+
+# ------------------------------------------------------ values far apart in size --
+
+def one_far_key(r, L, KV, D, at, power, small):
+    """Normal keys and values (times `small`), but at token `at` a key of -120 in channel 0 and values
+    2^power times as large.  For queries that hold 8 there."""
+    k, v = r.randn(L, KV, D).astype(np.float32), (small * r.randn(L, KV, D)).astype(np.float32)
+    k[:, :, 0] = 0
+    k[at], k[at, :, 0] = 0, -120
+    v[at] = v[at] * np.float32(2.0 ** power)
+    return k, v
+
+
+def far_query(r, rows, H, D):
+    q = r.randn(rows, H, D)
+    q[..., 0] = 8
+    return q
+
+
+def norm_error(got, want):
+    return np.linalg.norm(got - want) / np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("at", [0, 40, 290])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_kv4_large_values_of_no_weight(qm, typ, D, rows, at):
+    """A key of weight e^-40 and less whose values' step is 2^20 times the others': it has no part in
+    the result, so the result is as exact as without it (the bound for normal inputs, of whose
+    rounding terms the eight of a query's channel adds one of D as large as sqrt(D) others)."""
+    t = TYPES[typ]
+    r = rng_of(D, rows, at, 8)
+    L, H, KV = 300 + rows, 4, 2
+    k, v = one_far_key(r, L, KV, D, at, 20, 2.0 ** -8)
+    case = CacheCase(qm, r, [L], KV, D, 16, [k], [v])
+    q = to_type(far_query(r, rows, H, D), t)
+    got = values(run_kv4(qm, case, q, [rows], t, pad=0), t)
+    want = attention(values(q, t), case.k[0], case.v[0], L - rows + np.arange(rows), D ** -0.5)[0]
+    assert norm_error(got, want) <= 2 * kv4_bound(t, D, L)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_kv4_values_without_a_step(qm, typ, rows):
+    """All values of a token alike (a step of 0), those of a few tokens not, and of one that nothing sees."""
+    t = TYPES[typ]
+    r = rng_of(rows, 81)
+    L, H, KV, D = 400, 4, 2, 128
+    k = r.randn(L, KV, D).astype(np.float32)
+    v = np.repeat(r.randn(L, KV, 1), D, 2).astype(np.float32)
+    q = to_type(r.randn(rows, H, D), t)
+    for some in ([], [3], [200, 201], [399]):
+        v2 = v.copy()
+        v2[some] = 1000 * r.randn(len(some), KV, D)
+        case = CacheCase(qm, r, [L], KV, D, 16, [k], [v2])
+        got = values(run_kv4(qm, case, q, [rows], t, pad=0), t)
+        want, mag, es = attention(values(q, t), case.k[0], case.v[0], L - rows + np.arange(rows), D ** -0.5)
+        close(got, want, kv4_tol(t, D, L, want, 10 * mag, es), some)
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_kv4_a_nan_among_values(qm, typ, D, rows):
+    """It takes its 64 channels, and no digit of the others."""
+    t = TYPES[typ]
+    r = rng_of(D, rows, 82)
+    L, H, KV = 200 + rows, 4, 2
+    k, v = (r.randn(L, KV, D).astype(np.float32) for _ in range(2))
+    v[50, :, 70] = np.nan
+    case = CacheCase(qm, r, [L], KV, D, 16, [k], [v])
+    q = to_type(r.randn(rows, H, D), t)
+    got = values(run_kv4(qm, case, q, [rows], t, pad=0), t)
+    want = attention(values(q, t), case.k[0], case.v[0], L - rows + np.arange(rows), D ** -0.5)[0]
+    gone = np.arange(D) // 64 == 1
+    assert np.isnan(got[..., gone]).all() and np.isnan(want[..., gone]).all()
+    assert norm_error(got[..., ~gone], want[..., ~gone]) <= kv4_bound(t, D, L)
