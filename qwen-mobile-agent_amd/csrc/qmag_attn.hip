@@ -45,8 +45,7 @@ struct ApArgs {
     const int *cu;
     uint8_t *img;                         // [n_kv][tiles][K image | V image]
     float *scale;                         // [n_kv][tiles][32 of K | 32 of V], fp32 calls
-    int *flags;                           // [n_kv][tiles]: bit 0 V holds an infinity or a NaN; fp32 calls: 2 (128 + its
-                                          // largest power of two's exponent)
+    int *flags;                           // [n_kv][tiles]: V holds an infinity or a NaN
     int n_seq, T, tiles, n_kv, G;
     float sc;                             // scale * log2 e
     int q_vec, k_vec, v_vec, o_vec;
@@ -177,8 +176,8 @@ struct ApRows {
     }
 
     // into a tile's image and powers of two; odd: V had an infinity or a NaN (added
-    // where it is seen, not multiplied); most: the largest power's exponent
-    __device__ __forceinline__ void lay(bool v, E *img, float *scale, int *odd, int *most)
+    // where it is seen, not multiplied)
+    __device__ __forceinline__ void lay(bool v, E *img, float *scale, int *odd)
     {
         const int c = threadIdx.x % CH;
 #pragma unroll
@@ -204,7 +203,6 @@ struct ApRows {
                 }
                 *(V8 *)(row + PLANE) = lo;
                 if (c == 0) scale[(v ? AP_KEYS : 0) + key] = pow2i(e - 14);
-                *most = max(*most, e - 14);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) hi[i] = (E)x[u][i];
@@ -223,22 +221,13 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
     const int kvh = blockIdx.y;
     const int64_t tile = (int64_t)kvh * A.tiles + a / AP_KEYS + seq + part;
     const bool v = blockIdx.z;                     // K's image, or V's
-    int odd = 0, most = -126;
+    int odd = 0;
     R rows;
     rows.template fetch<true>(A, v, kvh, a, n, part * AP_KEYS);
-    rows.lay(v, (typename R::E *)A.img + tile * 2 * R::NS * R::PLANE, A.scale + tile * 2 * AP_KEYS, &odd, &most);
+    rows.lay(v, (typename R::E *)A.img + tile * 2 * R::NS * R::PLANE, A.scale + tile * 2 * AP_KEYS, &odd);
     if (v) {
-        if constexpr (R::NS == 2) {
-            __shared__ int wave_most[AP_WG / 64];
-#pragma unroll
-            for (int d = R::CH; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d));
-            if (lane_id() == 0) wave_most[threadIdx.x >> 6] = most;
-            odd = __syncthreads_or(odd);
-            for (int i = 0; i < AP_WG / 64; i++) most = max(most, wave_most[i]);
-        } else {
-            odd = __syncthreads_or(odd);
-        }
-        if (threadIdx.x == 0) A.flags[tile] = (odd ? 1 : 0) | 2 * (128 + most);
+        odd = __syncthreads_or(odd);
+        if (threadIdx.x == 0) A.flags[tile] = odd ? 1 : 0;
     }
 }
 
@@ -305,9 +294,6 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     } else {
         load(0, 0);
     }
-    // (as constants: scalar loads, which wait for no step)
-    const __attribute__((address_space(4))) int *flags = (const __attribute__((address_space(4))) int *)(uintptr_t)(A.flags + tile0);
-
     // ---- queries; a negative scale turns their sign, none makes them zero (the
     // scores are multiplied behind the mask, whose -inf has to stay)
     V8 qh[KS], ql[NS == 2 ? KS : 1];
@@ -347,7 +333,9 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 
     Acc o[DT];
     float m = -3e38f, l = 0.0f;                    // running maximum (of scaled scores), sum
-    int ve = -127;                                 // fp32: the row's weights carry 2^(7 - ve) and V's power of two
+    // fp32 calls: a weight's operand is p times V's power of two, 2^(7 - ve) of it: below 2^16, and near
+    // there to keep its bits
+    int ve = -110;
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -366,7 +354,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     }
 
     // One tile of 32 keys; EDGE: the one that holds the wave's own tokens.
-    auto tile = [&](const E *K, const float *sc, int flag, auto EDGE) {
+    auto tile = [&](const E *K, const float *sc, auto EDGE) {
         // ---- scores
         Acc sa[NA];
 #pragma unroll
@@ -416,59 +404,54 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         // ---- weights, by the maximum so far.  Whether it has to move is seen from
         // their sum, which is needed in any case: past 2^8, an infinity included.
         const float r = NS == 2 ? 1.0f : rs;
-        float p[NV], sum = 0.0f;
+        float p[NV], w[NS == 2 ? NV : 1], sum = 0.0f, far = 0.0f;    // w: times V's powers of two
         auto weigh = [&] {
-            sum = 0.0f;
+            sum = far = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 p[i] = __builtin_amdgcn_exp2f(NS == 2 ? s[i] - m : fmaf(s[i], r, -m));
                 sum += p[i];
+                if constexpr (NS == 2) {
+                    w[i] = p[i] * sc[AP_KEYS + KG * (i >> 2) + 4 * h + (i & 3)];
+                    far = fmaxf(far, w[i]);
+                }
             }
         };
         weigh();
-        bool move = sum > 256.0f;
-        int e = (flag >> 1) - 128;                 // of the largest V that the row sees here
-        if constexpr (NS == 2) {
-            if constexpr (EDGE.value || DIRECT) {
-                float vt = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NV; i++) vt = fmaxf(vt, s[i] == -INFINITY ? 0.0f : sc[AP_KEYS + KG * (i >> 2) + 4 * h + (i & 3)]);
-                e = max((int)(__float_as_uint(query_max<QW>(vt)) >> 23) - 127, -126);
-            }
-            move = move || e > ve;
-        }
-        if (__any(move)) {
-            float top = s[0], f = 1.0f;
+        // fp32 calls: nor may an operand pass 2^15.  Its power of two follows the largest w, not V's
+        // largest: a key of large values and no weight takes no bits from the others.
+        if (__any(sum > 256.0f || (NS == 2 && far > pow2i(min(ve + 8, 127))))) {
+            float top = s[0];
 #pragma unroll
             for (int i = 1; i < NV; i++) top = fmaxf(top, s[i]);
             top = query_max<QW>(top) * r;
             // (a query that need not move stays: what others see has no part in its rounding)
-            const float mn = query_max<QW>(sum) > 256.0f ? fmaxf(m, top) : m;
-            if (NS == 2 && e > ve) {
-                f = ve == -127 ? 0.0f : pow2i(max(ve - e, -126));
+            const bool moves = query_max<QW>(sum) > 256.0f, wide = NS == 2 && query_max<QW>(far) > pow2i(min(ve + 8, 127));
+            const float was = m;
+            m = moves ? fmaxf(m, top) : m;
+            weigh();
+            float f = __builtin_amdgcn_exp2f(was - m);
+            l *= f;
+            if constexpr (NS == 2) {
+                // what is summed so far shrinks with the maximum's move, and its power of two with it
+                const int sunk = ve - (int)fminf(m - was, 400.0f), here = (int)(__float_as_uint(query_max<QW>(far)) >> 23) - 126;
+                const int e = moves || wide ? max(max(sunk, here), -110) : ve;
+                f = __builtin_amdgcn_exp2f(was - m + (float)(ve - e));
                 ve = e;
             }
-            const float g = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= g;
-            f *= g;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int i = 0; i < R; i++) o[d][i] *= f;
-            weigh();
         }
         l += sum;
-        const float pv = NS == 2 ? pow2i(min(7 - ve, 127)) : 1.0f;
+        const float pv = NS == 2 ? pow2i(7 - ve) : 1.0f;
         V8 ph[PS], pl[NS == 2 ? PS : 1];
 #pragma unroll
         for (int i = 0; i < NV; i += 2) {
             if constexpr (NS == 2) {
                 half2v a, b;
-                float2 vp = *(const float2 *)(sc + AP_KEYS + KG * (i >> 2) + 4 * h + (i & 3));
-                vp.x *= pv, vp.y *= pv;                // up to 2^7; of keys not seen to infinity
-                if constexpr (EDGE.value) vp.x = fminf(vp.x, 128.0f), vp.y = fminf(vp.y, 128.0f);
-                split2(p[i] * vp.x, p[i + 1] * vp.y, &a, &b);
+                split2(w[i] * pv, w[i + 1] * pv, &a, &b);
                 ph[i >> 3][i & 7] = a[0], ph[i >> 3][(i & 7) + 1] = a[1];
                 pl[i >> 3][i & 7] = b[0], pl[i >> 3][(i & 7) + 1] = b[1];
             } else {
@@ -505,17 +488,13 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 
     const int mine = q0 < len ? q0 / AP_KEYS : -1;           // the wave's last tile
     const int steps = (tiles + KT - 1) / KT;
-    int flag[KT];
-#pragma unroll
-    for (int i = 0; i < KT; i++) flag[i] = NS == 2 && !DIRECT ? flags[i] : 0;
     unsigned long long odd = 0;                    // DIRECT: tiles whose V holds an infinity or a NaN
     for (int step = 0; step < steps; step++) {
         const int b = step & 1;
-        int next[KT] = {};
         if constexpr (DIRECT) {
-            int here = 0, most = 0;
-            kr.lay(false, lds[b], lsc[b], &here, &most);
-            vr.lay(true, lds[b], lsc[b], &here, &most);
+            int here = 0;
+            kr.lay(false, lds[b], lsc[b], &here);
+            vr.lay(true, lds[b], lsc[b], &here);
             if (__syncthreads_or(here)) odd |= 1ull << step;
             if (step + 1 < steps) {
                 kr.template fetch<false>(A, false, kvh, a, len, (step + 1) * AP_KEYS);
@@ -524,19 +503,15 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < KT; i++) next[i] = NS == 2 ? flags[(step + 1) * KT + i] : 0;
             if (step + 1 < steps) load(step + 1, b ^ 1);
         }
 #pragma unroll
         for (int i = 0; i < KT; i++) {
             const int kt = step * KT + i;
             const float *sc = lsc[b] + (NS == 2 ? i * 2 * AP_KEYS : 0);
-            if (kt < mine) tile(lds[b] + i * TILE, sc, flag[i], std::false_type{});
-            else if (kt == mine) tile(lds[b] + i * TILE, sc, 0, std::true_type{});
+            if (kt < mine) tile(lds[b] + i * TILE, sc, std::false_type{});
+            else if (kt == mine) tile(lds[b] + i * TILE, sc, std::true_type{});
         }
-#pragma unroll
-        for (int i = 0; i < KT; i++) flag[i] = next[i];
     }
     // ---- infinities and NaN of V, to the rows that see them: whatever else a
     // row sums, they decide its result, so they are added to it at the end
@@ -548,7 +523,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         for (int i = 0; i < R; i++) o[d][i] *= inv;
     for (int t0 = 0; t0 <= mine; t0 += 64) {       // (64 flags to a load: one after the other they took longer than a tile)
         if constexpr (DIRECT) odd = mine < 0 ? 0 : odd & (~0ull >> (63 - mine));
-        else odd = __ballot(t0 + lane <= mine && A.flags[tile0 + t0 + lane] & 1);
+        else odd = __ballot(t0 + lane <= mine && A.flags[tile0 + t0 + lane]);
         for (; odd; odd &= odd - 1) {
             const int k0 = (t0 + __ffsll(odd) - 1) * AP_KEYS, k1 = min(min(k0 + AP_KEYS, qi + 1), len);
             for (int k = k0; k < k1; k++) {

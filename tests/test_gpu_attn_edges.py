@@ -5,7 +5,7 @@ import pytest
 
 from attn_fixtures import BF16, F16, F32, HALF, TYPES, View, attention, held, ints, to_type, values
 from test_gpu_attn import CacheCase, check_kv4, close, kv4_tol, kv_values, rng_of, run_kv4, run_prompt
-from test_gpu_attn_wide import kv4_bound, prompt_bound
+from test_gpu_attn_wide import kv4_bound, many, prompt_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -95,12 +95,12 @@ def test_attn_kv4_scores_close_to_one_another(qm, typ, D, rows, large):
 
 # ------------------------------------------------------ values far apart in size --
 
-def one_far_key(r, L, KV, D, at, power, small):
+def one_far_key(r, L, KV, D, at, power, small, key=-120):
     """Normal keys and values (times `small`), but at token `at` a key of -120 in channel 0 and values
     2^power times as large.  For queries that hold 8 there."""
     k, v = r.randn(L, KV, D).astype(np.float32), (small * r.randn(L, KV, D)).astype(np.float32)
     k[:, :, 0] = 0
-    k[at], k[at, :, 0] = 0, -120
+    k[at], k[at, :, 0] = 0, key
     v[at] = v[at] * np.float32(2.0 ** power)
     return k, v
 
@@ -170,3 +170,36 @@ def test_attn_kv4_a_nan_among_values(qm, typ, D, rows):
     gone = np.arange(D) // 64 == 1
     assert np.isnan(got[..., gone]).all() and np.isnan(want[..., gone]).all()
     assert norm_error(got[..., ~gone], want[..., ~gone]) <= kv4_bound(t, D, L)
+
+
+PROMPT_FORMS = [(60, 4), (300, 4), (300, 0)]         # one launch; few workgroups; many (0: as many heads as it takes)
+
+
+def prompt_error(qm, q, k, v, t, heads, but):
+    """Norm-wise error of some of the heads of a prompt over one kv head, all rows but one."""
+    T, H, D = q.shape
+    got = values(run_prompt(qm, q, k, v, [T], t), t)[:, heads]
+    want = attention(values(q, t)[:, heads], values(k, t), values(v, t), np.arange(T), D ** -0.5)[0]
+    rows = np.arange(T) != but
+    return norm_error(got[rows], want[rows])
+
+
+@pytest.mark.parametrize("power", [12, 24, 60, 110])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,H", PROMPT_FORMS)
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_prompt_large_values_of_no_weight(qm, typ, T, H, D, power):
+    """As over the cache; the key is the second of the prompt or one of its last, so that rows meet it
+    before, with and after the others."""
+    t = TYPES[typ]
+    if t == F16:
+        power //= 10
+    r = rng_of(D, T, power, 9)
+    H = H or many(t, D)
+    for at in (1, T - 20):
+        # a weight of e^-60, or e^-120: 2^60 and 2^110 times that are nothing beside the others
+        k, v = one_far_key(r, T, 1, D, at, power, 1.0, -7.5 * D ** 0.5 * (2 if power > 60 else 1))
+        q = far_query(r, T, H, D)
+        q[at, :, 0] = 0                              # in its own row it has weight: that one is large
+        err = prompt_error(qm, *(to_type(x, t) for x in (q, k, v)), t, [0, H // 2, H - 1], at)
+        assert err <= 2 * prompt_bound(t, D, T), at
