@@ -402,7 +402,11 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             }
         }
         // ---- weights, by the maximum so far.  Whether it has to move is seen from
-        // their sum, which is needed in any case: past 2^8, an infinity included.
+        // their sum, which is needed in any case: past 2^8 of the largest weight after a
+        // move (an infinity included).  That is 1, and 2^7 in fp16: 2^15 is still in range,
+        // and weights down to 2^-32 of it are more than nothing (with 1 they ended at
+        // 2^-25, which thousands of keys together can reach).
+        constexpr float LIFT = std::is_same_v<T, TF16> ? 7.0f : 0.0f, FULL = std::is_same_v<T, TF16> ? 32768.0f : 256.0f;
         const float r = NS == 2 ? 1.0f : rs;
         float p[NV], w[NS == 2 ? NV : 1], sum = 0.0f, far = 0.0f;    // w: times V's powers of two
         auto weigh = [&] {
@@ -420,15 +424,15 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         weigh();
         // fp32 calls: nor may an operand pass 2^15.  Its power of two follows the largest w, not V's
         // largest: a key of large values and no weight takes no bits from the others.
-        if (__any(sum > 256.0f || (NS == 2 && far > pow2i(min(ve + 8, 127))))) {
+        if (__any(sum > FULL || (NS == 2 && far > pow2i(min(ve + 8, 127))))) {
             float top = s[0];
 #pragma unroll
             for (int i = 1; i < NV; i++) top = fmaxf(top, s[i]);
             top = query_max<QW>(top) * r;
             // (a query that need not move stays: what others see has no part in its rounding)
-            const bool moves = query_max<QW>(sum) > 256.0f, wide = NS == 2 && query_max<QW>(far) > pow2i(min(ve + 8, 127));
+            const bool moves = query_max<QW>(sum) > FULL, wide = NS == 2 && query_max<QW>(far) > pow2i(min(ve + 8, 127));
             const float was = m;
-            m = moves ? fmaxf(m, top) : m;
+            m = moves ? fmaxf(m, top - LIFT) : m;
             weigh();
             float f = __builtin_amdgcn_exp2f(was - m);
             l *= f;

@@ -203,3 +203,25 @@ def test_attn_prompt_large_values_of_no_weight(qm, typ, T, H, D, power):
         q[at, :, 0] = 0                              # in its own row it has weight: that one is large
         err = prompt_error(qm, *(to_type(x, t) for x in (q, k, v)), t, [0, H // 2, H - 1], at)
         assert err <= 2 * prompt_bound(t, D, T), at
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_prompt_many_small_weights(qm, typ, D):
+    """4095 keys of weights about e^-18 (2^-26) of the first one's, which has values of 0: together
+    they are the result.  Each weight is held to the type's half step, or in fp16 to half its smallest
+    step, 2^-25, of a largest weight of 2^7."""
+    t = TYPES[typ]
+    r = rng_of(D, 83)
+    T, H = 4096, 2
+    q, k, v = np.zeros((T, H, D)), 0.2 * r.randn(T, 1, D), r.randn(T, 1, D) + 2
+    q[..., 0], k[:, 0, 0], v[0] = D ** 0.5, 0.5 * r.randn(T), 0
+    k[0, 0, 0] = 18
+    q, k, v = (to_type(x, t) for x in (q, k, v))
+    got = values(run_prompt(qm, q, k, v, [T], t), t)
+    rows = [0, 1, 1000, 2047, 3000, 4095]
+    want, mag, es = attention(values(q, t)[rows], values(k, t), values(v, t), rows, D ** -0.5)
+    e = es * (3 * 2.0 ** -22 * (t == F32) + (D + 16) * 2.0 ** -24)
+    w = 3 * 2.0 ** -22 if t == F32 else HALF[t]
+    tol = (2 * e + w + (T + 64) * 2.0 ** -24) * mag + HALF[t] * np.abs(want)
+    close(got[rows], want, tol + (T * 2.0 ** -32 * 6 + 2.0 ** -25) * (t == F16) + 1e-30)
