@@ -616,7 +616,9 @@ int qmag_attn_kv4_dev(const qmag_kv4 *c, const qmag_kv_table *t, int type, const
    rows cu[i] .. cu[i + 1] - 1 of q, k, v and out (cu ascending, cu[n_seq] <= T;
    empty sequences are fine; rows behind cu[n_seq] are left as they were).  Heads
    of q share kv heads in runs of q->n_head / k->n_head.  Infinities and NaN at
-   keys that a row does not see have no effect on it. */
+   keys that a row does not see have no effect on it; at those that it sees they
+   count as the formula has them: a score of -inf is no weight, of +inf or NaN a row
+   of NaN, and an infinity of v comes through with its sign. */
 int qmag_attn_prompt_dev(int type, int head_dim, const qmag_heads *q, const qmag_heads *k, const qmag_heads *v,
                          const qmag_heads *out, const int *cu, int n_seq, int T, float scale);
 

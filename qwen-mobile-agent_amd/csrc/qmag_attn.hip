@@ -45,7 +45,7 @@ struct ApArgs {
     const int *cu;
     uint8_t *img;                         // [n_kv][tiles][K image | V image]
     float *scale;                         // [n_kv][tiles][32 of K | 32 of V], fp32 calls
-    int *flags;                           // [n_kv][tiles]: V holds an infinity or a NaN
+    int *flags;                           // [n_kv][tiles][2]: K (fp32 calls), V hold an infinity or a NaN
     int n_seq, T, tiles, n_kv, G;
     float sc;                             // scale * log2 e
     int q_vec, k_vec, v_vec, o_vec;
@@ -175,8 +175,8 @@ struct ApRows {
         }
     }
 
-    // into a tile's image and powers of two; odd: V had an infinity or a NaN (added
-    // where it is seen, not multiplied)
+    // into a tile's image and powers of two; odd: there was an infinity or a NaN, which
+    // is left out and added where it is seen (V's, and those of K that have no two parts)
     __device__ __forceinline__ void lay(bool v, E *img, float *scale, int *odd)
     {
         const int c = threadIdx.x % CH;
@@ -188,7 +188,7 @@ struct ApRows {
             for (int i = 0; i < 8; i++) {
                 const bool fine = fabsf(x[u][i]) <= 3.402823466e38f;
                 top = fmaxf(top, fine ? fabsf(x[u][i]) : 0.0f);
-                if (v && !fine) *odd = 1, x[u][i] = 0.0f;
+                if ((v || NS == 2) && !fine) *odd = 1, x[u][i] = 0.0f;
             }
             E *row = img + (v ? NS * PLANE : 0) + key * D + 8 * (v ? v_chunk<D, QW>(key, c) : k_chunk<D>(key, c));
             V8 hi, lo;
@@ -225,9 +225,9 @@ __global__ void __launch_bounds__(AP_WG) prompt_tiles_kernel(ApArgs A)
     R rows;
     rows.template fetch<true>(A, v, kvh, a, n, part * AP_KEYS);
     rows.lay(v, (typename R::E *)A.img + tile * 2 * R::NS * R::PLANE, A.scale + tile * 2 * AP_KEYS, &odd);
-    if (v) {
+    if (v || R::NS == 2) {
         odd = __syncthreads_or(odd);
-        if (threadIdx.x == 0) A.flags[tile] = odd ? 1 : 0;
+        if (threadIdx.x == 0) A.flags[2 * tile + v] = odd ? 1 : 0;
     }
 }
 
@@ -353,8 +353,9 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         v_at[i] = NS * PLANE + key * D + 8 * v_chunk<D, QW>(key, c >> 3) + (c & 7);
     }
 
-    // One tile of 32 keys; EDGE: the one that holds the wave's own tokens.
-    auto tile = [&](const E *K, const float *sc, auto EDGE) {
+    // One tile of 32 keys from t0; EDGE: the one that holds the wave's own tokens; odd: fp32 calls, K
+    // holds an infinity or a NaN.
+    auto tile = [&](const E *K, const float *sc, int t0, bool odd, auto EDGE) {
         // ---- scores
         Acc sa[NA];
 #pragma unroll
@@ -392,6 +393,23 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
                 const float4 ks = *(const float4 *)(sc + KG * g + 4 * h);
                 s[4 * g] *= rs * ks.x, s[4 * g + 1] *= rs * ks.y;
                 s[4 * g + 2] *= rs * ks.z, s[4 * g + 3] *= rs * ks.w;
+            }
+            if (odd) {
+                // what was left out of the scores, by the definition
+                int key = t0 + 4 * h, row = min(qi, len - 1);
+                asm volatile("" : "+v"(key), "+v"(row));       // (formed here: the registers do not hold addresses across tiles)
+                const float *qp = (const float *)A.q + (int64_t)(a + row) * A.qt + head * A.qh;
+#pragma unroll
+                for (int i = 0; i < NV; i++) {
+                    const float *kp = (const float *)A.k + (int64_t)(a + min(key, len - 1)) * A.kt + kvh * A.kh;
+                    float x = 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < D; c++)
+                        if (!(fabsf(kp[c]) <= 3.402823466e38f)) x = fmaf(kp[c] * A.sc, qp[c], x);
+                    s[i] += x;
+                    key += (i & 3) == 3 ? KG - 3 : 1;
+                    asm volatile("" : "+v"(key));
+                }
             }
         }
         if constexpr (EDGE.value) {                // (keys behind the end are behind every query)
@@ -492,14 +510,21 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 
     const int mine = q0 < len ? q0 / AP_KEYS : -1;           // the wave's last tile
     const int steps = (tiles + KT - 1) / KT;
+    // (as constants: scalar loads, which wait for no step)
+    const auto *flags = (const __attribute__((address_space(4))) int *)(uintptr_t)(A.flags + 2 * tile0);
+    int flag[KT];
+#pragma unroll
+    for (int i = 0; i < KT; i++) flag[i] = NS == 2 && !DIRECT ? flags[2 * i] : 0;
     unsigned long long odd = 0;                    // DIRECT: tiles whose V holds an infinity or a NaN
     for (int step = 0; step < steps; step++) {
         const int b = step & 1;
+        int next[KT] = {};
         if constexpr (DIRECT) {
             int here = 0;
             kr.lay(false, lds[b], lsc[b], &here);
             vr.lay(true, lds[b], lsc[b], &here);
-            if (__syncthreads_or(here)) odd |= 1ull << step;
+            flag[0] = __syncthreads_or(here);      // K's or V's
+            if (flag[0]) odd |= 1ull << step;
             if (step + 1 < steps) {
                 kr.template fetch<false>(A, false, kvh, a, len, (step + 1) * AP_KEYS);
                 vr.template fetch<false>(A, true, kvh, a, len, (step + 1) * AP_KEYS);
@@ -507,15 +532,19 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __syncthreads();
+#pragma unroll
+            for (int i = 0; i < KT; i++) next[i] = NS == 2 ? flags[2 * ((step + 1) * KT + i)] : 0;
             if (step + 1 < steps) load(step + 1, b ^ 1);
         }
 #pragma unroll
         for (int i = 0; i < KT; i++) {
             const int kt = step * KT + i;
             const float *sc = lsc[b] + (NS == 2 ? i * 2 * AP_KEYS : 0);
-            if (kt < mine) tile(lds[b] + i * TILE, sc, std::false_type{});
-            else if (kt == mine) tile(lds[b] + i * TILE, sc, std::true_type{});
+            if (kt < mine) tile(lds[b] + i * TILE, sc, kt * AP_KEYS, NS == 2 && flag[i], std::false_type{});
+            else if (kt == mine) tile(lds[b] + i * TILE, sc, kt * AP_KEYS, NS == 2 && flag[i], std::true_type{});
         }
+#pragma unroll
+        for (int i = 0; i < KT; i++) flag[i] = next[i];
     }
     // ---- infinities and NaN of V, to the rows that see them: whatever else a
     // row sums, they decide its result, so they are added to it at the end
@@ -527,7 +556,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         for (int i = 0; i < R; i++) o[d][i] *= inv;
     for (int t0 = 0; t0 <= mine; t0 += 64) {       // (64 flags to a load: one after the other they took longer than a tile)
         if constexpr (DIRECT) odd = mine < 0 ? 0 : odd & (~0ull >> (63 - mine));
-        else odd = __ballot(t0 + lane <= mine && A.flags[tile0 + t0 + lane]);
+        else odd = __ballot(t0 + lane <= mine && A.flags[2 * (tile0 + t0 + lane) + 1]);
         for (; odd; odd &= odd - 1) {
             const int k0 = (t0 + __ffsll(odd) - 1) * AP_KEYS, k1 = min(min(k0 + AP_KEYS, qi + 1), len);
             for (int k = k0; k < k1; k++) {
@@ -570,7 +599,7 @@ static int ap_run(ApArgs A, hipStream_t s)
         return QMAG_OK;
     }
     int st;
-    uint8_t *ws = (uint8_t *)workspace(WS_ATTN, n * (TILE + (NS == 2 ? 2 * AP_KEYS * sizeof(float) : 0) + sizeof(int)), &st);
+    uint8_t *ws = (uint8_t *)workspace(WS_ATTN, n * (TILE + (NS == 2 ? 2 * AP_KEYS * sizeof(float) : 0) + 2 * sizeof(int)), &st);
     if (st) return st;
     A.img = ws;
     A.scale = (float *)(ws + n * TILE);

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from attn_fixtures import BF16, F16, F32, HALF, TYPES, View, attention, held, ints, to_type, values
-from test_gpu_attn import CacheCase, check_kv4, close, kv4_tol, kv_values, rng_of, run_kv4, run_prompt
+from test_gpu_attn import CacheCase, check_kv4, close, kv4_tol, kv_values, prompt_tol, rng_of, run_kv4, run_prompt
 from test_gpu_attn_wide import kv4_bound, many, prompt_bound
 
 pytestmark = pytest.mark.gpu
@@ -225,3 +225,53 @@ def test_attn_prompt_many_small_weights(qm, typ, D):
     w = 3 * 2.0 ** -22 if t == F32 else HALF[t]
     tol = (2 * e + w + (T + 64) * 2.0 ** -24) * mag + HALF[t] * np.abs(want)
     close(got[rows], want, tol + (T * 2.0 ** -32 * 6 + 2.0 ** -25) * (t == F16) + 1e-30)
+
+
+# -------------------------------------------------------------------- infinite keys --
+
+def weigh64(q, k, v, scale):
+    """One head of one prompt in 64 bits, infinite and NaN scores as they fall."""
+    with np.errstate(all="ignore"):
+        s = (q[:, None] * k[None]).sum(-1) * scale
+        s[np.triu_indices(len(s), 1)] = -np.inf
+        seen = np.tril(np.ones(s.shape, bool))
+        p = np.where(seen, np.exp(s - np.where(seen, s, -np.inf).max(1, keepdims=True)), 0)
+        return p @ v / p.sum(1, keepdims=True)
+
+
+@pytest.mark.parametrize("scale", [0.125, -0.125, 0.0])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,H", PROMPT_FORMS)
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_prompt_infinite_keys(qm, typ, T, H, D, scale):
+    """A score of -inf is no weight, of +inf or NaN (infinities that meet, 0 times one) a row of NaN;
+    a row that sees nothing else is NaN.  Rows that do not see the key are as they were."""
+    t = TYPES[typ]
+    r = rng_of(D, T, 84)
+    H = H or many(t, D)
+    heads = [0, H // 2, H - 1]
+    q, k, v = r.randn(T, H, D), r.randn(T, 1, D), r.randn(T, 1, D)
+    q[..., 3] = -np.abs(q[..., 3])
+    q[30, :, 5], q[31, :, 3] = 0, 0
+    clean = [to_type(x, t) for x in (q, k, v)]
+    plain = values(run_prompt(qm, *clean, [T], t, scale=scale), t)[:, heads]
+    qf, _, vf = (values(x, t) for x in clean)
+    for places in ({(8, 3): np.inf}, {(0, 3): np.inf}, {(20, 5): -np.inf}, {(9, 3): np.inf, (9, 5): np.inf, (40, 3): np.inf},
+                   {(12, 3): np.inf, (33, 3): np.inf, (T - 1, 3): np.inf}, {(T - 2, 7): np.nan}):
+        k2 = k.copy()
+        for (at, c), x in places.items():
+            k2[at, 0, c] = x
+        a = [clean[0], to_type(k2, t), clean[2]]
+        got = values(run_prompt(qm, *a, [T], t, scale=scale), t)[:, heads]
+        first = min(at for at, _ in places)
+        assert np.array_equal(got[:first], plain[:first])
+        kf = values(a[1], t)
+        kz = np.where(np.isfinite(kf), kf, 0)
+        for j, h in enumerate(heads):
+            want = weigh64(qf[:, h], kf[:, 0], vf[:, 0], scale)
+            _, mag, es = attention(qf[:, h:h + 1], kz, vf, np.arange(T), scale)
+            nan = np.isnan(want)
+            assert np.array_equal(np.isnan(got[:, j]), nan), (places, h)
+            # a key without weight leaves the others the more: up to all of what the rows' first keys had
+            tol = prompt_tol(t, D, T, want, 8 * mag[:, 0] + 8, es[:, 0])
+            close(np.where(nan, 0, got[:, j]), np.where(nan, 0, want), np.where(nan, 1, tol), (places, h))
