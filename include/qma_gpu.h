@@ -538,7 +538,8 @@ typedef struct qmag_kv_table {
     int *free_list;     /* i32 [n_block] (not used by qmag_attn_kv4_dev) */
 } qmag_kv_table;
 
-/* What the bookkeeping calls leave in *status (device): */
+/* What the bookkeeping calls leave in *status (device); of several faults the
+   length's, then the row's, the list's, too few blocks: */
 #define QMAG_KV_OK 0
 #define QMAG_KV_FULL 1    /* too few free blocks */
 #define QMAG_KV_ROW 2     /* a sequence of more than max_blocks blocks */

@@ -90,7 +90,6 @@ __device__ __forceinline__ int pg_plan(const PgArgs &A, int *tok, int *blk, int 
             if (len < 0) bad |= 1;
             else if ((n = pg_blocks(len, A.shift)) > A.max_blocks) bad |= 2;
         }
-        if (bad) n = t = 0;
         if (ASSIGN) tok[i] = t, held[i] = len;
         blk[i] = n;
         mine.tok += t;

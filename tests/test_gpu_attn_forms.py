@@ -152,3 +152,28 @@ def test_assign_of_a_million_tokens(qm):
     back = [x for i in range(2) for x in want[1][i, :-(-want[5][i] // bs)]]
     assert st.download(np.int32)[0] == 0 and nf.download(np.int32)[0] == n_block
     assert np.array_equal(pool.read()[1][want[6]:want[6] + len(back)], back)
+
+
+@pytest.mark.parametrize("n_seq", [3, 256, 257, 600, 4096])
+def test_assign_and_release_of_several_faults(qm, n_seq):
+    """The status is the same whichever sequences have the faults: a length ahead of a row ahead of the
+    list ahead of too few blocks."""
+    bs, max_blocks, n_block, T = 16, 4, 12, 100
+    pool = Pool(qm, n_seq, max_blocks, bs, n_block, np.full((n_seq, max_blocks), -1), np.arange(n_block))
+    row, many_, neg = (70, 0), (0, 101), (0, -1)
+
+    def assign(faults, top):
+        held_, new = np.zeros(n_seq, int), np.zeros(n_seq, int)
+        for at, (h, w) in faults.items():
+            held_[at], new[at] = h, w
+        return run_assign(qm, pool, held_, new, top, T)["status"][0]
+    for i, j in ((0, 1), (1, 0), (0, n_seq - 1), (n_seq - 2, n_seq - 1), (n_seq - 1, n_seq - 2)):
+        assert assign({i: row, j: many_}, 12) == 3 and assign({i: row, j: neg}, 12) == 3
+        assert assign({i: row, j: (0, 30)}, 13) == 2 and assign({i: (0, 60), j: (0, 30)}, 13) == 4
+        assert assign({i: (0, 60), j: (0, 30)}, 5) == 1 and assign({i: (0, 60), j: (0, 30)}, 6) == 0
+        held_, ended = np.zeros(n_seq, int), np.zeros(n_seq, int)
+        held_[[i, j]], ended[[i, j]] = (70, -1), 1
+        ln, nf, st = ints(qm, held_), ints(qm, [9]), ints(qm, [9])
+        a, b, c = ints(qm, held_), ints(qm, ended), ints(qm, [0])
+        qm.kv_release_dev(pool.c, a.ptr, b.ptr, c.ptr, ln.ptr, nf.ptr, st.ptr)
+        assert st.download(np.int32)[0] == 3
