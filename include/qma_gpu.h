@@ -518,7 +518,7 @@ typedef struct qmag_rope {
     int sections[4];    /* pairs of each axis, n_rot / 2 together */
     int interleaved;    /* 0: the axes' pairs in runs; 1: in turns, an axis whose pairs are used up passed over */
     int adjacent;       /* 0: pair i is values i and i + n_rot / 2; 1: values 2 i and 2 i + 1 */
-    double theta;       /* > 0 */
+    double theta;       /* > 0, and no angle of a position of 2^31 beyond 64 bits */
 } qmag_rope;
 /* pos: i32 [n_axes][T].  src -> dst for n_views (1 or 2: q and k) views; a dst
    equal to its src turns in place.  Angles are formed in 64 bits. */

@@ -135,6 +135,7 @@ extern "C" int qmag_rope_dev(const qmag_rope *r, const int *pos, int T, int type
         left[a]--;
         if (r->interleaved) a = (a + 1) % r->n_axes;
         A.turns[i] = pow(r->theta, -2.0 * i / r->n_rot) / (2.0 * M_PI);
+        if (!isfinite(A.turns[i] * 2147483648.0)) return fail(QMAG_ERR_ARG, "rope: theta=%g, whose angles leave 64 bits", r->theta);
     }
     A.pos = pos;
     A.T = T;

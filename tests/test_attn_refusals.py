@@ -252,3 +252,10 @@ def test_read_results_over_what_it_reads(lib):
     assert read(s, k, v) == NODEV and read(s, k, k + n) == NODEV and read(s, k, k + n - 4) == ARG and read(s, k, k) == ARG
     assert read(k + n - 4, k, v) == ARG and read(v - 12, k, v) == ARG and read(k + n, k, v) == NODEV
     assert read(s, A, v) == ARG and read(s, k, A + size - 16) == ARG and read(s, k, A + size) == NODEV
+
+
+@pytest.mark.parametrize("theta,ok", [(1e-320, False), (1e-306, False), (1e-300, True), (1e-3, True), (1.0, True), (1e300, True)])
+def test_rope_frequencies_are_numbers(lib, theta, ok):
+    """theta^(-2 i / n_rot) times the largest position has to stay in range: 0 times an infinity is no angle.
+    (1e-300: 10^(300 x 126 / 128) 2^31 / 2 pi = 10^304.)"""
+    assert rope_call(lib, theta=theta, rot=128, sections=(64,)) == (NODEV if ok else ARG)
