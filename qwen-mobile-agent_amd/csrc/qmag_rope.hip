@@ -3,8 +3,9 @@
 //
 // Pair i of a head turns by a = pos[axis(i)][t] * theta^(-2 i / n_rot):
 //   y_i = x_i cos a - x_j sin a,   y_j = x_i sin a + x_j cos a.
-// Far positions make a large: it is formed in turns (a / 2 pi) in 64 bits, its
-// whole turns dropped exactly, and only the fraction goes to fp32.
+// Far positions make a large: it is formed in turns (a / 2 pi) in 64 bits and its
+// whole turns dropped exactly.  The fraction goes to fp32, and what that leaves of it
+// (up to 2 pi 2^-26, much beside a sine near half a turn) is added to first order.
 //
 // A workgroup takes one token and some of its heads: the token's cosines and
 // sines go to LDS once, then each thread turns 16 bytes of pairs.  Memory
@@ -50,9 +51,10 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs A)
         if (tid < A.pairs) {
             double r = (double)A.pos[A.axis[tid] * (int64_t)A.T + t] * A.turns[tid];
             r -= rint(r);
+            const float f = (float)r, rest = (float)((r - (double)f) * (2.0 * M_PI));
             float s, c;
-            sincospif(2.0f * (float)r, &s, &c);
-            cs[tid] = make_float2(c, s);
+            sincospif(2.0f * f, &s, &c);
+            cs[tid] = make_float2(fmaf(-rest, s, c), fmaf(rest, c, s));
         }
         __syncthreads();
         for (int h = h0 + (tid >> A.unit_shift); h < h1; h += per) {

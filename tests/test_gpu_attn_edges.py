@@ -3,7 +3,7 @@ none, values far apart in size, infinite keys, the forms that only large calls t
 import numpy as np
 import pytest
 
-from attn_fixtures import BF16, F16, F32, HALF, TYPES, View, attention, held, ints, to_type, values
+from attn_fixtures import BF16, F16, F32, HALF, TYPES, View, attention, held, ints, rope, to_type, values
 from test_gpu_attn import CacheCase, check_kv4, close, kv4_tol, kv_values, prompt_tol, rng_of, run_kv4, run_prompt
 from test_gpu_attn_wide import kv4_bound, many, prompt_bound
 
@@ -275,3 +275,24 @@ def test_attn_prompt_infinite_keys(qm, typ, T, H, D, scale):
             # a key without weight leaves the others the more: up to all of what the rows' first keys had
             tol = prompt_tol(t, D, T, want, 8 * mag[:, 0] + 8, es[:, 0])
             close(np.where(nan, 0, got[:, j]), np.where(nan, 0, want), np.where(nan, 1, tol), (places, h))
+
+
+# ------------------------------------------------------------------------- angles --
+
+def test_rope_near_half_turns(qm):
+    """Angles close to odd and even multiples of pi, whose sines are 1e-5 to 1e-2: each comes out with
+    the digits of fp32, as an angle formed in 64 bits has them (its frequency and product off by 2^-53
+    each, pi by as much; sine and cosine by 2 of their own steps, the rest roundings)."""
+    at = np.arange(1, 1 << 20)
+    pos = at[np.abs(np.sin(at)) < 2e-3]
+    T, D = len(pos), 64
+    assert 355 in pos and T > 1000
+    x = np.zeros((T, 1, D), np.float32)
+    x[..., 0], x[1::2, :, 32] = 1, 1e-4
+    xd, od = View(qm, x, F32), View(qm, np.zeros_like(x), F32)
+    qm.rope_dev(qm.Rope.make(D, D, (32,), False, False, 1e4), ints(qm, pos).ptr, T, F32, xd.heads, od.heads)
+    want = rope(x.astype(np.float64), pos[None], D, (32,), False, False, 1e4)
+    got = od.read()[0].astype(np.float64)
+    for c, other in ((0, 32), (32, 0)):
+        a, b = np.abs(x[:, 0, c] * np.cos(pos)), np.abs(x[:, 0, other] * np.sin(pos))
+        close(got[:, 0, c], want[:, 0, c], (a + b) * 5 * 2.0 ** -24 + 2.0 ** -51 * pos)
