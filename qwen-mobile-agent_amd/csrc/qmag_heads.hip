@@ -75,9 +75,10 @@ bool heads_overlap(const qmag_heads *a, const qmag_heads *b, int size, int dim, 
         side_by_side(apart, a->token_stride, extent(a, dim, 1), extent(b, dim, 1)))
         return false;
     const int64_t hs = a->n_head > 1 ? a->head_stride : b->head_stride;
+    const bool heads_alike = (a->n_head == 1 || a->head_stride == hs) && (b->n_head == 1 || b->head_stride == hs);
+    if (heads_alike && side_by_side(apart, hs, (n_tok - 1) * a->token_stride + dim, (n_tok - 1) * b->token_stride + dim)) return false;
     const bool whole = hs > 0 && a->token_stride % hs == 0 && b->token_stride % hs == 0;
-    if (whole && (a->n_head == 1 || a->head_stride == hs) && (b->n_head == 1 || b->head_stride == hs) &&
-        side_by_side(apart, hs, dim, dim))
+    if (whole && heads_alike && side_by_side(apart, hs, dim, dim))
         return false;
     return true;
 }

@@ -259,3 +259,15 @@ def test_rope_frequencies_are_numbers(lib, theta, ok):
     """theta^(-2 i / n_rot) times the largest position has to stay in range: 0 times an infinity is no angle.
     (1e-300: 10^(300 x 126 / 128) 2^31 / 2 pi = 10^304.)"""
     assert rope_call(lib, theta=theta, rot=128, sections=(64,)) == (NODEV if ok else ARG)
+
+
+def test_views_side_by_side_within_heads(lib):
+    """[head][q's tokens, k's tokens, ...] in one buffer: apart, unless a token reaches into the next view."""
+    S, D, T = 4096, 64, 8                                    # values to a head, of a token, tokens
+    at = lambda i, n=2: (A + int(4 * i * T * D), n, D, S)    # noqa: E731
+    assert rope_call(lib, dim=D, T=T, src=(at(0), at(1)), dst=(at(2), at(3))) == NODEV
+    assert rope_call(lib, dim=D, T=T, src=(at(0), at(1)), dst=(at(2), at(2.5))) == ARG
+    assert rope_call(lib, dim=D, T=T, src=(at(0), at(1)), dst=(at(0.5), at(3))) == ARG
+    assert rope_call(lib, dim=D, T=T + 1, src=(at(0), at(1)), dst=(at(2), at(3))) == ARG
+    assert rope_call(lib, dim=D, T=T, src=(at(0, 5), at(1, 1)), dst=(at(2, 5), at(3, 1))) == NODEV
+    assert rope_call(lib, dim=D, T=T, src=(at(0, 5), at(1)), dst=(at(7, 5), at(8))) == ARG      # behind its head: in the next one's first view

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 from attn_fixtures import BF16, F16, F32, HALF, TYPES, View, attention, held, ints, rope, to_type, values
-from test_gpu_attn import (CacheCase, Pool, assign_ref, check_kv4, close, kv4_tol, kv_values, rng_of, run_assign, run_kv4)
+from test_gpu_attn import (CacheCase, Pool, assign_ref, check_kv4, close, kv4_tol, kv_values, prompt_tol, rng_of, run_assign,
+                           run_kv4)
 
 pytestmark = pytest.mark.gpu
 
@@ -177,3 +178,72 @@ def test_assign_and_release_of_several_faults(qm, n_seq):
         a, b, c = ints(qm, held_), ints(qm, ended), ints(qm, [0])
         qm.kv_release_dev(pool.c, a.ptr, b.ptr, c.ptr, ln.ptr, nf.ptr, st.ptr)
         assert st.download(np.int32)[0] == 3
+
+
+# ------------------------------------------------------------------------- far apart --
+
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+def test_strides_beyond_32_bits(qm, layout):
+    """q, k, v and the results side by side in rows 2^31 values apart: by token, and by head."""
+    t, D, S, gap = BF16, 64, (1 << 31) + 64, 512
+    T, H = (3, 2) if layout == "tokens" else (40, 3)
+    rows, inner = (T, H) if layout == "tokens" else (H, T)                # rows far apart, values within them
+    r = rng_of(T, H, 97)
+    a = {n: to_type(r.randn(T, H, D), t) for n in "qkv"}
+    at = {n: i * inner * D for i, n in enumerate(("q", "k", "v", "rq", "rk", "op", "oc"))}
+    buf = qm.DBuf(2 * ((rows - 1) * S + 7 * inner * D + gap))
+    strides = (S, D) if layout == "tokens" else (D, S)
+    view = lambda n: qm.heads((buf.ptr + 2 * at[n], H, *strides))  # noqa: E731
+    near = lambda x: x if layout == "tokens" else x.transpose(1, 0, 2)  # noqa: E731
+
+    def put(n, x):
+        for i, row in enumerate(near(x)):
+            buf.upload(np.ascontiguousarray(row), 2 * (i * S + at[n]))
+
+    def get(n):
+        got = np.stack([buf.download(np.uint16, inner * D, 2 * (i * S + at[n])) for i in range(rows)])
+        return values(near(got.reshape(rows, inner, D)), t)
+    for n in "qkv":
+        put(n, a[n])
+    pos, cu, slot = ints(qm, np.arange(T)), ints(qm, [0, T]), ints(qm, np.arange(T))
+    both = lambda x, y: (qm.Heads * 2)(view(x)[0], view(y)[0])  # noqa: E731
+    qm.rope_dev(qm.Rope.make(D, D, (32,), theta=1e4), pos.ptr, T, t, both("q", "k"), both("rq", "rk"))
+    qf, kf, vf = (values(a[n], t) for n in "qkv")
+    for n, x in (("rq", qf), ("rk", kf)):
+        want = rope(x, np.arange(T)[None], D, (32,), False, False, 1e4)
+        close(get(n), want, (HALF[t] + 2.0 ** -20) * np.abs(x).max() * 2)
+    tq, tk = get("rq"), get("rk")
+    qm.attn_prompt_dev(t, D, view("rq"), view("rk"), view("v"), view("op"), cu.ptr, 1, T, 0.125)
+    want, mag, es = attention(tq, tk, vf, np.arange(T), 0.125)
+    close(get("op"), want, 2 * HALF[t] * (mag + np.abs(want)) + 1e-4)
+    cache = qm.DBuf(4 * H * 16 * (D + D // 8))
+    c = qm.Kv4(cache.ptr, 4, 16, H, D)
+    qm.kv4_append_dev(c, t, view("rk"), view("v"), slot.ptr, T)
+    table, lens = ints(qm, [[0, 1, 2, 3]]), ints(qm, [T])
+    kt = qm.KvTable(1, 4, 16, 4, table.ptr, None)
+    qm.attn_kv4_dev(c, kt, t, view("rq"), view("oc"), cu.ptr, lens.ptr, T, 0.125)
+    hk, hv = held(tk.astype(np.float32)), held(vf.astype(np.float32))
+    want, mag, es = attention(tq, hk, hv, np.arange(T), 0.125)
+    close(get("oc"), want, kv4_tol(t, D, T, want, mag, es))
+
+
+@pytest.mark.parametrize("typ", ["f16", "f32"])
+def test_attn_prompt_of_a_million_tokens(qm, typ):
+    """4096 prompts of up to 500 tokens, the largest list of them."""
+    t = TYPES[typ]
+    r = rng_of(98)
+    lens = r.randint(0, 500, 4096)
+    T, D = int(lens.sum()), 64
+    base = [to_type(r.randn(5000, 1, D), t) for _ in range(3)]
+    pick = [r.randint(0, 5000, T) for _ in range(3)]
+    q, k, v = (b[p] for b, p in zip(base, pick))
+    views = [View(qm, x, t) for x in (q, k, v)]
+    out = View(qm, np.zeros_like(q), t)
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    qm.attn_prompt_dev(t, D, *[x.heads for x in views], out.heads, ints(qm, cu).ptr, 4096, T, 0.125)
+    got = out.read()[0]
+    for i in [0, 1, 63, 64, 65, 2047, 4000, 4094, 4095]:
+        s = slice(cu[i], cu[i + 1])
+        if lens[i]:
+            want, mag, es = attention(*(values(x[s], t) for x in (q, k, v)), np.arange(lens[i]), 0.125)
+            close(values(got[s], t), want, prompt_tol(t, D, int(lens[i]), want, mag, es), i)
