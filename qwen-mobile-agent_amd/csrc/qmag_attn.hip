@@ -391,8 +391,9 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
             for (int g = 0; g < NV / 4; g++) {
                 const float4 ks = *(const float4 *)(sc + KG * g + 4 * h);
-                s[4 * g] *= rs * ks.x, s[4 * g + 1] *= rs * ks.y;
-                s[4 * g + 2] *= rs * ks.z, s[4 * g + 3] *= rs * ks.w;
+                // (one after the other: together the two may leave the range, and 0 times that is no score)
+                s[4 * g] = s[4 * g] * rs * ks.x, s[4 * g + 1] = s[4 * g + 1] * rs * ks.y;
+                s[4 * g + 2] = s[4 * g + 2] * rs * ks.z, s[4 * g + 3] = s[4 * g + 3] * rs * ks.w;
             }
             if (odd) {
                 // what was left out of the scores, by the definition

@@ -296,3 +296,19 @@ def test_rope_near_half_turns(qm):
     for c, other in ((0, 32), (32, 0)):
         a, b = np.abs(x[:, 0, c] * np.cos(pos)), np.abs(x[:, 0, other] * np.sin(pos))
         close(got[:, 0, c], want[:, 0, c], (a + b) * 5 * 2.0 ** -24 + 2.0 ** -51 * pos)
+
+
+@pytest.mark.parametrize("T,H", PROMPT_FORMS)
+@pytest.mark.parametrize("D", [64, 256])
+def test_attn_prompt_huge_and_apart(qm, T, H, D):
+    """Queries and keys of 1e38 in channels of their own: scores of 0, whose two powers of two together
+    leave fp32's range."""
+    r = rng_of(T, D, 85)
+    H = H or many(F32, D)
+    q, k, v = np.zeros((T, H, D), np.float32), np.zeros((T, 1, D), np.float32), r.randn(T, 1, D).astype(np.float32)
+    q[..., ::2], k[..., 1::2] = 1e38, -1e38
+    got = run_prompt(qm, q, k, v, [T], F32)[:, [0, H - 1]].astype(np.float64)
+    want = np.cumsum(v[:, 0].astype(np.float64), 0) / np.arange(1, T + 1)[:, None]
+    mag = np.cumsum(np.abs(v[:, 0]).astype(np.float64), 0) / np.arange(1, T + 1)[:, None]
+    for h in range(2):
+        close(got[:, h], want, (3 * 2.0 ** -22 + (T + 64) * 2.0 ** -24) * mag)
