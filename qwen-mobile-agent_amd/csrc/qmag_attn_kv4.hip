@@ -327,8 +327,13 @@ constexpr int ak_tile() { return 36 * D; }
 // 2 the join of the waves, the rest the launch.  A batch is bound by the vector
 // instructions that turn codes into operands and by memory together: 32 sequences
 // of up to 16,384 tokens (bf16, 32 heads of 128; 163 MB) 41 us, 4.0 TB/s.
+
+// how many of its workgroups of 4 waves LDS and registers let a CU hold
+template <class T, int D>
+constexpr int few_resident() { return D == 256 ? 2 : D == 128 && sizeof(typename T::S) == 4 ? 3 : 4; }
+
 template <class T, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 && sizeof(typename T::S) == 4 ? 3 : 4) attn_kv4_kernel(AkArgs A)
+__global__ void __launch_bounds__(64 * NW, (few_resident<T, D>())) attn_kv4_kernel(AkArgs A)
 {
     using S = typename T::S;
     constexpr int NS = sizeof(S) == 4 ? 2 : 1;
@@ -1018,11 +1023,13 @@ static int ak_launch(AkArgs A, hipStream_t s)
     constexpr int NW = ROWS ? 8 : 4, RG = ROWS ? 16 * NW : 16, STEP = ROWS ? 32 : 32 * NW;
     // Row groups at most.  Chunks are cut for as many workgroups as the chip holds at
     // once: of more the last ones run alone, of fewer some CUs get two and others none.
-    // (Heads of 256 for 4 of a CU instead of the 2 that its LDS holds: 41.2 us against
-    // 37.2 for 131,072 tokens, 31.4 against 27.6 for four sequences of up to 8192; of 128
-    // for 4 instead of 3: 48.5 against 47.5 for 32 sequences, 35.4 against 34.8 for 8.)
+    // (They are whole steps, so that between half and all of that many run.  Heads of 256
+    // for 4 of a CU instead of the 2 that its LDS holds: 40.4 us against 36.0 for 131,072
+    // tokens, 43.5 against 34.8 for 48 sequences; heads of 128 in 16 bits for 3 instead of 4:
+    // 52.1 against 50.8 for 32 sequences, 38.0 against 36.8 for 8, 42.5 against 43.2 for one
+    // of 131,072 tokens; of 64 for 3 instead of 4: 37.9 against 35.4, 25.7 against 24.7.)
     const int64_t groups = ak_most_groups(A.T, A.G, RG, A.n_seq);
-    const int64_t goal = (ROWS ? rows_resident<T, D>() : D == 256 ? 2 : 3) * (int64_t)ctx().n_cu;
+    const int64_t goal = (ROWS ? rows_resident<T, D>() : few_resident<T, D>()) * (int64_t)ctx().n_cu;
     A.target = (int)((goal + A.n_kv - 1) / A.n_kv);
     // enough row groups to fill the chip twice over: nothing is split
     A.min_chunk = ((int64_t)A.T * A.G / RG) * A.n_kv >= 2 * goal ? 0 : 128;

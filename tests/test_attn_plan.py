@@ -105,7 +105,7 @@ def test_any_lengths(walk, seed):
         blocks, shift = int(r.choice([1, 7, 100, 3000])), int(r.choice([4, 6]))
         cu = r.randint(-3, T + 4, n + 1) if r.rand() < 0.7 else r.choice([0, T, -2 ** 31, 2 ** 31 - 1, T // 2], n + 1)
         lens = np.where(r.rand(n) < 0.2, r.choice([0, 2 ** 31 - 1, -2 ** 31, blocks << shift], n), r.randint(0, (blocks << shift) + 9, n))
-        calls.append(call(cu, lens, T, n_kv, int(r.choice([1, 3, 8])), int(r.choice([16, 128])), int(r.choice([256, 512, 768])),
+        calls.append(call(cu, lens, T, n_kv, int(r.choice([1, 3, 8])), int(r.choice([16, 128])), int(r.choice([256, 512, 768, 1024])),
                           blocks, shift, int(r.choice([128, 128, 128, 0]))))
     walk(calls)
 
@@ -122,6 +122,6 @@ def test_ascending_lengths_have_room(walk, seed):
         cap = blocks << shift
         lens = r.choice([np.full(n, cap), r.randint(0, cap + 1, n), np.where(np.arange(n) == n // 2, cap, min(cap, 5)),
                          np.exp(r.uniform(0, np.log(cap + 1), n)).astype(np.int64).clip(0, cap)][r.randint(4)], n)
-        calls.append(call(cu, lens, T, n_kv, int(r.choice([1, 3, 8])), int(r.choice([16, 128])), int(r.choice([256, 512, 768])),
+        calls.append(call(cu, lens, T, n_kv, int(r.choice([1, 3, 8])), int(r.choice([16, 128])), int(r.choice([256, 512, 768, 1024])),
                           blocks, shift, int(r.choice([128, 128, 0]))))
     walk(calls)

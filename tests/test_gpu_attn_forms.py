@@ -34,7 +34,7 @@ def test_attn_kv4_a_wide_table_of_short_sequences(qm):
 
 
 @pytest.mark.parametrize("typ", TYPES)
-@pytest.mark.parametrize("D,n,H", [(64, 512, 48), (128, 768, 32), (256, 512, 32)])
+@pytest.mark.parametrize("D,n,H", [(64, 700, 48), (128, 1030, 32), (256, 512, 32)])
 def test_attn_kv4_rows_that_fill_the_chip(qm, typ, D, n, H):
     """Decode of so many rows that no sequence is split, a long one among them."""
     t = TYPES[typ]
