@@ -490,8 +490,10 @@ int qmag_sampler_sample_dev(int n_vocab, const float *logits, qmag_sampler *s, i
    at a time, as the other device entries.  Activations are f32, f16 or bf16
    (`type`: QMAG_TYPE_F32 / _F16 / _BF16), one type for all of a call's views.
    f32 calls keep fp32 accuracy (about 2^-22 of a row's largest value in each
-   operand); 16-bit calls hold weights to the type's own bits and round the
-   result once.  Scores, sums and maxima are fp32. */
+   operand, a weight times its value 2^-22 of itself down to 2^-32 of the row's
+   largest such product); 16-bit calls hold weights to the type's own bits (over
+   the cache to fp16's) and round the result once.  Scores, sums and maxima are
+   fp32. */
 
 /* Heads in memory: value c of head h of token t lies at
    ptr[t * token_stride + h * head_stride + c], strides in values.  q of the
@@ -607,8 +609,10 @@ int qmag_kv4_read_dev(const qmag_kv4 *c, const int *slot, int T, float *k, float
    be left as they were), and nothing but rows of out is written.  A table entry outside the cache stands for tokens that are not
    there.  What the cache holds where a row does not see has no effect on it.
    t->n_block and block_size are the cache's; max_blocks * block_size <= 2^30.
-   Sequences are split over the chip by their lengths and joined in a fixed
-   order: equal calls give equal bits. */
+   Sequences are split over the chip by their lengths, unless the call's rows
+   fill it twice over, and joined in a fixed order: equal calls give equal bits.
+   One call takes one form, by the mean number of rows to a sequence: a prompt's
+   chunk of some hundred tokens and sequences that decode are faster as two. */
 #define QMAG_ATTN_MAX_TOKENS (1 << 22)
 int qmag_attn_kv4_dev(const qmag_kv4 *c, const qmag_kv_table *t, int type, const qmag_heads *q, const qmag_heads *out,
                       const int *cu, const int *len, int T, float scale);

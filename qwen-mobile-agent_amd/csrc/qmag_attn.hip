@@ -14,7 +14,10 @@
 // 16-bit calls multiply in their own type.  fp32 calls are carried by the fp16
 // matrix cores, 16 times the fp32 ones' rate: every row of Q, K and V is scaled
 // by a power of two (exact) and split into two fp16 parts, x = hi + lo to 22
-// bits, and a product is hi hi + hi lo + lo hi.
+// bits, and a product is hi hi + hi lo + lo hi.  16-bit calls round a weight to
+// their type for the second product, not for the sum: as much again as the rounding
+// of the result (bf16 2.1e-3 of it in all, the result's rounding 1.6e-3; summed as
+// rounded it would be 1.8e-3 where few keys count and no less where many do).
 //
 // S^T = K Q^T by v_mfma_f32_32x32x16 leaves a lane with one query (n = lane % 32)
 // and keys 8 (r / 4) + 4 (lane / 32) + r % 4 of a tile, by v_mfma_f32_16x16x32
@@ -25,10 +28,10 @@
 // Bound by the matrix and vector units in turn: a tile of 32 x 32 scores of heads
 // of 128 is 512 cycles of products and about 500 of vector instructions, half of
 // them exponentials (a quarter rate), on a SIMD that three waves share.  Measured,
-// both launches: bf16, 8192 tokens in five prompts, 32 heads of 128 over 8: 371 us,
-// 826 TFLOP/s (a large bf16 product in the library: 1223); fp32, 4096 tokens, 16
-// heads of 256 over 2: 424 us, 324 TFLOP/s, or 972 of fp16 products (library: 1179;
-// its fp32 ones 153).  The first launch is 16 and 11 us of these.
+// both launches: bf16, 8192 tokens in five prompts, 32 heads of 128 over 8: 364 us,
+// 843 TFLOP/s (a large bf16 product in the library: 1223); fp32, 4096 tokens, 16
+// heads of 256 over 2: 421 us, 326 TFLOP/s, or 979 of fp16 products (library: 1179;
+// its fp32 ones 153).  The first launch is 16 and 12 us of these.
 #include <type_traits>
 
 #include "qmag_attn.h"
@@ -615,16 +618,16 @@ static int ap_launch(const ApArgs &A, hipStream_t s)
 {
     constexpr bool F32 = sizeof(typename T::S) == 4;
     // Few tokens: one launch, every workgroup lays its tiles out itself.  With / without:
-    // one token 8.6 / 11.7 us (fp32, 16 heads of 256) and 4.9 / 8.0 (bf16, 32 of 128), 64
-    // tokens 14.8 / 16.8 and 8.9 / 10.3, 128 tokens 27 / 22 and 12.1 / 11.3.  (The lengths
+    // one token 8.7 / 10.9 us (fp32, 16 heads of 256) and 4.9 / 7.2 (bf16, 32 of 128), 64
+    // tokens 15.3 / 16.7 and 8.9 / 10.2, 128 tokens 27.7 / 21.4 and 12.1 / 11.3.  (The lengths
     // are the device's: of several prompts none is taken to have all tokens.)
     if (A.T <= (D == 64 ? 128 : D == 128 ? 96 : 64) * (A.n_seq > 1 ? 3 : 2) / 2)
         return ap_run<T, D, D == 256 ? 8 : 4, 16, 1, 3, 2, true>(A, s);
     // Few workgroups of 128 queries: 64 to a workgroup, which leaves twice as many.  With /
-    // without, at these counts of the large ones: fp32, heads of 256: 208 129 / 132 us, 256
-    // 196 / 162; of 128: 416 91 / 95, 512 133 / 128; of 64: 800 130 / 135, 960 175 / 176; 16
-    // bits, of 256: 384 119 / 129, 640 279 / 273; of 128: 640 88 / 91, 768 123 / 114; of 64:
-    // 960 81 / 88, 1600 184 / 181.
+    // without, at these counts of the large ones: fp32, heads of 256: 208 125 / 132 us, 256
+    // 191 / 163; of 128: 416 88 / 93, 512 130 / 124; of 64: 800 129 / 134, 960 174 / 173; 16
+    // bits, of 256: 384 118 / 129, 640 277 / 272; of 128: 640 86 / 91, 768 117 / 112; of 64:
+    // 960 80 / 88, 1600 182 / 180.
     const int64_t wgs = ((int64_t)A.T / 128 + (A.T < A.n_seq ? A.T : A.n_seq)) * A.n_kv * A.G;
     if (wgs < (int64_t)ctx().n_cu * (F32 ? 1024 / D : D == 64 ? 16 : 11) / 4)
         return ap_run<T, D, 4, 16, 1, 3, F32 && D == 256 ? 1 : 2>(A, s);

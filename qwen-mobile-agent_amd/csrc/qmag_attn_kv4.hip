@@ -118,8 +118,8 @@ __device__ __forceinline__ bool ak_find(const AkArgs &A, int want, bool by_token
 // The workgroup's kv head and item.  Items in order, all heads of each, so that
 // those that have no work are the last to start: with the heads one behind
 // another the idle ones between them left some CUs two busy workgroups and others
-// none (32 sequences in bf16 52.4 us so, 48.3 in order; one of 32,768 tokens 22.1
-// and 19.7).
+// none (one sequence of 32,768 tokens 21.9 us so, 18.8 in order; of 32 sequences,
+// where few are idle, 51.9 and 52.1).
 __device__ __forceinline__ void ak_item(const AkArgs &A, int *item, int *kvh)
 {
     const unsigned i = blockIdx.x / (unsigned)A.n_kv;
@@ -324,9 +324,11 @@ constexpr int ak_tile() { return 36 * D; }
 // A step of one sequence is bound by a chain of round trips: of 14 us for 32,768
 // tokens (fp32, 16 heads of 256; 18.9 MB, 4 us at a large copy's rate) 0.8 are the
 // plan, 1.2 the table and the first tiles' requests, 1.2 the queries, 3.3 the tiles,
-// 2 the join of the waves, the rest the launch.  A batch is bound by the vector
-// instructions that turn codes into operands and by memory together: 32 sequences
-// of up to 16,384 tokens (bf16, 32 heads of 128; 163 MB) 41 us, 4.0 TB/s.
+// 2 the join of the waves; a launch alone takes 2.9, and what is left was not found.
+// (A chunk of 128 tokens becomes 256, see ak_chunk: one workgroup to a CU there.)  A
+// batch is bound by vector instructions, 12 of whose 16 rows are empty with four heads
+// to a kv head: 32 sequences of up to 16,384 tokens (bf16, 32 heads of 128; 163 MB) 46
+// us, 3.5 TB/s, 62,000 of a CU's 83,000 cycles.
 
 // how many of its workgroups of 4 waves LDS and registers let a CU hold
 template <class T, int D>
@@ -658,9 +660,9 @@ __global__ void __launch_bounds__(64 * NW, (few_resident<T, D>())) attn_kv4_kern
 // Bound by what a tile costs a wave besides its 64 products (fp32, heads of 256:
 // 1024 cycles): about 400 vector instructions, a quarter of them for steps and
 // minima, and as many cycles of LDS reads, which 8 waves share.  512 rows of 8 heads
-// each at 12,001 tokens: 316 us with the join, 312 TFLOP/s, or 623 of fp16 products.
-// (With 4 waves of it 544 us against 349; 64 rows that formed their codes themselves
-// 457; a step's exponent found once for a tile 332 against 334, not kept.)
+// each at 12,001 tokens: 305 us with the join, 323 TFLOP/s, or 646 of fp16 products.
+// (With 4 waves of an earlier form 544 us against 349; 64 rows that formed their codes
+// themselves 457.)
 
 // how many of its workgroups of 8 waves the registers let a CU hold
 template <class T, int D>
@@ -880,7 +882,8 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
         ak_weigh<NG>(s, p, m, l, ve, vs, o, [&](int i) { return size[i >> 2][i & 3]; }, [](float far) { return far; });
 
         // the next tile's codes, between the two products: its LDS reads and vector work run while
-        // the other waves multiply (ahead of the scores 334 us, behind the output 323, here 316)
+        // the other waves multiply (fp32, heads of 256: ahead of the scores 321 us, behind the output
+        // 333, here 305; bf16 of 128: 235, 238, 240)
         if (t0 + STEP < all) unpack(b ^ 1);
 
         // ---- output
@@ -1064,9 +1067,11 @@ static int ak_pick(const AkArgs &A, hipStream_t s)
 {
     // Few rows to a sequence: the waves share them and split the tokens, and every 16
     // rows read the cache again; of more the codes are formed once for 128.  With / without
-    // that, 256 rows: 25.9 / 22.4 us over 2000 tokens, 99 / 97 over 32,768 (bf16, 32 heads of
-    // 128), 37 / 21 and 89 / 80 (fp32, 16 heads of 256); 512 rows: 35 / 32, 175 / 182, 40 / 26
-    // and 137 / 138.
+    // that, 256 rows: 25.1 / 22.3 us over 2000 tokens, 98 / 114 over 32,768 (bf16, 32 heads of
+    // 128), 35 / 21 and 80 / 79 (fp32, 16 heads of 256); 512 rows: 35 / 31, 172 / 216, 38 / 25
+    // and 125 / 136.  The host knows the mean of a call only: beside 40 decoding sequences a
+    // chunk of 512 tokens is better a call of its own (bf16 161 us in one call, 141 in two), one
+    // of 128 is not (63 and 75).
     if ((int64_t)A.T * A.G <= 256 * (int64_t)A.n_seq) return ak_launch<T, D, false>(A, s);
     return ak_launch<T, D, true>(A, s);
 }
