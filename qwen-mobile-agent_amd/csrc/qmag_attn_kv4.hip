@@ -257,29 +257,35 @@ __device__ __forceinline__ float ak_size(uint32_t d) { return 0.25f * (float)(d 
 // would pass 2^8 or an operand 2^15.  The power follows the largest p d, not the largest
 // d: a token of large values and no weight takes no bits from the others (300 tokens,
 // one with a step 2^20 times theirs and a weight of e^-60: fp32 calls were off by 1e-3).
-// size(i): of a token's largest step, or more; exact(far): the largest score + size of
-// the lane, which is far where size gives no more.
+// size(i): of a token's largest step, or more; exact(x): the largest x + size of a lane
+// with no more.
 // (Arrays by reference: as members of a struct the compiler copied all of o in every tile.)
 template <int NG, class Size, class Exact>
 __device__ __forceinline__ void ak_weigh(const float (&s)[8], float (&p)[8], float &m, float &l, int &ve, float (&vs)[NG],
                                          f32x4 (&o)[NG][4], Size size, Exact exact)
 {
-    float top = s[0], far = s[0] + size(0);
+    // (from the differences: large scores have no room for a size)
+    float x[8], top = -INFINITY, far = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < 8; i++) {
-        top = fmaxf(top, s[i]);
-        far = fmaxf(far, s[i] + size(i));
+    for (int i = 0; i < 8; i++) {
+        x[i] = s[i] - m;
+        top = fmaxf(top, x[i]);
+        far = fmaxf(far, x[i] + size(i));
     }
-    if (__any(top > m + 8.0f || far > m + ((float)ve + 22.5f))) {
+    if (__any(top > 8.0f || far > (float)ve + 22.5f)) {
         // (a row that need not move stays: what others see has no part in its rounding)
-        top = row_max(top);
-        far = row_max(exact(far));
+        float high = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) high = fmaxf(high, s[i]);
+        high = row_max(high);
         const float was = m;
-        const bool wide = far > m + ((float)ve + 22.5f);
-        m = top > m + 8.0f ? top : m;
+        m = row_max(top) > 8.0f ? high : m;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = s[i] - m;
+        far = row_max(exact(x));
         // what is summed so far shrinks with the maximum's move, and its power of two with it
-        const int sunk = ve - (int)fminf(m - was, 200.0f), here = (int)ceilf(fminf(fmaxf(far - m - 14.5f, -60.0f), 40.0f));
-        const int e = wide || m != was ? max(max(here, sunk), -60) : ve;
+        const int sunk = ve - (int)fminf(m - was, 200.0f), here = (int)ceilf(fminf(fmaxf(far - 14.5f, -60.0f), 40.0f));
+        const int e = far > (float)ve + 22.5f || m != was ? max(max(here, sunk), -60) : ve;
         const float f = __builtin_amdgcn_exp2f(was - m), fo = __builtin_amdgcn_exp2f(was - m + (float)(ve - e));
         ve = e;
         l *= f;
@@ -292,7 +298,7 @@ __device__ __forceinline__ void ak_weigh(const float (&s)[8], float (&p)[8], flo
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        p[i] = __builtin_amdgcn_exp2f(s[i] - m);
+        p[i] = __builtin_amdgcn_exp2f(x[i]);
         l += p[i];
     }
 }
@@ -545,14 +551,14 @@ __global__ void __launch_bounds__(64 * NW, (few_resident<T, D>())) attn_kv4_kern
                 for (int g = 1; g < NG; g++) d = __builtin_elementwise_max(d, __builtin_bit_cast(s16x2, vdm[i][g]));
                 return ak_size(__builtin_bit_cast(uint32_t, d));
             },
-            [&](float) {
+            [&](const float (&x)[8]) {
                 float far = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 8; i++)
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
                         const float e = ak_size(vdm[i][g]);
-                        far = fmaxf(far, e < 31.0f ? s[i] + e : -INFINITY);        // (NaN has no part in it)
+                        far = fmaxf(far, e < 31.0f ? x[i] + e : -INFINITY);        // (NaN has no part in it)
                     }
                 return far;
             });
@@ -879,7 +885,14 @@ __global__ void __launch_bounds__(64 * NW, (2 * rows_resident<T, D>())) attn_kv4
         }
         float p[8];
         const f32x4 size[2] = {*(const f32x4 *)(isize[b] + 4 * h), *(const f32x4 *)(isize[b] + 16 + 4 * h)};
-        ak_weigh<NG>(s, p, m, l, ve, vs, o, [&](int i) { return size[i >> 2][i & 3]; }, [](float far) { return far; });
+        ak_weigh<NG>(
+            s, p, m, l, ve, vs, o, [&](int i) { return size[i >> 2][i & 3]; },
+            [&](const float (&x)[8]) {
+                float far = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++) far = fmaxf(far, x[i] + size[i >> 2][i & 3]);
+                return far;
+            });
 
         // the next tile's codes, between the two products: its LDS reads and vector work run while
         // the other waves multiply (fp32, heads of 256: ahead of the scores 321 us, behind the output

@@ -312,3 +312,32 @@ def test_attn_prompt_huge_and_apart(qm, T, H, D):
     mag = np.cumsum(np.abs(v[:, 0]).astype(np.float64), 0) / np.arange(1, T + 1)[:, None]
     for h in range(2):
         close(got[:, h], want, (3 * 2.0 ** -22 + (T + 64) * 2.0 ** -24) * mag)
+
+
+@pytest.mark.parametrize("sign,scale", [(1, 0.1), (-1, 0.1), (1, 4.0), (-1, 4.0)])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_kv4_scores_beyond_their_own_units(qm, typ, D, rows, sign, scale):
+    """Scores of 1e6 to 5e9, whose spacing in fp32 is up to 512: a row is the value of its largest key,
+    which leads by more than the sums round (257 x 2^-24 of 6 times a score) and the weights keep."""
+    t = TYPES[typ]
+    r = rng_of(D, rows, 86)
+    L, H, KV = 260 + rows, 4, 2
+    k, v = r.randn(L, KV, D), r.randn(L, KV, D)
+    k[..., 0] = sign * (3000 + 60000.0 * r.permutation(L)[:, None] / L)
+    q = r.randn(rows, H, D)
+    q[..., 0] = 20000 + 1000 * r.rand(rows, H)
+    q = to_type(q, t)
+    case = CacheCase(qm, r, [L], KV, D, 16, [k.astype(np.float32)], [v.astype(np.float32)])
+    got = values(run_kv4(qm, case, q, [rows], t, scale=scale, pad=0), t)
+    qf, want = values(q, t), np.zeros((rows, H, D))
+    for j in range(rows):
+        n = L - rows + j + 1
+        for h in range(H):
+            s = case.k[0][:n, h // 2] @ qf[j, h] * scale
+            two = np.partition(s, -2)[-2:]
+            assert two[1] - two[0] > 257 * 6 * 2.0 ** -24 * np.abs(s).max() + 100
+            want[j, h] = case.v[0][s.argmax(), h // 2]
+    part = 2.0 ** -21 if t == F32 else 2.0 ** -10
+    close(got, want, HALF[t] * np.abs(want) + 16 * part)
