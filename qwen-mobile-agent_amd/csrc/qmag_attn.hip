@@ -335,6 +335,10 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     }
 
     Acc o[DT];
+    // 16-bit calls: what is taken from the scores ahead of the scale.  Zero, unless scores are so large
+    // that the maximum's own rounding (8 and more beyond 2^27) would be the weights' exponent.
+    float ms = 0.0f;
+    bool large = false;                            // a query of the wave has one
     float m = -3e38f, l = 0.0f;                    // running maximum (of scaled scores), sum
     // fp32 calls: a weight's operand is p times V's power of two, 2^(7 - ve) of it: below 2^16, and near
     // there to keep its bits
@@ -431,6 +435,11 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         constexpr float LIFT = std::is_same_v<T, TF16> ? 7.0f : 0.0f, FULL = std::is_same_v<T, TF16> ? 32768.0f : 256.0f;
         const float r = NS == 2 ? 1.0f : rs;
         float p[NV], w[NS == 2 ? NV : 1], sum = 0.0f, far = 0.0f;    // w: times V's powers of two
+        if constexpr (NS == 1)
+            if (large) {
+#pragma unroll
+                for (int i = 0; i < NV; i++) s[i] -= ms;
+            }
         auto weigh = [&] {
             sum = far = 0.0f;
 #pragma unroll
@@ -450,14 +459,23 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             float top = s[0];
 #pragma unroll
             for (int i = 1; i < NV; i++) top = fmaxf(top, s[i]);
-            top = query_max<QW>(top) * r;
+            top = query_max<QW>(top);
             // (a query that need not move stays: what others see has no part in its rounding)
             const bool moves = query_max<QW>(sum) > FULL, wide = NS == 2 && query_max<QW>(far) > pow2i(min(ve + 8, 127));
             const float was = m;
-            m = moves ? fmaxf(m, top - LIFT) : m;
-            weigh();
+            m = moves ? fmaxf(m, top * r - LIFT) : m;
             float f = __builtin_amdgcn_exp2f(was - m);
             l *= f;
+            if constexpr (NS == 1)
+                if (__any(moves && fabsf(m) > 0x1p24f)) {
+                    const float by = moves && fabsf(m) > 0x1p24f ? top : 0.0f;
+                    m = by != 0.0f ? -LIFT : m;
+                    ms += by;
+                    large = true;
+#pragma unroll
+                    for (int i = 0; i < NV; i++) s[i] -= by;
+                }
+            weigh();
             if constexpr (NS == 2) {
                 // what is summed so far shrinks with the maximum's move, and its power of two with it
                 const int sunk = ve - (int)fminf(m - was, 400.0f), here = (int)(__float_as_uint(query_max<QW>(far)) >> 23) - 126;

@@ -341,3 +341,56 @@ def test_attn_kv4_scores_beyond_their_own_units(qm, typ, D, rows, sign, scale):
             want[j, h] = case.v[0][s.argmax(), h // 2]
     part = 2.0 ** -21 if t == F32 else 2.0 ** -10
     close(got, want, HALF[t] * np.abs(want) + 16 * part)
+
+
+@pytest.mark.parametrize("sign,scale", [(1, 0.1), (-1, 0.1), (1, 4.0), (-1, 4.0)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,H", PROMPT_FORMS)
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_prompt_scores_beyond_their_own_units(qm, typ, T, H, D, sign, scale):
+    """As over the cache: every row is the value of the largest key that it sees, or of several whose
+    scores are within what the sums round."""
+    t = TYPES[typ]
+    r = rng_of(D, T, 87)
+    H = H or many(t, D)
+    q, k, v = r.randn(T, H, D), r.randn(T, 1, D), r.randn(T, 1, D)
+    k[..., 0] = sign * (3000 + 60000.0 * r.permutation(T)[:, None] / T)
+    q[..., 0] = 20000 + 1000 * r.rand(T, H)
+    q, k, v = (to_type(x, t) for x in (q, k, v))
+    got = values(run_prompt(qm, q, k, v, [T], t, scale=scale), t)
+    qf, kf, vf = values(q, t), values(k, t)[:, 0], values(v, t)[:, 0]
+    sure = 0
+    for h in (0, H - 1):
+        s = qf[:, h] @ kf.T * scale
+        for j in range(T):
+            a = s[j, :j + 1]
+            near = a > a.max() - D * 6 * 2.0 ** -24 * np.abs(a).max() - 200
+            if near.sum() == 1:
+                sure += 1
+                close(got[j, h], vf[a.argmax()], 2 * HALF[t] * np.abs(vf[a.argmax()]) + 2.0 ** -20, (j, h))
+            else:
+                assert (got[j, h] <= vf[:j + 1][near].max(0) + 0.1).all() and (got[j, h] >= vf[:j + 1][near].min(0) - 0.1).all(), (j, h)
+    assert sure
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,H", PROMPT_FORMS)
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_prompt_huge_keys_that_are_seen(qm, typ, T, H, D):
+    """Finite keys near the type's largest value: a row whose score there is positive is that key's
+    value, for the others the key has no weight."""
+    t = TYPES[typ]
+    r = rng_of(D, T, 88)
+    H = H or many(t, D)
+    q, k, v = r.randn(T, H, D), r.randn(T, 1, D), r.randn(T, 1, D)
+    q[..., 3] = np.where(q[..., 3] < 0, -1, 1) * (0.5 + r.rand(T, H))
+    big = 6e4 if t == F16 else 1e38
+    k[20, 0, 3], k[41, 0, 3], k[T - 3, 0, 3] = big, big * 0.75, -big
+    q, k, v = (to_type(x, t) for x in (q, k, v))
+    got = values(run_prompt(qm, q, k, v, [T], t, scale=0.125), t)
+    calm = values(k, t)
+    calm = np.where(np.abs(calm) > 100, 0, calm)
+    for h in (0, H // 2, H - 1):
+        want = weigh64(values(q, t)[:, h], values(k, t)[:, 0], values(v, t)[:, 0], 0.125)
+        _, mag, es = attention(values(q, t)[:, h:h + 1], calm, values(v, t), np.arange(T), 0.125)
+        close(got[:, h], want, prompt_tol(t, D, T, want, 8 * mag[:, 0] + 8, es[:, 0]), h)
