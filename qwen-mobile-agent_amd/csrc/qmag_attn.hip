@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
     // that the maximum's own rounding (8 and more beyond 2^27) would be the weights' exponent.
     float ms = 0.0f;
     bool large = false;                            // a query of the wave has one
-    float m = -3e38f, l = 0.0f;                    // running maximum (of scaled scores), sum
+    float m = -3.402823466e38f, l = 0.0f;          // running maximum (of scaled scores), sum
     // fp32 calls: a weight's operand is p times V's power of two, 2^(7 - ve) of it: below 2^16, and near
     // there to keep its bits
     int ve = -110;

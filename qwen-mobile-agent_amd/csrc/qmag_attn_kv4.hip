@@ -156,9 +156,9 @@ union Frag {
     half8 h;
 };
 
-// The maximum of a row that has seen nothing: below any score, and finite, so that
+// The maximum of a row that has seen nothing: above no score, and finite, so that
 // differences from it are numbers.
-constexpr float AK_NONE = -3e38f;
+constexpr float AK_NONE = -3.402823466e38f;
 
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }

@@ -394,3 +394,21 @@ def test_attn_prompt_huge_keys_that_are_seen(qm, typ, T, H, D):
         want = weigh64(values(q, t)[:, h], values(k, t)[:, 0], values(v, t)[:, 0], 0.125)
         _, mag, es = attention(values(q, t)[:, h:h + 1], calm, values(v, t), np.arange(T), 0.125)
         close(got[:, h], want, prompt_tol(t, D, T, want, 8 * mag[:, 0] + 8, es[:, 0]), h)
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("T,H", PROMPT_FORMS)
+def test_attn_prompt_lowest_scores(qm, typ, T, H):
+    """All scores -2.2e38, times log2(e) near fp32's lowest value: they are equal, so a row is a mean."""
+    t = TYPES[typ]
+    r = rng_of(T, 89)
+    D, H = 64, H or many(t, 64)
+    q, k, v = np.zeros((T, H, D)), np.zeros((T, 1, D)), r.randn(T, 1, D)
+    q[..., 0], k[..., 0] = 1, -2.2e38
+    q, k, v = (to_type(x, t) for x in (q, k, v))
+    got = values(run_prompt(qm, q, k, v, [T], t, scale=1.0), t)
+    vf = values(v, t)[:, 0]
+    n = np.arange(1, T + 1)[:, None]
+    want, mag = np.cumsum(vf, 0) / n, np.cumsum(np.abs(vf), 0) / n
+    for h in (0, H - 1):
+        close(got[:, h], want, (3 * 2.0 ** -22 + (T + 64) * 2.0 ** -24) * mag + HALF[t] * np.abs(want))
