@@ -428,11 +428,14 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
             }
         }
         // ---- weights, by the maximum so far.  Whether it has to move is seen from
-        // their sum, which is needed in any case: past 2^8 of the largest weight after a
-        // move (an infinity included).  That is 1, and 2^7 in fp16: 2^15 is still in range,
-        // and weights down to 2^-32 of it are more than nothing (with 1 they ended at
-        // 2^-25, which thousands of keys together can reach).
-        constexpr float LIFT = std::is_same_v<T, TF16> ? 7.0f : 0.0f, FULL = std::is_same_v<T, TF16> ? 32768.0f : 256.0f;
+        // their sum, which is needed in any case: past 2^8 times the largest weight after a
+        // move (an infinity included).  That is 2^LIFT: 2^7 in fp16, where 2^15 is still in
+        // range, and weights down to 2^-32 of it are more than nothing (with 1 they ended at
+        // 2^-25, which thousands of keys together can reach); 2^-32 in bf16, whose values
+        // reach 2^128: their sums over 2^22 keys stay in fp32's range, those of 2^-94 and more
+        // in its normal one.
+        constexpr float LIFT = std::is_same_v<T, TF16> ? 7.0f : NS == 1 ? -32.0f : 0.0f;
+        constexpr float FULL = std::is_same_v<T, TF16> ? 0x1p15f : NS == 1 ? 0x1p-24f : 0x1p8f;
         const float r = NS == 2 ? 1.0f : rs;
         float p[NV], w[NS == 2 ? NV : 1], sum = 0.0f, far = 0.0f;    // w: times V's powers of two
         if constexpr (NS == 1)

@@ -412,3 +412,22 @@ def test_attn_prompt_lowest_scores(qm, typ, T, H):
     want, mag = np.cumsum(vf, 0) / n, np.cumsum(np.abs(vf), 0) / n
     for h in (0, H - 1):
         close(got[:, h], want, (3 * 2.0 ** -22 + (T + 64) * 2.0 ** -24) * mag + HALF[t] * np.abs(want))
+
+
+@pytest.mark.parametrize("size", ["largest", "small"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,H", PROMPT_FORMS + [(2500, 4)])
+@pytest.mark.parametrize("typ", TYPES)
+def test_attn_prompt_values_of_any_size(qm, typ, T, H, D, size):
+    """Values near the type's largest, whose sums would leave fp32's range, and small ones: their means
+    are as exact as those of others."""
+    t = TYPES[typ]
+    r = rng_of(T, D, 90)
+    H = H or many(t, D)
+    big = {F32: 3e38, BF16: 3e38, F16: 6e4}[t] if size == "largest" else {F32: 1e-25, BF16: 1e-25, F16: 1.0}[t]
+    q, k, v = (to_type(x, t) for x in (r.randn(T, H, D), r.randn(T, 1, D), big * (0.5 + 0.5 * r.rand(T, 1, D))))
+    got = values(run_prompt(qm, q, k, v, [T], t), t)
+    rows = np.unique(np.concatenate([np.arange(0, T, 61), [1, 31, 32, T - 1]]))
+    for h in (0, H - 1):
+        want, mag, es = attention(values(q, t)[rows, h:h + 1], values(k, t), values(v, t), rows, D ** -0.5)
+        assert norm_error(got[rows, h] / big, want[:, 0] / big) <= prompt_bound(t, D, T)
