@@ -15,9 +15,9 @@
 // matrix cores, 16 times the fp32 ones' rate: every row of Q, K and V is scaled
 // by a power of two (exact) and split into two fp16 parts, x = hi + lo to 22
 // bits, and a product is hi hi + hi lo + lo hi.  16-bit calls round a weight to
-// their type for the second product, not for the sum: as much again as the rounding
-// of the result (bf16 2.1e-3 of it in all, the result's rounding 1.6e-3; summed as
-// rounded it would be 1.8e-3 where few keys count and no less where many do).
+// their type, for the second product and for the sum: as much again as the rounding
+// of the result where many keys count (bf16 2.1e-3 of it in all, the result's rounding
+// 1.6e-3), less where few do, nothing where one does.
 //
 // S^T = K Q^T by v_mfma_f32_32x32x16 leaves a lane with one query (n = lane % 32)
 // and keys 8 (r / 4) + 4 (lane / 32) + r % 4 of a tile, by v_mfma_f32_16x16x32
@@ -149,6 +149,17 @@ __device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) { return __bu
 __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma(bf168 a, bf168 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(bf168 a, bf168 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// a + b + c, rounded once (subnormal a and b count)
+__device__ __forceinline__ float add_pair(_Float16 a, _Float16 b, float c)
+{
+    return __builtin_amdgcn_fdot2((half2v){a, b}, (half2v){1, 1}, c, false);
+}
+__device__ __forceinline__ float add_pair(__bf16 a, __bf16 b, float c)
+{
+    typedef __bf16 bf162v __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16((bf162v){a, b}, (bf162v){(__bf16)1.0f, (__bf16)1.0f}, c, false);
+}
 
 // ---------------------------------------------------------------- tiles ----
 // A thread's part of a tile of K or V, NT threads: 8 channels of every ROWSth of
@@ -443,15 +454,22 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
 #pragma unroll
                 for (int i = 0; i < NV; i++) s[i] -= ms;
             }
+        // (16-bit calls sum the weights as they are rounded for the second product: a row is a mean of
+        // values, of one key that key's value, and none leaves the type's range)
+        V8 ph[PS], pl[NS == 2 ? PS : 1];
         auto weigh = [&] {
             sum = far = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                p[i] = __builtin_amdgcn_exp2f(NS == 2 ? s[i] - m : fmaf(s[i], r, -m));
-                sum += p[i];
+            for (int i = 0; i < NV; i++) p[i] = __builtin_amdgcn_exp2f(NS == 2 ? s[i] - m : fmaf(s[i], r, -m));
+#pragma unroll
+            for (int i = 0; i < NV; i += NS == 2 ? 1 : 2) {
                 if constexpr (NS == 2) {
+                    sum += p[i];
                     w[i] = p[i] * sc[AP_KEYS + KG * (i >> 2) + 4 * h + (i & 3)];
                     far = fmaxf(far, w[i]);
+                } else {
+                    ph[i >> 3][i & 7] = (E)p[i], ph[i >> 3][(i & 7) + 1] = (E)p[i + 1];
+                    sum = add_pair(ph[i >> 3][i & 7], ph[i >> 3][(i & 7) + 1], sum);
                 }
             }
         };
@@ -493,18 +511,14 @@ __global__ void __launch_bounds__(64 * NW, WE) attn_prompt_kernel(ApArgs A)
         }
         l += sum;
         const float pv = NS == 2 ? pow2i(7 - ve) : 1.0f;
-        V8 ph[PS], pl[NS == 2 ? PS : 1];
+        if constexpr (NS == 2)
 #pragma unroll
-        for (int i = 0; i < NV; i += 2) {
-            if constexpr (NS == 2) {
+            for (int i = 0; i < NV; i += 2) {
                 half2v a, b;
                 split2(w[i] * pv, w[i + 1] * pv, &a, &b);
                 ph[i >> 3][i & 7] = a[0], ph[i >> 3][(i & 7) + 1] = a[1];
                 pl[i >> 3][i & 7] = b[0], pl[i >> 3][(i & 7) + 1] = b[1];
-            } else {
-                ph[i >> 3][i & 7] = (E)p[i], ph[i >> 3][(i & 7) + 1] = (E)p[i + 1];
             }
-        }
         // ---- output
 #pragma unroll
         for (int d = 0; d < DT; d++)

@@ -431,3 +431,21 @@ def test_attn_prompt_values_of_any_size(qm, typ, T, H, D, size):
     for h in (0, H - 1):
         want, mag, es = attention(values(q, t)[rows, h:h + 1], values(k, t), values(v, t), rows, D ** -0.5)
         assert norm_error(got[rows, h] / big, want[:, 0] / big) <= prompt_bound(t, D, T)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,H", PROMPT_FORMS + [(2500, 4)])
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+def test_attn_prompt_is_a_mean_of_values(qm, typ, T, H, D):
+    """All values the type's largest: so is every result, whatever the weights' rounding; and a row of
+    one or two keys, whose weights' rounding takes no part in it or little, is off by its own."""
+    t = TYPES[typ]
+    r = rng_of(T, D, 91)
+    H = H or many(t, D)
+    top = np.float32(65504) if t == F16 else np.array([0x7F7F0000], np.uint32).view(np.float32)[0]
+    q, k = to_type(r.randn(T, H, D), t), to_type(r.randn(T, 1, D), t)
+    got = values(run_prompt(qm, q, k, to_type(np.full((T, 1, D), top), t), [T], t), t)
+    assert (got == top).all()
+    v = to_type(r.randn(T, 1, D), t)
+    got = values(run_prompt(qm, q, k, v, [T], t), t)
+    assert np.array_equal(got[0], np.repeat(values(v, t)[0], H, 0))
