@@ -28,8 +28,8 @@
 // Bound by the matrix and vector units in turn: a tile of 32 x 32 scores of heads
 // of 128 is 512 cycles of products and about 500 of vector instructions, half of
 // them exponentials (a quarter rate), on a SIMD that three waves share.  Measured,
-// both launches: bf16, 8192 tokens in five prompts, 32 heads of 128 over 8: 364 us,
-// 843 TFLOP/s (a large bf16 product in the library: 1223); fp32, 4096 tokens, 16
+// both launches: bf16, 8192 tokens in five prompts, 32 heads of 128 over 8: 370 us,
+// 830 TFLOP/s (a large bf16 product in the library: 1223); fp32, 4096 tokens, 16
 // heads of 256 over 2: 421 us, 326 TFLOP/s, or 979 of fp16 products (library: 1179;
 // its fp32 ones 153).  The first launch is 16 and 12 us of these.
 #include <type_traits>

@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(64 * NW, (few_resident<T, D>())) attn_kv4_kern
 // Bound by what a tile costs a wave besides its 64 products (fp32, heads of 256:
 // 1024 cycles): about 400 vector instructions, a quarter of them for steps and
 // minima, and as many cycles of LDS reads, which 8 waves share.  512 rows of 8 heads
-// each at 12,001 tokens: 305 us with the join, 323 TFLOP/s, or 646 of fp16 products.
+// each at 12,001 tokens: 303 us with the join, 325 TFLOP/s, or 650 of fp16 products.
 // (With 4 waves of an earlier form 544 us against 349; 64 rows that formed their codes
 // themselves 457.)
 
