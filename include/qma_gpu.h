@@ -45,7 +45,8 @@ extern "C" {
    of this library with no counterpart in the reference or the GGUF; the same
    bytes per row, the same results as QMAG_TYPE_Q6_K). */
 #define QMAG_TYPE_Q6_K_R 270
-/* Activation types of the attention entries (GGML's type ids). */
+/* Activation types of the attention and recurrent entries and of logits (GGML's
+   type ids). */
 #define QMAG_TYPE_F32 0
 #define QMAG_TYPE_F16 1
 #define QMAG_TYPE_BF16 30
@@ -135,8 +136,10 @@ int qmag_event_elapsed(int a, int b, float *ms);
    3 Q8_K(h), 4 down+combine, 5 fused decode, 6 matvec (matmul entries),
    7 Q8_K quantisation (every launch of it), 8 grouping (prefill), 9 combine
    (prefill), 10 rotary positions, 11 cache bookkeeping, append and read,
-   12 attention (both launches of a call).  qmag_prof_read synchronises and
-   returns the launch count and summed milliseconds of one id. */
+   12 attention (both launches of a call), 13 short convolution, 14 linear
+   attention, 15 log probabilities (all launches of a call).  qmag_prof_read
+   synchronises and returns the launch count and summed milliseconds of one
+   id. */
 int qmag_prof_enable(int on);
 int qmag_prof_read(int kernel_id, long *count, double *total_ms);
 
@@ -626,6 +629,104 @@ int qmag_attn_kv4_dev(const qmag_kv4 *c, const qmag_kv_table *t, int type, const
    of NaN, and an infinity of v comes through with its sign. */
 int qmag_attn_prompt_dev(int type, int head_dim, const qmag_heads *q, const qmag_heads *k, const qmag_heads *v,
                          const qmag_heads *out, const int *cu, int n_seq, int T, float scale);
+
+/* ------------------------------------------------------------------------ */
+/* Log probabilities of device logits                                        */
+/* ------------------------------------------------------------------------ */
+
+/* For each of T rows of n_vocab logits x (row t from logits + t * stride, in
+   values; f32, f16 or bf16 as `type` says), beside the sampler's entries for a
+   program that scores text or answers with its alternatives:
+     logprob[t]      x[token[t]] - ln sum e^x; 0 for a token outside 0 .. n_vocab - 1
+                     (a row without one)
+     entropy[t]      - sum p ln p in nats, a token of no weight adding nothing
+     top_id[t][k], top_logprob[t][k]
+                     the k = top_k most likely tokens, the likeliest first, the
+                     lowest id first among equal logits (-0 is +0, NaN below
+                     every number)
+   logprob (with token), entropy and the top pair may be NULL: not wanted; top_k
+   is 0..QMAG_LOGPROBS_MAX_TOP, at most n_vocab, and 0 without the top pair.
+   Logits of -inf are tokens of no weight; a row with a NaN or +inf among its
+   logits, or with none above -inf, has NaN for every log probability and its
+   entropy (ids are ordered as ever).  Maxima and sums are fp32.  Equal calls
+   give equal bits.  What is written overlaps neither what is read nor itself. */
+#define QMAG_LOGPROBS_MAX_TOP 64
+int qmag_logprobs_dev(int n_vocab, int type, const void *logits, int64_t stride, const int *token, int T, int top_k,
+                      float *logprob, float *entropy, int *top_id, float *top_logprob);
+
+/* ------------------------------------------------------------------------ */
+/* Recurrent layers: short convolution, linear attention                     */
+/* ------------------------------------------------------------------------ */
+
+/* What a program calls between the projections of a recurrent layer (conv1d and
+   the gated delta net of the engine, nn.c:717-840) to keep its sequences on the
+   device:
+
+     conv -> linattn (q, k and v are heads of the convolution's output)
+
+   Both take sequences packed one behind another, sequence i being rows
+   cu[i] .. cu[i + 1] - 1 (cu: i32 [n_seq + 1], ascending within 0 .. T; empty
+   ones are fine, rows behind cu[n_seq] are left as they were; of others the
+   results are not defined, and nothing but rows of out and states is written),
+   and keep what a sequence hands on in a state of slot[i].  len (i32 [n_seq], as
+   qmag_kv_assign_dev takes it) counts the tokens that sequence i had before: with
+   none its state is taken as zeros, whatever the slot holds; NULL: every sequence
+   continues.  The state is read and then replaced; that of an empty sequence, and
+   slots nobody names, stay.  A slot outside 0 .. n_slot - 1 is no state: the
+   sequence begins from zeros and hands nothing on.  Each slot is named once: of
+   two sequences with the same the results are not defined.  One token of each
+   sequence, some, or whole prompts are one call each or together, and a prompt cut
+   into calls gives what one call gives within the accuracy.
+
+   Device pointers throughout, ordered on the library stream, one host thread at a
+   time, as the other device entries; activations are f32, f16 or bf16 (`type`),
+   states f32.  n_seq: 0..QMAG_KV_MAX_SEQ.  Equal calls give equal bits. */
+
+/* Short causal convolution, each channel by its own taps:
+     y[t][c] = bias[c] + sum_w weight[c][w] x[t - width + 1 + w][c],
+   x ahead of a sequence's rows from its state; with silu the result is
+   y / (1 + e^-y).  Sums are fp32, in the taps' order. */
+typedef struct qmag_conv {
+    int n_channel;        /* 1..QMAG_CONV_MAX_CHANNEL */
+    int width;            /* taps, 2..4 */
+    int silu;
+    int n_slot;
+    const float *weight;  /* f32 [n_channel][width], a token's own tap last (ssm_conv1d of the GGUF) */
+    const float *bias;    /* f32 [n_channel], or NULL */
+    float *state;         /* f32 [n_slot][width - 1][n_channel]: the last inputs, the oldest first */
+} qmag_conv;
+#define QMAG_CONV_MAX_CHANNEL (1 << 20)
+/* Row t of x from x + t * x_stride, in values, and so out; any strides of at least
+   n_channel.  out overlaps nothing that is read, the state none of the inputs. */
+int qmag_conv_dev(const qmag_conv *c, int type, const void *x, int64_t x_stride, void *out, int64_t out_stride,
+                  const int *slot, const int *len, const int *cu, int n_seq, int T);
+
+/* Linear attention with a decay for each head.  Head h of v and out has a state
+   S [dim_k][dim_v] and the key head h / (n_head / q's heads) of q and k, or with
+   turns the key head h % (q's heads).  A token does
+     S <- e^g S;  u = beta (v - delta S^T k);  S <- S + k u^T;  out = scale S^T q
+   (delta 0: a plain sum; 1: the delta rule, for keys of norm 1 and beta of 0 to 1,
+   or up to 2).  decay: g, f32 [T][n_head], at most 0 (above counts as 0; -inf
+   forgets all there was), or NULL: none.  beta: f32 [T][n_head], or NULL: 1.  With
+   norm_eps > 0, q and k are taken times (sum of their squares + norm_eps)^-1/2.
+   All in fp32: products on the matrix cores hold 2^-22 and better of each operand.
+   A NaN or infinity at a token has no effect on tokens ahead of it, on other
+   heads' states or other sequences; what follows it is as the recurrence has it.
+   q, k and v may be views of one buffer; out overlaps nothing that is read, the
+   state none of the inputs. */
+typedef struct qmag_linattn {
+    int n_head;           /* heads of v and out: 1..QMAG_MAX_HEADS */
+    int dim_k;            /* 64, 128 or 256 */
+    int dim_v;            /* a multiple of 16, 16..256 */
+    int delta;
+    int turns;
+    float norm_eps;
+    int n_slot;
+    float *state;         /* f32 [n_slot][n_head][dim_k][dim_v], 16-byte aligned */
+} qmag_linattn;
+int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_heads *q, const qmag_heads *k, const qmag_heads *v,
+                     const qmag_heads *out, const float *decay, const float *beta, const int *slot, const int *len,
+                     const int *cu, int n_seq, int T, float scale);
 
 /* ------------------------------------------------------------------------ */
 /* Synthetic inputs (bench/test utilities; not part of the reference)        */

@@ -137,8 +137,9 @@ struct DeviceScope {
 // of whole heads, or heads of whole tokens).
 int check_heads(const char *what, const qmag_heads *h, int type, int dim, int64_t n_tok, bool written);
 // whether the two may share a byte: false when their ranges are apart, or when
-// they lie side by side within the tokens, or the heads, of one buffer
-bool heads_overlap(const qmag_heads *a, const qmag_heads *b, int size, int dim, int64_t n_tok);
+// they lie side by side within the tokens, or the heads, of one buffer; dim_b: the
+// values of b's heads where they are others than a's
+bool heads_overlap(const qmag_heads *a, const qmag_heads *b, int size, int dim, int64_t n_tok, int dim_b = 0);
 // whether any of h's values lies in the `bytes` bytes from p
 bool heads_meet(const qmag_heads *h, int size, int dim, int64_t n_tok, const void *p, size_t bytes);
 // every head's first value 16-byte aligned

@@ -63,22 +63,23 @@ static bool side_by_side(int64_t apart, int64_t stride, int64_t ea, int64_t eb)
     return d >= eb && d + ea <= stride;
 }
 
-bool heads_overlap(const qmag_heads *a, const qmag_heads *b, int size, int dim, int64_t n_tok)
+bool heads_overlap(const qmag_heads *a, const qmag_heads *b, int size, int dim, int64_t n_tok, int dim_b)
 {
-    const int64_t na = extent(a, dim, n_tok), nb = extent(b, dim, n_tok);
+    const int db = dim_b ? dim_b : dim;
+    const int64_t na = extent(a, dim, n_tok), nb = extent(b, db, n_tok);
     if (na == 0 || nb == 0) return false;
     const intptr_t pa = (intptr_t)a->ptr, pb = (intptr_t)b->ptr;
     if (pa + na * size <= pb || pb + nb * size <= pa) return false;
     if ((pa - pb) % size) return true;
     const int64_t apart = (pa - pb) / size;
     if (a->token_stride == b->token_stride &&
-        side_by_side(apart, a->token_stride, extent(a, dim, 1), extent(b, dim, 1)))
+        side_by_side(apart, a->token_stride, extent(a, dim, 1), extent(b, db, 1)))
         return false;
     const int64_t hs = a->n_head > 1 ? a->head_stride : b->head_stride;
     const bool heads_alike = (a->n_head == 1 || a->head_stride == hs) && (b->n_head == 1 || b->head_stride == hs);
-    if (heads_alike && side_by_side(apart, hs, (n_tok - 1) * a->token_stride + dim, (n_tok - 1) * b->token_stride + dim)) return false;
+    if (heads_alike && side_by_side(apart, hs, (n_tok - 1) * a->token_stride + dim, (n_tok - 1) * b->token_stride + db)) return false;
     const bool whole = hs > 0 && a->token_stride % hs == 0 && b->token_stride % hs == 0;
-    if (whole && heads_alike && side_by_side(apart, hs, dim, dim))
+    if (whole && heads_alike && side_by_side(apart, hs, dim, db))
         return false;
     return true;
 }

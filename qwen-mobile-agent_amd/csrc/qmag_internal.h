@@ -52,6 +52,8 @@ enum WsSlot {
     WS_HOSTIO,                      // qmag_moe_ffn_host: the device copies of x and out
     WS_F32PART,                     // fp32 matmul rows longer than one LDS chunk: per-chunk partials
     WS_ATTN,                        // attention: partial results over a cache, tiles of a prompt's K and V
+    WS_LOGPROBS,                    // log probabilities: parts of rows
+    WS_LINATTN,                     // linear attention: what the chunks of prompts have in common
     WS_COUNT
 };
 void *workspace(int slot, size_t bytes, int *status);
@@ -59,7 +61,7 @@ void *workspace(int slot, size_t bytes, int *status);
 // ---- per-kernel event timing (qmag_prof_*) ----
 enum ProfId {
     PROF_ROUTER = 0, PROF_TOPK, PROF_GATEUP, PROF_HQUANT, PROF_DOWN, PROF_FUSED, PROF_MATVEC, PROF_Q8K,
-    PROF_GROUP, PROF_COMBINE, PROF_ROPE, PROF_KV, PROF_ATTN,
+    PROF_GROUP, PROF_COMBINE, PROF_ROPE, PROF_KV, PROF_ATTN, PROF_CONV, PROF_LINATTN, PROF_LOGPROBS,
     PROF_COUNT
 };
 bool prof_on();

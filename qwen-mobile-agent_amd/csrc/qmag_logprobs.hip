@@ -1,0 +1,332 @@
+// qmag_logprobs.hip -- log probabilities of given tokens, the entropy and the most
+// likely tokens of rows of logits, beside the sampler, in one pass over the logits.
+//
+// A thread keeps the largest value m it has met, s = sum e^(x - m) and
+// t = sum e^(x - m) (x - m), moved to a new m as s' = s c, t' = c (t + s (m - m')),
+// c = e^(m - m'); threads, waves and parts of a row join the same way.  Then
+//   ln sum e^x = m + ln s,   entropy = ln s - t / s.
+// A thread adds its values in groups of eight, and keeps what a sum's rounding
+// leaves: beside a token that stands out the others are each less than half a step
+// of the sum, and a thousand of them count (1e-6 of a row's result without).
+// Where the most likely tokens are asked for, a wave keeps the 64 best keys (a
+// value's order above its complemented place, so that no two are equal) sorted, one
+// to a lane, and a value of LDS room for 64 more; of a tile of values those above
+// the k-th best go there (few after the first tiles: a random row of n has about
+// k ln(n / k)), and a full one is sorted and merged in.
+//
+// A row is one workgroup's, or, where there are few, several workgroups' and joined
+// by a second launch.
+#include <float.h>
+
+#include "qmag_rows.h"
+#include "qmag_wavesort.h"
+
+namespace qmag {
+
+constexpr int LP_WG = 256, LP_WAVES = LP_WG / 64;
+constexpr int LP_PER = 8;                        // values of a thread in a tile
+constexpr int LP_TILE = 64 * LP_PER;             // a wave's tile
+
+struct LpArgs {
+    const void *x;
+    int64_t stride;
+    const int *token;
+    float *logprob, *entropy, *top_logprob;
+    int *top_id;
+    float *stat;             // parts: [T][parts][4] m, s, t
+    uint64_t *keys;          // [T][parts][64]
+    int n_vocab, T, top_k, parts, part_len;
+};
+
+constexpr uint32_t LP_KEY_NONE = 0x007FFFFFu;    // samp_key(-inf)
+constexpr float LOG2E = 1.44269504088896340736f;
+
+struct LpSum {
+    float m, s, t, rs, rt;            // rs, rt: what s and t are above their sums
+    __device__ void clear() { m = -FLT_MAX, s = 0.0f, t = 0.0f, rs = 0.0f, rt = 0.0f; }
+    __device__ void add(float es, float et)
+    {
+        const float ys = es - rs, yt = et - rt, ns = s + ys, nt = t + yt;
+        rs = (ns - s) - ys;
+        rt = (nt - t) - yt;
+        s = ns;
+        t = nt;
+    }
+    // to a maximum of at least m: a sum of nothing stays one
+    __device__ void move(float to)
+    {
+        const float d = fmaxf(m - to, -200.0f), c = exp2f(d * LOG2E);
+        t = s == 0.0f ? 0.0f : c * fmaf(s, d, t);
+        rt = s == 0.0f ? 0.0f : c * fmaf(rs, d, rt);
+        s *= c;
+        rs *= c;
+        m = to;
+    }
+    __device__ void join(float m2, float s2, float t2)
+    {
+        LpSum o;
+        o.clear();
+        o.m = m2, o.s = s2, o.t = t2;
+        const float to = fmaxf(m, m2);
+        move(to);
+        o.move(to);
+        s += o.s;
+        t += o.t;
+    }
+};
+
+__device__ __forceinline__ LpSum lp_wave_join(LpSum a)
+{
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        const float m = __uint_as_float(xor_lane(__float_as_uint(a.m), d)), s = __uint_as_float(xor_lane(__float_as_uint(a.s), d)),
+                    t = __uint_as_float(xor_lane(__float_as_uint(a.t), d));
+        a.join(m, s, t);
+    }
+    return a;
+}
+
+// keys sorted descending and others ascending: the 64 largest of both, descending
+__device__ __forceinline__ uint64_t lp_merge(uint64_t best, uint64_t ascending)
+{
+    return wave_clean64(best > ascending ? best : ascending);
+}
+
+// a wave's best keys
+struct LpTop {
+    uint64_t best;        // one to a lane, descending
+    float bound;          // the k-th best value
+    bool full;            // there are k numbers: what is not above the bound is none of the best
+    int n;                // keys waiting in LDS
+    __device__ void clear() { best = 0, bound = 0.0f, full = false, n = 0; }
+    __device__ void take(const uint64_t *wait, int k)
+    {
+        __builtin_amdgcn_wave_barrier();
+        const uint64_t v = lane_id() < n ? wait[lane_id()] : 0ull;
+        __builtin_amdgcn_wave_barrier();
+        best = lp_merge(best, ~wave_sort64(~v));
+        n = 0;
+        const uint64_t kth = readlane64(best, k - 1);
+        full = (uint32_t)(kth >> 32) > 1u;           // 0: no key, 1: NaN
+        bound = samp_value(kth);
+    }
+    // What of a tile may be among the best, hi being the lane's largest value in it: values above the bound, or,
+    // while there is none, keys from the k-th best of the lanes' largest on (k lanes hold one of that size).  It holds
+    // for the whole tile, whose values do not come in the order of their places.
+    __device__ bool filter(float hi, int k, uint32_t *from) const
+    {
+        if (full) {
+            *from = 0;
+            return __ballot(hi > bound) != 0;
+        }
+        *from = (uint32_t)__builtin_amdgcn_readlane((int)wave_sort64_u32(samp_key(hi)), k - 1);
+        if (*from <= LP_KEY_NONE) *from = 0;             // a lane's largest may be no value of the row
+        return true;
+    }
+    __device__ void add(float v, int id, bool in, bool first, uint32_t from, float above, uint64_t *wait, int k)
+    {
+        const uint32_t key = samp_key(v);
+        const uint64_t who = __ballot(in && (first ? key >= from : v > above));
+        if (!who) return;
+        const int more = __popcll(who);
+        if (n + more > 64) take(wait, k);
+        const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+        if ((who >> lane_id()) & 1u) wait[n + at] = samp_comp(key, id, v);
+        n += more;
+    }
+};
+
+// The results of a row from its sums, by one wave; key: its best keys, one to a lane.
+template <class T>
+__device__ __forceinline__ void lp_finish(const LpArgs &A, int64_t row, LpSum a, uint64_t key)
+{
+    const int lane = lane_id();
+    const float nan = __builtin_nanf("");
+    // a NaN among the sums is one among the logits, or an infinite maximum
+    const bool ok = a.s > 0.0f && a.m < INFINITY;
+    const float ln = logf(a.s);
+    if (lane == 0 && A.logprob) {
+        const int tok = A.token[row];
+        float lp = 0.0f;
+        if (tok >= 0 && tok < A.n_vocab) lp = ok ? (T::up(((const typename T::S *)A.x)[row * A.stride + tok]) - a.m) - ln : nan;
+        A.logprob[row] = lp;
+    }
+    if (lane == 0 && A.entropy) A.entropy[row] = ok ? fmaxf(ln - a.t / a.s, 0.0f) : nan;
+    if (lane < A.top_k) {
+        A.top_id[row * A.top_k + lane] = samp_id(key);
+        A.top_logprob[row * A.top_k + lane] = ok ? (samp_value(key) - a.m) - ln : nan;
+    }
+}
+
+template <class T, bool TOP>
+__global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
+{
+    using S = typename T::S;
+    __shared__ uint64_t s_wait[TOP ? LP_WAVES : 1][64];
+    __shared__ float s_sum[LP_WAVES][3];
+    const int lane = lane_id(), w = threadIdx.x >> 6;
+    uint64_t *wait = s_wait[TOP ? w : 0];
+    for (int64_t job = blockIdx.x; job < (int64_t)A.T * A.parts; job += gridDim.x) {
+        const int64_t row = job / A.parts;
+        const int part = (int)(job - row * A.parts);
+        const int v0 = part * A.part_len, v1 = (int)min((int64_t)v0 + A.part_len, (int64_t)A.n_vocab);
+        const S *x = (const S *)A.x + row * A.stride;
+        LpSum a;
+        a.clear();
+        LpTop top;
+        top.clear();
+        for (int64_t at = (int64_t)v0 + w * LP_TILE; at < v1; at += LP_WAVES * LP_TILE) {
+            const int64_t i0 = at + lane * LP_PER;
+            float v[LP_PER];
+            if (i0 + LP_PER <= v1) {
+                load_row<T, LP_PER>(x + i0, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < LP_PER; i++) v[i] = i0 + i < v1 ? T::up(x[i0 + i]) : -INFINITY;
+            }
+            float hi = v[0];
+#pragma unroll
+            for (int i = 1; i < LP_PER; i++) hi = fmaxf(hi, v[i]);
+            if (hi > a.m) a.move(hi);
+            float es = 0.0f, et = 0.0f;
+#pragma unroll
+            for (int i = 0; i < LP_PER; i++) {
+                const float d = v[i] - a.m, e = exp2f(d * LOG2E);
+                es += e;                                              // a NaN stays
+                et = fmaf(e, fmaxf(d, -200.0f), et);
+            }
+            a.add(es, et);
+            if constexpr (TOP) {
+                uint32_t from;
+                const bool first = !top.full;
+                const float above = top.bound;
+                if (top.filter(hi, A.top_k, &from)) {
+#pragma unroll
+                    for (int i = 0; i < LP_PER; i++) top.add(v[i], (int)(i0 + i), i0 + i < v1, first, from, above, wait, A.top_k);
+                    if (first) top.take(wait, A.top_k);
+                }
+            }
+        }
+        if constexpr (TOP) {
+            top.take(wait, A.top_k);
+            wait[lane] = top.best;
+        }
+        a = lp_wave_join(a);
+        if (lane == 0) s_sum[w][0] = a.m, s_sum[w][1] = a.s, s_sum[w][2] = a.t;
+        __syncthreads();
+        if (w == 0) {
+#pragma unroll
+            for (int o = 1; o < LP_WAVES; o++) a.join(s_sum[o][0], s_sum[o][1], s_sum[o][2]);
+            uint64_t key = top.best;
+            if constexpr (TOP)
+                for (int o = 1; o < LP_WAVES; o++) key = lp_merge(key, s_wait[o][63 - lane]);
+            if (A.parts == 1) {
+                lp_finish<T>(A, row, a, key);
+            } else {
+                if (lane == 0) {
+                    float *st = A.stat + job * 4;
+                    st[0] = a.m, st[1] = a.s, st[2] = a.t;
+                }
+                if constexpr (TOP) A.keys[job * 64 + lane] = key;
+            }
+        }
+        __syncthreads();                 // the next job's sums
+    }
+}
+
+template <class T, bool TOP>
+__global__ void __launch_bounds__(LP_WG) logprobs_join_kernel(LpArgs A)
+{
+    __shared__ uint64_t s_key[TOP ? LP_WAVES : 1][64];
+    __shared__ float s_sum[LP_WAVES][3];
+    const int lane = lane_id(), w = threadIdx.x >> 6;
+    for (int64_t row = blockIdx.x; row < A.T; row += gridDim.x) {
+        LpSum a;
+        a.clear();
+        uint64_t key = 0;
+        for (int p = w * 64 + lane; p < A.parts; p += LP_WG) {
+            const float *st = A.stat + (row * A.parts + p) * 4;
+            a.join(st[0], st[1], st[2]);
+        }
+        a = lp_wave_join(a);
+        if constexpr (TOP) {
+            for (int p = w; p < A.parts; p += LP_WAVES) key = lp_merge(key, A.keys[(row * A.parts + p) * 64 + 63 - lane]);
+            s_key[w][lane] = key;
+        }
+        if (lane == 0) s_sum[w][0] = a.m, s_sum[w][1] = a.s, s_sum[w][2] = a.t;
+        __syncthreads();
+        if (w == 0) {
+#pragma unroll
+            for (int o = 1; o < LP_WAVES; o++) a.join(s_sum[o][0], s_sum[o][1], s_sum[o][2]);
+            if constexpr (TOP)
+                for (int o = 1; o < LP_WAVES; o++) key = lp_merge(key, s_key[o][63 - lane]);
+            lp_finish<T>(A, row, a, key);
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace qmag
+
+using namespace qmag;
+
+extern "C" int qmag_logprobs_dev(int n_vocab, int type, const void *logits, int64_t stride, const int *token, int T,
+                                 int top_k, float *logprob, float *entropy, int *top_id, float *top_logprob)
+{
+    const int size = attn_type_size(type);
+    if (!size) return fail(QMAG_ERR_ARG, "logprobs: type %d", type);
+    if (n_vocab < 1 || T < 0 || top_k < 0 || top_k > QMAG_LOGPROBS_MAX_TOP || top_k > n_vocab)
+        return fail(QMAG_ERR_ARG, "logprobs: n_vocab=%d T=%d top_k=%d", n_vocab, T, top_k);
+    if (((uintptr_t)token | (uintptr_t)logprob | (uintptr_t)entropy | (uintptr_t)top_id | (uintptr_t)top_logprob) % 4)
+        return fail(QMAG_ERR_ARG, "logprobs: an unaligned pointer");
+    if (T > 0 && ((logprob && !token) || (top_k > 0 && (!top_id || !top_logprob))))
+        return fail(QMAG_ERR_ARG, "logprobs: logprob without token, or top_k=%d without its results", top_k);
+    const qmag_heads hx = {(void *)logits, 1, stride, 0};
+    int st = check_heads("logprobs logits", &hx, type, n_vocab, T, false);
+    if (st) return st;
+    const size_t n = sizeof(float) * (size_t)T;
+    const struct { const void *p; size_t n; } out[] = {{logprob, logprob ? n : 0}, {entropy, entropy ? n : 0},
+                                                       {top_id, n * (size_t)top_k}, {top_logprob, n * (size_t)top_k}};
+    for (int i = 0; i < 4; i++) {
+        if (heads_meet(&hx, size, n_vocab, T, out[i].p, out[i].n) || ranges_meet(out[i].p, out[i].n, token, logprob ? n : 0))
+            return fail(QMAG_ERR_ARG, "logprobs: a result overlaps an input");
+        for (int j = 0; j < i; j++)
+            if (ranges_meet(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(QMAG_ERR_ARG, "logprobs: results overlap");
+    }
+    if ((st = require_ready())) return st;
+    if (T == 0 || (!logprob && !entropy && top_k == 0)) return QMAG_OK;
+
+    LpArgs A = {logits, stride, token, logprob, entropy, top_logprob, top_id, nullptr, nullptr, n_vocab, T, top_k, 1, n_vocab};
+    // rows in parts while there are fewer than 1024 of them, parts of 2048 values and more
+    const int64_t want = (1024 + (int64_t)T - 1) / T, fit = ((int64_t)n_vocab + LP_WAVES * LP_TILE - 1) / (LP_WAVES * LP_TILE);
+    A.parts = (int)(want < fit ? want : fit);
+    if (A.parts > 1) {
+        const int64_t tiles = (fit + A.parts - 1) / A.parts;
+        A.part_len = (int)(tiles * LP_WAVES * LP_TILE);
+        A.parts = (int)((fit + tiles - 1) / tiles);
+    }
+    DeviceScope dev;
+    if (dev.st) return dev.st;
+    hipStream_t s = ctx().stream;
+    if (A.parts > 1) {
+        const size_t jobs = (size_t)T * (size_t)A.parts;
+        uint8_t *p = (uint8_t *)workspace(WS_LOGPROBS, jobs * (16 + (top_k ? 512 : 0)), &st);
+        if (st) return st;
+        A.keys = (uint64_t *)p;
+        A.stat = (float *)(p + jobs * (top_k ? 512 : 0));
+    }
+    const int64_t jobs = (int64_t)T * A.parts, most = 1 << 23;
+    const unsigned grid = (unsigned)(jobs < most ? jobs : most), rows = (unsigned)(T < most ? T : most);
+    prof_begin(PROF_LOGPROBS, s);
+    with_type(type, [&](auto t) {
+        using TT = decltype(t);
+        if (top_k) logprobs_kernel<TT, true><<<grid, LP_WG, 0, s>>>(A);
+        else logprobs_kernel<TT, false><<<grid, LP_WG, 0, s>>>(A);
+        if (A.parts > 1 && top_k) logprobs_join_kernel<TT, true><<<rows, LP_WG, 0, s>>>(A);
+        else if (A.parts > 1) logprobs_join_kernel<TT, false><<<rows, LP_WG, 0, s>>>(A);
+        return 0;
+    });
+    prof_end(PROF_LOGPROBS, s);
+    QMAG_HIP(hipGetLastError());
+    return QMAG_OK;
+}

@@ -99,6 +99,9 @@ SIGNATURES = {
     "qmag_kv4_read_dev": (C.c_int, [P, P, C.c_int, P, P]),
     "qmag_attn_kv4_dev": (C.c_int, [P, P, C.c_int, P, P, P, P, C.c_int, C.c_float]),
     "qmag_attn_prompt_dev": (C.c_int, [C.c_int, C.c_int, P, P, P, P, P, C.c_int, C.c_int, C.c_float]),
+    "qmag_logprobs_dev": (C.c_int, [C.c_int, C.c_int, P, C.c_int64, P, C.c_int, C.c_int, P, P, P, P]),
+    "qmag_conv_dev": (C.c_int, [P, C.c_int, P, C.c_int64, P, C.c_int64, P, P, P, C.c_int, C.c_int]),
+    "qmag_linattn_dev": (C.c_int, [P, C.c_int, P, P, P, P, P, P, P, P, P, C.c_int, C.c_int, C.c_float]),
     "qmag_synth_normal": (C.c_int, [C.c_uint64, C.c_size_t, C.c_float, C.c_float, P]),
     "qmag_synth_weights": (C.c_int, [C.c_uint64, C.c_size_t, C.c_float, C.c_int, P]),
     "qmag_quantize_dev": (C.c_int, [P, C.c_size_t, C.c_int, P]),
@@ -414,6 +417,38 @@ def attn_prompt_dev(type: int, head_dim: int, q, k, v, out, cu_ptr: int, n_seq: 
     check(lib().qmag_attn_prompt_dev(type, head_dim, q, k, v, out, cu_ptr, n_seq, T, scale))
 
 
+class Conv(C.Structure):
+    """qmag_conv"""
+    _fields_ = [("n_channel", C.c_int), ("width", C.c_int), ("silu", C.c_int), ("n_slot", C.c_int), ("weight", P), ("bias", P),
+                ("state", P)]
+
+
+class Linattn(C.Structure):
+    """qmag_linattn"""
+    _fields_ = [("n_head", C.c_int), ("dim_k", C.c_int), ("dim_v", C.c_int), ("delta", C.c_int), ("turns", C.c_int),
+                ("norm_eps", C.c_float), ("n_slot", C.c_int), ("state", P)]
+
+
+def conv_dev(c: Conv, type: int, x_ptr: int, x_stride: int, out_ptr: int, out_stride: int, slot_ptr: int, len_ptr,
+             cu_ptr: int, n_seq: int, T: int) -> None:
+    """len_ptr: None where every sequence continues its state."""
+    check(lib().qmag_conv_dev(C.byref(c), type, x_ptr, x_stride, out_ptr, out_stride, slot_ptr, len_ptr, cu_ptr, n_seq, T))
+
+
+def linattn_dev(a: Linattn, type: int, q, k, v, out, decay_ptr, beta_ptr, slot_ptr: int, len_ptr, cu_ptr: int, n_seq: int,
+                T: int, scale: float) -> None:
+    """q, k, v, out: heads(); decay_ptr, beta_ptr, len_ptr: None for none."""
+    check(lib().qmag_linattn_dev(C.byref(a), type, q, k, v, out, decay_ptr, beta_ptr, slot_ptr, len_ptr, cu_ptr, n_seq, T,
+                                 scale))
+
+
+def logprobs_dev(n_vocab: int, type: int, logits_ptr: int, stride: int, token_ptr, T: int, top_k: int, logprob_ptr,
+                 entropy_ptr, top_id_ptr, top_logprob_ptr) -> None:
+    """None for a result that is not wanted."""
+    check(lib().qmag_logprobs_dev(n_vocab, type, logits_ptr, stride, token_ptr, T, top_k, logprob_ptr, entropy_ptr,
+                                  top_id_ptr, top_logprob_ptr))
+
+
 def synth_normal(seed: int, n: int, mean: float, std: float, out_ptr: int) -> None:
     check(lib().qmag_synth_normal(C.c_uint64(seed), n, mean, std, out_ptr))
 
@@ -427,7 +462,8 @@ def quantize_dev(x_ptr: int, n: int, wtype: int, out_ptr: int) -> None:
 
 
 PROF_IDS = {"router": 0, "topk": 1, "gateup": 2, "hquant": 3, "down": 4, "fused": 5, "matvec": 6,
-            "q8k": 7, "group": 8, "combine": 9, "rope": 10, "kv": 11, "attn": 12}
+            "q8k": 7, "group": 8, "combine": 9, "rope": 10, "kv": 11, "attn": 12, "conv": 13, "linattn": 14,
+            "logprobs": 15}
 
 
 def prof_enable(on: bool) -> None:
