@@ -4,16 +4,34 @@
 //
 //   S <- a S;  u = b (v - delta S^T k);  S <- S + k u^T;  o = scale S^T q,  a = e^g
 //
-// The columns of S have nothing to do with one another.  A wave takes 16 of them: lane
-// l rows (l % 16) dim_k / 16 .. of columns 4 (l / 16) .., all in registers for as
-// many tokens as there are.  With S0 the state ahead of a token,
+// The columns of S have nothing to do with one another.  Two forms:
+//
+// Token by token (la_recurrence).  A wave takes 16 columns: lane l rows
+// (l % 16) dim_k / 16 .. of columns 4 (l / 16) .., all in registers for as many tokens
+// as there are.  With S0 the state ahead of a token,
 //   S^T q = a S0^T q + (k . q) u,
 // so that both of a token's products with the state are formed from S0, side by side,
 // and one exchange over 16 lanes sums them.
+//
+// In chunks of 64 tokens, for prompts.  With G the sums of g from a chunk's start and S0
+// the state ahead of it,
+//   (I + L) U = b (V - e^G K S0),  L_ij = b_i (k_i . k_j) e^(G_i - G_j), j < i  (delta)
+//   O = scale (e^G Q S0 + P U),    P_ij = (q_i . k_j) e^(G_i - G_j), j <= i
+//   S1 = e^G_63 S0 + sum_j e^(G_63 - G_j) k_j u_j^T.
+// P and (I + L)^-1 do not depend on the state: a first kernel forms them for all chunks
+// at once, a second walks down each sequence's chunks, 16 columns of a head to a
+// workgroup.  Sums of g are held in 64 bits, since their differences count.
+//
+// Products are the bf16 matrix cores': an fp32 operand is three bf16 parts (24 bits, the
+// range of fp32; fp16 values are two exactly, bf16 ones one), and of the products of
+// parts those are formed whose places add up to less than three (2^-24 of the operands).
+// An accumulator holds four rows of a column in a lane, which is half of what the next
+// product's operand holds of 32 rows: products whose 32 terms are taken in the order
+// [4 g .. 4 g + 3, 16 + 4 g ..] for lane group g need no move between lanes.
 #include <math.h>
 
 #include "qmag_rows.h"
-#include "qmag_seq.h"
+#include "qmag_linattn_plan.h"
 
 namespace qmag {
 
@@ -31,9 +49,19 @@ struct LaArgs {
     const float *decay, *beta;
     float *state;
     const int *slot, *len, *cu;
-    int n_head, share, turns, dim_v, n_slot, n_seq, T;
+    int n_head, n_key, share, turns, dim_v, n_slot, n_seq, T;
     float norm_eps, scale;
+    // the chunked form
+    int r0, r1;               // the window's rows
+    int n_tile;
+    uint8_t *keys, *heads;    // what chunks have for each key head, and for each head
+    const float *carry_in;    // [n_head][dim_k][dim_v]: the state of a sequence begun ahead of the window
+    float *carry_out;
 };
+
+// the key head of a head, and the i-th head of a key head
+__device__ __forceinline__ int la_key_of(const LaArgs &A, int head) { return A.turns ? head % A.n_key : head / A.share; }
+__device__ __forceinline__ int la_head_of(const LaArgs &A, int key, int i) { return A.turns ? key + i * A.n_key : key * A.share + i; }
 
 // e^g: at most 1, nothing left of what a fp32 weight does not hold; a NaN stays
 __device__ __forceinline__ float la_decay(float g)
@@ -41,49 +69,57 @@ __device__ __forceinline__ float la_decay(float g)
     return g > 0.0f ? 1.0f : expf(g);
 }
 
-template <class T, int N>
+// Where a sequence's state comes from and goes to, at row 0 and column 0 of a head; null: nowhere.
+struct LaState {
+    const float *from;
+    float *to;
+};
+__device__ __forceinline__ LaState la_state(const LaArgs &A, int seq, int head, int dim_k, bool begun, bool goes_on)
+{
+    const int64_t size = (int64_t)dim_k * A.dim_v;
+    const int slot = A.slot ? ldg(A.slot + seq) : -1;
+    float *own = slot >= 0 && slot < A.n_slot ? A.state + ((int64_t)slot * A.n_head + head) * size : nullptr;
+    LaState s;
+    s.from = begun ? A.carry_in + head * size : own && !(A.len && ldg(A.len + seq) <= 0) ? own : nullptr;
+    s.to = goes_on ? A.carry_out + head * size : own;
+    return s;
+}
+
+template <int N>
 struct LaToken {
     float k[N], q[N], v[4], a, b;
 };
 
-// A sequence's rows, one after another, of one head and 16 columns, by one wave.
-template <class T, int DK, bool DELTA>
-__device__ void la_recurrence(const LaArgs &A, int seq, int head, int c0, int first, int n)
+// n rows from `first` on, one after another, of one head and 16 columns, by one wave;
+// from(row, x): four values of the state ahead of them, from the lane's column on.  The
+// first `quiet` rows' results are there already.
+template <class T, int DK, bool DELTA, class F>
+__device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int n, int quiet, F from, float *to)
 {
     using S = typename T::S;
     constexpr int N = DK / 16;
     const int lane = lane_id(), rg = lane & 15, col = c0 + 4 * (lane >> 4);
-    const int kh = A.turns ? head % A.share : head / A.share;
-    const int slot = A.slot ? ldg(A.slot + seq) : -1;
-    const bool held = slot >= 0 && slot < A.n_slot;
-    float *state = A.state + (((int64_t)(held ? slot : 0) * A.n_head + head) * DK + rg * N) * A.dim_v + col;
+    const int kh = la_key_of(A, head);
     float s[N][4];
-    if (held && !(A.len && ldg(A.len + seq) <= 0)) {
 #pragma unroll
-        for (int r = 0; r < N; r++) load_row<TF32, 4>(state + (int64_t)r * A.dim_v, s[r]);
-    } else {
-#pragma unroll
-        for (int r = 0; r < N; r++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) s[r][c] = 0.0f;
-    }
+    for (int r = 0; r < N; r++) from(rg * N + r, s[r]);
     const S *kp = (const S *)A.k.p + first * A.k.ts + kh * A.k.hs + rg * N;
     const S *qp = (const S *)A.q.p + first * A.q.ts + kh * A.q.hs + rg * N;
     const S *vp = (const S *)A.v.p + first * A.v.ts + head * A.v.hs + col;
     S *op = (S *)A.out + first * A.ots + head * A.ohs + col;
     const float *gp = A.decay ? A.decay + (int64_t)first * A.n_head + head : nullptr;
     const float *bp = A.beta ? A.beta + (int64_t)first * A.n_head + head : nullptr;
-    auto load = [&](int t, LaToken<T, N> &x) {
+    auto load = [&](int t, LaToken<N> &x) {
         load_row<T, N>(kp + t * A.k.ts, x.k);
         load_row<T, N>(qp + t * A.q.ts, x.q);
         load_row<T, 4>(vp + t * A.v.ts, x.v);
         x.a = gp ? ldg(gp + (int64_t)t * A.n_head) : 0.0f;
         x.b = bp ? ldg(bp + (int64_t)t * A.n_head) : 1.0f;
     };
-    LaToken<T, N> x;
+    LaToken<N> x;
     load(0, x);
     for (int t = 0; t < n; t++) {
-        LaToken<T, N> next;
+        LaToken<N> next;
         if (t + 1 < n) load(t + 1, next);
         if (A.norm_eps > 0.0f) {
             // ahead of the products: a large key's would leave fp32's range
@@ -120,13 +156,28 @@ __device__ void la_recurrence(const LaArgs &A, int seq, int head, int c0, int fi
         for (int r = 0; r < N; r++)
 #pragma unroll
             for (int c = 0; c < 4; c++) s[r][c] = fmaf(x.k[r], u[c], a * s[r][c]);
-        if (rg == 0) store_row<T, 4>(op + t * A.ots, o);
+        if (rg == 0 && t >= quiet) store_row<T, 4>(op + t * A.ots, o);
         x = next;
     }
-    if (held) {
+    if (to) {
 #pragma unroll
-        for (int r = 0; r < N; r++) store_row<TF32, 4>(state + (int64_t)r * A.dim_v, s[r]);
+        for (int r = 0; r < N; r++) store_row<TF32, 4>(to + (int64_t)(rg * N + r) * A.dim_v + col, s[r]);
     }
+}
+
+// the same from a sequence's own state
+template <class T, int DK, bool DELTA>
+__device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int n, LaState st)
+{
+    const int col = c0 + 4 * (lane_id() >> 4);
+    la_recurrence<T, DK, DELTA>(A, head, c0, first, n, 0, [&](int row, float (&x)[4]) {
+        if (st.from) {
+            load_row<TF32, 4>(st.from + (int64_t)row * A.dim_v + col, x);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) x[c] = 0.0f;
+        }
+    }, st.to);
 }
 
 template <class T, int DK, bool DELTA>
@@ -139,7 +190,616 @@ __global__ void __launch_bounds__(LA_WG) linattn_step_kernel(LaArgs A)
         const int seq = __builtin_amdgcn_readfirstlane((int)(sh / A.n_head)), head = __builtin_amdgcn_readfirstlane((int)(sh % A.n_head));
         const int c0 = __builtin_amdgcn_readfirstlane((int)(j % slices) * 16);
         const int first = seq_row(ldg(A.cu + seq), A.T), n = seq_row(ldg(A.cu + seq + 1), A.T) - first;
-        if (n > 0) la_recurrence<T, DK, DELTA>(A, seq, head, c0, first, n);
+        if (n > 0) la_recurrence<T, DK, DELTA>(A, head, c0, first, n, la_state(A, seq, head, DK, false, false));
+    }
+}
+
+// ------------------------------------------------------------ in chunks --
+
+// bf16 parts of a value of the type, and of what the heads' matrices are held in
+template <class T> constexpr int LA_PARTS = 3;
+template <> constexpr int LA_PARTS<TF16> = 2;
+template <> constexpr int LA_PARTS<TBF16> = 1;
+// For results of 16 bits two parts of P, U and the state: 2^-16 of them beside the result's own rounding of 2^-9 or 2^-12.
+template <class T> constexpr int LA_OUT_PARTS = 2;
+template <> constexpr int LA_OUT_PARTS<TF32> = 3;
+
+// Operands lie in the workspace as the matrix cores take them: 64 lanes of 16 bytes.
+constexpr int LA_FRAG = 1024;
+constexpr int LA_TRI = 6;             // operands of a lower triangle: 16 rows by 32 columns, those all above it left out
+constexpr int la_tri(int rt, int tb) { return rt < 2 ? rt : 2 * rt - 2 + tb; }
+template <class T, int DK>
+struct LaLayout {
+    static constexpr int NP = LA_PARTS<T>, NKB = DK / 32;
+    // a chunk and key head: K and Q [16 rows: 4][NKB][NP], K^T [DK / 16][32 tokens: 2][NP]
+    static constexpr int K = 0, Q = 4 * NKB * NP * LA_FRAG, KT = 2 * Q, KEY_BYTES = 3 * Q;
+    // a chunk and head: (I + L)^-1 and P [LA_TRI][parts], then rows of 64: what the chunk's tokens are multiplied by
+    static constexpr int TI = 0, P = LA_TRI * 3 * LA_FRAG, VEC = P + LA_TRI * LA_OUT_PARTS<T> * LA_FRAG;
+    static constexpr int KD = 0, QD = 64, KE = 128, B = 192, END = 256, BAD = 257;     // floats; END: e^G_63; BAD: the first row the form does not hold, 64: none
+    static constexpr int HEAD_BYTES = VEC + 272 * 4;
+};
+
+// x as N parts, the first the nearest bf16 to it, each other to what those ahead leave
+template <int N, int V>
+__device__ __forceinline__ void la_split(const float (&x)[V], __bf16 (&o)[N][V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        float r = x[i];
+#pragma unroll
+        for (int p = 0; p < N; p++) {
+            o[p][i] = (__bf16)r;
+            r -= (float)o[p][i];
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void la_split8(const float (&x)[8], bf168 (&o)[N])
+{
+    __bf16 s[N][8];
+    la_split<N, 8>(x, s);
+#pragma unroll
+    for (int p = 0; p < N; p++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[p][i] = s[p][i];
+}
+
+// c += a b, of the products of parts those of places adding up to at most UP
+template <int NA, int NB, int UP>
+__device__ __forceinline__ f32x4 la_mul(const bf168 (&a)[NA], const bf168 (&b)[NB], f32x4 c)
+{
+#pragma unroll
+    for (int s = UP; s >= 0; s--)                     // the small ones first
+#pragma unroll
+        for (int i = 0; i < NA; i++)
+            if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
+    return c;
+}
+
+template <int N>
+__device__ __forceinline__ void la_load(const uint8_t *p, bf168 (&o)[N])
+{
+    const int at = lane_id() * 16;
+#pragma unroll
+    for (int i = 0; i < N; i++) o[i] = *(const QMAG_GLOBAL bf168 *)(p + i * LA_FRAG + at);
+}
+template <int N>
+__device__ __forceinline__ void la_store(uint8_t *p, const bf168 (&x)[N])
+{
+    const int at = lane_id() * 16;
+#pragma unroll
+    for (int i = 0; i < N; i++) *(QMAG_GLOBAL bf168 *)(p + i * LA_FRAG + at) = x[i];
+}
+
+// sums over the four lanes of a column (or row)
+__device__ __forceinline__ float la_sum4(float v)
+{
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// A wave looks for long sequences: of chunk number j the sequence (-1: none), its rows and which of its chunks.
+struct LaTile {
+    LaRows rows;
+    int chunk;
+    bool any;
+};
+__device__ LaTile la_find(const LaArgs &A, int j)
+{
+    const int lane = lane_id();
+    int rank = 0;
+    for (int s0 = 0; s0 < A.n_seq; s0 += 64) {
+        const int i = s0 + lane;
+        LaRows x = {0, 0, false, false};
+        if (i < A.n_seq) x = la_rows(ldg(A.cu + i), ldg(A.cu + i + 1), A.T, A.r0, A.r1);
+        const uint64_t is_long = __ballot(la_long(x.n));
+        const int tile0 = la_tile0(x.first, A.r0, rank + __popcll(is_long & ((1ull << lane) - 1)));
+        const uint64_t hit = __ballot(la_long(x.n) && j >= tile0 && j < tile0 + seq_tiles(x.n, LA_SHIFT));
+        if (hit) {
+            const int at = __ffsll((unsigned long long)hit) - 1;
+            x.first = __builtin_amdgcn_readlane(x.first, at);
+            x.n = __builtin_amdgcn_readlane(x.n, at);
+            return {x, j - __builtin_amdgcn_readlane(tile0, at), true};
+        }
+        rank += __popcll(is_long);
+    }
+    return {{0, 0, false, false}, 0, false};
+}
+// the number of a long sequence's first chunk
+__device__ int la_first_tile(const LaArgs &A, int seq, int first)
+{
+    const int lane = lane_id();
+    int rank = 0;
+    for (int s0 = 0; s0 < seq; s0 += 64) {
+        const int i = s0 + lane;
+        bool is_long = false;
+        if (i < seq) is_long = la_long(la_rows(ldg(A.cu + i), ldg(A.cu + i + 1), A.T, A.r0, A.r1).n);
+        rank += __popcll(__ballot(is_long));
+    }
+    return la_tile0(first, A.r0, rank);
+}
+
+// What a chunk of a key head and its heads has that does not depend on the state: a wave takes 16 of the chunk's rows.
+// Products of rows j with rows i leave lane group g with j = 4 g .. of a row i: as P and the inverse are operands.
+template <class T, int DK, bool DELTA>
+__global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
+{
+    using S = typename T::S;
+    using Y = LaLayout<T, DK>;
+    constexpr int NP = Y::NP, NKB = Y::NKB, ROW = DK + 8;
+    __shared__ __attribute__((aligned(16))) __bf16 s_k[NP][64][ROW];
+    __shared__ __attribute__((aligned(16))) float s_lt[64][68];           // L, rows and columns exchanged
+    __shared__ __attribute__((aligned(16))) float s_dt[4][16][20];        // inverses of its diagonal blocks, exchanged
+    __shared__ double s_g[64];
+    __shared__ float s_fk[64], s_fq[64], s_kk[64], s_b[64];
+    __shared__ int s_odd[4], s_good;
+    const int lane = lane_id(), w = threadIdx.x >> 6, l16 = lane & 15, g4 = (lane >> 4) * 4;
+    const int tile = blockIdx.x / A.n_key, key = blockIdx.x % A.n_key;
+    const LaTile at = la_find(A, tile);
+    if (!at.any) return;
+    const int n = min(64, at.rows.n - 64 * at.chunk);
+    const int64_t row0 = at.rows.first + 64 * (int64_t)at.chunk;
+    uint8_t *mine = A.keys + ((int64_t)tile * A.n_key + key) * Y::KEY_BYTES;
+
+    // rows of K and Q as operands, their sums of squares
+    bf168 kf[NKB][NP], qf[NKB][NP];
+    float kk = 0.0f, qq = 0.0f;
+    const int my = 16 * w + l16;
+#pragma unroll
+    for (int kb = 0; kb < NKB; kb++) {
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.0f, y[e] = 0.0f;
+        if (my < n) {
+            const S *kp = (const S *)A.k.p + (row0 + my) * A.k.ts + key * A.k.hs + 32 * kb + g4;
+            const S *qp = (const S *)A.q.p + (row0 + my) * A.q.ts + key * A.q.hs + 32 * kb + g4;
+            float h[4];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                load_row<T, 4>(kp + 16 * half, h);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[4 * half + e] = h[e];
+                load_row<T, 4>(qp + 16 * half, h);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[4 * half + e] = h[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            kk = fmaf(x[e], x[e], kk);
+            qq = fmaf(y[e], y[e], qq);
+        }
+        la_split8<NP>(x, kf[kb]);
+        la_split8<NP>(y, qf[kb]);
+        la_store<NP>(mine + Y::K + (w * NKB + kb) * NP * LA_FRAG, kf[kb]);
+        la_store<NP>(mine + Y::Q + (w * NKB + kb) * NP * LA_FRAG, qf[kb]);
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            const s16x4 *h = (const s16x4 *)&kf[kb][p];
+            *(s16x4 *)&s_k[p][my][32 * kb + g4] = h[0];
+            *(s16x4 *)&s_k[p][my][32 * kb + 16 + g4] = h[1];
+        }
+    }
+    kk = la_sum4(kk);
+    qq = la_sum4(qq);
+    const bool norm = A.norm_eps > 0.0f;
+    if (lane < 16) {
+        s_kk[my] = norm ? kk / (kk + A.norm_eps) : kk;
+        s_fk[my] = norm ? rsqrtf(kk + A.norm_eps) : 1.0f;
+        s_fq[my] = norm ? rsqrtf(qq + A.norm_eps) : 1.0f;
+    }
+    // From a row whose values the products' fp32 sums, or the sums of squares, do not hold on the chunk goes token by
+    // token; the rows ahead of it are as if there were none behind.
+    constexpr float MOST = 0x1p80f, LEAST = 0x1p-60f;
+    const uint64_t odd = __ballot(!(kk <= MOST) || !(qq <= MOST) || (norm && ((kk > 0.0f && kk < LEAST) || (qq > 0.0f && qq < LEAST))));
+    if (lane == 0) s_odd[w] = odd ? 16 * w + (__ffsll((unsigned long long)odd) - 1) % 16 : 64;
+    __syncthreads();
+    const int even = min(min(s_odd[0], s_odd[1]), min(s_odd[2], s_odd[3]));
+
+    f32x4 ck[4], cq[4];
+#pragma unroll
+    for (int ct = 0; ct < 4; ct++) {
+        ck[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, cq[ct] = ck[ct];
+        if (ct > w) continue;
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++) {
+            bf168 a[NP];
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                s16x4 *h = (s16x4 *)&a[p];
+                h[0] = *(const s16x4 *)&s_k[p][16 * ct + l16][32 * kb + g4];
+                h[1] = *(const s16x4 *)&s_k[p][16 * ct + l16][32 * kb + 16 + g4];
+            }
+            if constexpr (DELTA) ck[ct] = la_mul<NP, NP, 2>(a, kf[kb], ck[ct]);
+            cq[ct] = la_mul<NP, NP, 2>(a, qf[kb], cq[ct]);
+        }
+    }
+    // K^T, 16 channels by 32 tokens
+    for (int f = w; f < DK / 16 * 2; f += 4) {
+        const int ch = 16 * (f >> 1) + l16, t0 = 32 * (f & 1) + g4;
+        bf168 a[NP];
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) a[p][e] = s_k[p][t0 + (e & 3) + 16 * (e >> 2)][ch];
+        la_store<NP>(mine + Y::KT + f * NP * LA_FRAG, a);
+    }
+
+    const int sharing = A.n_head / A.n_key;
+    for (int i = 0; i < sharing; i++) {
+        const int head = la_head_of(A, key, i);
+        uint8_t *to = A.heads + ((int64_t)tile * A.n_head + head) * Y::HEAD_BYTES;
+        if (w == 0) {
+            float g = 0.0f, b = 0.0f;
+            if (lane < n) {
+                g = A.decay ? ldg(A.decay + (row0 + lane) * A.n_head + head) : 0.0f;
+                b = A.beta ? ldg(A.beta + (row0 + lane) * A.n_head + head) : 1.0f;
+            }
+            const bool none = g != g;
+            g = g > 0.0f ? 0.0f : g < -200.0f ? -200.0f : g;              // e^-200 is 0 in fp32
+            double sum = g;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const double o = __shfl_up(sum, d);
+                if (lane >= d) sum += o;
+            }
+            const double all = __shfl(sum, 63);
+            const float bk = b * s_kk[lane];
+            // the delta rule grows past b |k|^2 = 2, and its inverse with it
+            const bool out = none || (DELTA ? !(bk >= 0.0f && bk <= 2.01f) || !(b <= 0x1p60f) : !(fabsf(b) <= 0x1p40f));
+            const uint64_t bad = __ballot(out);
+            s_g[lane] = sum;
+            s_b[lane] = b;
+            const int good = bad ? min(even, __ffsll((unsigned long long)bad) - 1) : even;
+            float *vec = (float *)(to + Y::VEC);
+            const float now = expf((float)sum), fk = s_fk[lane];
+            vec[Y::KD + lane] = now * fk;
+            vec[Y::QD + lane] = A.scale * s_fq[lane] * now;
+            vec[Y::KE + lane] = expf((float)(all - sum)) * fk;
+            vec[Y::B + lane] = b;
+            if (lane == 0) {
+                vec[Y::END] = expf((float)all);
+                ((int *)vec)[Y::BAD] = s_good = good;
+            }
+        }
+        __syncthreads();
+        const double gi = s_g[my];
+        const bool row = my < s_good;
+        const float pq = A.scale * s_fq[my], lk = s_b[my] * s_fk[my];
+        float pv[4][4];
+#pragma unroll
+        for (int ct = 0; ct < 4; ct++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                pv[ct][r] = 0.0f;
+                if (ct > w) continue;
+                const int j = 16 * ct + g4 + r;
+                const float e = s_fk[j] * expf((float)(gi - s_g[j]));
+                pv[ct][r] = row && j <= my ? pq * (cq[ct][r] * e) : 0.0f;
+                if constexpr (DELTA) s_lt[j][my] = row && j < my ? lk * (ck[ct][r] * e) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int tb = 0; tb < 2; tb++) {
+            if (2 * tb > w) continue;
+            float x[8];
+            bf168 p[LA_OUT_PARTS<T>];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = pv[2 * tb + (e >> 2)][e & 3];
+            la_split8<LA_OUT_PARTS<T>>(x, p);
+            la_store<LA_OUT_PARTS<T>>(to + Y::P + la_tri(w, tb) * LA_OUT_PARTS<T> * LA_FRAG, p);
+        }
+        if constexpr (DELTA) {
+            // the inverse of the wave's diagonal block, a column to a lane (four lanes the same)
+            __builtin_amdgcn_wave_barrier();
+            float d[16];
+#pragma unroll
+            for (int r = 0; r < 16; r++) d[r] = r == l16 ? 1.0f : 0.0f;
+#pragma unroll
+            for (int m = 0; m < 15; m++)
+#pragma unroll
+                for (int r = m + 1; r < 16; r++) d[r] = fmaf(-s_lt[16 * w + m][16 * w + r], d[m], d[r]);
+            if (lane < 16) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) *(f32x4 *)&s_dt[w][l16][r] = f32x4{d[r], d[r + 1], d[r + 2], d[r + 3]};
+            }
+            __syncthreads();
+            // row w of the inverse, from the diagonal on: T_wb = -(sum over c in b + 1 .. w of T_wc L_cb) T_bb
+            f32x4 t[4];
+#pragma unroll
+            for (int b = 3; b >= 0; b--) {
+                t[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (b > w) continue;
+                if (b == w) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) t[b][r] = s_dt[w][g4 + r][l16];
+                    continue;
+                }
+                f32x4 m = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = b + 1; c < 4; c++) {
+                    if (c > w) continue;
+                    const f32x4 a = *(const f32x4 *)&s_lt[16 * b + l16][16 * c + g4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) m = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], t[c][r], m, 0, 0, 0);
+                }
+                const f32x4 a = *(const f32x4 *)&s_dt[b][l16][g4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) t[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(-a[r], m[r], t[b], 0, 0, 0);
+            }
+#pragma unroll
+            for (int tb = 0; tb < 2; tb++) {
+                if (2 * tb > w) continue;
+                float x[8];
+                bf168 p[3];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = t[2 * tb + (e >> 2)][e & 3];
+                la_split8<3>(x, p);
+                la_store<3>(to + Y::TI + la_tri(w, tb) * 3 * LA_FRAG, p);
+            }
+        }
+        __syncthreads();                    // the next head's gates and L
+    }
+}
+
+// Down a sequence's chunks: one head, 16 columns of the state.  Waves 0 .. 3 form U and the next state, 16 of the
+// chunk's rows and a quarter of the state's each; waves 4 .. 7 the results.  What a wave forms the others take from LDS
+// as operands.
+template <class T, int DK, bool DELTA>
+__global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
+{
+    using S = typename T::S;
+    using Y = LaLayout<T, DK>;
+    constexpr int NP = Y::NP, NKB = Y::NKB, NO = LA_OUT_PARTS<T>, UP = NO - 1;
+    constexpr int OWN = (NKB + 3) / 4;                    // blocks of 32 rows of the state that a wave holds
+    __shared__ __attribute__((aligned(16))) uint8_t s_s[NKB][3][LA_FRAG];
+    __shared__ __attribute__((aligned(16))) uint8_t s_x[DELTA ? 2 : 1][3][LA_FRAG], s_u[2][NO][LA_FRAG], s_e[2][3][LA_FRAG];
+    __shared__ int s_bad;
+    const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = (lane >> 4) * 4;
+    const bool chain = w < 4;
+    const int rt = w & 3, at = lane * 16, half = at + 8 * (rt & 1);
+    const int slices = A.dim_v / 16;
+    const int64_t jobs = (int64_t)A.n_seq * A.n_head * slices;
+    // workgroups go round the 8 XCDs: the slices of a head, and heads of one key, on one of them
+    const int64_t per = (jobs + 7) / 8;
+    for (int64_t b = blockIdx.x; b < 8 * per; b += gridDim.x) {
+        const int64_t job = (b & 7) * per + (b >> 3);
+        if (job >= jobs) continue;
+        const int c0 = (int)(job % slices) * 16, head0 = (int)(job / slices % A.n_head), seq = (int)(job / slices / A.n_head);
+        const int head = la_head_of(A, head0 / (A.n_head / A.n_key), head0 % (A.n_head / A.n_key));
+        const LaRows rows = la_rows(ldg(A.cu + seq), ldg(A.cu + seq + 1), A.T, A.r0, A.r1);
+        if (rows.n <= 0) continue;
+        const LaState st = la_state(A, seq, head, DK, rows.begun, rows.goes_on);
+        __syncthreads();                                  // the job before has left LDS
+        const int chunks = seq_tiles(rows.n, LA_SHIFT), tile0 = la_long(rows.n) ? la_first_tile(A, seq, rows.first) : 0;
+        // (sequences that lap over one another may have more chunks than the host counts)
+        if (!la_long(rows.n) || !la_room(tile0, chunks, A.n_tile)) {
+            if (w == 0) la_recurrence<T, DK, DELTA>(A, head, c0, rows.first, rows.n, st);
+            continue;
+        }
+        const int key = la_key_of(A, head);
+        f32x4 s[OWN][2];
+        bool odd = false;
+#pragma unroll
+        for (int o = 0; o < OWN; o++) {
+            const int kb = rt + 4 * o;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    s[o][h][r] = 0.0f;
+                    if (chain && kb < NKB && st.from) s[o][h][r] = ldg(st.from + (int64_t)(32 * kb + 16 * h + g4 + r) * A.dim_v + c0 + l16);
+                    odd |= !(fabsf(s[o][h][r]) <= 0x1p100f);
+                }
+        }
+        auto publish = [&]() {
+#pragma unroll
+            for (int o = 0; o < OWN; o++) {
+                const int kb = rt + 4 * o;
+                if (!chain || kb >= NKB) continue;
+                float x[8];
+                bf168 p[3];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = s[o][e >> 2][e & 3];
+                la_split8<3>(x, p);
+#pragma unroll
+                for (int i = 0; i < 3; i++) *(bf168 *)&s_s[kb][i][at] = p[i];
+            }
+        };
+        publish();
+        if (threadIdx.x == 0) s_bad = 64;
+        int c = 0, upto = 0;                              // the first chunk that is not done, the first such row of it
+        if (!__syncthreads_or(odd)) {
+            bf168 kf[NKB][NP], tf[2][3], ktf[OWN][2][2][NP], pf[2][NO];
+            auto keys = [&](int i) { return A.keys + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_key + key) * Y::KEY_BYTES; };
+            auto heads = [&](int i) { return A.heads + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_head + head) * Y::HEAD_BYTES; };
+            auto load_k = [&](int i) {
+                const uint8_t *p = keys(i) + (chain ? Y::K : Y::Q) + rt * NKB * NP * LA_FRAG;
+#pragma unroll
+                for (int kb = 0; kb < NKB; kb++) la_load<NP>(p + kb * NP * LA_FRAG, kf[kb]);
+            };
+            auto load_kt = [&](int i) {
+                const uint8_t *p = keys(i) + Y::KT;
+#pragma unroll
+                for (int o = 0; o < OWN; o++) {
+                    const int kb = rt + 4 * o;
+                    if (kb >= NKB) continue;
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int tb = 0; tb < 2; tb++) la_load<NP>(p + ((2 * kb + h) * 2 + tb) * NP * LA_FRAG, ktf[o][h][tb]);
+                }
+            };
+            auto load_t = [&](int i) {
+                const uint8_t *p = heads(i) + Y::TI;
+#pragma unroll
+                for (int tb = 0; tb < 2; tb++)
+                    if (2 * tb <= rt) la_load<3>(p + la_tri(rt, tb) * 3 * LA_FRAG, tf[tb]);
+            };
+            auto load_p = [&](int i) {
+                const uint8_t *p = heads(i) + Y::P;
+#pragma unroll
+                for (int tb = 0; tb < 2; tb++)
+                    if (2 * tb <= rt) la_load<NO>(p + la_tri(rt, tb) * NO * LA_FRAG, pf[tb]);
+            };
+            float v[4];
+            auto load_v = [&](int i) {
+                const int t = 64 * min(i, chunks - 1) + 16 * rt + g4;
+                const S *p = (const S *)A.v.p + (rows.first + (int64_t)t) * A.v.ts + head * A.v.hs + c0 + l16;
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[r] = t + r < rows.n ? T::up(p[r * A.v.ts]) : 0.0f;
+            };
+            if (!chain || DELTA) load_k(0);
+            if (chain) {
+                load_v(0);
+                if constexpr (DELTA) load_t(0);
+                load_kt(0);
+            } else {
+                load_p(0);
+            }
+            for (; c < chunks; c++) {
+                const float *vec = (const float *)(heads(c) + Y::VEC);
+                f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (!chain || DELTA) {
+#pragma unroll
+                    for (int kb = 0; kb < NKB; kb++) {
+                        bf168 b[3];
+#pragma unroll
+                        for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
+                        if (chain) acc = la_mul<NP, 3, 2>(kf[kb], b, acc);
+                        else acc = la_mul<NP, 3, UP>(kf[kb], b, acc);
+                    }
+                    load_k(c + 1);
+                }
+                float x[4], ke[4];
+                if (chain) {
+                    const f32x4 kd = *(const QMAG_GLOBAL f32x4 *)(vec + Y::KD + 16 * rt + g4), bt = *(const QMAG_GLOBAL f32x4 *)(vec + Y::B + 16 * rt + g4),
+                                e4 = *(const QMAG_GLOBAL f32x4 *)(vec + Y::KE + 16 * rt + g4);
+                    const int good = ((const QMAG_GLOBAL int *)vec)[Y::BAD];
+                    int bad = good;
+#pragma unroll
+                    for (int r = 3; r >= 0; r--) {
+                        const int row = 16 * rt + g4 + r;
+                        const bool fine = row < good && fabsf(v[r]) <= 0x1p60f;
+                        x[r] = fine ? bt[r] * (DELTA ? fmaf(-kd[r], acc[r], v[r]) : v[r]) : 0.0f;
+                        bad = fine ? bad : min(bad, row);
+                        ke[r] = e4[r];
+                    }
+                    load_v(c + 1);
+                    if (bad < 64) atomicMin(&s_bad, bad);
+                    if constexpr (DELTA) {
+                        __bf16 p[3][4];
+                        la_split<3, 4>(x, p);
+#pragma unroll
+                        for (int i = 0; i < 3; i++) *(s16x4 *)&s_x[rt >> 1][i][half] = *(const s16x4 *)p[i];
+                    }
+                }
+                if constexpr (DELTA) {
+                    __syncthreads();
+                    if (chain) {
+                        f32x4 u = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int tb = 0; tb < 2; tb++) {
+                            if (2 * tb > rt) continue;
+                            bf168 b[3];
+#pragma unroll
+                            for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_x[tb][i][at];
+                            u = la_mul<3, 3, 2>(tf[tb], b, u);
+                        }
+                        load_t(c + 1);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) x[r] = u[r];
+                    }
+                }
+                if (chain) {
+                    __bf16 p[NO][4], pe[3][4];
+                    float xe[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) xe[r] = x[r] * ke[r];
+                    la_split<NO, 4>(x, p);
+                    la_split<3, 4>(xe, pe);
+#pragma unroll
+                    for (int i = 0; i < NO; i++) *(s16x4 *)&s_u[rt >> 1][i][half] = *(const s16x4 *)p[i];
+#pragma unroll
+                    for (int i = 0; i < 3; i++) *(s16x4 *)&s_e[rt >> 1][i][half] = *(const s16x4 *)pe[i];
+                }
+                __syncthreads();
+                upto = s_bad;
+                if (chain && upto == 64) {
+                    const float end = ((const QMAG_GLOBAL float *)vec)[Y::END];
+#pragma unroll
+                    for (int o = 0; o < OWN; o++) {
+                        if (rt + 4 * o >= NKB) continue;
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) s[o][h][r] *= end;
+                    }
+#pragma unroll
+                    for (int tb = 0; tb < 2; tb++) {
+                        bf168 b[3];
+#pragma unroll
+                        for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_e[tb][i][at];
+#pragma unroll
+                        for (int o = 0; o < OWN; o++) {
+                            if (rt + 4 * o >= NKB) continue;
+#pragma unroll
+                            for (int h = 0; h < 2; h++) s[o][h] = la_mul<NP, 3, 2>(ktf[o][h][tb], b, s[o][h]);
+                        }
+                    }
+                    load_kt(c + 1);
+                    publish();
+                } else if (!chain) {
+                    const f32x4 qd = *(const QMAG_GLOBAL f32x4 *)(vec + Y::QD + 16 * rt + g4);
+                    f32x4 o = acc * qd;
+#pragma unroll
+                    for (int tb = 0; tb < 2; tb++) {
+                        if (2 * tb > rt) continue;
+                        bf168 b[NO];
+#pragma unroll
+                        for (int i = 0; i < NO; i++) b[i] = *(const bf168 *)&s_u[tb][i][at];
+                        o = la_mul<NO, NO, UP>(pf[tb], b, o);
+                    }
+                    load_p(c + 1);
+                    const int t = 64 * c + 16 * rt + g4;
+                    S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + l16;
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (t + r < rows.n && 16 * rt + g4 + r < upto) p[r * A.ots] = T::down(o[r]);
+                }
+                if (upto < 64) break;
+                __syncthreads();
+            }
+        }
+        if (c < chunks) {
+            // a row with values that the products do not hold, or a state: from there on token by token
+            static_assert(sizeof(s_s) >= DK * 16 * sizeof(float), "room for the state");
+            float (*hand)[16] = (float (*)[16])s_s;
+            __syncthreads();
+#pragma unroll
+            for (int o = 0; o < OWN; o++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (chain && rt + 4 * o < NKB) hand[32 * (rt + 4 * o) + 16 * h + g4 + r][l16] = s[o][h][r];
+            __syncthreads();
+            if (w == 0)
+                la_recurrence<T, DK, DELTA>(A, head, c0, rows.first + 64 * c, rows.n - 64 * c, upto, [&](int row, float (&x)[4]) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] = hand[row][g4 + e];
+                }, st.to);
+        } else if (chain && st.to) {
+#pragma unroll
+            for (int o = 0; o < OWN; o++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (rt + 4 * o < NKB) st.to[(int64_t)(32 * (rt + 4 * o) + 16 * h + g4 + r) * A.dim_v + c0 + l16] = s[o][h][r];
+        }
     }
 }
 
@@ -149,6 +809,23 @@ static int with_dim_k(int dim, F f)
     if (dim == 64) return f(std::integral_constant<int, 64>{});
     if (dim == 128) return f(std::integral_constant<int, 128>{});
     return f(std::integral_constant<int, 256>{});
+}
+
+constexpr int LA_MEAN = 16;                          // tokens to a sequence from which on a call goes in chunks
+constexpr size_t LA_WORKSPACE = (size_t)1 << 30;
+
+// bytes of the workspace for a chunk number
+static size_t la_tile_bytes(int type, int dim_k, int n_key, int n_head)
+{
+    size_t bytes = 0;
+    with_type(type, [&](auto t) {
+        return with_dim_k(dim_k, [&](auto d) {
+            using Y = LaLayout<decltype(t), decltype(d)::value>;
+            bytes = (size_t)n_key * Y::KEY_BYTES + (size_t)n_head * Y::HEAD_BYTES;
+            return 0;
+        });
+    });
+    return bytes;
 }
 
 }  // namespace qmag
@@ -203,19 +880,59 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
     A.out = out->ptr, A.ots = out->token_stride, A.ohs = out->head_stride;
     A.decay = decay, A.beta = beta, A.state = a->state;
     A.slot = a->n_slot ? slot : nullptr, A.len = len, A.cu = cu;
-    A.n_head = a->n_head, A.turns = a->turns, A.share = a->turns ? q->n_head : a->n_head / q->n_head;
+    A.n_head = a->n_head, A.n_key = q->n_head, A.share = a->n_head / q->n_head, A.turns = a->turns;
     A.dim_v = a->dim_v, A.n_slot = a->n_slot, A.n_seq = n_seq, A.T = T;
     A.norm_eps = a->norm_eps, A.scale = scale;
     DeviceScope dev;
     if (dev.st) return dev.st;
     hipStream_t s = ctx().stream;
-    const int64_t wgs = ((int64_t)n_seq * a->n_head * (a->dim_v / 16) + LA_WG / 64 - 1) / (LA_WG / 64);
-    const unsigned grid = (unsigned)(wgs < 1 << 23 ? wgs : 1 << 23);
+    const int64_t slices = (int64_t)n_seq * a->n_head * (a->dim_v / 16);
+    // prompts in chunks; few tokens to a sequence one after another
+    const bool chunks = (int64_t)T > (int64_t)LA_MEAN * n_seq;
+    size_t state = 0;
+    int window = 0;
+    if (chunks) {
+        // windows that keep the workspace under a bound
+        const size_t per = la_tile_bytes(type, a->dim_k, q->n_head, a->n_head);
+        state = sizeof(float) * (size_t)a->n_head * (size_t)a->dim_k * (size_t)a->dim_v;
+        window = (int)(((int64_t)T + LA_CHUNK - 1) / LA_CHUNK < (1 << 20) ? (T + LA_CHUNK - 1) / LA_CHUNK * LA_CHUNK : 1 << 26);
+        while (window > 4 * LA_CHUNK && (size_t)la_most_tiles(window, n_seq) * per > LA_WORKSPACE) window = window / (2 * LA_CHUNK) * LA_CHUNK;
+        uint8_t *p = (uint8_t *)workspace(WS_LINATTN, (size_t)la_most_tiles(window, n_seq) * per + (T > window ? 2 * state : 0), &st);
+        if (st) return st;
+        A.carry_in = (float *)p;
+        A.keys = p + (T > window ? 2 * state : 0);
+    }
     prof_begin(PROF_LINATTN, s);
     with_type(type, [&](auto t) {
         return with_dim_k(a->dim_k, [&](auto d) {
-            if (a->delta) linattn_step_kernel<decltype(t), decltype(d)::value, true><<<grid, LA_WG, 0, s>>>(A);
-            else linattn_step_kernel<decltype(t), decltype(d)::value, false><<<grid, LA_WG, 0, s>>>(A);
+            using TT = decltype(t);
+            constexpr int DK = decltype(d)::value;
+            if (!chunks) {
+                const int64_t wgs = (slices + LA_WG / 64 - 1) / (LA_WG / 64);
+                const unsigned grid = (unsigned)(wgs < 1 << 23 ? wgs : 1 << 23);
+                if (a->delta) linattn_step_kernel<TT, DK, true><<<grid, LA_WG, 0, s>>>(A);
+                else linattn_step_kernel<TT, DK, false><<<grid, LA_WG, 0, s>>>(A);
+                return 0;
+            }
+            float *carry = (float *)A.carry_in;
+            const int64_t wgs = (slices + 7) / 8 * 8;
+            const unsigned grid = (unsigned)(wgs < 1 << 22 ? wgs : 1 << 22);
+            for (int64_t r0 = 0, odd = 0; r0 < T; r0 += window, odd ^= 1) {
+                A.r0 = (int)r0;
+                A.r1 = (int)(r0 + window < T ? r0 + window : T);
+                A.n_tile = la_most_tiles(A.r1 - A.r0, n_seq);
+                A.heads = A.keys + (size_t)A.n_tile * (size_t)A.n_key * LaLayout<TT, DK>::KEY_BYTES;
+                A.carry_in = carry + (odd ? state / sizeof(float) : 0);
+                A.carry_out = carry + (odd ? 0 : state / sizeof(float));
+                const unsigned tiles = (unsigned)A.n_tile * (unsigned)A.n_key;
+                if (a->delta) {
+                    linattn_chunk_kernel<TT, DK, true><<<tiles, 256, 0, s>>>(A);
+                    linattn_chain_kernel<TT, DK, true><<<grid, 512, 0, s>>>(A);
+                } else {
+                    linattn_chunk_kernel<TT, DK, false><<<tiles, 256, 0, s>>>(A);
+                    linattn_chain_kernel<TT, DK, false><<<grid, 512, 0, s>>>(A);
+                }
+            }
             return 0;
         });
     });

@@ -304,3 +304,23 @@ def test_linattn_profile(qm):
     c.run(qm)
     assert qm.prof_read("linattn")[0] == 1
     qm.prof_enable(False)
+
+
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+def test_linattn_windows(qm, typ):
+    """A call whose chunks are more than a workspace holds is taken in windows; a sequence that goes on behind one
+    hands its state on, with a slot or without."""
+    t, r = TYPES[typ], rng_of(12)
+    rows = 20000 if typ == "f32" else 30000
+    s = Sequences(qm, r, [40, rows - 5000, 1, 300, 4500, 0, 130], pad=1, slots=[3, -1, 1, 0, 2, 5, 4], had="all")
+    c = Case(r, s, t, 32, 32, 64, 16)
+    got, after = c.run(qm)
+    for h in (0, 17):
+        for i in range(s.n):
+            a, n = s.cu[i], s.lens[i]
+            S = c.state[s.slots[i], h].astype(np.float64) if s.slots[i] >= 0 else np.zeros((64, 16))
+            out, off, S, e = c.one(i, h, S)
+            near(values(got[a:a + n, h], t), out, off, t, "sequence %d head %d" % (i, h))
+            if s.keeps(i):
+                near(after[s.slots[i], h].astype(np.float64), S, e[None], 0, "state of sequence %d head %d" % (i, h))
+    assert (got[-1] == 7).all()

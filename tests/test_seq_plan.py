@@ -88,3 +88,72 @@ def test_sums_of_any_kind(walk):
         cu = r.choice([r.randint(-T, 2 * T), 0, T, -2 ** 31, 2 ** 31 - 1], n + 1) if r.rand() < 0.3 else r.randint(-9, T + 9, n + 1)
         calls.append((T, shift, cu))
     walk(calls)
+
+
+CHUNKS = r"""
+#include <stdio.h>
+#include <vector>
+#include "qmag_linattn_plan.h"
+using namespace qmag;
+
+// stdin: calls of T window n_seq, then cu: what the kernels do with them, window by window
+int main()
+{
+    int T, window, n;
+    for (int call = 0; scanf("%d%d%d", &T, &window, &n) == 3; call++) {
+        std::vector<int> cu(n + 1), rows(T);
+        for (int &v : cu) if (scanf("%d", &v) != 1) return 1;
+        bool ascending = cu[0] >= 0 && cu[n] <= T;
+        for (int i = 0; i < n; i++) ascending = ascending && cu[i] <= cu[i + 1];
+        for (int r0 = 0; r0 < T; r0 += window) {
+            const int r1 = r0 + window < T ? r0 + window : T, most = la_most_tiles(r1 - r0, n);
+            std::vector<int> taken(most);
+            int rank = 0, begun = 0, goes_on = 0;
+            for (int i = 0; i < n; i++) {
+                const LaRows x = la_rows(cu[i], cu[i + 1], T, r0, r1);
+                if (x.n < 0 || (x.n && (x.first < r0 || x.first + x.n > r1))) return printf("call %d: rows outside the window\n", call), 1;
+                for (int r = 0; r < x.n; r++) rows[x.first + r]++;
+                begun += x.n && x.begun;
+                goes_on += x.n && x.goes_on;
+                if (!la_long(x.n)) continue;
+                const int t0 = la_tile0(x.first, r0, rank++), c = seq_tiles(x.n, LA_SHIFT);
+                if (!la_room(t0, c, most)) {
+                    if (ascending) return printf("call %d: no room for sequence %d\n", call, i), 1;
+                    continue;
+                }
+                for (int j = t0; j < t0 + c; j++)
+                    if (j < 0 || j >= most || (taken[j]++ && ascending)) return printf("call %d: chunk number %d of %d\n", call, j, most), 1;
+            }
+            if (ascending && (begun > 1 || goes_on > 1)) return printf("call %d: two sequences hand a state on\n", call), 1;
+        }
+        if (ascending)
+            for (int r = 0; r < T; r++)
+                if (rows[r] != (r >= cu[0] && r < cu[n])) return printf("call %d: row %d\n", call, r), 1;
+    }
+    return puts("ok"), 0;
+}
+"""
+
+
+def test_chunks_and_windows(tmp_path):
+    """Chunks of linear attention: numbers apart and within what the host counts, windows that take every row once."""
+    cc = shutil.which("g++")
+    if not cc:
+        pytest.skip("no host compiler")
+    (tmp_path / "chunks.cpp").write_text(CHUNKS)
+    exe = str(tmp_path / "chunks")
+    subprocess.run([cc, "-std=c++17", "-O1", "-D_GLIBCXX_ASSERTIONS", "-I", os.path.join(ROOT, "qwen-mobile-agent_amd", "csrc"),
+                    str(tmp_path / "chunks.cpp"), "-o", exe], check=True)
+    r, calls = np.random.RandomState(3), []
+    for _ in range(500):
+        n = r.randint(1, 60)
+        lens = r.randint(0, r.choice([2, 18, 70, 400]) + 1, n) * (r.rand(n) < 0.8)
+        cu = np.concatenate([[0], np.cumsum(lens)])
+        calls.append((max(1, int(cu[-1]) + r.choice([0, 0, 3])), 64 * r.choice([4, 5, 9, 1000]), cu))
+    calls += [(17 * 500, 64 * w, np.arange(501) * 17) for w in (4, 7, 200)] + [(4096, 256, np.array([0, 4096]))]
+    for _ in range(300):
+        n, T = r.randint(1, 40), r.randint(1, 900)
+        calls.append((T, 64 * r.choice([4, 6, 100]), r.choice([-2 ** 31, -5, 0, T // 2, T - 3, T, T + 9, 2 ** 31 - 1], n + 1)))
+    text = "\n".join(" ".join(map(str, [T, w, len(cu) - 1] + list(cu))) for T, w, cu in calls)
+    out = subprocess.run([exe], input=text, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
