@@ -611,113 +611,103 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
         publish();
         if (threadIdx.x == 0) s_bad = 64;
         int c = 0, upto = 0;                              // the first chunk that is not done, the first such row of it
-        if (!__syncthreads_or(odd)) {
-            bf168 kf[NKB][NP], tf[2][3], ktf[OWN][2][2][NP], pf[2][NO];
-            auto keys = [&](int i) { return A.keys + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_key + key) * Y::KEY_BYTES; };
-            auto heads = [&](int i) { return A.heads + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_head + head) * Y::HEAD_BYTES; };
-            auto load_k = [&](int i) {
-                const uint8_t *p = keys(i) + (chain ? Y::K : Y::Q) + rt * NKB * NP * LA_FRAG;
+        const bool go = !__syncthreads_or(odd);
+        auto keys = [&](int i) { return A.keys + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_key + key) * Y::KEY_BYTES; };
+        auto heads = [&](int i) { return A.heads + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_head + head) * Y::HEAD_BYTES; };
+        // 16 rows of K or Q
+        auto load_rows = [&](const uint8_t *p, bf168 (&o)[NKB][NP]) {
 #pragma unroll
-                for (int kb = 0; kb < NKB; kb++) la_load<NP>(p + kb * NP * LA_FRAG, kf[kb]);
-            };
+            for (int kb = 0; kb < NKB; kb++) la_load<NP>(p + (rt * NKB + kb) * NP * LA_FRAG, o[kb]);
+        };
+        // Each of the two walks asks for a chunk's operands a chunk ahead, as soon as it has used the last one's, and
+        // without a branch: loads come back in turn, and one that is waited for early is waited for with all ahead of it.
+        if (chain && go) {
+            bf168 kf[NKB][NP], tf[2][3], ktf[OWN][2][2][NP];
+            f32x4 kd, bt, ke;
+            float v[4], end;
+            int good, none = 0;
+            asm("" : "+v"(none));                         // a scalar load would be waited for with LDS
             auto load_kt = [&](int i) {
                 const uint8_t *p = keys(i) + Y::KT;
 #pragma unroll
-                for (int o = 0; o < OWN; o++) {
-                    const int kb = rt + 4 * o;
-                    if (kb >= NKB) continue;
+                for (int o = 0; o < OWN; o++)
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int tb = 0; tb < 2; tb++) la_load<NP>(p + ((2 * kb + h) * 2 + tb) * NP * LA_FRAG, ktf[o][h][tb]);
-                }
+                        for (int tb = 0; tb < 2; tb++)
+                            la_load<NP>(p + ((2 * min(rt + 4 * o, NKB - 1) + h) * 2 + tb) * NP * LA_FRAG, ktf[o][h][tb]);
             };
             auto load_t = [&](int i) {
                 const uint8_t *p = heads(i) + Y::TI;
 #pragma unroll
-                for (int tb = 0; tb < 2; tb++)
-                    if (2 * tb <= rt) la_load<3>(p + la_tri(rt, tb) * 3 * LA_FRAG, tf[tb]);
+                for (int tb = 0; tb < 2; tb++) la_load<3>(p + la_tri(rt, rt < 2 ? 0 : tb) * 3 * LA_FRAG, tf[tb]);
             };
-            auto load_p = [&](int i) {
-                const uint8_t *p = heads(i) + Y::P;
-#pragma unroll
-                for (int tb = 0; tb < 2; tb++)
-                    if (2 * tb <= rt) la_load<NO>(p + la_tri(rt, tb) * NO * LA_FRAG, pf[tb]);
-            };
-            float v[4];
             auto load_v = [&](int i) {
+                const uint8_t *vec = heads(i) + Y::VEC;
+                kd = *(const QMAG_GLOBAL f32x4 *)(vec + 4 * (Y::KD + 16 * rt + g4));
+                bt = *(const QMAG_GLOBAL f32x4 *)(vec + 4 * (Y::B + 16 * rt + g4));
+                ke = *(const QMAG_GLOBAL f32x4 *)(vec + 4 * (Y::KE + 16 * rt + g4));
+                end = *(const QMAG_GLOBAL float *)(vec + 4 * (Y::END + none));
+                good = *(const QMAG_GLOBAL int *)(vec + 4 * (Y::BAD + none));
                 const int t = 64 * min(i, chunks - 1) + 16 * rt + g4;
-                const S *p = (const S *)A.v.p + (rows.first + (int64_t)t) * A.v.ts + head * A.v.hs + c0 + l16;
+                const S *p = (const S *)A.v.p + (int64_t)rows.first * A.v.ts + head * A.v.hs + c0 + l16;
 #pragma unroll
-                for (int r = 0; r < 4; r++) v[r] = t + r < rows.n ? T::up(p[r * A.v.ts]) : 0.0f;
+                for (int r = 0; r < 4; r++) v[r] = T::up(*(const QMAG_GLOBAL S *)(p + min(t + r, rows.n - 1) * A.v.ts));
             };
-            if (!chain || DELTA) load_k(0);
-            if (chain) {
-                load_v(0);
-                if constexpr (DELTA) load_t(0);
-                load_kt(0);
-            } else {
-                load_p(0);
-            }
+            if constexpr (DELTA) load_rows(keys(0) + Y::K, kf);
+            load_v(0);
+            if constexpr (DELTA) load_t(0);
+            load_kt(0);
             for (; c < chunks; c++) {
-                const float *vec = (const float *)(heads(c) + Y::VEC);
                 f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (!chain || DELTA) {
+                if constexpr (DELTA) {
 #pragma unroll
                     for (int kb = 0; kb < NKB; kb++) {
                         bf168 b[3];
 #pragma unroll
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
-                        if (chain) acc = la_mul<NP, 3, 2>(kf[kb], b, acc);
-                        else acc = la_mul<NP, 3, UP>(kf[kb], b, acc);
+                        acc = la_mul<NP, 3, 2>(kf[kb], b, acc);
                     }
-                    load_k(c + 1);
+                    load_rows(keys(c + 1) + Y::K, kf);
                 }
-                float x[4], ke[4];
-                if (chain) {
-                    const f32x4 kd = *(const QMAG_GLOBAL f32x4 *)(vec + Y::KD + 16 * rt + g4), bt = *(const QMAG_GLOBAL f32x4 *)(vec + Y::B + 16 * rt + g4),
-                                e4 = *(const QMAG_GLOBAL f32x4 *)(vec + Y::KE + 16 * rt + g4);
-                    const int good = ((const QMAG_GLOBAL int *)vec)[Y::BAD];
-                    int bad = good;
+                const int left = min(rows.n - 64 * c, good);
+                int bad = good;
+                float x[4];
 #pragma unroll
-                    for (int r = 3; r >= 0; r--) {
-                        const int row = 16 * rt + g4 + r;
-                        const bool fine = row < good && fabsf(v[r]) <= 0x1p60f;
-                        x[r] = fine ? bt[r] * (DELTA ? fmaf(-kd[r], acc[r], v[r]) : v[r]) : 0.0f;
-                        bad = fine ? bad : min(bad, row);
-                        ke[r] = e4[r];
-                    }
-                    load_v(c + 1);
-                    if (bad < 64) atomicMin(&s_bad, bad);
-                    if constexpr (DELTA) {
-                        __bf16 p[3][4];
-                        la_split<3, 4>(x, p);
-#pragma unroll
-                        for (int i = 0; i < 3; i++) *(s16x4 *)&s_x[rt >> 1][i][half] = *(const s16x4 *)p[i];
-                    }
+                for (int r = 3; r >= 0; r--) {
+                    const int row = 16 * rt + g4 + r;
+                    const bool fine = fabsf(v[r]) <= 0x1p60f;
+                    x[r] = row < left && fine ? bt[r] * (DELTA ? fmaf(-kd[r], acc[r], v[r]) : v[r]) : 0.0f;
+                    bad = row < left && !fine ? min(bad, row) : bad;
                 }
+                const float now = end;
+                const f32x4 e4 = ke;
+                load_v(c + 1);
+                if (bad < 64) atomicMin(&s_bad, bad);
                 if constexpr (DELTA) {
+                    __bf16 p[3][4];
+                    la_split<3, 4>(x, p);
+#pragma unroll
+                    for (int i = 0; i < 3; i++) *(s16x4 *)&s_x[rt >> 1][i][half] = *(const s16x4 *)p[i];
                     __syncthreads();
-                    if (chain) {
-                        f32x4 u = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    f32x4 u = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int tb = 0; tb < 2; tb++) {
-                            if (2 * tb > rt) continue;
-                            bf168 b[3];
+                    for (int tb = 0; tb < 2; tb++) {
+                        if (2 * tb > rt) continue;
+                        bf168 b[3];
 #pragma unroll
-                            for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_x[tb][i][at];
-                            u = la_mul<3, 3, 2>(tf[tb], b, u);
-                        }
-                        load_t(c + 1);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) x[r] = u[r];
+                        for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_x[tb][i][at];
+                        u = la_mul<3, 3, 2>(tf[tb], b, u);
                     }
+                    load_t(c + 1);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[r] = u[r];
                 }
-                if (chain) {
+                {
                     __bf16 p[NO][4], pe[3][4];
                     float xe[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) xe[r] = x[r] * ke[r];
+                    for (int r = 0; r < 4; r++) xe[r] = x[r] * e4[r];
                     la_split<NO, 4>(x, p);
                     la_split<3, 4>(xe, pe);
 #pragma unroll
@@ -727,48 +717,64 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
                 }
                 __syncthreads();
                 upto = s_bad;
-                if (chain && upto == 64) {
-                    const float end = ((const QMAG_GLOBAL float *)vec)[Y::END];
+                if (upto < 64) break;
 #pragma unroll
-                    for (int o = 0; o < OWN; o++) {
-                        if (rt + 4 * o >= NKB) continue;
+                for (int o = 0; o < OWN; o++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < 2; h++) s[o][h] *= now;
 #pragma unroll
-                            for (int r = 0; r < 4; r++) s[o][h][r] *= end;
-                    }
+                for (int tb = 0; tb < 2; tb++) {
+                    bf168 b[3];
 #pragma unroll
-                    for (int tb = 0; tb < 2; tb++) {
-                        bf168 b[3];
+                    for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_e[tb][i][at];
 #pragma unroll
-                        for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_e[tb][i][at];
+                    for (int o = 0; o < OWN; o++)
 #pragma unroll
-                        for (int o = 0; o < OWN; o++) {
-                            if (rt + 4 * o >= NKB) continue;
-#pragma unroll
-                            for (int h = 0; h < 2; h++) s[o][h] = la_mul<NP, 3, 2>(ktf[o][h][tb], b, s[o][h]);
-                        }
-                    }
-                    load_kt(c + 1);
-                    publish();
-                } else if (!chain) {
-                    const f32x4 qd = *(const QMAG_GLOBAL f32x4 *)(vec + Y::QD + 16 * rt + g4);
-                    f32x4 o = acc * qd;
-#pragma unroll
-                    for (int tb = 0; tb < 2; tb++) {
-                        if (2 * tb > rt) continue;
-                        bf168 b[NO];
-#pragma unroll
-                        for (int i = 0; i < NO; i++) b[i] = *(const bf168 *)&s_u[tb][i][at];
-                        o = la_mul<NO, NO, UP>(pf[tb], b, o);
-                    }
-                    load_p(c + 1);
-                    const int t = 64 * c + 16 * rt + g4;
-                    S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + l16;
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (t + r < rows.n && 16 * rt + g4 + r < upto) p[r * A.ots] = T::down(o[r]);
+                        for (int h = 0; h < 2; h++) s[o][h] = la_mul<NP, 3, 2>(ktf[o][h][tb], b, s[o][h]);
                 }
+                load_kt(c + 1);
+                publish();
+                __syncthreads();
+            }
+        } else if (go) {
+            bf168 qf[NKB][NP], pf[2][NO];
+            f32x4 qd;
+            auto load_p = [&](int i) {
+                const uint8_t *p = heads(i);
+                qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::VEC + 4 * (Y::QD + 16 * rt + g4));
+#pragma unroll
+                for (int tb = 0; tb < 2; tb++) la_load<NO>(p + Y::P + la_tri(rt, rt < 2 ? 0 : tb) * NO * LA_FRAG, pf[tb]);
+            };
+            load_rows(keys(0) + Y::Q, qf);
+            load_p(0);
+            for (; c < chunks; c++) {
+                f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int kb = 0; kb < NKB; kb++) {
+                    bf168 b[3];
+#pragma unroll
+                    for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
+                    o = la_mul<NP, 3, UP>(qf[kb], b, o);
+                }
+                load_rows(keys(c + 1) + Y::Q, qf);
+                o *= qd;
+                if constexpr (DELTA) __syncthreads();
+                __syncthreads();
+                upto = s_bad;
+#pragma unroll
+                for (int tb = 0; tb < 2; tb++) {
+                    if (2 * tb > rt) continue;
+                    bf168 b[NO];
+#pragma unroll
+                    for (int i = 0; i < NO; i++) b[i] = *(const bf168 *)&s_u[tb][i][at];
+                    o = la_mul<NO, NO, UP>(pf[tb], b, o);
+                }
+                load_p(c + 1);
+                const int t = 64 * c + 16 * rt + g4, to = min(rows.n, 64 * c + upto);
+                S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + l16;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (t + r < to) p[r * A.ots] = T::down(o[r]);
                 if (upto < 64) break;
                 __syncthreads();
             }
