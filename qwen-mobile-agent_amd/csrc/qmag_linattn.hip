@@ -208,15 +208,21 @@ template <> constexpr int LA_OUT_PARTS<TF32> = 3;
 constexpr int LA_FRAG = 1024;
 constexpr int LA_TRI = 6;             // operands of a lower triangle: 16 rows by 32 columns, those all above it left out
 constexpr int la_tri(int rt, int tb) { return rt < 2 ? rt : 2 * rt - 2 + tb; }
+// What a chunk has for each key head: the parts of K, rows of whole 16 bytes whose places are exchanged so that 16 rows'
+// lie in different banks, and of Q as operands, [16 rows: 4][DK / 32][parts].
 template <class T, int DK>
+struct LaKeys {
+    static constexpr int K = 0, PLANE = 64 * DK * 2, Q = LA_PARTS<T> * PLANE, BYTES = 2 * Q;
+};
+// where 16 bytes of a row of K lie, in 16 bytes
+__host__ __device__ constexpr int la_place(int row, int piece) { return piece ^ (row & 7); }
+// What a chunk has for each head: (I + L)^-1 and P [LA_TRI][parts], then rows of 64 that the chunk's tokens are
+// multiplied by.
+template <class T>
 struct LaLayout {
-    static constexpr int NP = LA_PARTS<T>, NKB = DK / 32;
-    // a chunk and key head: K and Q [16 rows: 4][NKB][NP], K^T [DK / 16][32 tokens: 2][NP]
-    static constexpr int K = 0, Q = 4 * NKB * NP * LA_FRAG, KT = 2 * Q, KEY_BYTES = 3 * Q;
-    // a chunk and head: (I + L)^-1 and P [LA_TRI][parts], then rows of 64: what the chunk's tokens are multiplied by
-    static constexpr int TI = 0, P = LA_TRI * 3 * LA_FRAG, VEC = P + LA_TRI * LA_OUT_PARTS<T> * LA_FRAG;
-    static constexpr int KD = 0, QD = 64, KE = 128, B = 192, END = 256, BAD = 257;     // floats; END: e^G_63; BAD: the first row the form does not hold, 64: none
-    static constexpr int HEAD_BYTES = VEC + 272 * 4;
+    static constexpr int TI = 0, P = LA_TRI * 3 * LA_FRAG, VEC = P + LA_TRI * LA_OUT_PARTS<T> * LA_FRAG, QD = VEC + 1024;
+    static constexpr int KD = 0, KE = 64, B = 128, END = 192, BAD = 193;     // floats of VEC; END: e^G_63; BAD: the first row the form does not hold, 64: none
+    static constexpr int HEAD_BYTES = QD + 256;
 };
 
 // x as N parts, the first the nearest bf16 to it, each other to what those ahead leave
@@ -244,17 +250,34 @@ __device__ __forceinline__ void la_split8(const float (&x)[8], bf168 (&o)[N])
         for (int i = 0; i < 8; i++) o[p][i] = s[p][i];
 }
 
-// c += a b, of the products of parts those of places adding up to at most UP
-template <int NA, int NB, int UP>
-__device__ __forceinline__ f32x4 la_mul(const bf168 (&a)[NA], const bf168 (&b)[NB], f32x4 c)
-{
+// A sum of products of parts, one accumulator for each place that two parts' places add up to: a product that adds to
+// the one ahead of it waits for it (one accumulator for all: 253 us for 4096 tokens against 199 in fp32).
+template <int UP>
+struct LaSum {
+    f32x4 c[UP + 1];
+    __device__ __forceinline__ void clear()
+    {
 #pragma unroll
-    for (int s = UP; s >= 0; s--)                     // the small ones first
+        for (int i = 0; i <= UP; i++) c[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // += a b, of the products of parts those of places adding up to at most UP
+    template <int NA, int NB>
+    __device__ __forceinline__ void add(const bf168 (&a)[NA], const bf168 (&b)[NB])
+    {
 #pragma unroll
         for (int i = 0; i < NA; i++)
-            if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
-    return c;
-}
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+                if (i + j <= UP) c[i + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], c[i + j], 0, 0, 0);
+    }
+    __device__ __forceinline__ f32x4 sum() const
+    {
+        f32x4 s = c[UP];
+#pragma unroll
+        for (int i = UP - 1; i >= 0; i--) s += c[i];
+        return s;
+    }
+};
 
 template <int N>
 __device__ __forceinline__ void la_load(const uint8_t *p, bf168 (&o)[N])
@@ -327,22 +350,22 @@ template <class T, int DK, bool DELTA>
 __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
 {
     using S = typename T::S;
-    using Y = LaLayout<T, DK>;
-    constexpr int NP = Y::NP, NKB = Y::NKB, ROW = DK + 8;
+    using Y = LaLayout<T>;
+    constexpr int NP = LA_PARTS<T>, NKB = DK / 32, ROW = DK + 8;
     __shared__ __attribute__((aligned(16))) __bf16 s_k[NP][64][ROW];
     __shared__ __attribute__((aligned(16))) float s_lt[64][68];           // L, rows and columns exchanged
     __shared__ __attribute__((aligned(16))) float s_dt[4][16][20];        // inverses of its diagonal blocks, exchanged
     __shared__ double s_g[64];
     __shared__ float s_fk[64], s_fq[64], s_kk[64], s_b[64];
     __shared__ int s_odd[4], s_good;
-    const int lane = lane_id(), w = threadIdx.x >> 6, l16 = lane & 15, g4 = (lane >> 4) * 4;
+    const int lane = lane_id(), w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4, g4 = g * 4;
     const int tile = blockIdx.x / A.n_key, key = blockIdx.x % A.n_key;
     const LaTile at = la_find(A, tile);
     if (!at.any) return;
     const int n = min(64, at.rows.n - 64 * at.chunk);
     const int64_t row0 = at.rows.first + 64 * (int64_t)at.chunk;
-    uint8_t *mine = A.keys + ((int64_t)tile * A.n_key + key) * Y::KEY_BYTES;
 
+    uint8_t *mine = A.keys + ((int64_t)tile * A.n_key + key) * LaKeys<T, DK>::BYTES;
     // rows of K and Q as operands, their sums of squares
     bf168 kf[NKB][NP], qf[NKB][NP];
     float kk = 0.0f, qq = 0.0f;
@@ -353,18 +376,8 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = 0.0f, y[e] = 0.0f;
         if (my < n) {
-            const S *kp = (const S *)A.k.p + (row0 + my) * A.k.ts + key * A.k.hs + 32 * kb + g4;
-            const S *qp = (const S *)A.q.p + (row0 + my) * A.q.ts + key * A.q.hs + 32 * kb + g4;
-            float h[4];
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                load_row<T, 4>(kp + 16 * half, h);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[4 * half + e] = h[e];
-                load_row<T, 4>(qp + 16 * half, h);
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[4 * half + e] = h[e];
-            }
+            load_row<T, 8>((const S *)A.k.p + (row0 + my) * A.k.ts + key * A.k.hs + 32 * kb + 8 * g, x);
+            load_row<T, 8>((const S *)A.q.p + (row0 + my) * A.q.ts + key * A.q.hs + 32 * kb + 8 * g, y);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -373,14 +386,12 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
         }
         la_split8<NP>(x, kf[kb]);
         la_split8<NP>(y, qf[kb]);
-        la_store<NP>(mine + Y::K + (w * NKB + kb) * NP * LA_FRAG, kf[kb]);
-        la_store<NP>(mine + Y::Q + (w * NKB + kb) * NP * LA_FRAG, qf[kb]);
 #pragma unroll
         for (int p = 0; p < NP; p++) {
-            const s16x4 *h = (const s16x4 *)&kf[kb][p];
-            *(s16x4 *)&s_k[p][my][32 * kb + g4] = h[0];
-            *(s16x4 *)&s_k[p][my][32 * kb + 16 + g4] = h[1];
+            *(bf168 *)&s_k[p][my][32 * kb + 8 * g] = kf[kb][p];
+            *(QMAG_GLOBAL bf168 *)(mine + p * LaKeys<T, DK>::PLANE + my * DK * 2 + la_place(my, 4 * kb + g) * 16) = kf[kb][p];
         }
+        la_store<NP>(mine + LaKeys<T, DK>::Q + (w * NKB + kb) * NP * LA_FRAG, qf[kb]);
     }
     kk = la_sum4(kk);
     qq = la_sum4(qq);
@@ -401,32 +412,21 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
     f32x4 ck[4], cq[4];
 #pragma unroll
     for (int ct = 0; ct < 4; ct++) {
-        ck[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, cq[ct] = ck[ct];
         if (ct > w) continue;
+        LaSum<NP == 1 ? 0 : 2> sk, sq;
+        sk.clear();
+        sq.clear();
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
             bf168 a[NP];
 #pragma unroll
-            for (int p = 0; p < NP; p++) {
-                s16x4 *h = (s16x4 *)&a[p];
-                h[0] = *(const s16x4 *)&s_k[p][16 * ct + l16][32 * kb + g4];
-                h[1] = *(const s16x4 *)&s_k[p][16 * ct + l16][32 * kb + 16 + g4];
-            }
-            if constexpr (DELTA) ck[ct] = la_mul<NP, NP, 2>(a, kf[kb], ck[ct]);
-            cq[ct] = la_mul<NP, NP, 2>(a, qf[kb], cq[ct]);
+            for (int p = 0; p < NP; p++) a[p] = *(const bf168 *)&s_k[p][16 * ct + l16][32 * kb + 8 * g];
+            if constexpr (DELTA) sk.add(a, kf[kb]);
+            sq.add(a, qf[kb]);
         }
+        ck[ct] = sk.sum();
+        cq[ct] = sq.sum();
     }
-    // K^T, 16 channels by 32 tokens
-    for (int f = w; f < DK / 16 * 2; f += 4) {
-        const int ch = 16 * (f >> 1) + l16, t0 = 32 * (f & 1) + g4;
-        bf168 a[NP];
-#pragma unroll
-        for (int p = 0; p < NP; p++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) a[p][e] = s_k[p][t0 + (e & 3) + 16 * (e >> 2)][ch];
-        la_store<NP>(mine + Y::KT + f * NP * LA_FRAG, a);
-    }
-
     const int sharing = A.n_head / A.n_key;
     for (int i = 0; i < sharing; i++) {
         const int head = la_head_of(A, key, i);
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
             float *vec = (float *)(to + Y::VEC);
             const float now = expf((float)sum), fk = s_fk[lane];
             vec[Y::KD + lane] = now * fk;
-            vec[Y::QD + lane] = A.scale * s_fq[lane] * now;
+            ((float *)(to + Y::QD))[lane] = A.scale * s_fq[lane] * now;
             vec[Y::KE + lane] = expf((float)(all - sum)) * fk;
             vec[Y::B + lane] = b;
             if (lane == 0) {
@@ -544,31 +544,58 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
     }
 }
 
-// Down a sequence's chunks: one head, 16 columns of the state.  Waves 0 .. 3 form U and the next state, 16 of the
-// chunk's rows and a quarter of the state's each; waves 4 .. 7 the results.  What a wave forms the others take from LDS
-// as operands.
+// Down a sequence's chunks: one head, 16 columns of the state, by 12 waves.  Waves 0 .. 3 form U and the next state, 16
+// of the chunk's rows and a quarter of the state's each; waves 4 .. 7 the results; what a wave forms the others take
+// from LDS as operands.  Waves 8 .. 11 bring LDS what the first four read of a chunk, ahead of them: a CU takes in some
+// 40 bytes a clock, and a wave that asks for its own operands waits in line with all others.
+template <class T, int DK>
+struct LaRoom {
+    static constexpr int K = LaKeys<T, DK>::Q, REST = LA_TRI * 3 * LA_FRAG + DK / 32 * 3 * LA_FRAG + 2 * (6 + LA_OUT_PARTS<T>) * LA_FRAG + 5 * LA_FRAG + 64;
+    static constexpr int BUFS = 2 * K + REST <= 160 * 1024 ? 2 : 1;      // chunks of K in LDS
+    static constexpr bool OVER = K + REST > 160 * 1024;                  // a chunk's V lies where its U goes
+};
+
+// A loader's waits: all but the last N of its loads are there, and its writes to LDS; then the workgroup's barrier.
+// (An ordinary one would wait for every load to LDS.)
+__device__ __forceinline__ uint32_t la_lds(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p; }
+__device__ __forceinline__ void la_write(uint8_t *to, f32x4 v) { asm volatile("ds_write_b128 %0, %1" ::"v"(la_lds(to)), "v"(v) : "memory"); }
+// a value as if it were new in every turn of a loop, so that places formed from it are not kept (and then spilled)
+__device__ __forceinline__ void la_fresh(int &v) { asm volatile("" : "+v"(v)); }
+template <int N>
+__device__ __forceinline__ void la_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void la_bring(const uint8_t *from, uint8_t *to)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + lane_id() * 16),
+                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
 template <class T, int DK, bool DELTA>
-__global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
+__global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
 {
     using S = typename T::S;
-    using Y = LaLayout<T, DK>;
-    constexpr int NP = Y::NP, NKB = Y::NKB, NO = LA_OUT_PARTS<T>, UP = NO - 1;
+    using Y = LaLayout<T>;
+    using M = LaRoom<T, DK>;
+    using X = LaKeys<T, DK>;
+    constexpr int NP = LA_PARTS<T>, NKB = DK / 32, NO = LA_OUT_PARTS<T>, UP = NO - 1, BUFS = M::BUFS;
     constexpr int OWN = (NKB + 3) / 4;                    // blocks of 32 rows of the state that a wave holds
-    __shared__ __attribute__((aligned(16))) uint8_t s_s[NKB][3][LA_FRAG];
+    __shared__ __attribute__((aligned(16))) uint8_t s_k[BUFS][X::Q];
+    __shared__ __attribute__((aligned(16))) uint8_t s_t[DELTA ? LA_TRI * 3 : 1][LA_FRAG], s_s[NKB][3][LA_FRAG];
     __shared__ __attribute__((aligned(16))) uint8_t s_x[DELTA ? 2 : 1][3][LA_FRAG], s_u[2][NO][LA_FRAG], s_e[2][3][LA_FRAG];
-    __shared__ int s_bad;
-    const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g4 = (lane >> 4) * 4;
-    const bool chain = w < 4;
-    const int rt = w & 3, at = lane * 16, half = at + 8 * (rt & 1);
-    const int slices = A.dim_v / 16;
-    const int64_t jobs = (int64_t)A.n_seq * A.n_head * slices;
-    // workgroups go round the 8 XCDs: the slices of a head, and heads of one key, on one of them
-    const int64_t per = (jobs + 7) / 8;
-    for (int64_t b = blockIdx.x; b < 8 * per; b += gridDim.x) {
-        const int64_t job = (b & 7) * per + (b >> 3);
-        if (job >= jobs) continue;
-        const int c0 = (int)(job % slices) * 16, head0 = (int)(job / slices % A.n_head), seq = (int)(job / slices / A.n_head);
-        const int head = la_head_of(A, head0 / (A.n_head / A.n_key), head0 % (A.n_head / A.n_key));
+    __shared__ __attribute__((aligned(16))) float s_in[M::OVER ? 1 : 1280];
+    float *const s_vec = M::OVER ? (float *)s_u : s_in, *const s_v = s_vec + 256;
+    __shared__ __attribute__((aligned(16))) int s_bad[4];         // each wave's first row that the form does not hold, 64: none
+    const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4, g4 = g * 4;
+    const bool chain = w < 4, loader = w >= 8;
+    const int rt = w & 3;
+    int at = lane * 16, half = at + 8 * (rt & 1);
+    // workgroups go round the 8 XCDs: the slices of a key head's heads on one of them, a sequence's key heads on all
+    const int slices = A.dim_v / 16, each = A.n_head / A.n_key * slices;
+    const int64_t units = (int64_t)A.n_seq * A.n_key, jobs = (units + 7) / 8 * 8 * each;
+    for (int64_t b = blockIdx.x; b < jobs; b += gridDim.x) {
+        const int64_t unit = (b >> 3) / each * 8 + (b & 7);
+        if (unit >= units) continue;
+        const int seq = (int)(unit / A.n_key), key = (int)(unit % A.n_key), part = (int)((b >> 3) % each);
+        const int head = la_head_of(A, key, part / slices), c0 = part % slices * 16;
         const LaRows rows = la_rows(ldg(A.cu + seq), ldg(A.cu + seq + 1), A.T, A.r0, A.r1);
         if (rows.n <= 0) continue;
         const LaState st = la_state(A, seq, head, DK, rows.begun, rows.goes_on);
@@ -579,7 +606,7 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
             if (w == 0) la_recurrence<T, DK, DELTA>(A, head, c0, rows.first, rows.n, st);
             continue;
         }
-        const int key = la_key_of(A, head);
+        // a wave's block kb of the state holds rows 32 kb + 8 g + 4 h + r
         f32x4 s[OWN][2];
         bool odd = false;
 #pragma unroll
@@ -590,7 +617,7 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     s[o][h][r] = 0.0f;
-                    if (chain && kb < NKB && st.from) s[o][h][r] = ldg(st.from + (int64_t)(32 * kb + 16 * h + g4 + r) * A.dim_v + c0 + l16);
+                    if (chain && kb < NKB && st.from) s[o][h][r] = ldg(st.from + (int64_t)(32 * kb + 8 * g + 4 * h + r) * A.dim_v + c0 + l16);
                     odd |= !(fabsf(s[o][h][r]) <= 0x1p100f);
                 }
         }
@@ -609,68 +636,105 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
             }
         };
         publish();
-        if (threadIdx.x == 0) s_bad = 64;
         int c = 0, upto = 0;                              // the first chunk that is not done, the first such row of it
         const bool go = !__syncthreads_or(odd);
-        auto keys = [&](int i) { return A.keys + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_key + key) * Y::KEY_BYTES; };
         auto heads = [&](int i) { return A.heads + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_head + head) * Y::HEAD_BYTES; };
-        // 16 rows of K or Q
-        auto load_rows = [&](const uint8_t *p, bf168 (&o)[NKB][NP]) {
+        auto keys = [&](int i) { return A.keys + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_key + key) * X::BYTES; };
+        // a row of chunk i, or the sequence's last
+        auto row_of = [&](int i, int row) { return (int64_t)rows.first + min(64 * i + row, rows.n - 1); };
+        if (loader && go) {
+            constexpr int MINE = X::Q / LA_FRAG / 4, MINE_T = DELTA ? (LA_TRI * 3 + 3) / 4 : 0, MINE_V = 5;      // loads of a loader
+            float v[4];
+            f32x4 vec;
+            auto bring_k = [&](int i) {
 #pragma unroll
-            for (int kb = 0; kb < NKB; kb++) la_load<NP>(p + (rt * NKB + kb) * NP * LA_FRAG, o[kb]);
-        };
-        // Each of the two walks asks for a chunk's operands a chunk ahead, as soon as it has used the last one's, and
-        // without a branch: loads come back in turn, and one that is waited for early is waited for with all ahead of it.
-        if (chain && go) {
-            bf168 kf[NKB][NP], tf[2][3], ktf[OWN][2][2][NP];
-            f32x4 kd, bt, ke;
-            float v[4], end;
-            int good, none = 0;
-            asm("" : "+v"(none));                         // a scalar load would be waited for with LDS
-            auto load_kt = [&](int i) {
-                const uint8_t *p = keys(i) + Y::KT;
-#pragma unroll
-                for (int o = 0; o < OWN; o++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int tb = 0; tb < 2; tb++)
-                            la_load<NP>(p + ((2 * min(rt + 4 * o, NKB - 1) + h) * 2 + tb) * NP * LA_FRAG, ktf[o][h][tb]);
+                for (int u = 0; u < MINE; u++) la_bring(keys(i) + (rt + 4 * u) * LA_FRAG, s_k[i % BUFS] + (rt + 4 * u) * LA_FRAG);
             };
-            auto load_t = [&](int i) {
-                const uint8_t *p = heads(i) + Y::TI;
+            auto bring_t = [&](int i) {
 #pragma unroll
-                for (int tb = 0; tb < 2; tb++) la_load<3>(p + la_tri(rt, rt < 2 ? 0 : tb) * 3 * LA_FRAG, tf[tb]);
+                for (int u = 0; u < MINE_T; u++) {
+                    const int f = min(rt + 4 * u, LA_TRI * 3 - 1);
+                    la_bring(heads(i) + Y::TI + f * LA_FRAG, s_t[f]);
+                }
             };
-            auto load_v = [&](int i) {
-                const uint8_t *vec = heads(i) + Y::VEC;
-                kd = *(const QMAG_GLOBAL f32x4 *)(vec + 4 * (Y::KD + 16 * rt + g4));
-                bt = *(const QMAG_GLOBAL f32x4 *)(vec + 4 * (Y::B + 16 * rt + g4));
-                ke = *(const QMAG_GLOBAL f32x4 *)(vec + 4 * (Y::KE + 16 * rt + g4));
-                end = *(const QMAG_GLOBAL float *)(vec + 4 * (Y::END + none));
-                good = *(const QMAG_GLOBAL int *)(vec + 4 * (Y::BAD + none));
-                const int t = 64 * min(i, chunks - 1) + 16 * rt + g4;
-                const S *p = (const S *)A.v.p + (int64_t)rows.first * A.v.ts + head * A.v.hs + c0 + l16;
+            auto ask = [&](int i) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) v[r] = T::up(*(const QMAG_GLOBAL S *)(p + min(t + r, rows.n - 1) * A.v.ts));
+                for (int r = 0; r < 4; r++) v[r] = T::up(*(const QMAG_GLOBAL S *)((const S *)A.v.p + row_of(i, 16 * rt + g4 + r) * A.v.ts + head * A.v.hs + c0 + l16));
+                vec = *(const QMAG_GLOBAL f32x4 *)(heads(i) + Y::VEC + at);
             };
-            if constexpr (DELTA) load_rows(keys(0) + Y::K, kf);
-            load_v(0);
-            if constexpr (DELTA) load_t(0);
-            load_kt(0);
+            auto put = [&]() {
+                la_write((uint8_t *)&s_v[256 * rt + 4 * lane], f32x4{v[0], v[1], v[2], v[3]});
+                if (rt == 0) la_write((uint8_t *)&s_vec[4 * lane], vec);
+            };
+            ask(0);
+            put();
+            bring_k(0);
+            bring_t(0);
+            ask(1);
+            la_meet<0>();
             for (; c < chunks; c++) {
-                f32x4 acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (BUFS == 2) bring_k(c + 1);
                 if constexpr (DELTA) {
+                    la_meet<BUFS == 2 ? MINE : 0>();      // the inverse is there; V and what it is multiplied by are taken next
+                    if constexpr (BUFS == 2) {
+                        put();
+                        ask(c + 2);
+                    }
+                }
+                la_meet<63>();
+                // (an ordinary read of LDS would wait for all that is on its way there)
+                int4 bad;
+                asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(bad) : "v"(la_lds(s_bad)) : "memory");
+                upto = min(min(bad.x, bad.y), min(bad.z, bad.w));
+                if (upto < 64) break;
+                if constexpr (!DELTA && BUFS == 2) {
+                    put();
+                    ask(c + 2);
+                }
+                bring_t(c + 1);
+                if constexpr (BUFS == 2) {
+                    la_meet<MINE_T + MINE_V>();           // K is there
+                } else {
+                    la_meet<63>();
+                    put();
+                    ask(c + 2);
+                    bring_k(c + 1);
+                    la_meet<0>();
+                }
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else if (chain && go) {
+            // places in K that differ by more than a constant: a row's even and odd blocks, the wave's rows of K^T
+            int row_at[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) row_at[i] = (16 * rt + l16) * DK * 2 + la_place(l16, 4 * i + g) * 16;
+            const int own = min(rt, NKB - 1), tok = g4 + (l16 >> 2);
+            const int col_at = tok * DK * 2 + (own >> 1) * 128 + la_place(tok, 4 * (own & 1) + (l16 & 3)) * 16;
+            __syncthreads();
+            for (; c < chunks; c++) {
+                la_fresh(at);
+                la_fresh(half);
+                const uint8_t *K = s_k[c % BUFS];
+                f32x4 acc;
+                if constexpr (DELTA) {
+                    LaSum<2> ks[2];
+                    ks[0].clear();
+                    ks[1].clear();
 #pragma unroll
                     for (int kb = 0; kb < NKB; kb++) {
-                        bf168 b[3];
+                        bf168 a[NP], b[3];
 #pragma unroll
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
-                        acc = la_mul<NP, 3, 2>(kf[kb], b, acc);
+#pragma unroll
+                        for (int i = 0; i < NP; i++) a[i] = *(const bf168 *)(K + row_at[kb & 1] + i * X::PLANE + (kb >> 1) * 128);
+                        ks[kb & 1].add(a, b);
                     }
-                    load_rows(keys(c + 1) + Y::K, kf);
+                    acc = ks[0].sum() + ks[1].sum();
                 }
-                const int left = min(rows.n - 64 * c, good);
+                const f32x4 kd = *(const f32x4 *)&s_vec[Y::KD + 16 * rt + g4], bt = *(const f32x4 *)&s_vec[Y::B + 16 * rt + g4],
+                            ke = *(const f32x4 *)&s_vec[Y::KE + 16 * rt + g4], v = *(const f32x4 *)&s_v[256 * rt + 4 * lane];
+                const float end = s_vec[Y::END];
+                const int good = ((const int *)s_vec)[Y::BAD], left = min(rows.n - 64 * c, good);
                 int bad = good;
                 float x[4];
 #pragma unroll
@@ -680,26 +744,30 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
                     x[r] = row < left && fine ? bt[r] * (DELTA ? fmaf(-kd[r], acc[r], v[r]) : v[r]) : 0.0f;
                     bad = row < left && !fine ? min(bad, row) : bad;
                 }
-                const float now = end;
-                const f32x4 e4 = ke;
-                load_v(c + 1);
-                if (bad < 64) atomicMin(&s_bad, bad);
                 if constexpr (DELTA) {
                     __bf16 p[3][4];
                     la_split<3, 4>(x, p);
 #pragma unroll
                     for (int i = 0; i < 3; i++) *(s16x4 *)&s_x[rt >> 1][i][half] = *(const s16x4 *)p[i];
+                }
+                bad = group_min_i<64>(bad);
+                if (lane == 0) s_bad[rt] = bad;
+                if constexpr (DELTA) {
                     __syncthreads();
-                    f32x4 u = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    LaSum<2> us[2];
+                    us[0].clear();
+                    us[1].clear();
 #pragma unroll
                     for (int tb = 0; tb < 2; tb++) {
                         if (2 * tb > rt) continue;
-                        bf168 b[3];
+                        bf168 a[3], b[3];
 #pragma unroll
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_x[tb][i][at];
-                        u = la_mul<3, 3, 2>(tf[tb], b, u);
+#pragma unroll
+                        for (int i = 0; i < 3; i++) a[i] = *(const bf168 *)&s_t[la_tri(rt, tb) * 3 + i][at];
+                        us[tb].add(a, b);
                     }
-                    load_t(c + 1);
+                    const f32x4 u = us[0].sum() + us[1].sum();
 #pragma unroll
                     for (int r = 0; r < 4; r++) x[r] = u[r];
                 }
@@ -707,7 +775,7 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
                     __bf16 p[NO][4], pe[3][4];
                     float xe[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++) xe[r] = x[r] * e4[r];
+                    for (int r = 0; r < 4; r++) xe[r] = x[r] * ke[r];
                     la_split<NO, 4>(x, p);
                     la_split<3, 4>(xe, pe);
 #pragma unroll
@@ -716,12 +784,13 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
                     for (int i = 0; i < 3; i++) *(s16x4 *)&s_e[rt >> 1][i][half] = *(const s16x4 *)pe[i];
                 }
                 __syncthreads();
-                upto = s_bad;
+                upto = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
                 if (upto < 64) break;
+                LaSum<2> more[OWN][2];
 #pragma unroll
                 for (int o = 0; o < OWN; o++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) s[o][h] *= now;
+                    for (int h = 0; h < 2; h++) more[o][h].clear();
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) {
                     bf168 b[3];
@@ -730,46 +799,76 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
 #pragma unroll
                     for (int o = 0; o < OWN; o++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) s[o][h] = la_mul<NP, 3, 2>(ktf[o][h][tb], b, s[o][h]);
+                        for (int h = 0; h < 2; h++) {
+                            // K^T by transposing reads: 16 lanes take 4 tokens by 4 times 4 channels, and lane n gets
+                            // the tokens of the n-th
+                            union { s16x4 half[2]; bf168 v; } a[NP];
+                            bf168 av[NP];
+#pragma unroll
+                            for (int i = 0; i < NP; i++) {
+#pragma unroll
+                                for (int u = 0; u < 2; u++)
+                                    a[i].half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        (__attribute__((address_space(3))) s16x4 *)(K + col_at + i * X::PLANE + (32 * tb + 16 * u) * DK * 2 + 256 * o + 8 * h));
+                                av[i] = a[i].v;
+                            }
+                            more[o][h].add(av, b);
+                        }
                 }
-                load_kt(c + 1);
+#pragma unroll
+                for (int o = 0; o < OWN; o++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) s[o][h] = s[o][h] * end + more[o][h].sum();
                 publish();
                 __syncthreads();
+                if constexpr (BUFS == 1) __syncthreads();
             }
         } else if (go) {
             bf168 qf[NKB][NP], pf[2][NO];
             f32x4 qd;
-            auto load_p = [&](int i) {
+            auto ask_q = [&](int i) {
+                const uint8_t *p = keys(i) + X::Q + rt * NKB * NP * LA_FRAG;
+#pragma unroll
+                for (int kb = 0; kb < NKB; kb++) la_load<NP>(p + kb * NP * LA_FRAG, qf[kb]);
+            };
+            auto ask_p = [&](int i) {
                 const uint8_t *p = heads(i);
-                qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::VEC + 4 * (Y::QD + 16 * rt + g4));
+                qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::QD + 4 * (16 * rt + g4));
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) la_load<NO>(p + Y::P + la_tri(rt, rt < 2 ? 0 : tb) * NO * LA_FRAG, pf[tb]);
             };
-            load_rows(keys(0) + Y::Q, qf);
-            load_p(0);
+            ask_q(0);
+            ask_p(0);
+            __syncthreads();
             for (; c < chunks; c++) {
-                f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                la_fresh(at);
+                LaSum<UP> qs[2], ps[2];
+                qs[0].clear();
+                qs[1].clear();
+                ps[0].clear();
+                ps[1].clear();
 #pragma unroll
                 for (int kb = 0; kb < NKB; kb++) {
-                    bf168 b[3];
+                    bf168 b[UP + 1];
 #pragma unroll
-                    for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
-                    o = la_mul<NP, 3, UP>(qf[kb], b, o);
+                    for (int i = 0; i <= UP; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
+                    qs[kb & 1].add(qf[kb], b);
                 }
-                load_rows(keys(c + 1) + Y::Q, qf);
-                o *= qd;
+                ask_q(c + 1);
+                f32x4 o = (qs[0].sum() + qs[1].sum()) * qd;
                 if constexpr (DELTA) __syncthreads();
                 __syncthreads();
-                upto = s_bad;
+                upto = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) {
                     if (2 * tb > rt) continue;
                     bf168 b[NO];
 #pragma unroll
                     for (int i = 0; i < NO; i++) b[i] = *(const bf168 *)&s_u[tb][i][at];
-                    o = la_mul<NO, NO, UP>(pf[tb], b, o);
+                    ps[tb].add(pf[tb], b);
                 }
-                load_p(c + 1);
+                ask_p(c + 1);
+                o += ps[0].sum() + ps[1].sum();
                 const int t = 64 * c + 16 * rt + g4, to = min(rows.n, 64 * c + upto);
                 S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + l16;
 #pragma unroll
@@ -777,6 +876,7 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
                     if (t + r < to) p[r * A.ots] = T::down(o[r]);
                 if (upto < 64) break;
                 __syncthreads();
+                if constexpr (BUFS == 1) __syncthreads();
             }
         }
         if (c < chunks) {
@@ -790,7 +890,7 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        if (chain && rt + 4 * o < NKB) hand[32 * (rt + 4 * o) + 16 * h + g4 + r][l16] = s[o][h][r];
+                        if (chain && rt + 4 * o < NKB) hand[32 * (rt + 4 * o) + 8 * g + 4 * h + r][l16] = s[o][h][r];
             __syncthreads();
             if (w == 0)
                 la_recurrence<T, DK, DELTA>(A, head, c0, rows.first + 64 * c, rows.n - 64 * c, upto, [&](int row, float (&x)[4]) {
@@ -804,7 +904,7 @@ __global__ void __launch_bounds__(512) linattn_chain_kernel(LaArgs A)
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        if (rt + 4 * o < NKB) st.to[(int64_t)(32 * (rt + 4 * o) + 16 * h + g4 + r) * A.dim_v + c0 + l16] = s[o][h][r];
+                        if (rt + 4 * o < NKB) st.to[(int64_t)(32 * (rt + 4 * o) + 8 * g + 4 * h + r) * A.dim_v + c0 + l16] = s[o][h][r];
         }
     }
 }
@@ -826,8 +926,8 @@ static size_t la_tile_bytes(int type, int dim_k, int n_key, int n_head)
     size_t bytes = 0;
     with_type(type, [&](auto t) {
         return with_dim_k(dim_k, [&](auto d) {
-            using Y = LaLayout<decltype(t), decltype(d)::value>;
-            bytes = (size_t)n_key * Y::KEY_BYTES + (size_t)n_head * Y::HEAD_BYTES;
+            using TT = decltype(t);
+            bytes = (size_t)n_key * LaKeys<TT, decltype(d)::value>::BYTES + (size_t)n_head * LaLayout<TT>::HEAD_BYTES;
             return 0;
         });
     });
@@ -921,22 +1021,22 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
                 return 0;
             }
             float *carry = (float *)A.carry_in;
-            const int64_t wgs = (slices + 7) / 8 * 8;
+            const int64_t wgs = ((int64_t)n_seq * q->n_head + 7) / 8 * 8 * (a->n_head / q->n_head) * (a->dim_v / 16);
             const unsigned grid = (unsigned)(wgs < 1 << 22 ? wgs : 1 << 22);
             for (int64_t r0 = 0, odd = 0; r0 < T; r0 += window, odd ^= 1) {
                 A.r0 = (int)r0;
                 A.r1 = (int)(r0 + window < T ? r0 + window : T);
                 A.n_tile = la_most_tiles(A.r1 - A.r0, n_seq);
-                A.heads = A.keys + (size_t)A.n_tile * (size_t)A.n_key * LaLayout<TT, DK>::KEY_BYTES;
+                A.heads = A.keys + (size_t)A.n_tile * (size_t)A.n_key * LaKeys<TT, DK>::BYTES;
                 A.carry_in = carry + (odd ? state / sizeof(float) : 0);
                 A.carry_out = carry + (odd ? 0 : state / sizeof(float));
                 const unsigned tiles = (unsigned)A.n_tile * (unsigned)A.n_key;
                 if (a->delta) {
                     linattn_chunk_kernel<TT, DK, true><<<tiles, 256, 0, s>>>(A);
-                    linattn_chain_kernel<TT, DK, true><<<grid, 512, 0, s>>>(A);
+                    linattn_chain_kernel<TT, DK, true><<<grid, 768, 0, s>>>(A);
                 } else {
                     linattn_chunk_kernel<TT, DK, false><<<tiles, 256, 0, s>>>(A);
-                    linattn_chain_kernel<TT, DK, false><<<grid, 512, 0, s>>>(A);
+                    linattn_chain_kernel<TT, DK, false><<<grid, 768, 0, s>>>(A);
                 }
             }
             return 0;
