@@ -21,7 +21,7 @@ struct ConvArgs {
     const float *weight, *bias;
     float *state;
     const int *slot, *len, *cu;
-    int n_channel, n_slot, n_seq, T, shift, n_tile, silu;
+    int n_channel, n_slot, n_seq, T, shift, n_tile, across, silu;
 };
 
 // the n <= V values from p, the others zero
@@ -47,12 +47,19 @@ __device__ __forceinline__ void store_some(typename T::S *p, int n, const float 
     }
 }
 
+// y / (1 + e^-y), both sides times 2^-64, so that what is divided by has no reciprocal below fp32's normal numbers
+// while the result has
+__device__ __forceinline__ float conv_silu(float y)
+{
+    return (y * 0x1p-64f) * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(y * -1.44269504088896340736f), 0x1p-64f, 0x1p-64f));
+}
+
 template <class T, int W>
 __global__ void __launch_bounds__(256) conv_kernel(ConvArgs A)
 {
     using S = typename T::S;
     constexpr int V = 16 / (int)sizeof(S), AT_ONCE = 4;
-    const int c0 = (int)(blockIdx.y * blockDim.x + threadIdx.x) * V;
+    const int c0 = (int)(blockIdx.x % A.across * blockDim.x + threadIdx.x) * V;
     if (c0 >= A.n_channel) return;
     const int nc = min(V, A.n_channel - c0);
     float w[V][W], bias[V];
@@ -65,7 +72,7 @@ __global__ void __launch_bounds__(256) conv_kernel(ConvArgs A)
     const S *x = (const S *)A.x + c0;
     S *out = (S *)A.out + c0;
     const int tokens = 1 << A.shift;
-    for (int j = blockIdx.x; j < A.n_tile; j += gridDim.x) {
+    for (int j = blockIdx.x / A.across; j < A.n_tile; j += gridDim.x / A.across) {
         const SeqTile s = seq_find([&](int i) { return ldg(A.cu + i); }, A.n_seq, A.T, A.shift, j);
         if (s.seq < 0) continue;
         const int64_t row = (int64_t)s.first + ((int64_t)s.tile << A.shift);
@@ -86,11 +93,15 @@ __global__ void __launch_bounds__(256) conv_kernel(ConvArgs A)
 #pragma unroll
                 for (int i = 0; i < V; i++) past[k][i] = 0.0f;
         }
-        for (int t0 = 0; t0 < n; t0 += AT_ONCE) {
-            float v[AT_ONCE][V];
+        float v[AT_ONCE][V];
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; u++)
-                if (t0 + u < n) load_some<T, V>(x + (row + t0 + u) * A.xs, nc, v[u]);
+        for (int u = 0; u < AT_ONCE; u++) load_some<T, V>(x + (row + min(u, n - 1)) * A.xs, nc, v[u]);
+        for (int t0 = 0; t0 < n; t0 += AT_ONCE) {
+            float next[AT_ONCE][V];
+            if (t0 + AT_ONCE < n) {
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; u++) load_some<T, V>(x + (row + min(t0 + AT_ONCE + u, n - 1)) * A.xs, nc, next[u]);
+            }
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) {
                 if (t0 + u >= n) break;
@@ -101,13 +112,17 @@ __global__ void __launch_bounds__(256) conv_kernel(ConvArgs A)
 #pragma unroll
                     for (int k = 0; k < W - 1; k++) a = fmaf(w[i][k], past[k][i], a);
                     a = fmaf(w[i][W - 1], v[u][i], a);
-                    y[i] = A.silu ? a / (1.0f + expf(-a)) : a;
+                    y[i] = A.silu ? conv_silu(a) : a;
 #pragma unroll
                     for (int k = 0; k + 1 < W - 1; k++) past[k][i] = past[k + 1][i];
                     past[W - 2][i] = v[u][i];
                 }
                 store_some<T, V>(out + (row + t0 + u) * A.os, nc, y);
             }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+                for (int i = 0; i < V; i++) v[u][i] = next[u][i];
         }
         if (held) {
             // a sequence longer than its first tile: its last rows; else what the tile ends with
@@ -158,17 +173,19 @@ extern "C" int qmag_conv_dev(const qmag_conv *c, int type, const void *x, int64_
     if (T == 0 || n_seq == 0) return QMAG_OK;
 
     ConvArgs A = {x, out, x_stride, out_stride, c->weight, c->bias, c->state, c->n_slot ? slot : nullptr, len, cu,
-                  C, c->n_slot, n_seq, T, 2, 0, c->silu};
+                  C, c->n_slot, n_seq, T, 2, 0, 0, c->silu};
     const int per = 16 / size, threads = (C + per - 1) / per;
-    const int wg = threads >= 256 ? 256 : (threads + 63) / 64 * 64, across = (threads + wg - 1) / wg;
+    // workgroups of up to four waves, as few of which are empty as may be
+    const int waves = (threads + 63) / 64, across = (waves + 3) / 4, wg = (waves + across - 1) / across * 64;
     // tiles as long as leave the chip its waves
     while (A.shift < 5 && (int64_t)seq_most_tiles(T, n_seq, A.shift + 1) * across * (wg / 64) >= 4096) A.shift++;
     A.n_tile = seq_most_tiles(T, n_seq, A.shift);
+    A.across = across;                                // a tile's workgroups side by side: rows are read whole
     DeviceScope dev;
     if (dev.st) return dev.st;
     hipStream_t s = ctx().stream;
     const int most = (1 << 22) / across + 1;          // a launch holds fewer than 2^32 threads
-    const dim3 grid((unsigned)(A.n_tile < most ? A.n_tile : most), (unsigned)across);
+    const unsigned grid = (unsigned)(A.n_tile < most ? A.n_tile : most) * (unsigned)across;
     prof_begin(PROF_CONV, s);
     with_type(type, [&](auto t) {
         using TT = decltype(t);

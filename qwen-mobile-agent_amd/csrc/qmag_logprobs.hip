@@ -26,6 +26,7 @@ namespace qmag {
 constexpr int LP_WG = 256, LP_WAVES = LP_WG / 64;
 constexpr int LP_PER = 8;                        // values of a thread in a tile
 constexpr int LP_TILE = 64 * LP_PER;             // a wave's tile
+constexpr int LP_AHEAD = 4;
 
 struct LpArgs {
     const void *x;
@@ -55,7 +56,7 @@ struct LpSum {
     // to a maximum of at least m: a sum of nothing stays one
     __device__ void move(float to)
     {
-        const float d = fmaxf(m - to, -200.0f), c = exp2f(d * LOG2E);
+        const float d = fmaxf(m - to, -200.0f), c = __builtin_amdgcn_exp2f(d * LOG2E);
         t = s == 0.0f ? 0.0f : c * fmaf(s, d, t);
         rt = s == 0.0f ? 0.0f : c * fmaf(rs, d, rt);
         s *= c;
@@ -158,6 +159,28 @@ __device__ __forceinline__ void lp_finish(const LpArgs &A, int64_t row, LpSum a,
     }
 }
 
+// a thread's values of a tile as they are read
+template <class T>
+struct LpRaw {
+    static constexpr int N = LP_PER * (int)sizeof(typename T::S) / 16, PER = LP_PER / N;
+    uint4 r[N];
+    __device__ __forceinline__ void load(const typename T::S *p)
+    {
+#pragma unroll
+        for (int i = 0; i < N; i++) r[i] = ld16((const uint8_t *)(p + i * PER));
+    }
+    __device__ __forceinline__ void get(float (&v)[LP_PER]) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            union { uint4 u; typename T::S s[PER]; } x;
+            x.u = r[i];
+#pragma unroll
+            for (int e = 0; e < PER; e++) v[i * PER + e] = T::up(x.s[e]);
+        }
+    }
+};
+
 template <class T, bool TOP>
 __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
 {
@@ -175,15 +198,7 @@ __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
         a.clear();
         LpTop top;
         top.clear();
-        for (int64_t at = (int64_t)v0 + w * LP_TILE; at < v1; at += LP_WAVES * LP_TILE) {
-            const int64_t i0 = at + lane * LP_PER;
-            float v[LP_PER];
-            if (i0 + LP_PER <= v1) {
-                load_row<T, LP_PER>(x + i0, v);
-            } else {
-#pragma unroll
-                for (int i = 0; i < LP_PER; i++) v[i] = i0 + i < v1 ? T::up(x[i0 + i]) : -INFINITY;
-            }
+        auto tile = [&](const float (&v)[LP_PER], int64_t i0) {
             float hi = v[0];
 #pragma unroll
             for (int i = 1; i < LP_PER; i++) hi = fmaxf(hi, v[i]);
@@ -191,7 +206,7 @@ __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
             float es = 0.0f, et = 0.0f;
 #pragma unroll
             for (int i = 0; i < LP_PER; i++) {
-                const float d = v[i] - a.m, e = exp2f(d * LOG2E);
+                const float d = v[i] - a.m, e = __builtin_amdgcn_exp2f(d * LOG2E);
                 es += e;                                              // a NaN stays
                 et = fmaf(e, fmaxf(d, -200.0f), et);
             }
@@ -206,6 +221,32 @@ __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
                     if (first) top.take(wait, A.top_k);
                 }
             }
+        };
+        // whole tiles, several asked for ahead: a CU's share of the memory is some 16 KB for each microsecond of a load
+        const int64_t w0 = (int64_t)v0 + w * LP_TILE;
+        const int whole = v1 - w0 >= LP_TILE ? (int)((v1 - w0 - LP_TILE) / (LP_WAVES * LP_TILE)) + 1 : 0;
+        LpRaw<T> raw[LP_AHEAD];
+        if (whole > 0) {
+#pragma unroll
+            for (int u = 0; u < LP_AHEAD; u++) raw[u].load(x + w0 + (int64_t)min(u, whole - 1) * (LP_WAVES * LP_TILE) + lane * LP_PER);
+            for (int k0 = 0; k0 < whole; k0 += LP_AHEAD) {
+#pragma unroll
+                for (int u = 0; u < LP_AHEAD; u++) {
+                    if (k0 + u >= whole) break;
+                    float v[LP_PER];
+                    raw[u].get(v);
+                    raw[u].load(x + w0 + (int64_t)min(k0 + u + LP_AHEAD, whole - 1) * (LP_WAVES * LP_TILE) + lane * LP_PER);
+                    tile(v, w0 + (int64_t)(k0 + u) * (LP_WAVES * LP_TILE) + lane * LP_PER);
+                }
+            }
+        }
+        const int64_t rest = w0 + (int64_t)whole * (LP_WAVES * LP_TILE);
+        if (rest < v1) {
+            const int64_t i0 = rest + lane * LP_PER;
+            float v[LP_PER];
+#pragma unroll
+            for (int i = 0; i < LP_PER; i++) v[i] = i0 + i < v1 ? T::up(x[i0 + i]) : -INFINITY;
+            tile(v, i0);
         }
         if constexpr (TOP) {
             top.take(wait, A.top_k);
@@ -234,33 +275,52 @@ __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
     }
 }
 
+// Parts of a row: a wave takes every 16th, four asked for at once, then the waves' results in pairs.
+constexpr int LP_JOIN = 1024, LP_JOINERS = LP_JOIN / 64;
 template <class T, bool TOP>
-__global__ void __launch_bounds__(LP_WG) logprobs_join_kernel(LpArgs A)
+__global__ void __launch_bounds__(LP_JOIN) logprobs_join_kernel(LpArgs A)
 {
-    __shared__ uint64_t s_key[TOP ? LP_WAVES : 1][64];
-    __shared__ float s_sum[LP_WAVES][3];
+    __shared__ uint64_t s_key[TOP ? LP_JOINERS : 1][64];
+    __shared__ float s_sum[LP_JOINERS][3];
     const int lane = lane_id(), w = threadIdx.x >> 6;
     for (int64_t row = blockIdx.x; row < A.T; row += gridDim.x) {
         LpSum a;
         a.clear();
         uint64_t key = 0;
-        for (int p = w * 64 + lane; p < A.parts; p += LP_WG) {
+        for (int p = w + LP_JOINERS * lane; p < A.parts; p += LP_JOIN) {
             const float *st = A.stat + (row * A.parts + p) * 4;
             a.join(st[0], st[1], st[2]);
         }
-        a = lp_wave_join(a);
         if constexpr (TOP) {
-            for (int p = w; p < A.parts; p += LP_WAVES) key = lp_merge(key, A.keys[(row * A.parts + p) * 64 + 63 - lane]);
+            for (int p = w; p < A.parts; p += 4 * LP_JOINERS) {
+                uint64_t k[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    k[u] = p + u * LP_JOINERS < A.parts ? A.keys[(row * A.parts + p + u * LP_JOINERS) * 64 + 63 - lane] : 0ull;
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (p + u * LP_JOINERS < A.parts) key = lp_merge(key, k[u]);
+            }
             s_key[w][lane] = key;
         }
+        a = lp_wave_join(a);
         if (lane == 0) s_sum[w][0] = a.m, s_sum[w][1] = a.s, s_sum[w][2] = a.t;
         __syncthreads();
-        if (w == 0) {
+        if constexpr (TOP) {
 #pragma unroll
-            for (int o = 1; o < LP_WAVES; o++) a.join(s_sum[o][0], s_sum[o][1], s_sum[o][2]);
-            if constexpr (TOP)
-                for (int o = 1; o < LP_WAVES; o++) key = lp_merge(key, s_key[o][63 - lane]);
-            lp_finish<T>(A, row, a, key);
+            for (int half = LP_JOINERS / 2; half > 0; half >>= 1) {
+                if (w < half && w + half < A.parts) {
+                    key = lp_merge(key, s_key[w + half][63 - lane]);
+                    s_key[w][lane] = key;
+                }
+                if (half > 1) __syncthreads();
+            }
+        }
+        if (w == 0) {
+            LpSum b;
+            b.clear();
+            if (lane < LP_JOINERS) b.m = s_sum[lane][0], b.s = s_sum[lane][1], b.t = s_sum[lane][2];
+            lp_finish<T>(A, row, lp_wave_join(b), key);
         }
         __syncthreads();
     }
@@ -322,8 +382,8 @@ extern "C" int qmag_logprobs_dev(int n_vocab, int type, const void *logits, int6
         using TT = decltype(t);
         if (top_k) logprobs_kernel<TT, true><<<grid, LP_WG, 0, s>>>(A);
         else logprobs_kernel<TT, false><<<grid, LP_WG, 0, s>>>(A);
-        if (A.parts > 1 && top_k) logprobs_join_kernel<TT, true><<<rows, LP_WG, 0, s>>>(A);
-        else if (A.parts > 1) logprobs_join_kernel<TT, false><<<rows, LP_WG, 0, s>>>(A);
+        if (A.parts > 1 && top_k) logprobs_join_kernel<TT, true><<<rows, LP_JOIN, 0, s>>>(A);
+        else if (A.parts > 1) logprobs_join_kernel<TT, false><<<rows, LP_JOIN, 0, s>>>(A);
         return 0;
     });
     prof_end(PROF_LOGPROBS, s);
