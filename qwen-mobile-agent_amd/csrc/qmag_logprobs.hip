@@ -10,9 +10,9 @@
 // of the sum, and a thousand of them count (1e-6 of a row's result without).
 // Where the most likely tokens are asked for, a wave keeps the 64 best keys (a
 // value's order above its complemented place, so that no two are equal) sorted, one
-// to a lane, and a value of LDS room for 64 more; of a tile of values those above
-// the k-th best go there (few after the first tiles: a random row of n has about
-// k ln(n / k)), and a full one is sorted and merged in.
+// to a lane; of a tile of values those above the k-th best wait in LDS (few after the
+// first tiles: a random row of n has about k ln(n / k)), and k that wait are sorted
+// and merged in.
 //
 // A row is one workgroup's, or, where there are few, several workgroups' and joined
 // by a second launch.
@@ -27,6 +27,7 @@ constexpr int LP_WG = 256, LP_WAVES = LP_WG / 64;
 constexpr int LP_PER = 8;                        // values of a thread in a tile
 constexpr int LP_TILE = 64 * LP_PER;             // a wave's tile
 constexpr int LP_AHEAD = 4;
+constexpr int LP_ROOM = 64 + LP_TILE;           // keys that wait: fewer than k ahead of a tile, all of its values
 
 struct LpArgs {
     const void *x;
@@ -41,6 +42,14 @@ struct LpArgs {
 
 constexpr uint32_t LP_KEY_NONE = 0x007FFFFFu;    // samp_key(-inf)
 constexpr float LOG2E = 1.44269504088896340736f;
+
+// the largest of three; not as fmaxf has it where one is a NaN, which then costs an instruction for each operand
+__device__ __forceinline__ float lp_max(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 struct LpSum {
     float m, s, t, rs, rt;            // rs, rt: what s and t are above their sums
@@ -100,13 +109,15 @@ struct LpTop {
     bool full;            // there are k numbers: what is not above the bound is none of the best
     int n;                // keys waiting in LDS
     __device__ void clear() { best = 0, bound = 0.0f, full = false, n = 0; }
+    // the last of those that wait, up to 64 of them
     __device__ void take(const uint64_t *wait, int k)
     {
+        const int from = max(n - 64, 0);
         __builtin_amdgcn_wave_barrier();
-        const uint64_t v = lane_id() < n ? wait[lane_id()] : 0ull;
+        const uint64_t v = from + lane_id() < n ? wait[from + lane_id()] : 0ull;
         __builtin_amdgcn_wave_barrier();
         best = lp_merge(best, ~wave_sort64(~v));
-        n = 0;
+        n = from;
         const uint64_t kth = readlane64(best, k - 1);
         full = (uint32_t)(kth >> 32) > 1u;           // 0: no key, 1: NaN
         bound = samp_value(kth);
@@ -114,26 +125,25 @@ struct LpTop {
     // What of a tile may be among the best, hi being the lane's largest value in it: values above the bound, or,
     // while there is none, keys from the k-th best of the lanes' largest on (k lanes hold one of that size).  It holds
     // for the whole tile, whose values do not come in the order of their places.
-    __device__ bool filter(float hi, int k, uint32_t *from) const
+    // (odd: a NaN among the lane's values, which may be its largest)
+    __device__ bool filter(float hi, bool odd, int k, uint32_t *from) const
     {
         if (full) {
             *from = 0;
-            return __ballot(hi > bound) != 0;
+            return __ballot(hi > bound || odd) != 0;
         }
         *from = (uint32_t)__builtin_amdgcn_readlane((int)wave_sort64_u32(samp_key(hi)), k - 1);
         if (*from <= LP_KEY_NONE) *from = 0;             // a lane's largest may be no value of the row
         return true;
     }
-    __device__ void add(float v, int id, bool in, bool first, uint32_t from, float above, uint64_t *wait, int k)
+    // a value of each lane joins those that wait
+    __device__ __forceinline__ void add(float v, int id, bool in, bool first, uint32_t from, uint64_t *wait)
     {
         const uint32_t key = samp_key(v);
-        const uint64_t who = __ballot(in && (first ? key >= from : v > above));
-        if (!who) return;
-        const int more = __popcll(who);
-        if (n + more > 64) take(wait, k);
+        const uint64_t who = __ballot(in && (first ? key >= from : v > bound));
         const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
         if ((who >> lane_id()) & 1u) wait[n + at] = samp_comp(key, id, v);
-        n += more;
+        n += __popcll(who);
     }
 };
 
@@ -169,10 +179,12 @@ struct LpRaw {
 #pragma unroll
         for (int i = 0; i < N; i++) r[i] = ld16((const uint8_t *)(p + i * PER));
     }
-    __device__ __forceinline__ void get(float (&v)[LP_PER]) const
+    // (what is made of them is not moved up to where they were asked for, which would wait for them there)
+    __device__ __forceinline__ void get(float (&v)[LP_PER])
     {
 #pragma unroll
         for (int i = 0; i < N; i++) {
+            asm volatile("" : "+v"(r[i].x), "+v"(r[i].y), "+v"(r[i].z), "+v"(r[i].w));
             union { uint4 u; typename T::S s[PER]; } x;
             x.u = r[i];
 #pragma unroll
@@ -185,7 +197,7 @@ template <class T, bool TOP>
 __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
 {
     using S = typename T::S;
-    __shared__ uint64_t s_wait[TOP ? LP_WAVES : 1][64];
+    __shared__ uint64_t s_wait[TOP ? LP_WAVES : 1][LP_ROOM];
     __shared__ float s_sum[LP_WAVES][3];
     const int lane = lane_id(), w = threadIdx.x >> 6;
     uint64_t *wait = s_wait[TOP ? w : 0];
@@ -199,9 +211,7 @@ __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
         LpTop top;
         top.clear();
         auto tile = [&](const float (&v)[LP_PER], int64_t i0) {
-            float hi = v[0];
-#pragma unroll
-            for (int i = 1; i < LP_PER; i++) hi = fmaxf(hi, v[i]);
+            const float hi = lp_max(lp_max(v[0], v[1], v[2]), lp_max(v[3], v[4], v[5]), lp_max(v[6], v[7], v[7]));
             if (hi > a.m) a.move(hi);
             float es = 0.0f, et = 0.0f;
 #pragma unroll
@@ -214,33 +224,41 @@ __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
             if constexpr (TOP) {
                 uint32_t from;
                 const bool first = !top.full;
-                const float above = top.bound;
-                if (top.filter(hi, A.top_k, &from)) {
+                if (top.filter(hi, es != es, A.top_k, &from)) {
 #pragma unroll
-                    for (int i = 0; i < LP_PER; i++) top.add(v[i], (int)(i0 + i), i0 + i < v1, first, from, above, wait, A.top_k);
-                    if (first) top.take(wait, A.top_k);
+                    for (int i = 0; i < LP_PER; i++) top.add(v[i], (int)(i0 + i), i0 + i < v1, first, from, wait);
+                    // (as many as are asked for move the bound; waiting for 64 lets half of all tiles through at k = 1)
+                    while (top.n >= A.top_k || (first && top.n > 0)) top.take(wait, A.top_k);
                 }
             }
         };
         // whole tiles, several asked for ahead: a CU's share of the memory is some 16 KB for each microsecond of a load
         const int64_t w0 = (int64_t)v0 + w * LP_TILE;
         const int whole = v1 - w0 >= LP_TILE ? (int)((v1 - w0 - LP_TILE) / (LP_WAVES * LP_TILE)) + 1 : 0;
+        constexpr int64_t STEP = LP_WAVES * LP_TILE;
         LpRaw<T> raw[LP_AHEAD];
-        if (whole > 0) {
+        const S *from = x + w0 + lane * LP_PER;
+        const int groups = whole / LP_AHEAD * LP_AHEAD;
+        if (groups > 0) {
 #pragma unroll
-            for (int u = 0; u < LP_AHEAD; u++) raw[u].load(x + w0 + (int64_t)min(u, whole - 1) * (LP_WAVES * LP_TILE) + lane * LP_PER);
-            for (int k0 = 0; k0 < whole; k0 += LP_AHEAD) {
+            for (int u = 0; u < LP_AHEAD; u++) raw[u].load(from + u * STEP);
+            for (int k = 0; k < groups; k += LP_AHEAD) {
 #pragma unroll
                 for (int u = 0; u < LP_AHEAD; u++) {
-                    if (k0 + u >= whole) break;
                     float v[LP_PER];
                     raw[u].get(v);
-                    raw[u].load(x + w0 + (int64_t)min(k0 + u + LP_AHEAD, whole - 1) * (LP_WAVES * LP_TILE) + lane * LP_PER);
-                    tile(v, w0 + (int64_t)(k0 + u) * (LP_WAVES * LP_TILE) + lane * LP_PER);
+                    raw[u].load(from + min(k + u + LP_AHEAD, whole - 1) * STEP);
+                    tile(v, w0 + (k + u) * STEP + lane * LP_PER);
                 }
             }
         }
-        const int64_t rest = w0 + (int64_t)whole * (LP_WAVES * LP_TILE);
+        for (int k = groups; k < whole; k++) {
+            float v[LP_PER];
+            raw[0].load(from + k * STEP);
+            raw[0].get(v);
+            tile(v, w0 + k * STEP + lane * LP_PER);
+        }
+        const int64_t rest = w0 + whole * STEP;
         if (rest < v1) {
             const int64_t i0 = rest + lane * LP_PER;
             float v[LP_PER];
@@ -249,7 +267,7 @@ __global__ void __launch_bounds__(LP_WG) logprobs_kernel(LpArgs A)
             tile(v, i0);
         }
         if constexpr (TOP) {
-            top.take(wait, A.top_k);
+            if (top.n > 0) top.take(wait, A.top_k);
             wait[lane] = top.best;
         }
         a = lp_wave_join(a);
