@@ -55,6 +55,7 @@ struct LaArgs {
     int r0, r1;               // the window's rows
     int n_tile;
     uint8_t *keys, *heads;    // what chunks have for each key head, and for each head
+    int *left;                // [n_tile][n_head][dim_v / 16] of a sequence's first chunk: the first row the walk did not do
     const float *carry_in;    // [n_head][dim_k][dim_v]: the state of a sequence begun ahead of the window
     float *carry_out;
 };
@@ -69,6 +70,8 @@ __device__ __forceinline__ float la_decay(float g)
     return g > 0.0f ? 1.0f : expf(g);
 }
 
+__device__ __forceinline__ int la_one(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Where a sequence's state comes from and goes to, at row 0 and column 0 of a head; null: nowhere.
 struct LaState {
     const float *from;
@@ -77,10 +80,10 @@ struct LaState {
 __device__ __forceinline__ LaState la_state(const LaArgs &A, int seq, int head, int dim_k, bool begun, bool goes_on)
 {
     const int64_t size = (int64_t)dim_k * A.dim_v;
-    const int slot = A.slot ? ldg(A.slot + seq) : -1;
+    const int slot = A.slot ? la_one(ldg(A.slot + seq)) : -1;
     float *own = slot >= 0 && slot < A.n_slot ? A.state + ((int64_t)slot * A.n_head + head) * size : nullptr;
     LaState s;
-    s.from = begun ? A.carry_in + head * size : own && !(A.len && ldg(A.len + seq) <= 0) ? own : nullptr;
+    s.from = begun ? A.carry_in + head * size : own && !(A.len && la_one(ldg(A.len + seq)) <= 0) ? own : nullptr;
     s.to = goes_on ? A.carry_out + head * size : own;
     return s;
 }
@@ -90,11 +93,10 @@ struct LaToken {
     float k[N], q[N], v[4], a, b;
 };
 
-// n rows from `first` on, one after another, of one head and 16 columns, by one wave;
-// from(row, x): four values of the state ahead of them, from the lane's column on.  The
+// n rows from `first` on, one after another, of one head and 16 columns, by one wave.  The
 // first `quiet` rows' results are there already.
-template <class T, int DK, bool DELTA, class F>
-__device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int n, int quiet, F from, float *to)
+template <class T, int DK, bool DELTA>
+__device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int n, int quiet, LaState st)
 {
     using S = typename T::S;
     constexpr int N = DK / 16;
@@ -102,7 +104,14 @@ __device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int 
     const int kh = la_key_of(A, head);
     float s[N][4];
 #pragma unroll
-    for (int r = 0; r < N; r++) from(rg * N + r, s[r]);
+    for (int r = 0; r < N; r++) {
+        if (st.from) {
+            load_row<TF32, 4>(st.from + (int64_t)(rg * N + r) * A.dim_v + col, s[r]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) s[r][c] = 0.0f;
+        }
+    }
     const S *kp = (const S *)A.k.p + first * A.k.ts + kh * A.k.hs + rg * N;
     const S *qp = (const S *)A.q.p + first * A.q.ts + kh * A.q.hs + rg * N;
     const S *vp = (const S *)A.v.p + first * A.v.ts + head * A.v.hs + col;
@@ -159,38 +168,9 @@ __device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int 
         if (rg == 0 && t >= quiet) store_row<T, 4>(op + t * A.ots, o);
         x = next;
     }
-    if (to) {
+    if (st.to) {
 #pragma unroll
-        for (int r = 0; r < N; r++) store_row<TF32, 4>(to + (int64_t)(rg * N + r) * A.dim_v + col, s[r]);
-    }
-}
-
-// the same from a sequence's own state
-template <class T, int DK, bool DELTA>
-__device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int n, LaState st)
-{
-    const int col = c0 + 4 * (lane_id() >> 4);
-    la_recurrence<T, DK, DELTA>(A, head, c0, first, n, 0, [&](int row, float (&x)[4]) {
-        if (st.from) {
-            load_row<TF32, 4>(st.from + (int64_t)row * A.dim_v + col, x);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 4; c++) x[c] = 0.0f;
-        }
-    }, st.to);
-}
-
-template <class T, int DK, bool DELTA>
-__global__ void __launch_bounds__(LA_WG) linattn_step_kernel(LaArgs A)
-{
-    const int slices = A.dim_v / 16;
-    const int64_t jobs = (int64_t)A.n_seq * A.n_head * slices;
-    for (int64_t j = (int64_t)blockIdx.x * (LA_WG / 64) + (threadIdx.x >> 6); j < jobs; j += (int64_t)gridDim.x * (LA_WG / 64)) {
-        const int64_t sh = j / slices;
-        const int seq = __builtin_amdgcn_readfirstlane((int)(sh / A.n_head)), head = __builtin_amdgcn_readfirstlane((int)(sh % A.n_head));
-        const int c0 = __builtin_amdgcn_readfirstlane((int)(j % slices) * 16);
-        const int first = seq_row(ldg(A.cu + seq), A.T), n = seq_row(ldg(A.cu + seq + 1), A.T) - first;
-        if (n > 0) la_recurrence<T, DK, DELTA>(A, head, c0, first, n, la_state(A, seq, head, DK, false, false));
+        for (int r = 0; r < N; r++) store_row<TF32, 4>(st.to + (int64_t)(rg * N + r) * A.dim_v + col, s[r]);
     }
 }
 
@@ -214,8 +194,13 @@ template <class T, int DK>
 struct LaKeys {
     static constexpr int K = 0, PLANE = 64 * DK * 2, Q = LA_PARTS<T> * PLANE, BYTES = 2 * Q;
 };
-// where 16 bytes of a row of K lie, in 16 bytes
-__host__ __device__ constexpr int la_place(int row, int piece) { return piece ^ (row & 7); }
+// Where 16 bytes of a row of K lie, in 16 bytes: 16 rows' of one piece in different banks, and so four rows' of four
+// pieces side by side, which a transposing read takes.
+template <int DK>
+__host__ __device__ constexpr int la_place(int row, int piece)
+{
+    return piece ^ (DK == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3));
+}
 // What a chunk has for each head: (I + L)^-1 and P [LA_TRI][parts], then rows of 64 that the chunk's tokens are
 // multiplied by.
 template <class T>
@@ -282,7 +267,7 @@ struct LaSum {
 template <int N>
 __device__ __forceinline__ void la_load(const uint8_t *p, bf168 (&o)[N])
 {
-    const int at = lane_id() * 16;
+    const uint32_t at = (uint32_t)lane_id() * 16;
 #pragma unroll
     for (int i = 0; i < N; i++) o[i] = *(const QMAG_GLOBAL bf168 *)(p + i * LA_FRAG + at);
 }
@@ -344,6 +329,29 @@ __device__ int la_first_tile(const LaArgs &A, int seq, int first)
     return la_tile0(first, A.r0, rank);
 }
 
+// Token by token: whole calls, or what the walk down a window's chunks leaves, sequences of few rows and those with
+// values that its products do not hold, from their first row on.
+template <class T, int DK, bool DELTA, bool REST>
+__global__ void __launch_bounds__(LA_WG) linattn_step_kernel(LaArgs A)
+{
+    const int slices = A.dim_v / 16;
+    const int64_t jobs = (int64_t)A.n_seq * A.n_head * slices;
+    for (int64_t j = (int64_t)blockIdx.x * (LA_WG / 64) + (threadIdx.x >> 6); j < jobs; j += (int64_t)gridDim.x * (LA_WG / 64)) {
+        const int64_t sh = j / slices;
+        const int seq = __builtin_amdgcn_readfirstlane((int)(sh / A.n_head)), head = __builtin_amdgcn_readfirstlane((int)(sh % A.n_head));
+        const int c0 = __builtin_amdgcn_readfirstlane((int)(j % slices) * 16);
+        const LaRows rows = la_rows(ldg(A.cu + seq), ldg(A.cu + seq + 1), A.T, A.r0, A.r1);
+        if (rows.n <= 0) continue;
+        int quiet = 0;
+        if (REST && la_long(rows.n)) {
+            const int tile0 = la_first_tile(A, seq, rows.first);
+            if (la_room(tile0, seq_tiles(rows.n, LA_SHIFT), A.n_tile)) quiet = ldg(A.left + ((int64_t)tile0 * A.n_head + head) * slices + c0 / 16);
+            if (quiet < 0) continue;
+        }
+        la_recurrence<T, DK, DELTA>(A, head, c0, rows.first, rows.n, quiet, la_state(A, seq, head, DK, rows.begun, rows.goes_on));
+    }
+}
+
 // What a chunk of a key head and its heads has that does not depend on the state: a wave takes 16 of the chunk's rows.
 // Products of rows j with rows i leave lane group g with j = 4 g .. of a row i: as P and the inverse are operands.
 template <class T, int DK, bool DELTA>
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
 #pragma unroll
         for (int p = 0; p < NP; p++) {
             *(bf168 *)&s_k[p][my][32 * kb + 8 * g] = kf[kb][p];
-            *(QMAG_GLOBAL bf168 *)(mine + p * LaKeys<T, DK>::PLANE + my * DK * 2 + la_place(my, 4 * kb + g) * 16) = kf[kb][p];
+            *(QMAG_GLOBAL bf168 *)(mine + p * LaKeys<T, DK>::PLANE + my * DK * 2 + la_place<DK>(my, 4 * kb + g) * 16) = kf[kb][p];
         }
         la_store<NP>(mine + LaKeys<T, DK>::Q + (w * NKB + kb) * NP * LA_FRAG, qf[kb]);
     }
@@ -544,33 +552,23 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
     }
 }
 
-// Down a sequence's chunks: one head, 16 columns of the state, by 12 waves.  Waves 0 .. 3 form U and the next state, 16
-// of the chunk's rows and a quarter of the state's each; waves 4 .. 7 the results; what a wave forms the others take
-// from LDS as operands.  Waves 8 .. 11 bring LDS what the first four read of a chunk, ahead of them: a CU takes in some
-// 40 bytes a clock, and a wave that asks for its own operands waits in line with all others.
+// Down a sequence's chunks: one head, 16 columns of the state, by 8 waves.  Waves 0 .. 3 form U and the next state, 16
+// of the chunk's rows and a quarter of the state's each; what a wave forms the others take from LDS as operands.  Waves
+// 4 .. 7 form the results, and bring LDS what the first four read of a chunk, ahead of them: a CU takes in some 40
+// bytes a clock, and a wave that asks for its own operands waits in line with all others.
 template <class T, int DK>
 struct LaRoom {
-    static constexpr int K = LaKeys<T, DK>::Q, REST = LA_TRI * 3 * LA_FRAG + DK / 32 * 3 * LA_FRAG + 2 * (6 + LA_OUT_PARTS<T>) * LA_FRAG + 5 * LA_FRAG + 64;
+    static constexpr int K = LaKeys<T, DK>::Q, REST = DK / 32 * 3 * LA_FRAG + 2 * (6 + LA_OUT_PARTS<T>) * LA_FRAG + 5 * LA_FRAG + 64;
     static constexpr int BUFS = 2 * K + REST <= 160 * 1024 ? 2 : 1;      // chunks of K in LDS
-    static constexpr bool OVER = K + REST > 160 * 1024;                  // a chunk's V lies where its U goes
+    // two workgroups to a CU, where their LDS allows it: each waits most of its time for a product or a move through LDS
+    static constexpr int WGS = 2 * (2 * K + REST) <= 160 * 1024 ? 2 : 1;
 };
 
-// A loader's waits: all but the last N of its loads are there, and its writes to LDS; then the workgroup's barrier.
-// (An ordinary one would wait for every load to LDS.)
-__device__ __forceinline__ uint32_t la_lds(const void *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p; }
-__device__ __forceinline__ void la_write(uint8_t *to, f32x4 v) { asm volatile("ds_write_b128 %0, %1" ::"v"(la_lds(to)), "v"(v) : "memory"); }
 // a value as if it were new in every turn of a loop, so that places formed from it are not kept (and then spilled)
-__device__ __forceinline__ void la_fresh(int &v) { asm volatile("" : "+v"(v)); }
-template <int N>
-__device__ __forceinline__ void la_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void la_bring(const uint8_t *from, uint8_t *to)
-{
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(from + lane_id() * 16),
-                                     (__attribute__((address_space(3))) void *)to, 16, 0, 0);
-}
+__device__ __forceinline__ void la_fresh(uint32_t &v) { asm volatile("" : "+v"(v)); }
 
 template <class T, int DK, bool DELTA>
-__global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
+__global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_kernel(LaArgs A)
 {
     using S = typename T::S;
     using Y = LaLayout<T>;
@@ -579,15 +577,14 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
     constexpr int NP = LA_PARTS<T>, NKB = DK / 32, NO = LA_OUT_PARTS<T>, UP = NO - 1, BUFS = M::BUFS;
     constexpr int OWN = (NKB + 3) / 4;                    // blocks of 32 rows of the state that a wave holds
     __shared__ __attribute__((aligned(16))) uint8_t s_k[BUFS][X::Q];
-    __shared__ __attribute__((aligned(16))) uint8_t s_t[DELTA ? LA_TRI * 3 : 1][LA_FRAG], s_s[NKB][3][LA_FRAG];
+    __shared__ __attribute__((aligned(16))) uint8_t s_s[NKB][3][LA_FRAG];
     __shared__ __attribute__((aligned(16))) uint8_t s_x[DELTA ? 2 : 1][3][LA_FRAG], s_u[2][NO][LA_FRAG], s_e[2][3][LA_FRAG];
-    __shared__ __attribute__((aligned(16))) float s_in[M::OVER ? 1 : 1280];
-    float *const s_vec = M::OVER ? (float *)s_u : s_in, *const s_v = s_vec + 256;
+    __shared__ __attribute__((aligned(16))) float s_vec[256], s_v[1024];
     __shared__ __attribute__((aligned(16))) int s_bad[4];         // each wave's first row that the form does not hold, 64: none
     const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4, g4 = g * 4;
-    const bool chain = w < 4, loader = w >= 8;
+    const bool chain = w < 4;
     const int rt = w & 3;
-    int at = lane * 16, half = at + 8 * (rt & 1);
+    uint32_t at = lane * 16, half = at + 8 * (rt & 1);
     // workgroups go round the 8 XCDs: the slices of a key head's heads on one of them, a sequence's key heads on all
     const int slices = A.dim_v / 16, each = A.n_head / A.n_key * slices;
     const int64_t units = (int64_t)A.n_seq * A.n_key, jobs = (units + 7) / 8 * 8 * each;
@@ -596,16 +593,14 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
         if (unit >= units) continue;
         const int seq = (int)(unit / A.n_key), key = (int)(unit % A.n_key), part = (int)((b >> 3) % each);
         const int head = la_head_of(A, key, part / slices), c0 = part % slices * 16;
-        const LaRows rows = la_rows(ldg(A.cu + seq), ldg(A.cu + seq + 1), A.T, A.r0, A.r1);
+        // (what the workgroup has in common in scalar registers, places formed from it too)
+        const LaRows rows = la_rows(la_one(ldg(A.cu + seq)), la_one(ldg(A.cu + seq + 1)), A.T, A.r0, A.r1);
         if (rows.n <= 0) continue;
         const LaState st = la_state(A, seq, head, DK, rows.begun, rows.goes_on);
         __syncthreads();                                  // the job before has left LDS
-        const int chunks = seq_tiles(rows.n, LA_SHIFT), tile0 = la_long(rows.n) ? la_first_tile(A, seq, rows.first) : 0;
+        const int chunks = seq_tiles(rows.n, LA_SHIFT), tile0 = la_one(la_long(rows.n) ? la_first_tile(A, seq, rows.first) : 0);
         // (sequences that lap over one another may have more chunks than the host counts)
-        if (!la_long(rows.n) || !la_room(tile0, chunks, A.n_tile)) {
-            if (w == 0) la_recurrence<T, DK, DELTA>(A, head, c0, rows.first, rows.n, st);
-            continue;
-        }
+        if (!la_long(rows.n) || !la_room(tile0, chunks, A.n_tile)) continue;
         // a wave's block kb of the state holds rows 32 kb + 8 g + 4 h + r
         f32x4 s[OWN][2];
         bool odd = false;
@@ -642,74 +637,20 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
         auto keys = [&](int i) { return A.keys + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_key + key) * X::BYTES; };
         // a row of chunk i, or the sequence's last
         auto row_of = [&](int i, int row) { return (int64_t)rows.first + min(64 * i + row, rows.n - 1); };
-        if (loader && go) {
-            constexpr int MINE = X::Q / LA_FRAG / 4, MINE_T = DELTA ? (LA_TRI * 3 + 3) / 4 : 0, MINE_V = 5;      // loads of a loader
-            float v[4];
-            f32x4 vec;
-            auto bring_k = [&](int i) {
+        if (chain && go) {
+            // places in K that differ by more than a constant: a row's blocks, the wave's rows of K^T
+            constexpr int KINDS = NKB < 4 ? NKB : 4;
+            int row_at[KINDS];
 #pragma unroll
-                for (int u = 0; u < MINE; u++) la_bring(keys(i) + (rt + 4 * u) * LA_FRAG, s_k[i % BUFS] + (rt + 4 * u) * LA_FRAG);
-            };
-            auto bring_t = [&](int i) {
+            for (int i = 0; i < KINDS; i++) row_at[i] = (16 * rt + l16) * DK * 2 + la_place<DK>(l16, 4 * i + g) * 16;
+            bf168 tf[2][3];                               // the wave's rows of the inverse, a chunk ahead
+            auto ask_t = [&](int i) {
 #pragma unroll
-                for (int u = 0; u < MINE_T; u++) {
-                    const int f = min(rt + 4 * u, LA_TRI * 3 - 1);
-                    la_bring(heads(i) + Y::TI + f * LA_FRAG, s_t[f]);
-                }
+                for (int tb = 0; tb < 2; tb++) la_load<3>(heads(i) + Y::TI + la_tri(rt, rt < 2 ? 0 : tb) * 3 * LA_FRAG, tf[tb]);
             };
-            auto ask = [&](int i) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) v[r] = T::up(*(const QMAG_GLOBAL S *)((const S *)A.v.p + row_of(i, 16 * rt + g4 + r) * A.v.ts + head * A.v.hs + c0 + l16));
-                vec = *(const QMAG_GLOBAL f32x4 *)(heads(i) + Y::VEC + at);
-            };
-            auto put = [&]() {
-                la_write((uint8_t *)&s_v[256 * rt + 4 * lane], f32x4{v[0], v[1], v[2], v[3]});
-                if (rt == 0) la_write((uint8_t *)&s_vec[4 * lane], vec);
-            };
-            ask(0);
-            put();
-            bring_k(0);
-            bring_t(0);
-            ask(1);
-            la_meet<0>();
-            for (; c < chunks; c++) {
-                if constexpr (BUFS == 2) bring_k(c + 1);
-                if constexpr (DELTA) {
-                    la_meet<BUFS == 2 ? MINE : 0>();      // the inverse is there; V and what it is multiplied by are taken next
-                    if constexpr (BUFS == 2) {
-                        put();
-                        ask(c + 2);
-                    }
-                }
-                la_meet<63>();
-                // (an ordinary read of LDS would wait for all that is on its way there)
-                int4 bad;
-                asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(bad) : "v"(la_lds(s_bad)) : "memory");
-                upto = min(min(bad.x, bad.y), min(bad.z, bad.w));
-                if (upto < 64) break;
-                if constexpr (!DELTA && BUFS == 2) {
-                    put();
-                    ask(c + 2);
-                }
-                bring_t(c + 1);
-                if constexpr (BUFS == 2) {
-                    la_meet<MINE_T + MINE_V>();           // K is there
-                } else {
-                    la_meet<63>();
-                    put();
-                    ask(c + 2);
-                    bring_k(c + 1);
-                    la_meet<0>();
-                }
-            }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        } else if (chain && go) {
-            // places in K that differ by more than a constant: a row's even and odd blocks, the wave's rows of K^T
-            int row_at[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) row_at[i] = (16 * rt + l16) * DK * 2 + la_place(l16, 4 * i + g) * 16;
-            const int own = min(rt, NKB - 1), tok = g4 + (l16 >> 2);
-            const int col_at = tok * DK * 2 + (own >> 1) * 128 + la_place(tok, 4 * (own & 1) + (l16 & 3)) * 16;
+            if constexpr (DELTA) ask_t(0);
+            const int tok = g4 + (l16 >> 2);
+            const int col_at = tok * DK * 2 + la_place<DK>(tok, 4 * min(rt, NKB - 1) + (l16 & 3)) * 16;
             __syncthreads();
             for (; c < chunks; c++) {
                 la_fresh(at);
@@ -726,7 +667,7 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
 #pragma unroll
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
 #pragma unroll
-                        for (int i = 0; i < NP; i++) a[i] = *(const bf168 *)(K + row_at[kb & 1] + i * X::PLANE + (kb >> 1) * 128);
+                        for (int i = 0; i < NP; i++) a[i] = *(const bf168 *)(K + row_at[kb % KINDS] + i * X::PLANE + kb / KINDS * 256);
                         ks[kb & 1].add(a, b);
                     }
                     acc = ks[0].sum() + ks[1].sum();
@@ -750,7 +691,7 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
 #pragma unroll
                     for (int i = 0; i < 3; i++) *(s16x4 *)&s_x[rt >> 1][i][half] = *(const s16x4 *)p[i];
                 }
-                bad = group_min_i<64>(bad);
+                if (__ballot(bad < 64)) bad = group_min_i<64>(bad);
                 if (lane == 0) s_bad[rt] = bad;
                 if constexpr (DELTA) {
                     __syncthreads();
@@ -760,13 +701,12 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
 #pragma unroll
                     for (int tb = 0; tb < 2; tb++) {
                         if (2 * tb > rt) continue;
-                        bf168 a[3], b[3];
+                        bf168 b[3];
 #pragma unroll
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_x[tb][i][at];
-#pragma unroll
-                        for (int i = 0; i < 3; i++) a[i] = *(const bf168 *)&s_t[la_tri(rt, tb) * 3 + i][at];
-                        us[tb].add(a, b);
+                        us[tb].add(tf[tb], b);
                     }
+                    ask_t(c + 1);
                     const f32x4 u = us[0].sum() + us[1].sum();
 #pragma unroll
                     for (int r = 0; r < 4; r++) x[r] = u[r];
@@ -824,8 +764,13 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
                 if constexpr (BUFS == 1) __syncthreads();
             }
         } else if (go) {
+            // All that a chunk is taken from is asked for a chunk and more ahead, and goes on to LDS as soon as its
+            // place there is free: K beside the last one's, V and what it is multiplied by once the first barrier has
+            // passed.
+            constexpr int MINE = X::Q / LA_FRAG / 4;
             bf168 qf[NKB][NP], pf[2][NO];
-            f32x4 qd;
+            f32x4 qd, kr[MINE], vec;
+            float v[4];
             auto ask_q = [&](int i) {
                 const uint8_t *p = keys(i) + X::Q + rt * NKB * NP * LA_FRAG;
 #pragma unroll
@@ -833,12 +778,35 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
             };
             auto ask_p = [&](int i) {
                 const uint8_t *p = heads(i);
-                qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::QD + 4 * (16 * rt + g4));
+                qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::QD + 64 * rt + (uint32_t)(4 * g4));
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) la_load<NO>(p + Y::P + la_tri(rt, rt < 2 ? 0 : tb) * NO * LA_FRAG, pf[tb]);
             };
+            auto ask_k = [&](int i) {
+#pragma unroll
+                for (int u = 0; u < MINE; u++) kr[u] = *(const QMAG_GLOBAL f32x4 *)(keys(i) + (rt + 4 * u) * LA_FRAG + (uint32_t)at);
+            };
+            auto put_k = [&](int i) {
+#pragma unroll
+                for (int u = 0; u < MINE; u++) *(f32x4 *)(s_k[i % BUFS] + (rt + 4 * u) * LA_FRAG + at) = kr[u];
+            };
+            auto ask_v = [&](int i) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[r] = T::up(*(const QMAG_GLOBAL S *)((const S *)A.v.p + row_of(i, 16 * rt + g4 + r) * A.v.ts + head * A.v.hs + c0 + l16));
+                vec = *(const QMAG_GLOBAL f32x4 *)(heads(i) + Y::VEC + (uint32_t)at);
+            };
+            auto put_v = [&]() {
+                *(f32x4 *)&s_v[256 * rt + 4 * lane] = f32x4{v[0], v[1], v[2], v[3]};
+                if (rt == 0) *(f32x4 *)&s_vec[4 * lane] = vec;
+            };
+            ask_k(0);
+            ask_v(0);
             ask_q(0);
             ask_p(0);
+            put_k(0);
+            put_v();
+            ask_k(1);
+            ask_v(1);
             __syncthreads();
             for (; c < chunks; c++) {
                 la_fresh(at);
@@ -856,7 +824,17 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
                 }
                 ask_q(c + 1);
                 f32x4 o = (qs[0].sum() + qs[1].sum()) * qd;
-                if constexpr (DELTA) __syncthreads();
+                if constexpr (BUFS == 2) {
+                    put_k(c + 1);
+                    ask_k(c + 2);
+                }
+                if constexpr (DELTA) {
+                    __syncthreads();
+                    if constexpr (BUFS == 2) {
+                        put_v();
+                        ask_v(c + 2);
+                    }
+                }
                 __syncthreads();
                 upto = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
 #pragma unroll
@@ -868,6 +846,10 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
                     ps[tb].add(pf[tb], b);
                 }
                 ask_p(c + 1);
+                if constexpr (!DELTA && BUFS == 2) {
+                    put_v();
+                    ask_v(c + 2);
+                }
                 o += ps[0].sum() + ps[1].sum();
                 const int t = 64 * c + 16 * rt + g4, to = min(rows.n, 64 * c + upto);
                 S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + l16;
@@ -876,28 +858,18 @@ __global__ void __launch_bounds__(768) linattn_chain_kernel(LaArgs A)
                     if (t + r < to) p[r * A.ots] = T::down(o[r]);
                 if (upto < 64) break;
                 __syncthreads();
-                if constexpr (BUFS == 1) __syncthreads();
+                if constexpr (BUFS == 1) {
+                    put_k(c + 1);
+                    put_v();
+                    ask_k(c + 2);
+                    ask_v(c + 2);
+                    __syncthreads();
+                }
             }
         }
-        if (c < chunks) {
-            // a row with values that the products do not hold, or a state: from there on token by token
-            static_assert(sizeof(s_s) >= DK * 16 * sizeof(float), "room for the state");
-            float (*hand)[16] = (float (*)[16])s_s;
-            __syncthreads();
-#pragma unroll
-            for (int o = 0; o < OWN; o++)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (chain && rt + 4 * o < NKB) hand[32 * (rt + 4 * o) + 8 * g + 4 * h + r][l16] = s[o][h][r];
-            __syncthreads();
-            if (w == 0)
-                la_recurrence<T, DK, DELTA>(A, head, c0, rows.first + 64 * c, rows.n - 64 * c, upto, [&](int row, float (&x)[4]) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = hand[row][g4 + e];
-                }, st.to);
-        } else if (chain && st.to) {
+        // a row with values that the products do not hold, or a state: all is left as it was from there on
+        if (threadIdx.x == 0) A.left[((int64_t)tile0 * A.n_head + head) * slices + c0 / 16] = c < chunks ? 64 * c + upto : -1;
+        if (c >= chunks && chain && st.to) {
 #pragma unroll
             for (int o = 0; o < OWN; o++)
 #pragma unroll
@@ -927,7 +899,7 @@ static size_t la_tile_bytes(int type, int dim_k, int n_key, int n_head)
     with_type(type, [&](auto t) {
         return with_dim_k(dim_k, [&](auto d) {
             using TT = decltype(t);
-            bytes = (size_t)n_key * LaKeys<TT, decltype(d)::value>::BYTES + (size_t)n_head * LaLayout<TT>::HEAD_BYTES;
+            bytes = (size_t)n_key * LaKeys<TT, decltype(d)::value>::BYTES + (size_t)n_head * (LaLayout<TT>::HEAD_BYTES + 64);
             return 0;
         });
     });
@@ -988,7 +960,7 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
     A.slot = a->n_slot ? slot : nullptr, A.len = len, A.cu = cu;
     A.n_head = a->n_head, A.n_key = q->n_head, A.share = a->n_head / q->n_head, A.turns = a->turns;
     A.dim_v = a->dim_v, A.n_slot = a->n_slot, A.n_seq = n_seq, A.T = T;
-    A.norm_eps = a->norm_eps, A.scale = scale;
+    A.norm_eps = a->norm_eps, A.scale = scale, A.r1 = T;
     DeviceScope dev;
     if (dev.st) return dev.st;
     hipStream_t s = ctx().stream;
@@ -1013,11 +985,11 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
         return with_dim_k(a->dim_k, [&](auto d) {
             using TT = decltype(t);
             constexpr int DK = decltype(d)::value;
+            const int64_t step_wgs = (slices + LA_WG / 64 - 1) / (LA_WG / 64);
+            const unsigned steps = (unsigned)(step_wgs < 1 << 23 ? step_wgs : 1 << 23);
             if (!chunks) {
-                const int64_t wgs = (slices + LA_WG / 64 - 1) / (LA_WG / 64);
-                const unsigned grid = (unsigned)(wgs < 1 << 23 ? wgs : 1 << 23);
-                if (a->delta) linattn_step_kernel<TT, DK, true><<<grid, LA_WG, 0, s>>>(A);
-                else linattn_step_kernel<TT, DK, false><<<grid, LA_WG, 0, s>>>(A);
+                if (a->delta) linattn_step_kernel<TT, DK, true, false><<<steps, LA_WG, 0, s>>>(A);
+                else linattn_step_kernel<TT, DK, false, false><<<steps, LA_WG, 0, s>>>(A);
                 return 0;
             }
             float *carry = (float *)A.carry_in;
@@ -1028,15 +1000,18 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
                 A.r1 = (int)(r0 + window < T ? r0 + window : T);
                 A.n_tile = la_most_tiles(A.r1 - A.r0, n_seq);
                 A.heads = A.keys + (size_t)A.n_tile * (size_t)A.n_key * LaKeys<TT, DK>::BYTES;
+                A.left = (int *)(A.heads + (size_t)A.n_tile * (size_t)A.n_head * LaLayout<TT>::HEAD_BYTES);
                 A.carry_in = carry + (odd ? state / sizeof(float) : 0);
                 A.carry_out = carry + (odd ? 0 : state / sizeof(float));
                 const unsigned tiles = (unsigned)A.n_tile * (unsigned)A.n_key;
                 if (a->delta) {
                     linattn_chunk_kernel<TT, DK, true><<<tiles, 256, 0, s>>>(A);
-                    linattn_chain_kernel<TT, DK, true><<<grid, 768, 0, s>>>(A);
+                    linattn_chain_kernel<TT, DK, true><<<grid, 512, 0, s>>>(A);
+                    linattn_step_kernel<TT, DK, true, true><<<steps, LA_WG, 0, s>>>(A);
                 } else {
                     linattn_chunk_kernel<TT, DK, false><<<tiles, 256, 0, s>>>(A);
-                    linattn_chain_kernel<TT, DK, false><<<grid, 768, 0, s>>>(A);
+                    linattn_chain_kernel<TT, DK, false><<<grid, 512, 0, s>>>(A);
+                    linattn_step_kernel<TT, DK, false, true><<<steps, LA_WG, 0, s>>>(A);
                 }
             }
             return 0;
