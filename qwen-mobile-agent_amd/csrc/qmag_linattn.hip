@@ -796,8 +796,8 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 vec = *(const QMAG_GLOBAL f32x4 *)(heads(i) + Y::VEC + (uint32_t)at);
             };
             auto put_v = [&]() {
-                *(f32x4 *)&s_v[256 * rt + 4 * lane] = f32x4{v[0], v[1], v[2], v[3]};
-                if (rt == 0) *(f32x4 *)&s_vec[4 * lane] = vec;
+                *(f32x4 *)((uint8_t *)s_v + 1024 * rt + at) = f32x4{v[0], v[1], v[2], v[3]};
+                if (rt == 0) *(f32x4 *)((uint8_t *)s_vec + at) = vec;
             };
             ask_k(0);
             ask_v(0);
