@@ -24,21 +24,21 @@ struct ConvArgs {
     int n_channel, n_slot, n_seq, T, shift, n_tile, across, silu;
 };
 
-// the n <= V values from p, the others zero
-template <class T, int V>
+// V values from p, or only the first n of them, the others zero
+template <class T, int V, bool FULL>
 __device__ __forceinline__ void load_some(const typename T::S *p, int n, float (&o)[V])
 {
-    if (n == V) {
+    if constexpr (FULL) {
         load_row<T, V>(p, o);
     } else {
 #pragma unroll
         for (int i = 0; i < V; i++) o[i] = i < n ? T::up(p[i]) : 0.0f;
     }
 }
-template <class T, int V>
+template <class T, int V, bool FULL>
 __device__ __forceinline__ void store_some(typename T::S *p, int n, const float (&v)[V])
 {
-    if (n == V) {
+    if constexpr (FULL) {
         store_row<T, V>(p, v);
     } else {
 #pragma unroll
@@ -54,86 +54,92 @@ __device__ __forceinline__ float conv_silu(float y)
     return (y * 0x1p-64f) * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(y * -1.44269504088896340736f), 0x1p-64f, 0x1p-64f));
 }
 
-template <class T, int W>
-__global__ void __launch_bounds__(256) conv_kernel(ConvArgs A)
+// a tile's channels from c0 on: V of them, or the row's last nc
+template <class T, int W, bool FULL>
+__device__ __forceinline__ void conv_tile(const ConvArgs &A, const SeqTile &s, int c0, int nc)
 {
     using S = typename T::S;
     constexpr int V = 16 / (int)sizeof(S), AT_ONCE = 4;
-    const int c0 = (int)(blockIdx.x % A.across * blockDim.x + threadIdx.x) * V;
-    if (c0 >= A.n_channel) return;
-    const int nc = min(V, A.n_channel - c0);
-    float w[V][W], bias[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        bias[i] = A.bias && i < nc ? A.bias[c0 + i] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; k++) w[i][k] = i < nc ? A.weight[(int64_t)(c0 + i) * W + k] : 0.0f;
-    }
     const S *x = (const S *)A.x + c0;
     S *out = (S *)A.out + c0;
     const int tokens = 1 << A.shift;
-    for (int j = blockIdx.x / A.across; j < A.n_tile; j += gridDim.x / A.across) {
-        const SeqTile s = seq_find([&](int i) { return ldg(A.cu + i); }, A.n_seq, A.T, A.shift, j);
-        if (s.seq < 0) continue;
-        const int64_t row = (int64_t)s.first + ((int64_t)s.tile << A.shift);
-        const int n = min(tokens, s.n - (s.tile << A.shift));
-        const int slot = A.slot ? ldg(A.slot + s.seq) : -1;
-        const bool held = s.tile == 0 && slot >= 0 && slot < A.n_slot;
-        float *state = A.state + (int64_t)(held ? slot : 0) * (W - 1) * A.n_channel + c0;
-        float past[W - 1][V];
-        if (s.tile > 0) {
+    const int64_t row = (int64_t)s.first + ((int64_t)s.tile << A.shift);
+    const int n = min(tokens, s.n - (s.tile << A.shift));
+    float v[AT_ONCE][V], past[W - 1][V], w[V * W], bias[V];
 #pragma unroll
-            for (int k = 0; k < W - 1; k++) load_some<T, V>(x + (row - (W - 1) + k) * A.xs, nc, past[k]);
-        } else if (held && !(A.len && ldg(A.len + s.seq) <= 0)) {
+    for (int u = 0; u < AT_ONCE; u++) load_some<T, V, FULL>(x + (row + min(u, n - 1)) * A.xs, nc, v[u]);
+    load_some<TF32, V * W, FULL>(A.weight + (int64_t)c0 * W, nc * W, w);
+    if (A.bias) {
+        load_some<TF32, V, FULL>(A.bias + c0, nc, bias);
+    } else {
 #pragma unroll
-            for (int k = 0; k < W - 1; k++) load_some<TF32, V>(state + (int64_t)k * A.n_channel, nc, past[k]);
-        } else {
+        for (int i = 0; i < V; i++) bias[i] = 0.0f;
+    }
+    const int slot = A.slot ? __builtin_amdgcn_readfirstlane(ldg(A.slot + s.seq)) : -1;
+    const bool held = s.tile == 0 && slot >= 0 && slot < A.n_slot;
+    float *state = A.state + (int64_t)(held ? slot : 0) * (W - 1) * A.n_channel + c0;
+    if (s.tile > 0) {
+#pragma unroll
+        for (int k = 0; k < W - 1; k++) load_some<T, V, FULL>(x + (row - (W - 1) + k) * A.xs, nc, past[k]);
+    } else if (held && !(A.len && __builtin_amdgcn_readfirstlane(ldg(A.len + s.seq)) <= 0)) {
+#pragma unroll
+        for (int k = 0; k < W - 1; k++) load_some<TF32, V, FULL>(state + (int64_t)k * A.n_channel, nc, past[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < W - 1; k++)
+#pragma unroll
+            for (int i = 0; i < V; i++) past[k][i] = 0.0f;
+    }
+    for (int t0 = 0; t0 < n; t0 += AT_ONCE) {
+        // (asked for behind the tile's end too, its last row: a load in a branch is waited for at the branch's end)
+        float next[AT_ONCE][V];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) load_some<T, V, FULL>(x + (row + min(t0 + AT_ONCE + u, n - 1)) * A.xs, nc, next[u]);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) {
+            if (t0 + u >= n) break;
+            float y[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                float a = bias[i];
+#pragma unroll
+                for (int k = 0; k < W - 1; k++) a = fmaf(w[i * W + k], past[k][i], a);
+                a = fmaf(w[i * W + W - 1], v[u][i], a);
+                y[i] = A.silu ? conv_silu(a) : a;
+#pragma unroll
+                for (int k = 0; k + 1 < W - 1; k++) past[k][i] = past[k + 1][i];
+                past[W - 2][i] = v[u][i];
+            }
+            store_some<T, V, FULL>(out + (row + t0 + u) * A.os, nc, y);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+            for (int i = 0; i < V; i++) v[u][i] = next[u][i];
+    }
+    if (held) {
+        // a sequence longer than its first tile: its last rows; else what the tile ends with
+        if (s.n > tokens) {
 #pragma unroll
             for (int k = 0; k < W - 1; k++)
-#pragma unroll
-                for (int i = 0; i < V; i++) past[k][i] = 0.0f;
+                load_some<T, V, FULL>(x + ((int64_t)s.first + s.n - (W - 1) + k) * A.xs, nc, past[k]);
         }
-        float v[AT_ONCE][V];
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; u++) load_some<T, V>(x + (row + min(u, n - 1)) * A.xs, nc, v[u]);
-        for (int t0 = 0; t0 < n; t0 += AT_ONCE) {
-            float next[AT_ONCE][V];
-            if (t0 + AT_ONCE < n) {
-#pragma unroll
-                for (int u = 0; u < AT_ONCE; u++) load_some<T, V>(x + (row + min(t0 + AT_ONCE + u, n - 1)) * A.xs, nc, next[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; u++) {
-                if (t0 + u >= n) break;
-                float y[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    float a = bias[i];
-#pragma unroll
-                    for (int k = 0; k < W - 1; k++) a = fmaf(w[i][k], past[k][i], a);
-                    a = fmaf(w[i][W - 1], v[u][i], a);
-                    y[i] = A.silu ? conv_silu(a) : a;
-#pragma unroll
-                    for (int k = 0; k + 1 < W - 1; k++) past[k][i] = past[k + 1][i];
-                    past[W - 2][i] = v[u][i];
-                }
-                store_some<T, V>(out + (row + t0 + u) * A.os, nc, y);
-            }
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; u++)
-#pragma unroll
-                for (int i = 0; i < V; i++) v[u][i] = next[u][i];
-        }
-        if (held) {
-            // a sequence longer than its first tile: its last rows; else what the tile ends with
-            if (s.n > tokens) {
-#pragma unroll
-                for (int k = 0; k < W - 1; k++)
-                    load_some<T, V>(x + ((int64_t)s.first + s.n - (W - 1) + k) * A.xs, nc, past[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < W - 1; k++) store_some<TF32, V>(state + (int64_t)k * A.n_channel, nc, past[k]);
-        }
+        for (int k = 0; k < W - 1; k++) store_some<TF32, V, FULL>(state + (int64_t)k * A.n_channel, nc, past[k]);
+    }
+}
+
+template <class T, int W>
+__global__ void __launch_bounds__(256) conv_kernel(ConvArgs A)
+{
+    constexpr int V = 16 / (int)sizeof(typename T::S);
+    const int c0 = (int)(blockIdx.x % A.across * blockDim.x + threadIdx.x) * V;
+    for (int j = blockIdx.x / A.across; j < A.n_tile; j += gridDim.x / A.across) {
+        const SeqTile s = seq_find([&](int i) { return ldg(A.cu + i); }, [&](auto f) { return __ballot(f(lane_id())); },
+                                   A.n_seq, A.T, A.shift, j);
+        if (s.seq < 0) continue;
+        if (c0 + V <= A.n_channel) conv_tile<T, W, true>(A, s, c0, V);
+        else if (c0 < A.n_channel) conv_tile<T, W, false>(A, s, c0, A.n_channel - c0);
     }
 }
 

@@ -26,15 +26,21 @@ struct SeqTile {
 };
 
 // Tile number j: the last sequence that begins at or ahead of it, if it reaches j.
-// n_seq >= 1; cu(i) gives the sum at i.
-template <class F>
-constexpr SeqTile seq_find(F cu, int n_seq, int T, int shift, int j)
+// n_seq >= 1; cu(i) gives the sum at i, vote(f) the bits f(0) .. f(63), all of which a
+// wave asks at once: 4096 sequences in two rounds.
+template <class F, class V>
+constexpr SeqTile seq_find(F cu, V vote, int n_seq, int T, int shift, int j)
 {
-    int lo = 0, hi = n_seq - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (seq_tile0(seq_row(cu(mid), T), mid, shift) <= j) lo = mid;
-        else hi = mid - 1;
+    int lo = 0;
+    for (int left = n_seq; left > 1;) {
+        const int step = (left - 1) / 64 + 1;
+        const uint64_t ahead = vote([&](int i) {
+            const int at = lo + (i * step < left ? i * step : 0);
+            return i * step < left && seq_tile0(seq_row(cu(at), T), at, shift) <= j;
+        });
+        const int hit = ahead ? 63 - __builtin_clzll(ahead) : 0;
+        lo += hit * step;
+        left = left - hit * step < step ? left - hit * step : step;
     }
     const int first = seq_row(cu(lo), T), n = seq_row(cu(lo + 1), T) - first;
     const int tile = j - seq_tile0(first, lo, shift);

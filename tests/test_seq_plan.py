@@ -20,6 +20,11 @@ using namespace qmag;
 // stdin: calls of T shift n_seq, then cu
 int main()
 {
+    auto vote = [](auto f) {
+        uint64_t bits = 0;
+        for (int i = 0; i < 64; i++) bits |= (uint64_t)f(i) << i;
+        return bits;
+    };
     int T, shift, n;
     for (int call = 0; scanf("%d%d%d", &T, &shift, &n) == 3; call++) {
         std::vector<int> cu(n + 1), rows(T);
@@ -28,7 +33,7 @@ int main()
         for (int i = 0; i < n; i++) ascending = ascending && cu[i] <= cu[i + 1];
         const int most = seq_most_tiles(T, n, shift);
         for (int j = 0; j < most; j++) {
-            const SeqTile s = seq_find([&](int i) { return cu.at(i); }, n, T, shift, j);
+            const SeqTile s = seq_find([&](int i) { return cu.at(i); }, vote, n, T, shift, j);
             if (s.seq < 0) continue;
             if (s.seq >= n || s.tile < 0 || s.tile >= seq_tiles(s.n, shift) || s.first < 0 || s.first + s.n > T)
                 return printf("call %d: tile %d is %d of sequence %d, rows %d + %d of %d\n", call, j, s.tile, s.seq, s.first, s.n, T), 1;
@@ -76,7 +81,7 @@ def test_ascending_sequences(walk):
         lens = r.randint(0, r.choice([2, 5, 65, 200]) + 1, n) * (r.rand(n) < 0.8)
         cu = np.concatenate([[0], np.cumsum(lens)])
         calls.append((int(cu[-1]) + r.choice([0, 0, 3]), shift, cu))
-    calls += [(64 * n, 6, np.arange(n + 1) * 64) for n in (1, 2, 63)] + [(4096, 6, np.arange(4097))]
+    calls += [(64 * n, 6, np.arange(n + 1) * 64) for n in (1, 2, 63)] + [(4096, 6, np.arange(4097)), (9000, 2, np.arange(9001)), (300, 3, np.arange(131) // 2)]
     walk(calls)
 
 
@@ -84,7 +89,7 @@ def test_sums_of_any_kind(walk):
     r = np.random.RandomState(2)
     calls = []
     for _ in range(400):
-        n, shift, T = r.randint(1, 30), r.randint(2, 7), r.randint(1, 400)
+        n, shift, T = r.randint(1, r.choice([30, 300])), r.randint(2, 7), r.randint(1, 400)
         cu = r.choice([r.randint(-T, 2 * T), 0, T, -2 ** 31, 2 ** 31 - 1], n + 1) if r.rand() < 0.3 else r.randint(-9, T + 9, n + 1)
         calls.append((T, shift, cu))
     walk(calls)
