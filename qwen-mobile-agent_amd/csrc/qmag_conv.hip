@@ -9,6 +9,12 @@
 // tile's first W - 1 rows.  Tiles are of 4 tokens or more: only a sequence's first
 // tile reaches ahead of its rows, so that the thread that reads a channel's state
 // is the one that replaces it, and no other looks at it.
+//
+// Bound by memory: 4096 tokens of 8192 fp32 channels and 4 taps take 58.5 us, of
+// which reading and writing them alone is 56 at the 4.8 TB/s of a copy; 5003 tokens
+// of 4100 bf16 channels 23.6 us (3.5 TB/s; no row begins at 16 bytes, and a tile of 8
+// tokens reads 10 rows).  Five tokens take 3.9 us, a launch and four loads that wait
+// for one another: cu, the slot, the state, the rows.
 #include "qmag_rows.h"
 #include "qmag_seq.h"
 
@@ -54,12 +60,13 @@ __device__ __forceinline__ float conv_silu(float y)
     return (y * 0x1p-64f) * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(y * -1.44269504088896340736f), 0x1p-64f, 0x1p-64f));
 }
 
-// a tile's channels from c0 on: V of them, or the row's last nc
+// a tile's channels from c0 on: V of them, or the row's last nc.  Rows are asked for 16 values ahead of those at work:
+// 32 of bf16 ones take so many registers that three waves fit where four do (26.4 us against 23.6).
 template <class T, int W, bool FULL>
 __device__ __forceinline__ void conv_tile(const ConvArgs &A, const SeqTile &s, int c0, int nc)
 {
     using S = typename T::S;
-    constexpr int V = 16 / (int)sizeof(S), AT_ONCE = 4;
+    constexpr int V = 16 / (int)sizeof(S), AT_ONCE = 16 / V;
     const S *x = (const S *)A.x + c0;
     S *out = (S *)A.out + c0;
     const int tokens = 1 << A.shift;
@@ -130,7 +137,7 @@ __device__ __forceinline__ void conv_tile(const ConvArgs &A, const SeqTile &s, i
 }
 
 template <class T, int W>
-__global__ void __launch_bounds__(256) conv_kernel(ConvArgs A)
+__global__ void __launch_bounds__(256, 4) conv_kernel(ConvArgs A)
 {
     constexpr int V = 16 / (int)sizeof(typename T::S);
     const int c0 = (int)(blockIdx.x % A.across * blockDim.x + threadIdx.x) * V;
@@ -183,10 +190,11 @@ extern "C" int qmag_conv_dev(const qmag_conv *c, int type, const void *x, int64_
     const int per = 16 / size, threads = (C + per - 1) / per;
     // workgroups of up to four waves, as few of which are empty as may be
     const int waves = (threads + 63) / 64, across = (waves + 3) / 4, wg = (waves + across - 1) / across * 64;
-    // tiles as long as leave the chip its waves
+    // tiles as long as leave the chip its waves: longer ones read fewer rows twice, shorter ones keep more loads on
+    // their way (4100 bf16 channels: 23.6 us from 4096 waves on, 26.1 from 2048, 25.2 from 8192; 8192 fp32: 58.5, 58.5, 57.7)
     while (A.shift < 5 && (int64_t)seq_most_tiles(T, n_seq, A.shift + 1) * across * (wg / 64) >= 4096) A.shift++;
     A.n_tile = seq_most_tiles(T, n_seq, A.shift);
-    A.across = across;                                // a tile's workgroups side by side: rows are read whole
+    A.across = across;                                // a tile's workgroups side by side: rows are read whole (80 us else)
     DeviceScope dev;
     if (dev.st) return dev.st;
     hipStream_t s = ctx().stream;
