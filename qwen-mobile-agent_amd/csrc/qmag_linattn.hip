@@ -53,7 +53,7 @@ struct LaArgs {
     float norm_eps, scale;
     // the chunked form
     int r0, r1;               // the window's rows
-    int n_tile;
+    int n_tile, n_long, brief;
     uint8_t *keys, *heads;    // what chunks have for each key head, and for each head
     int *left;                // [n_tile][n_head][dim_v / 16] of a sequence's first chunk: the first row the walk did not do
     const float *carry_in;    // [n_head][dim_k][dim_v]: the state of a sequence begun ahead of the window
@@ -80,10 +80,10 @@ struct LaState {
 __device__ __forceinline__ LaState la_state(const LaArgs &A, int seq, int head, int dim_k, bool begun, bool goes_on)
 {
     const int64_t size = (int64_t)dim_k * A.dim_v;
-    const int slot = A.slot ? la_one(ldg(A.slot + seq)) : -1;
+    const int slot = A.slot ? la_one(ldg(A.slot + seq)) : -1, behind = A.len ? la_one(ldg(A.len + seq)) : 1;
     float *own = slot >= 0 && slot < A.n_slot ? A.state + ((int64_t)slot * A.n_head + head) * size : nullptr;
     LaState s;
-    s.from = begun ? A.carry_in + head * size : own && !(A.len && la_one(ldg(A.len + seq)) <= 0) ? own : nullptr;
+    s.from = begun ? A.carry_in + head * size : own && behind > 0 ? own : nullptr;
     s.to = goes_on ? A.carry_out + head * size : own;
     return s;
 }
@@ -129,7 +129,7 @@ __device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int 
     load(0, x);
     for (int t = 0; t < n; t++) {
         LaToken<N> next;
-        if (t + 1 < n) load(t + 1, next);
+        load(min(t + 1, n - 1), next);
         if (A.norm_eps > 0.0f) {
             // ahead of the products: a large key's would leave fp32's range
             float kk = 0.0f, qq = 0.0f;
@@ -302,9 +302,9 @@ __device__ LaTile la_find(const LaArgs &A, int j)
         const int i = s0 + lane;
         LaRows x = {0, 0, false, false};
         if (i < A.n_seq) x = la_rows(ldg(A.cu + i), ldg(A.cu + i + 1), A.T, A.r0, A.r1);
-        const uint64_t is_long = __ballot(la_long(x.n));
+        const uint64_t is_long = __ballot(la_long(x.n, A.brief));
         const int tile0 = la_tile0(x.first, A.r0, rank + __popcll(is_long & ((1ull << lane) - 1)));
-        const uint64_t hit = __ballot(la_long(x.n) && j >= tile0 && j < tile0 + seq_tiles(x.n, LA_SHIFT));
+        const uint64_t hit = __ballot(la_long(x.n, A.brief) && j >= tile0 && j < tile0 + seq_tiles(x.n, LA_SHIFT));
         if (hit) {
             const int at = __ffsll((unsigned long long)hit) - 1;
             x.first = __builtin_amdgcn_readlane(x.first, at);
@@ -315,18 +315,36 @@ __device__ LaTile la_find(const LaArgs &A, int j)
     }
     return {{0, 0, false, false}, 0, false};
 }
-// the number of a long sequence's first chunk
-__device__ int la_first_tile(const LaArgs &A, int seq, int first)
+// how many long sequences are ahead of one
+__device__ int la_rank(const LaArgs &A, int seq)
 {
     const int lane = lane_id();
     int rank = 0;
     for (int s0 = 0; s0 < seq; s0 += 64) {
         const int i = s0 + lane;
         bool is_long = false;
-        if (i < seq) is_long = la_long(la_rows(ldg(A.cu + i), ldg(A.cu + i + 1), A.T, A.r0, A.r1).n);
+        if (i < seq) is_long = la_long(la_rows(ldg(A.cu + i), ldg(A.cu + i + 1), A.T, A.r0, A.r1).n, A.brief);
         rank += __popcll(__ballot(is_long));
     }
-    return la_tile0(first, A.r0, rank);
+    return rank;
+}
+// the long sequence that has `rank` ahead of it; -1: none
+__device__ int la_ranked(const LaArgs &A, int rank)
+{
+    const int lane = lane_id();
+    for (int s0 = 0; s0 < A.n_seq; s0 += 64) {
+        const int i = s0 + lane;
+        bool is_long = false;
+        if (i < A.n_seq) is_long = la_long(la_rows(ldg(A.cu + i), ldg(A.cu + i + 1), A.T, A.r0, A.r1).n, A.brief);
+        uint64_t m = __ballot(is_long);
+        const int n = __popcll(m);
+        if (rank < n) {
+            for (; rank > 0; rank--) m &= m - 1;
+            return s0 + __ffsll((unsigned long long)m) - 1;
+        }
+        rank -= n;
+    }
+    return -1;
 }
 
 // Token by token: whole calls, or what the walk down a window's chunks leaves, sequences of few rows and those with
@@ -334,18 +352,16 @@ __device__ int la_first_tile(const LaArgs &A, int seq, int first)
 template <class T, int DK, bool DELTA, bool REST>
 __global__ void __launch_bounds__(LA_WG) linattn_step_kernel(LaArgs A)
 {
-    const int slices = A.dim_v / 16;
-    const int64_t jobs = (int64_t)A.n_seq * A.n_head * slices;
-    for (int64_t j = (int64_t)blockIdx.x * (LA_WG / 64) + (threadIdx.x >> 6); j < jobs; j += (int64_t)gridDim.x * (LA_WG / 64)) {
-        const int64_t sh = j / slices;
-        const int seq = __builtin_amdgcn_readfirstlane((int)(sh / A.n_head)), head = __builtin_amdgcn_readfirstlane((int)(sh % A.n_head));
-        const int c0 = __builtin_amdgcn_readfirstlane((int)(j % slices) * 16);
-        const LaRows rows = la_rows(ldg(A.cu + seq), ldg(A.cu + seq + 1), A.T, A.r0, A.r1);
+    const uint32_t slices = (uint32_t)A.dim_v / 16, jobs = (uint32_t)A.n_seq * (uint32_t)A.n_head * slices;
+    for (uint32_t j = blockIdx.x * (LA_WG / 64) + (uint32_t)la_one(threadIdx.x >> 6); j < jobs; j += gridDim.x * (LA_WG / 64)) {
+        const uint32_t sh = j / slices;
+        const int seq = (int)(sh / (uint32_t)A.n_head), head = (int)(sh % (uint32_t)A.n_head), c0 = (int)(j % slices) * 16;
+        const LaRows rows = la_rows(la_one(ldg(A.cu + seq)), la_one(ldg(A.cu + seq + 1)), A.T, A.r0, A.r1);
         if (rows.n <= 0) continue;
         int quiet = 0;
-        if (REST && la_long(rows.n)) {
-            const int tile0 = la_first_tile(A, seq, rows.first);
-            if (la_room(tile0, seq_tiles(rows.n, LA_SHIFT), A.n_tile)) quiet = ldg(A.left + ((int64_t)tile0 * A.n_head + head) * slices + c0 / 16);
+        if (REST && la_long(rows.n, A.brief)) {
+            const int rank = la_rank(A, seq), tile0 = la_tile0(rows.first, A.r0, rank);
+            if (la_room(rank, tile0, seq_tiles(rows.n, LA_SHIFT), A.n_long, A.n_tile)) quiet = ldg(A.left + ((int64_t)tile0 * A.n_head + head) * slices + c0 / 16);
             if (quiet < 0) continue;
         }
         la_recurrence<T, DK, DELTA>(A, head, c0, rows.first, rows.n, quiet, la_state(A, seq, head, DK, rows.begun, rows.goes_on));
@@ -586,21 +602,20 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
     const int rt = w & 3;
     uint32_t at = lane * 16, half = at + 8 * (rt & 1);
     // workgroups go round the 8 XCDs: the slices of a key head's heads on one of them, a sequence's key heads on all
-    const int slices = A.dim_v / 16, each = A.n_head / A.n_key * slices;
-    const int64_t units = (int64_t)A.n_seq * A.n_key, jobs = (units + 7) / 8 * 8 * each;
-    for (int64_t b = blockIdx.x; b < jobs; b += gridDim.x) {
-        const int64_t unit = (b >> 3) / each * 8 + (b & 7);
+    const uint32_t slices = (uint32_t)A.dim_v / 16, each = (uint32_t)A.share * slices, units = (uint32_t)A.n_long * (uint32_t)A.n_key;
+    for (uint32_t b = blockIdx.x; b < (units + 7) / 8 * 8 * each; b += gridDim.x) {
+        const uint32_t unit = (b >> 3) / each * 8 + (b & 7);
         if (unit >= units) continue;
-        const int seq = (int)(unit / A.n_key), key = (int)(unit % A.n_key), part = (int)((b >> 3) % each);
-        const int head = la_head_of(A, key, part / slices), c0 = part % slices * 16;
+        const int rank = la_one((int)(unit / (uint32_t)A.n_key)), seq = la_one(la_ranked(A, rank));
+        if (seq < 0) break;
+        const int key = la_one((int)(unit % (uint32_t)A.n_key)), part = la_one((int)((b >> 3) % each));
+        const int head = la_head_of(A, key, part / (int)slices), c0 = la_one(part % (int)slices * 16);
         // (what the workgroup has in common in scalar registers, places formed from it too)
         const LaRows rows = la_rows(la_one(ldg(A.cu + seq)), la_one(ldg(A.cu + seq + 1)), A.T, A.r0, A.r1);
-        if (rows.n <= 0) continue;
+        const int chunks = seq_tiles(rows.n, LA_SHIFT), tile0 = la_one(la_tile0(rows.first, A.r0, rank));
+        if (!la_room(rank, tile0, chunks, A.n_long, A.n_tile)) continue;
         const LaState st = la_state(A, seq, head, DK, rows.begun, rows.goes_on);
         __syncthreads();                                  // the job before has left LDS
-        const int chunks = seq_tiles(rows.n, LA_SHIFT), tile0 = la_one(la_long(rows.n) ? la_first_tile(A, seq, rows.first) : 0);
-        // (sequences that lap over one another may have more chunks than the host counts)
-        if (!la_long(rows.n) || !la_room(tile0, chunks, A.n_tile)) continue;
         // a wave's block kb of the state holds rows 32 kb + 8 g + 4 h + r
         f32x4 s[OWN][2];
         bool odd = false;
@@ -778,7 +793,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
             };
             auto ask_p = [&](int i) {
                 const uint8_t *p = heads(i);
-                qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::QD + 64 * rt + (uint32_t)(4 * g4));
+                qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::QD + 64 * rt + (at >> 8) * 16);
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) la_load<NO>(p + Y::P + la_tri(rt, rt < 2 ? 0 : tb) * NO * LA_FRAG, pf[tb]);
             };
@@ -791,8 +806,9 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 for (int u = 0; u < MINE; u++) *(f32x4 *)(s_k[i % BUFS] + (rt + 4 * u) * LA_FRAG + at) = kr[u];
             };
             auto ask_v = [&](int i) {
+                const int row = 16 * rt + (int)(at >> 8) * 4, col = (int)(at >> 4) & 15;      // (the lane's, new in every turn)
 #pragma unroll
-                for (int r = 0; r < 4; r++) v[r] = T::up(*(const QMAG_GLOBAL S *)((const S *)A.v.p + row_of(i, 16 * rt + g4 + r) * A.v.ts + head * A.v.hs + c0 + l16));
+                for (int r = 0; r < 4; r++) v[r] = T::up(*(const QMAG_GLOBAL S *)((const S *)A.v.p + row_of(i, row + r) * A.v.ts + head * A.v.hs + c0 + col));
                 vec = *(const QMAG_GLOBAL f32x4 *)(heads(i) + Y::VEC + (uint32_t)at);
             };
             auto put_v = [&]() {
@@ -851,8 +867,8 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                     ask_v(c + 2);
                 }
                 o += ps[0].sum() + ps[1].sum();
-                const int t = 64 * c + 16 * rt + g4, to = min(rows.n, 64 * c + upto);
-                S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + l16;
+                const int t = 64 * c + 16 * rt + (int)(at >> 8) * 4, to = min(rows.n, 64 * c + upto);
+                S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + ((at >> 4) & 15);
 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (t + r < to) p[r * A.ots] = T::down(o[r]);
@@ -889,7 +905,6 @@ static int with_dim_k(int dim, F f)
     return f(std::integral_constant<int, 256>{});
 }
 
-constexpr int LA_MEAN = 16;                          // tokens to a sequence from which on a call goes in chunks
 constexpr size_t LA_WORKSPACE = (size_t)1 << 30;
 
 // bytes of the workspace for a chunk number
@@ -966,7 +981,8 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
     hipStream_t s = ctx().stream;
     const int64_t slices = (int64_t)n_seq * a->n_head * (a->dim_v / 16);
     // prompts in chunks; few tokens to a sequence one after another
-    const bool chunks = (int64_t)T > (int64_t)LA_MEAN * n_seq;
+    A.brief = la_brief(slices);
+    const bool chunks = la_cut(T, n_seq, A.brief);
     size_t state = 0;
     int window = 0;
     if (chunks) {
@@ -974,8 +990,8 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
         const size_t per = la_tile_bytes(type, a->dim_k, q->n_head, a->n_head);
         state = sizeof(float) * (size_t)a->n_head * (size_t)a->dim_k * (size_t)a->dim_v;
         window = (int)(((int64_t)T + LA_CHUNK - 1) / LA_CHUNK < (1 << 20) ? (T + LA_CHUNK - 1) / LA_CHUNK * LA_CHUNK : 1 << 26);
-        while (window > 4 * LA_CHUNK && (size_t)la_most_tiles(window, n_seq) * per > LA_WORKSPACE) window = window / (2 * LA_CHUNK) * LA_CHUNK;
-        uint8_t *p = (uint8_t *)workspace(WS_LINATTN, (size_t)la_most_tiles(window, n_seq) * per + (T > window ? 2 * state : 0), &st);
+        while (window > 4 * LA_CHUNK && (size_t)la_most_tiles(window, n_seq, A.brief) * per > LA_WORKSPACE) window = window / (2 * LA_CHUNK) * LA_CHUNK;
+        uint8_t *p = (uint8_t *)workspace(WS_LINATTN, (size_t)la_most_tiles(window, n_seq, A.brief) * per + (T > window ? 2 * state : 0), &st);
         if (st) return st;
         A.carry_in = (float *)p;
         A.keys = p + (T > window ? 2 * state : 0);
@@ -993,24 +1009,30 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
                 return 0;
             }
             float *carry = (float *)A.carry_in;
-            const int64_t wgs = ((int64_t)n_seq * q->n_head + 7) / 8 * 8 * (a->n_head / q->n_head) * (a->dim_v / 16);
-            const unsigned grid = (unsigned)(wgs < 1 << 22 ? wgs : 1 << 22);
             for (int64_t r0 = 0, odd = 0; r0 < T; r0 += window, odd ^= 1) {
                 A.r0 = (int)r0;
                 A.r1 = (int)(r0 + window < T ? r0 + window : T);
-                A.n_tile = la_most_tiles(A.r1 - A.r0, n_seq);
+                A.n_tile = la_most_tiles(A.r1 - A.r0, n_seq, A.brief);
+                A.n_long = la_most_long(A.r1 - A.r0, n_seq, A.brief);
+                // (a workgroup that finds no sequence ends: few of them, where none may be long enough)
+                const int64_t wgs = ((int64_t)A.n_long * A.n_key + 7) / 8 * 8 * A.share * (a->dim_v / 16);
+                const unsigned grid = (unsigned)(wgs < 2048 ? wgs : 2048);
                 A.heads = A.keys + (size_t)A.n_tile * (size_t)A.n_key * LaKeys<TT, DK>::BYTES;
                 A.left = (int *)(A.heads + (size_t)A.n_tile * (size_t)A.n_head * LaLayout<TT>::HEAD_BYTES);
                 A.carry_in = carry + (odd ? state / sizeof(float) : 0);
                 A.carry_out = carry + (odd ? 0 : state / sizeof(float));
                 const unsigned tiles = (unsigned)A.n_tile * (unsigned)A.n_key;
                 if (a->delta) {
-                    linattn_chunk_kernel<TT, DK, true><<<tiles, 256, 0, s>>>(A);
-                    linattn_chain_kernel<TT, DK, true><<<grid, 512, 0, s>>>(A);
+                    if (grid) {
+                        linattn_chunk_kernel<TT, DK, true><<<tiles, 256, 0, s>>>(A);
+                        linattn_chain_kernel<TT, DK, true><<<grid, 512, 0, s>>>(A);
+                    }
                     linattn_step_kernel<TT, DK, true, true><<<steps, LA_WG, 0, s>>>(A);
                 } else {
-                    linattn_chunk_kernel<TT, DK, false><<<tiles, 256, 0, s>>>(A);
-                    linattn_chain_kernel<TT, DK, false><<<grid, 512, 0, s>>>(A);
+                    if (grid) {
+                        linattn_chunk_kernel<TT, DK, false><<<tiles, 256, 0, s>>>(A);
+                        linattn_chain_kernel<TT, DK, false><<<grid, 512, 0, s>>>(A);
+                    }
                     linattn_step_kernel<TT, DK, false, true><<<steps, LA_WG, 0, s>>>(A);
                 }
             }

@@ -4,7 +4,7 @@
 //
 // A call is taken in windows of rows, so that its workspace has a bound; a sequence that
 // goes on behind its window hands its state on.  Within a window a sequence of more than
-// LA_SHORT rows is cut into chunks of LA_CHUNK; shorter ones go token by token.  The
+// `brief` rows is cut into chunks of LA_CHUNK; those as brief go token by token.  The
 // chunks of the i-th long sequence are numbered from (first row >> 6) + i on:
 // ceil(n / 64) <= (n >> 6) + 1, so that no two share a number.
 #pragma once
@@ -15,7 +15,23 @@
 
 namespace qmag {
 
-constexpr int LA_CHUNK = 64, LA_SHIFT = 6, LA_SHORT = 16;
+constexpr int LA_CHUNK = 64, LA_SHIFT = 6;
+
+// Up to how many rows a sequence goes token by token, for the waves that this takes, 16
+// columns of a head and sequence each.  Few waves wait for one another's sums, some 0.7 us
+// a token, and a chunk takes 26 us whatever rows it has: one sequence of 32 heads and 128
+// channels 27 us in either form for 32 tokens, 50 against 27 for 64.  Where the chip is
+// full a token costs what it computes: 64 such sequences of 64 tokens 468 us against 687
+// in chunks (bf16 461 and 549), 64 of 8 heads and 256 channels 430 and 298.
+constexpr int la_brief(int64_t waves) { return waves <= 1024 ? 32 : 64; }
+// Whether a call is cut: its sequences have more rows than that on average, or one of them
+// may have twice as many, the others a row each.  If then none has, the two launches that
+// find nothing take 10 us, of 80 for 64 sequences of 8 tokens; a prompt of 512 tokens among
+// single ones would take 360 us token by token, and takes 60.
+constexpr bool la_cut(int T, int n_seq, int brief)
+{
+    return T > (int64_t)brief * n_seq || (int64_t)T - n_seq >= 2 * brief;
+}
 
 // a sequence's rows within the window [r0, r1)
 struct LaRows {
@@ -28,16 +44,20 @@ constexpr LaRows la_rows(int cu0, int cu1, int T, int r0, int r1)
     const int first = a < r0 ? r0 : a, last = b > r1 ? r1 : b;
     return {first, last > first ? last - first : 0, a < r0, b > r1};
 }
-constexpr bool la_long(int n) { return n > LA_SHORT; }
+constexpr bool la_long(int n, int brief) { return n > brief; }
 constexpr int la_tile0(int first, int r0, int rank) { return ((first - r0) >> LA_SHIFT) + rank; }
-constexpr bool la_room(int tile0, int chunks, int most) { return tile0 + chunks <= most; }
 
-// numbers of a window of `rows` rows: its long sequences are at most n_seq, and have
-// LA_SHORT + 1 rows each
-constexpr int la_most_tiles(int rows, int n_seq)
+// A window's long sequences, each of brief + 1 rows or more, and their chunks' numbers.  (Sequences that lap over one
+// another may be more, or have more: what is behind these goes token by token.)
+constexpr int la_most_long(int rows, int n_seq, int brief)
 {
-    const int most = rows / (LA_SHORT + 1) + 1;
-    return (rows >> LA_SHIFT) + (n_seq < most ? n_seq : most);
+    const int most = rows / (brief + 1);
+    return n_seq < most ? n_seq : most;
+}
+constexpr int la_most_tiles(int rows, int n_seq, int brief) { return (rows >> LA_SHIFT) + la_most_long(rows, n_seq, brief); }
+constexpr bool la_room(int rank, int tile0, int chunks, int most_long, int most_tiles)
+{
+    return rank < most_long && tile0 + chunks <= most_tiles;
 }
 
 }  // namespace qmag

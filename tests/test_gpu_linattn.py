@@ -72,7 +72,7 @@ class Case:
         assert np.array_equal(after[left], self.state[left], equal_nan=True) and other[left].all()
 
 
-LENS = {"step": [1] * 7, "some": [3, 1, 0, 9, 16, 2], "edges": [15, 17, 63, 64, 65, 0, 1, 130], "one": [300], "two": [129, 127]}
+LENS = {"step": [1] * 7, "some": [3, 1, 0, 9, 16, 2], "edges": [15, 17, 63, 64, 65, 0, 1, 130], "brief": [31, 32, 33, 34, 1, 0], "one": [300], "two": [129, 127]}
 
 
 @pytest.mark.parametrize("typ", TYPES)
@@ -82,6 +82,16 @@ def test_linattn_lengths(qm, typ, lens, delta):
     r = rng_of(len(lens), delta, 1)
     s = Sequences(qm, r, LENS[lens], pad=3)
     c = Case(r, s, TYPES[typ], delta=delta, norm=delta, beta=delta)
+    c.check(*c.run(qm))
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("delta", [True, False])
+def test_linattn_many_sequences(qm, typ, delta):
+    """More waves than the chip holds at once: 64 rows go token by token, 65 in a chunk and one row."""
+    r = rng_of(13, delta)
+    s = Sequences(qm, r, [1, 64, 65, 2, 0, 33, 66, 1, 128, 63] + [1] * 30, pad=1)
+    c = Case(r, s, TYPES[typ], 4, 8, 64, 64, delta=delta, norm=delta, beta=delta)
     c.check(*c.run(qm))
 
 

@@ -101,17 +101,17 @@ CHUNKS = r"""
 #include "qmag_linattn_plan.h"
 using namespace qmag;
 
-// stdin: calls of T window n_seq, then cu: what the kernels do with them, window by window
+// stdin: calls of T window brief n_seq, then cu: what the kernels do with them, window by window
 int main()
 {
-    int T, window, n;
-    for (int call = 0; scanf("%d%d%d", &T, &window, &n) == 3; call++) {
+    int T, window, brief, n;
+    for (int call = 0; scanf("%d%d%d%d", &T, &window, &brief, &n) == 4; call++) {
         std::vector<int> cu(n + 1), rows(T);
         for (int &v : cu) if (scanf("%d", &v) != 1) return 1;
         bool ascending = cu[0] >= 0 && cu[n] <= T;
         for (int i = 0; i < n; i++) ascending = ascending && cu[i] <= cu[i + 1];
         for (int r0 = 0; r0 < T; r0 += window) {
-            const int r1 = r0 + window < T ? r0 + window : T, most = la_most_tiles(r1 - r0, n);
+            const int r1 = r0 + window < T ? r0 + window : T, most = la_most_tiles(r1 - r0, n, brief), most_long = la_most_long(r1 - r0, n, brief);
             std::vector<int> taken(most);
             int rank = 0, begun = 0, goes_on = 0;
             for (int i = 0; i < n; i++) {
@@ -120,9 +120,9 @@ int main()
                 for (int r = 0; r < x.n; r++) rows[x.first + r]++;
                 begun += x.n && x.begun;
                 goes_on += x.n && x.goes_on;
-                if (!la_long(x.n)) continue;
-                const int t0 = la_tile0(x.first, r0, rank++), c = seq_tiles(x.n, LA_SHIFT);
-                if (!la_room(t0, c, most)) {
+                if (!la_long(x.n, brief)) continue;
+                const int t0 = la_tile0(x.first, r0, rank), c = seq_tiles(x.n, LA_SHIFT);
+                if (!la_room(rank++, t0, c, most_long, most)) {
                     if (ascending) return printf("call %d: no room for sequence %d\n", call, i), 1;
                     continue;
                 }
@@ -152,13 +152,13 @@ def test_chunks_and_windows(tmp_path):
     r, calls = np.random.RandomState(3), []
     for _ in range(500):
         n = r.randint(1, 60)
-        lens = r.randint(0, r.choice([2, 18, 70, 400]) + 1, n) * (r.rand(n) < 0.8)
+        lens = r.randint(0, r.choice([2, 34, 70, 400]) + 1, n) * (r.rand(n) < 0.8)
         cu = np.concatenate([[0], np.cumsum(lens)])
         calls.append((max(1, int(cu[-1]) + r.choice([0, 0, 3])), 64 * r.choice([4, 5, 9, 1000]), cu))
-    calls += [(17 * 500, 64 * w, np.arange(501) * 17) for w in (4, 7, 200)] + [(4096, 256, np.array([0, 4096]))]
+    calls += [(n * 500, 64 * w, np.arange(501) * n) for w in (4, 7, 200) for n in (33, 65)] + [(4096, 256, np.array([0, 4096]))]
     for _ in range(300):
         n, T = r.randint(1, 40), r.randint(1, 900)
         calls.append((T, 64 * r.choice([4, 6, 100]), r.choice([-2 ** 31, -5, 0, T // 2, T - 3, T, T + 9, 2 ** 31 - 1], n + 1)))
-    text = "\n".join(" ".join(map(str, [T, w, len(cu) - 1] + list(cu))) for T, w, cu in calls)
+    text = "\n".join(" ".join(map(str, [T, w, brief, len(cu) - 1] + list(cu))) for T, w, cu in calls for brief in (32, 64))
     out = subprocess.run([exe], input=text, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
