@@ -576,8 +576,10 @@ template <class T, int DK>
 struct LaRoom {
     static constexpr int K = LaKeys<T, DK>::Q, REST = DK / 32 * 3 * LA_FRAG + 2 * (6 + LA_OUT_PARTS<T>) * LA_FRAG + 5 * LA_FRAG + 64;
     static constexpr int BUFS = 2 * K + REST <= 160 * 1024 ? 2 : 1;      // chunks of K in LDS
-    // two workgroups to a CU, where their LDS allows it: each waits most of its time for a product or a move through LDS
-    static constexpr int WGS = 2 * (2 * K + REST) <= 160 * 1024 ? 2 : 1;
+    // two workgroups to a CU, where their LDS allows it and half the registers do: each waits most of its time for a
+    // product or a move through LDS.  (fp32's three parts of Q and K ahead do not fit 128: 4096 tokens, 32 heads and 64
+    // channels 367 us against 165.)
+    static constexpr int WGS = sizeof(typename T::S) == 2 && 2 * (2 * K + REST) <= 160 * 1024 ? 2 : 1;
 };
 
 // a value as if it were new in every turn of a loop, so that places formed from it are not kept (and then spilled)
@@ -783,10 +785,13 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
             // place there is free: K beside the last one's, V and what it is multiplied by once the first barrier has
             // passed.
             constexpr int MINE = X::Q / LA_FRAG / 4;
+            // (256 fp32 channels: Q where it is used, or registers spill: 2 x 2048 tokens of 4 heads 355 us against 577)
+            constexpr bool HOLD = NKB * NP <= 16;
             bf168 qf[NKB][NP], pf[2][NO];
             f32x4 qd, kr[MINE], vec;
             float v[4];
             auto ask_q = [&](int i) {
+                if (!HOLD) return;
                 const uint8_t *p = keys(i) + X::Q + rt * NKB * NP * LA_FRAG;
 #pragma unroll
                 for (int kb = 0; kb < NKB; kb++) la_load<NP>(p + kb * NP * LA_FRAG, qf[kb]);
@@ -836,6 +841,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                     bf168 b[UP + 1];
 #pragma unroll
                     for (int i = 0; i <= UP; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
+                    if constexpr (!HOLD) la_load<NP>(keys(c) + X::Q + (rt * NKB + kb) * NP * LA_FRAG, qf[kb]);
                     qs[kb & 1].add(qf[kb], b);
                 }
                 ask_q(c + 1);
