@@ -26,8 +26,23 @@
 // range of fp32; fp16 values are two exactly, bf16 ones one), and of the products of
 // parts those are formed whose places add up to less than three (2^-24 of the operands).
 // An accumulator holds four rows of a column in a lane, which is half of what the next
-// product's operand holds of 32 rows: products whose 32 terms are taken in the order
-// [4 g .. 4 g + 3, 16 + 4 g ..] for lane group g need no move between lanes.
+// product's operand holds of 32 rows.  Products over tokens take their 32 terms in the
+// order [4 g .. 4 g + 3, 16 + 4 g ..] for lane group g, products over channels a group's
+// eight side by side, the state's rows being laid out for it: neither moves between lanes.
+//
+// What they are bound by (32 heads over 16 key heads, 128 channels both):
+//   a token each of 96 sequences, bf16: 89 us for 403 MB of states, 4.5 TB/s, memory.
+//   one token of one sequence: 5.3 us; 61 tokens of 13 sequences: 16.2.  Some 0.7 us a
+//   token for two sums over 16 lanes and what hangs on them; where the chip is full, 250
+//   instructions for each token and wave.  Not kept: more tokens asked for ahead and
+//   normalised early (registers for three waves where four were: 96 sequences 118 us),
+//   half the columns a wave (18.7 us for the 61 tokens), a quarter (27).
+//   prompts, fp32, 4096 tokens: 60 us for all chunks' matrices, 179 MB written and read
+//   back, and 200 for the walk, 64 chunks in a row of 3.1 us: three products of 6 pairs
+//   of parts that wait for one another through LDS, with a barrier after each.
+//   8192 tokens of 7 prompts, bf16: 84 and 245 us; the longest prompt's chunks.
+//   Not kept in the walk: operands by transfers straight to LDS, by 4 waves more (227 us
+//   for fp32, 325 for bf16); Q and K split into parts in the walk (244 and 395).
 #include <math.h>
 
 #include "qmag_rows.h"
@@ -235,8 +250,8 @@ __device__ __forceinline__ void la_split8(const float (&x)[8], bf168 (&o)[N])
         for (int i = 0; i < 8; i++) o[p][i] = s[p][i];
 }
 
-// A sum of products of parts, one accumulator for each place that two parts' places add up to: a product that adds to
-// the one ahead of it waits for it (one accumulator for all: 253 us for 4096 tokens against 199 in fp32).
+// A sum of products of parts, one accumulator for each place that two parts' places add up to: small ones are added
+// among themselves first.
 template <int UP>
 struct LaSum {
     f32x4 c[UP + 1];
@@ -369,6 +384,8 @@ __global__ void __launch_bounds__(LA_WG) linattn_step_kernel(LaArgs A)
 }
 
 // What a chunk of a key head and its heads has that does not depend on the state: a wave takes 16 of the chunk's rows.
+// Bound by what it writes: 60 us for 4096 tokens of 16 key heads and 32 heads in fp32, 96 KB of K and Q and twice 37 KB
+// of matrices for each chunk and key head, 179 MB (3 TB/s).
 // Products of rows j with rows i leave lane group g with j = 4 g .. of a row i: as P and the inverse are operands.
 template <class T, int DK, bool DELTA>
 __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)

@@ -16,6 +16,11 @@
 //
 // A row is one workgroup's, or, where there are few, several workgroups' and joined
 // by a second launch.
+//
+// Bound by memory where there are many rows: 1024 of 151936 bf16 logits with the best
+// token take 87 us for 311 MB, 3.6 TB/s (a large read alone reaches 3.8).  One row, fp32,
+// 20 tokens: 7.2 us and 7.3 for the join, sorts of 64 keys one after another in both;
+// 77 rows of 32003 fp16, 5 tokens: 12.8 and 5.0.
 #include <float.h>
 
 #include "qmag_rows.h"
@@ -26,7 +31,7 @@ namespace qmag {
 constexpr int LP_WG = 256, LP_WAVES = LP_WG / 64;
 constexpr int LP_PER = 8;                        // values of a thread in a tile
 constexpr int LP_TILE = 64 * LP_PER;             // a wave's tile
-constexpr int LP_AHEAD = 4;
+constexpr int LP_AHEAD = 4;                      // tiles asked for ahead (8: 92 us for 1024 rows against 87)
 constexpr int LP_ROOM = 64 + LP_TILE;           // keys that wait: fewer than k ahead of a tile, all of its values
 
 struct LpArgs {
@@ -375,7 +380,8 @@ extern "C" int qmag_logprobs_dev(int n_vocab, int type, const void *logits, int6
     if (T == 0 || (!logprob && !entropy && top_k == 0)) return QMAG_OK;
 
     LpArgs A = {logits, stride, token, logprob, entropy, top_logprob, top_id, nullptr, nullptr, n_vocab, T, top_k, 1, n_vocab};
-    // rows in parts while there are fewer than 1024 of them, parts of 2048 values and more
+    // rows in parts while there are fewer than 1024 of them (2048: 102 us and 16 for the join, for 1024 rows, against 87),
+    // parts of 2048 values and more
     const int64_t want = (1024 + (int64_t)T - 1) / T, fit = ((int64_t)n_vocab + LP_WAVES * LP_TILE - 1) / (LP_WAVES * LP_TILE);
     A.parts = (int)(want < fit ? want : fit);
     if (A.parts > 1) {
