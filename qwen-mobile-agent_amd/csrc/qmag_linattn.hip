@@ -250,34 +250,18 @@ __device__ __forceinline__ void la_split8(const float (&x)[8], bf168 (&o)[N])
         for (int i = 0; i < 8; i++) o[p][i] = s[p][i];
 }
 
-// A sum of products of parts, one accumulator for each place that two parts' places add up to: small ones are added
-// among themselves first.
-template <int UP>
-struct LaSum {
-    f32x4 c[UP + 1];
-    __device__ __forceinline__ void clear()
-    {
+// c += a b, of the products of parts those of places adding up to at most UP, the smallest first
+template <int UP, int NA, int NB>
+__device__ __forceinline__ void la_mac(const bf168 (&a)[NA], const bf168 (&b)[NB], f32x4 &c)
+{
 #pragma unroll
-        for (int i = 0; i <= UP; i++) c[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    // += a b, of the products of parts those of places adding up to at most UP
-    template <int NA, int NB>
-    __device__ __forceinline__ void add(const bf168 (&a)[NA], const bf168 (&b)[NB])
-    {
+    for (int places = UP; places >= 0; places--)
 #pragma unroll
-        for (int i = 0; i < NA; i++)
-#pragma unroll
-            for (int j = 0; j < NB; j++)
-                if (i + j <= UP) c[i + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], c[i + j], 0, 0, 0);
-    }
-    __device__ __forceinline__ f32x4 sum() const
-    {
-        f32x4 s = c[UP];
-#pragma unroll
-        for (int i = UP - 1; i >= 0; i--) s += c[i];
-        return s;
-    }
-};
+        for (int i = 0; i < NA; i++) {
+            const int j = places - i;
+            if (j >= 0 && j < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], c, 0, 0, 0);
+        }
+}
 
 template <int N>
 __device__ __forceinline__ void la_load(const uint8_t *p, bf168 (&o)[N])
@@ -454,19 +438,15 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
 #pragma unroll
     for (int ct = 0; ct < 4; ct++) {
         if (ct > w) continue;
-        LaSum<NP == 1 ? 0 : 2> sk, sq;
-        sk.clear();
-        sq.clear();
+        ck[ct] = cq[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
             bf168 a[NP];
 #pragma unroll
             for (int p = 0; p < NP; p++) a[p] = *(const bf168 *)&s_k[p][16 * ct + l16][32 * kb + 8 * g];
-            if constexpr (DELTA) sk.add(a, kf[kb]);
-            sq.add(a, qf[kb]);
+            if constexpr (DELTA) la_mac<2>(a, kf[kb], ck[ct]);
+            la_mac<2>(a, qf[kb], cq[ct]);
         }
-        ck[ct] = sk.sum();
-        cq[ct] = sq.sum();
     }
     const int sharing = A.n_head / A.n_key;
     for (int i = 0; i < sharing; i++) {
@@ -692,9 +672,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 const uint8_t *K = s_k[c % BUFS];
                 f32x4 acc;
                 if constexpr (DELTA) {
-                    LaSum<2> ks[2];
-                    ks[0].clear();
-                    ks[1].clear();
+                    f32x4 ks[2] = {};
 #pragma unroll
                     for (int kb = 0; kb < NKB; kb++) {
                         bf168 a[NP], b[3];
@@ -702,22 +680,33 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
 #pragma unroll
                         for (int i = 0; i < NP; i++) a[i] = *(const bf168 *)(K + row_at[kb % KINDS] + i * X::PLANE + kb / KINDS * 256);
-                        ks[kb & 1].add(a, b);
+                        la_mac<2>(a, b, ks[kb & 1]);
                     }
-                    acc = ks[0].sum() + ks[1].sum();
+                    acc = ks[0] + ks[1];
                 }
                 const f32x4 kd = *(const f32x4 *)&s_vec[Y::KD + 16 * rt + g4], bt = *(const f32x4 *)&s_vec[Y::B + 16 * rt + g4],
                             ke = *(const f32x4 *)&s_vec[Y::KE + 16 * rt + g4], v = *(const f32x4 *)&s_v[256 * rt + 4 * lane];
                 const float end = s_vec[Y::END];
                 const int good = ((const int *)s_vec)[Y::BAD], left = min(rows.n - 64 * c, good);
-                int bad = good;
                 float x[4];
+                bool odd = good < 64;
 #pragma unroll
-                for (int r = 3; r >= 0; r--) {
-                    const int row = 16 * rt + g4 + r;
-                    const bool fine = fabsf(v[r]) <= 0x1p60f;
-                    x[r] = row < left && fine ? bt[r] * (DELTA ? fmaf(-kd[r], acc[r], v[r]) : v[r]) : 0.0f;
-                    bad = row < left && !fine ? min(bad, row) : bad;
+                for (int r = 0; r < 4; r++) {
+                    // (b is 0 behind the sequence's end)
+                    x[r] = bt[r] * (DELTA ? fmaf(-kd[r], acc[r], v[r]) : v[r]);
+                    odd |= !(fabsf(v[r]) <= 0x1p60f);
+                }
+                int bad = 64;
+                if (__ballot(odd)) {
+                    bad = good;
+#pragma unroll
+                    for (int r = 3; r >= 0; r--) {
+                        const int row = 16 * rt + g4 + r;
+                        const bool fine = fabsf(v[r]) <= 0x1p60f;
+                        if (row < left && !fine) bad = min(bad, row);
+                        if (row >= left || !fine) x[r] = 0.0f;              // not even times 0 in the rows ahead
+                    }
+                    bad = group_min_i<64>(bad);
                 }
                 if constexpr (DELTA) {
                     __bf16 p[3][4];
@@ -725,23 +714,20 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
 #pragma unroll
                     for (int i = 0; i < 3; i++) *(s16x4 *)&s_x[rt >> 1][i][half] = *(const s16x4 *)p[i];
                 }
-                if (__ballot(bad < 64)) bad = group_min_i<64>(bad);
                 if (lane == 0) s_bad[rt] = bad;
                 if constexpr (DELTA) {
                     __syncthreads();
-                    LaSum<2> us[2];
-                    us[0].clear();
-                    us[1].clear();
+                    f32x4 us[2] = {};
 #pragma unroll
                     for (int tb = 0; tb < 2; tb++) {
                         if (2 * tb > rt) continue;
                         bf168 b[3];
 #pragma unroll
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_x[tb][i][at];
-                        us[tb].add(tf[tb], b);
+                        la_mac<2>(tf[tb], b, us[tb]);
                     }
                     ask_t(c + 1);
-                    const f32x4 u = us[0].sum() + us[1].sum();
+                    const f32x4 u = us[0] + us[1];
 #pragma unroll
                     for (int r = 0; r < 4; r++) x[r] = u[r];
                 }
@@ -760,11 +746,10 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 __syncthreads();
                 upto = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
                 if (upto < 64) break;
-                LaSum<2> more[OWN][2];
 #pragma unroll
                 for (int o = 0; o < OWN; o++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) more[o][h].clear();
+                    for (int h = 0; h < 2; h++) s[o][h] *= end;
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) {
                     bf168 b[3];
@@ -786,13 +771,9 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                                         (__attribute__((address_space(3))) s16x4 *)(K + col_at + i * X::PLANE + (32 * tb + 16 * u) * DK * 2 + 256 * o + 8 * h));
                                 av[i] = a[i].v;
                             }
-                            more[o][h].add(av, b);
+                            la_mac<2>(av, b, s[o][h]);
                         }
                 }
-#pragma unroll
-                for (int o = 0; o < OWN; o++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) s[o][h] = s[o][h] * end + more[o][h].sum();
                 publish();
                 __syncthreads();
                 if constexpr (BUFS == 1) __syncthreads();
@@ -848,21 +829,17 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
             __syncthreads();
             for (; c < chunks; c++) {
                 la_fresh(at);
-                LaSum<UP> qs[2], ps[2];
-                qs[0].clear();
-                qs[1].clear();
-                ps[0].clear();
-                ps[1].clear();
+                f32x4 qs[2] = {};
 #pragma unroll
                 for (int kb = 0; kb < NKB; kb++) {
                     bf168 b[UP + 1];
 #pragma unroll
                     for (int i = 0; i <= UP; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
                     if constexpr (!HOLD) la_load<NP>(keys(c) + X::Q + (rt * NKB + kb) * NP * LA_FRAG, qf[kb]);
-                    qs[kb & 1].add(qf[kb], b);
+                    la_mac<UP>(qf[kb], b, qs[kb & 1]);
                 }
                 ask_q(c + 1);
-                f32x4 o = (qs[0].sum() + qs[1].sum()) * qd;
+                f32x4 o = (qs[0] + qs[1]) * qd;
                 if constexpr (BUFS == 2) {
                     put_k(c + 1);
                     ask_k(c + 2);
@@ -882,14 +859,13 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                     bf168 b[NO];
 #pragma unroll
                     for (int i = 0; i < NO; i++) b[i] = *(const bf168 *)&s_u[tb][i][at];
-                    ps[tb].add(pf[tb], b);
+                    la_mac<UP>(pf[tb], b, o);
                 }
                 ask_p(c + 1);
                 if constexpr (!DELTA && BUFS == 2) {
                     put_v();
                     ask_v(c + 2);
                 }
-                o += ps[0].sum() + ps[1].sum();
                 const int t = 64 * c + 16 * rt + (int)(at >> 8) * 4, to = min(rows.n, 64 * c + upto);
                 S *p = (S *)A.out + (rows.first + (int64_t)t) * A.ots + head * A.ohs + c0 + ((at >> 4) & 15);
 #pragma unroll
