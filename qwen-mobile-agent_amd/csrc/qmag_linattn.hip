@@ -37,12 +37,13 @@
 //   instructions for each token and wave.  Not kept: more tokens asked for ahead and
 //   normalised early (registers for three waves where four were: 96 sequences 118 us),
 //   half the columns a wave (18.7 us for the 61 tokens), a quarter (27).
-//   prompts, fp32, 4096 tokens: 60 us for all chunks' matrices, 179 MB written and read
-//   back, and 200 for the walk, 64 chunks in a row of 3.1 us: three products of 6 pairs
+//   prompts, fp32, 4096 tokens: 54 us for all chunks' matrices, 179 MB written and read
+//   back, and 183 for the walk, 64 chunks in a row of 2.9 us: three products of 6 pairs
 //   of parts that wait for one another through LDS, with a barrier after each.
-//   8192 tokens of 7 prompts, bf16: 84 and 245 us; the longest prompt's chunks.
-//   Not kept in the walk: operands by transfers straight to LDS, by 4 waves more (227 us
-//   for fp32, 325 for bf16); Q and K split into parts in the walk (244 and 395).
+//   8192 tokens of 7 prompts, bf16: 60 and 206 us, the chip full of chunks of two
+//   workgroups to a CU at 3.2 us each.
+//   Not kept in the walk, at 200 us for fp32 and 245 for bf16: operands by transfers
+//   straight to LDS, by 4 waves more (227, 325); Q and K split into parts there (244, 395).
 #include <math.h>
 
 #include "qmag_rows.h"
@@ -368,11 +369,19 @@ __global__ void __launch_bounds__(LA_WG) linattn_step_kernel(LaArgs A)
 }
 
 // What a chunk of a key head and its heads has that does not depend on the state: a wave takes 16 of the chunk's rows.
-// Bound by what it writes: 60 us for 4096 tokens of 16 key heads and 32 heads in fp32, 96 KB of K and Q and twice 37 KB
-// of matrices for each chunk and key head, 179 MB (3 TB/s).
+// 54 us for 4096 tokens of 16 key heads and 32 heads in fp32, 96 KB of K and Q and twice 37 KB of matrices for each chunk
+// and key head: 179 MB written and 64 read, 4.5 TB/s, the memory's rate.
 // Products of rows j with rows i leave lane group g with j = 4 g .. of a row i: as P and the inverse are operands.
+constexpr double LOG2E = 1.4426950408889634;
+__device__ __forceinline__ float la_power(double x) { return __builtin_amdgcn_exp2f((float)x); }
+
+// workgroups to a CU, as many as their LDS leaves, three at most: more than two waves to a SIMD take fewer registers than
+// the compiler would (8192 tokens bf16 60 us with three, 72 with two)
+template <class T, int DK>
+constexpr int LA_CHUNK_WGS = 160 * 1024 / (LA_PARTS<T> * 128 * (DK + 8) + 28 * 1024) < 3 ? 160 * 1024 / (LA_PARTS<T> * 128 * (DK + 8) + 28 * 1024) : 3;
+
 template <class T, int DK, bool DELTA>
-__global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
+__global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kernel(LaArgs A)
 {
     using S = typename T::S;
     using Y = LaLayout<T>;
@@ -380,9 +389,9 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
     __shared__ __attribute__((aligned(16))) __bf16 s_k[NP][64][ROW];
     __shared__ __attribute__((aligned(16))) float s_lt[64][68];           // L, rows and columns exchanged
     __shared__ __attribute__((aligned(16))) float s_dt[4][16][20];        // inverses of its diagonal blocks, exchanged
-    __shared__ double s_g[64];
-    __shared__ float s_fk[64], s_fq[64], s_kk[64], s_b[64];
-    __shared__ int s_odd[4], s_good;
+    __shared__ double s_g[4][64];
+    __shared__ float s_fk[64], s_fq[64], s_kk[64], s_b[4][64];
+    __shared__ int s_odd[4], s_good[4];
     const int lane = lane_id(), w = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4, g4 = g * 4;
     const int tile = blockIdx.x / A.n_key, key = blockIdx.x % A.n_key;
     const LaTile at = la_find(A, tile);
@@ -395,15 +404,19 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
     bf168 kf[NKB][NP], qf[NKB][NP];
     float kk = 0.0f, qq = 0.0f;
     const int my = 16 * w + l16;
+    const S *kp = (const S *)A.k.p + (row0 + min(my, n - 1)) * A.k.ts + key * A.k.hs + 8 * g;
+    const S *qp = (const S *)A.q.p + (row0 + min(my, n - 1)) * A.q.ts + key * A.q.hs + 8 * g;
+    float kx[NKB][8], qx[NKB][8];
+#pragma unroll
+    for (int kb = 0; kb < NKB; kb++) {
+        load_row<T, 8>(kp + 32 * kb, kx[kb]);
+        load_row<T, 8>(qp + 32 * kb, qx[kb]);
+    }
 #pragma unroll
     for (int kb = 0; kb < NKB; kb++) {
         float x[8], y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = 0.0f, y[e] = 0.0f;
-        if (my < n) {
-            load_row<T, 8>((const S *)A.k.p + (row0 + my) * A.k.ts + key * A.k.hs + 32 * kb + 8 * g, x);
-            load_row<T, 8>((const S *)A.q.p + (row0 + my) * A.q.ts + key * A.q.hs + 32 * kb + 8 * g, y);
-        }
+        for (int e = 0; e < 8; e++) x[e] = my < n ? kx[kb][e] : 0.0f, y[e] = my < n ? qx[kb][e] : 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             kk = fmaf(x[e], x[e], kk);
@@ -450,9 +463,10 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
     }
     const int sharing = A.n_head / A.n_key;
     for (int i = 0; i < sharing; i++) {
-        const int head = la_head_of(A, key, i);
-        uint8_t *to = A.heads + ((int64_t)tile * A.n_head + head) * Y::HEAD_BYTES;
-        if (w == 0) {
+        // the gates of four heads at once, a wave to each
+        if (i % 4 == 0 && i + w < sharing) {
+            const int head = la_head_of(A, key, i + w);
+            uint8_t *to = A.heads + ((int64_t)tile * A.n_head + head) * Y::HEAD_BYTES;
             float g = 0.0f, b = 0.0f;
             if (lane < n) {
                 g = A.decay ? ldg(A.decay + (row0 + lane) * A.n_head + head) : 0.0f;
@@ -466,29 +480,32 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
                 const double o = __shfl_up(sum, d);
                 if (lane >= d) sum += o;
             }
+            sum *= LOG2E;
             const double all = __shfl(sum, 63);
             const float bk = b * s_kk[lane];
             // the delta rule grows past b |k|^2 = 2, and its inverse with it
             const bool out = none || (DELTA ? !(bk >= 0.0f && bk <= 2.01f) || !(b <= 0x1p60f) : !(fabsf(b) <= 0x1p40f));
             const uint64_t bad = __ballot(out);
-            s_g[lane] = sum;
-            s_b[lane] = b;
+            s_g[w][lane] = sum;
+            s_b[w][lane] = b;
             const int good = bad ? min(even, __ffsll((unsigned long long)bad) - 1) : even;
             float *vec = (float *)(to + Y::VEC);
-            const float now = expf((float)sum), fk = s_fk[lane];
+            const float now = la_power(sum), fk = s_fk[lane];
             vec[Y::KD + lane] = now * fk;
             ((float *)(to + Y::QD))[lane] = A.scale * s_fq[lane] * now;
-            vec[Y::KE + lane] = expf((float)(all - sum)) * fk;
+            vec[Y::KE + lane] = la_power(all - sum) * fk;
             vec[Y::B + lane] = b;
             if (lane == 0) {
-                vec[Y::END] = expf((float)all);
-                ((int *)vec)[Y::BAD] = s_good = good;
+                vec[Y::END] = la_power(all);
+                ((int *)vec)[Y::BAD] = s_good[w] = good;
             }
         }
-        __syncthreads();
-        const double gi = s_g[my];
-        const bool row = my < s_good;
-        const float pq = A.scale * s_fq[my], lk = s_b[my] * s_fk[my];
+        if (i % 4 == 0) __syncthreads();
+        const int head = la_head_of(A, key, i), gate = i % 4;
+        uint8_t *to = A.heads + ((int64_t)tile * A.n_head + head) * Y::HEAD_BYTES;
+        const double gi = s_g[gate][my];
+        const bool row = my < s_good[gate];
+        const float pq = A.scale * s_fq[my], lk = s_b[gate][my] * s_fk[my];
         float pv[4][4];
 #pragma unroll
         for (int ct = 0; ct < 4; ct++) {
@@ -497,7 +514,7 @@ __global__ void __launch_bounds__(256) linattn_chunk_kernel(LaArgs A)
                 pv[ct][r] = 0.0f;
                 if (ct > w) continue;
                 const int j = 16 * ct + g4 + r;
-                const float e = s_fk[j] * expf((float)(gi - s_g[j]));
+                const float e = s_fk[j] * la_power(gi - s_g[gate][j]);
                 pv[ct][r] = row && j <= my ? pq * (cq[ct][r] * e) : 0.0f;
                 if constexpr (DELTA) s_lt[j][my] = row && j < my ? lk * (ck[ct][r] * e) : 0.0f;
             }
