@@ -997,7 +997,7 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
     hipStream_t s = ctx().stream;
     const int64_t slices = (int64_t)n_seq * a->n_head * (a->dim_v / 16);
     // prompts in chunks; few tokens to a sequence one after another
-    A.brief = la_brief(slices);
+    A.brief = la_brief(slices, type == QMAG_TYPE_F32);
     const bool chunks = la_cut(T, n_seq, A.brief);
     size_t state = 0;
     int window = 0;

@@ -19,18 +19,19 @@ constexpr int LA_CHUNK = 64, LA_SHIFT = 6;
 
 // Up to how many rows a sequence goes token by token, for the waves that this takes, 16
 // columns of a head and sequence each.  Few waves wait for one another's sums, some 0.7 us
-// a token, and a chunk takes 26 us whatever rows it has: one sequence of 32 heads and 128
-// channels 27 us in either form for 32 tokens, 50 against 27 for 64.  Where the chip is
-// full a token costs what it computes: 64 such sequences of 64 tokens 468 us against 687
-// in chunks (bf16 461 and 549), 64 of 8 heads and 256 channels 430 and 298.
-constexpr int la_brief(int64_t waves) { return waves <= 1024 ? 32 : 64; }
+// a token, and a chunk takes 26 us whatever rows it has (one sequence of 32 heads and 128
+// channels fp32, tokens and a chunk: 27 us and 26 for 32 rows, 50 and 26 for 64).  Where
+// the chip is full a token costs what it computes, and a chunk what begins and ends it: 64
+// such sequences in fp32, one workgroup to a CU, of 64 rows 468 and 638, of 96 689 and 830,
+// of 128 910 and 840; in bf16, two to a CU, of 32 rows 242 and 293, of 48 350 and 307.
+constexpr int la_brief(int64_t waves, bool wide) { return waves <= 1024 ? 32 : wide ? 96 : 40; }
 // Whether a call is cut: its sequences have more rows than that on average, or one of them
-// may have twice as many, the others a row each.  A prompt of 512 tokens beside 31 single
+// may have many more, the others a row each.  A prompt of 512 tokens beside 31 single
 // ones takes 81 us, token by token 436; where none is long after all, the launches that
-// find nothing take 64 sequences of 8 tokens from 88 us to 94.
+// find nothing take 64 sequences of 8 tokens from 88 us to 92.
 constexpr bool la_cut(int T, int n_seq, int brief)
 {
-    return T > (int64_t)brief * n_seq || (int64_t)T - n_seq >= 2 * brief;
+    return T > (int64_t)brief * n_seq || (int64_t)T - n_seq >= (brief <= 32 ? 64 : 128);
 }
 
 // a sequence's rows within the window [r0, r1)

@@ -88,9 +88,9 @@ def test_linattn_lengths(qm, typ, lens, delta):
 @pytest.mark.parametrize("typ", TYPES)
 @pytest.mark.parametrize("delta", [True, False])
 def test_linattn_many_sequences(qm, typ, delta):
-    """More waves than the chip holds at once: 64 rows go token by token, 65 in a chunk and one row."""
+    """More waves than the chip holds at once: 40 rows of 16-bit types go token by token, 96 of fp32."""
     r = rng_of(13, delta)
-    s = Sequences(qm, r, [1, 64, 65, 2, 0, 33, 66, 1, 128, 63] + [1] * 30, pad=1)
+    s = Sequences(qm, r, [1, 64, 65, 2, 0, 40, 41, 1, 128, 63, 96, 97] + [1] * 30, pad=1)
     c = Case(r, s, TYPES[typ], 4, 8, 64, 64, delta=delta, norm=delta, beta=delta)
     c.check(*c.run(qm))
 

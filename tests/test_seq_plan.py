@@ -155,10 +155,10 @@ def test_chunks_and_windows(tmp_path):
         lens = r.randint(0, r.choice([2, 34, 70, 400]) + 1, n) * (r.rand(n) < 0.8)
         cu = np.concatenate([[0], np.cumsum(lens)])
         calls.append((max(1, int(cu[-1]) + r.choice([0, 0, 3])), 64 * r.choice([4, 5, 9, 1000]), cu))
-    calls += [(n * 500, 64 * w, np.arange(501) * n) for w in (4, 7, 200) for n in (33, 65)] + [(4096, 256, np.array([0, 4096]))]
+    calls += [(n * 500, 64 * w, np.arange(501) * n) for w in (4, 7, 200) for n in (33, 41, 97)] + [(4096, 256, np.array([0, 4096]))]
     for _ in range(300):
         n, T = r.randint(1, 40), r.randint(1, 900)
         calls.append((T, 64 * r.choice([4, 6, 100]), r.choice([-2 ** 31, -5, 0, T // 2, T - 3, T, T + 9, 2 ** 31 - 1], n + 1)))
-    text = "\n".join(" ".join(map(str, [T, w, brief, len(cu) - 1] + list(cu))) for T, w, cu in calls for brief in (32, 64))
+    text = "\n".join(" ".join(map(str, [T, w, brief, len(cu) - 1] + list(cu))) for T, w, cu in calls for brief in (32, 40, 96))
     out = subprocess.run([exe], input=text, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
