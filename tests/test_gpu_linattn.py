@@ -1,5 +1,7 @@
 """Linear attention with a decay for each head (qmag_linattn_dev), plain and by the delta
 rule, against its recurrence in 64 bits."""
+import copy
+
 import numpy as np
 import pytest
 
@@ -95,7 +97,25 @@ def test_linattn_many_sequences(qm, typ, delta):
     c.check(*c.run(qm))
 
 
-SHAPES = [(1, 1, 64, 16), (2, 6, 64, 48), (3, 3, 128, 128), (1, 4, 128, 144), (2, 2, 256, 64), (1, 2, 256, 256), (5, 5, 64, 112)]
+@pytest.mark.parametrize("typ,least", [("f32", 97), ("bf16", 41)])
+def test_linattn_more_walks_than_workgroups(qm, typ, least):
+    """4096 walks of 16 columns: a workgroup takes one after another, of sequences with and without values that end one."""
+    r = rng_of(14, least)
+    s = Sequences(qm, r, [least + 3 * (i % 5) for i in range(16)], pad=1, had="all")
+    c = Case(r, s, TYPES[typ], 4, 16, 64, 256)
+    c.check(*c.run(qm))
+    d = copy.copy(c)
+    d.v = c.v.copy()
+    d.v[s.cu[3] + 5, 2, 7] = to_type(np.float32(np.inf), TYPES[typ])
+    (got, after), (clean, clean_after) = d.run(qm), c.run(qm)
+    same = np.ones(got.shape, bool)
+    same[s.cu[3] + 5:s.cu[4], 2] = False
+    assert np.array_equal(got[same], clean[same])
+    others = [j for j in range(s.n_slot) if j != s.slots[3]]
+    assert np.array_equal(after[others], clean_after[others], equal_nan=True)
+
+
+SHAPES = [(1, 1, 64, 16), (2, 6, 64, 48), (3, 3, 128, 128), (1, 4, 128, 144), (2, 2, 256, 64), (1, 2, 256, 256), (5, 5, 64, 112), (1, 6, 64, 32), (2, 18, 64, 16)]
 
 
 @pytest.mark.parametrize("typ", TYPES)
