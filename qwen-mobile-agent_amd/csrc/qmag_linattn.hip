@@ -192,13 +192,11 @@ __device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int 
 
 // ------------------------------------------------------------ in chunks --
 
-// bf16 parts of a value of the type, and of what the heads' matrices are held in
+// bf16 parts of a value of the type; what is formed of them is fp32, three parts, for results of any type: a 16-bit one
+// is rounded once, from what the recurrence in fp32 has.
 template <class T> constexpr int LA_PARTS = 3;
 template <> constexpr int LA_PARTS<TF16> = 2;
 template <> constexpr int LA_PARTS<TBF16> = 1;
-// For results of 16 bits two parts of P, U and the state: 2^-16 of them beside the result's own rounding of 2^-9 or 2^-12.
-template <class T> constexpr int LA_OUT_PARTS = 2;
-template <> constexpr int LA_OUT_PARTS<TF32> = 3;
 
 // Operands lie in the workspace as the matrix cores take them: 64 lanes of 16 bytes.
 constexpr int LA_FRAG = 1024;
@@ -219,9 +217,8 @@ __host__ __device__ constexpr int la_place(int row, int piece)
 }
 // What a chunk has for each head: (I + L)^-1 and P [LA_TRI][parts], then rows of 64 that the chunk's tokens are
 // multiplied by.
-template <class T>
 struct LaLayout {
-    static constexpr int TI = 0, P = LA_TRI * 3 * LA_FRAG, VEC = P + LA_TRI * LA_OUT_PARTS<T> * LA_FRAG, QD = VEC + 1024;
+    static constexpr int TI = 0, P = LA_TRI * 3 * LA_FRAG, VEC = P + LA_TRI * 3 * LA_FRAG, QD = VEC + 1024;
     static constexpr int KD = 0, KE = 64, B = 128, END = 192, BAD = 193;     // floats of VEC; END: e^G_63; BAD: the first row the form does not hold, 64: none
     static constexpr int HEAD_BYTES = QD + 256;
 };
@@ -251,12 +248,12 @@ __device__ __forceinline__ void la_split8(const float (&x)[8], bf168 (&o)[N])
         for (int i = 0; i < 8; i++) o[p][i] = s[p][i];
 }
 
-// c += a b, of the products of parts those of places adding up to at most UP, the smallest first
-template <int UP, int NA, int NB>
+// c += a b, of the products of parts those of places adding up to less than three, the smallest first
+template <int NA, int NB>
 __device__ __forceinline__ void la_mac(const bf168 (&a)[NA], const bf168 (&b)[NB], f32x4 &c)
 {
 #pragma unroll
-    for (int places = UP; places >= 0; places--)
+    for (int places = 2; places >= 0; places--)
 #pragma unroll
         for (int i = 0; i < NA; i++) {
             const int j = places - i;
@@ -384,7 +381,7 @@ template <class T, int DK, bool DELTA>
 __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kernel(LaArgs A)
 {
     using S = typename T::S;
-    using Y = LaLayout<T>;
+    using Y = LaLayout;
     constexpr int NP = LA_PARTS<T>, NKB = DK / 32, ROW = DK + 8;
     __shared__ __attribute__((aligned(16))) __bf16 s_k[NP][64][ROW];
     __shared__ __attribute__((aligned(16))) float s_lt[64][68];           // L, rows and columns exchanged
@@ -457,8 +454,8 @@ __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kern
             bf168 a[NP];
 #pragma unroll
             for (int p = 0; p < NP; p++) a[p] = *(const bf168 *)&s_k[p][16 * ct + l16][32 * kb + 8 * g];
-            if constexpr (DELTA) la_mac<2>(a, kf[kb], ck[ct]);
-            la_mac<2>(a, qf[kb], cq[ct]);
+            if constexpr (DELTA) la_mac(a, kf[kb], ck[ct]);
+            la_mac(a, qf[kb], cq[ct]);
         }
     }
     const int sharing = A.n_head / A.n_key;
@@ -523,11 +520,11 @@ __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kern
         for (int tb = 0; tb < 2; tb++) {
             if (2 * tb > w) continue;
             float x[8];
-            bf168 p[LA_OUT_PARTS<T>];
+            bf168 p[3];
 #pragma unroll
             for (int e = 0; e < 8; e++) x[e] = pv[2 * tb + (e >> 2)][e & 3];
-            la_split8<LA_OUT_PARTS<T>>(x, p);
-            la_store<LA_OUT_PARTS<T>>(to + Y::P + la_tri(w, tb) * LA_OUT_PARTS<T> * LA_FRAG, p);
+            la_split8<3>(x, p);
+            la_store<3>(to + Y::P + la_tri(w, tb) * 3 * LA_FRAG, p);
         }
         if constexpr (DELTA) {
             // the inverse of the wave's diagonal block, a column to a lane (four lanes the same)
@@ -588,7 +585,7 @@ __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kern
 // bytes a clock, and a wave that asks for its own operands waits in line with all others.
 template <class T, int DK>
 struct LaRoom {
-    static constexpr int K = LaKeys<T, DK>::Q, REST = DK / 32 * 3 * LA_FRAG + 2 * (6 + LA_OUT_PARTS<T>) * LA_FRAG + 5 * LA_FRAG + 64;
+    static constexpr int K = LaKeys<T, DK>::Q, REST = DK / 32 * 3 * LA_FRAG + 2 * 9 * LA_FRAG + 5 * LA_FRAG + 64;
     static constexpr int BUFS = 2 * K + REST <= 160 * 1024 ? 2 : 1;      // chunks of K in LDS
     // two workgroups to a CU, where their LDS allows it and half the registers do: each waits most of its time for a
     // product or a move through LDS.  (fp32's three parts of Q and K ahead do not fit 128: 4096 tokens, 32 heads and 64
@@ -603,14 +600,14 @@ template <class T, int DK, bool DELTA>
 __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_kernel(LaArgs A)
 {
     using S = typename T::S;
-    using Y = LaLayout<T>;
+    using Y = LaLayout;
     using M = LaRoom<T, DK>;
     using X = LaKeys<T, DK>;
-    constexpr int NP = LA_PARTS<T>, NKB = DK / 32, NO = LA_OUT_PARTS<T>, UP = NO - 1, BUFS = M::BUFS;
+    constexpr int NP = LA_PARTS<T>, NKB = DK / 32, BUFS = M::BUFS;
     constexpr int OWN = (NKB + 3) / 4;                    // blocks of 32 rows of the state that a wave holds
     __shared__ __attribute__((aligned(16))) uint8_t s_k[BUFS][X::Q];
     __shared__ __attribute__((aligned(16))) uint8_t s_s[NKB][3][LA_FRAG];
-    __shared__ __attribute__((aligned(16))) uint8_t s_x[DELTA ? 2 : 1][3][LA_FRAG], s_u[2][NO][LA_FRAG], s_e[2][3][LA_FRAG];
+    __shared__ __attribute__((aligned(16))) uint8_t s_x[DELTA ? 2 : 1][3][LA_FRAG], s_u[2][3][LA_FRAG], s_e[2][3][LA_FRAG];
     __shared__ __attribute__((aligned(16))) float s_vec[256], s_v[1024];
     __shared__ __attribute__((aligned(16))) int s_bad[4];         // each wave's first row that the form does not hold, 64: none
     const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4, g4 = g * 4;
@@ -697,7 +694,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
 #pragma unroll
                         for (int i = 0; i < NP; i++) a[i] = *(const bf168 *)(K + row_at[kb % KINDS] + i * X::PLANE + kb / KINDS * 256);
-                        la_mac<2>(a, b, ks[kb & 1]);
+                        la_mac(a, b, ks[kb & 1]);
                     }
                     acc = ks[0] + ks[1];
                 }
@@ -741,7 +738,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                         bf168 b[3];
 #pragma unroll
                         for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_x[tb][i][at];
-                        la_mac<2>(tf[tb], b, us[tb]);
+                        la_mac(tf[tb], b, us[tb]);
                     }
                     ask_t(c + 1);
                     const f32x4 u = us[0] + us[1];
@@ -749,16 +746,17 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                     for (int r = 0; r < 4; r++) x[r] = u[r];
                 }
                 {
-                    __bf16 p[NO][4], pe[3][4];
+                    __bf16 p[3][4], pe[3][4];
                     float xe[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) xe[r] = x[r] * ke[r];
-                    la_split<NO, 4>(x, p);
+                    la_split<3, 4>(x, p);
                     la_split<3, 4>(xe, pe);
 #pragma unroll
-                    for (int i = 0; i < NO; i++) *(s16x4 *)&s_u[rt >> 1][i][half] = *(const s16x4 *)p[i];
-#pragma unroll
-                    for (int i = 0; i < 3; i++) *(s16x4 *)&s_e[rt >> 1][i][half] = *(const s16x4 *)pe[i];
+                    for (int i = 0; i < 3; i++) {
+                        *(s16x4 *)&s_u[rt >> 1][i][half] = *(const s16x4 *)p[i];
+                        *(s16x4 *)&s_e[rt >> 1][i][half] = *(const s16x4 *)pe[i];
+                    }
                 }
                 __syncthreads();
                 upto = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
@@ -788,7 +786,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                                         (__attribute__((address_space(3))) s16x4 *)(K + col_at + i * X::PLANE + (32 * tb + 16 * u) * DK * 2 + 256 * o + 8 * h));
                                 av[i] = a[i].v;
                             }
-                            la_mac<2>(av, b, s[o][h]);
+                            la_mac(av, b, s[o][h]);
                         }
                 }
                 publish();
@@ -802,7 +800,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
             constexpr int MINE = X::Q / LA_FRAG / 4;
             // (256 fp32 channels: Q where it is used, or registers spill: 2 x 2048 tokens of 4 heads 355 us against 577)
             constexpr bool HOLD = NKB * NP <= 16;
-            bf168 qf[NKB][NP], pf[2][NO];
+            bf168 qf[NKB][NP], pf[2][3];
             f32x4 qd, kr[MINE], vec;
             float v[4];
             auto ask_q = [&](int i) {
@@ -815,7 +813,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 const uint8_t *p = heads(i);
                 qd = *(const QMAG_GLOBAL f32x4 *)(p + Y::QD + 64 * rt + (at >> 8) * 16);
 #pragma unroll
-                for (int tb = 0; tb < 2; tb++) la_load<NO>(p + Y::P + la_tri(rt, rt < 2 ? 0 : tb) * NO * LA_FRAG, pf[tb]);
+                for (int tb = 0; tb < 2; tb++) la_load<3>(p + Y::P + la_tri(rt, rt < 2 ? 0 : tb) * 3 * LA_FRAG, pf[tb]);
             };
             auto ask_k = [&](int i) {
 #pragma unroll
@@ -849,11 +847,11 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 f32x4 qs[2] = {};
 #pragma unroll
                 for (int kb = 0; kb < NKB; kb++) {
-                    bf168 b[UP + 1];
+                    bf168 b[3];
 #pragma unroll
-                    for (int i = 0; i <= UP; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
+                    for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_s[kb][i][at];
                     if constexpr (!HOLD) la_load<NP>(keys(c) + X::Q + (rt * NKB + kb) * NP * LA_FRAG, qf[kb]);
-                    la_mac<UP>(qf[kb], b, qs[kb & 1]);
+                    la_mac(qf[kb], b, qs[kb & 1]);
                 }
                 ask_q(c + 1);
                 f32x4 o = (qs[0] + qs[1]) * qd;
@@ -873,10 +871,10 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) {
                     if (2 * tb > rt) continue;
-                    bf168 b[NO];
+                    bf168 b[3];
 #pragma unroll
-                    for (int i = 0; i < NO; i++) b[i] = *(const bf168 *)&s_u[tb][i][at];
-                    la_mac<UP>(pf[tb], b, o);
+                    for (int i = 0; i < 3; i++) b[i] = *(const bf168 *)&s_u[tb][i][at];
+                    la_mac(pf[tb], b, o);
                 }
                 ask_p(c + 1);
                 if constexpr (!DELTA && BUFS == 2) {
@@ -930,7 +928,7 @@ static size_t la_tile_bytes(int type, int dim_k, int n_key, int n_head)
     with_type(type, [&](auto t) {
         return with_dim_k(dim_k, [&](auto d) {
             using TT = decltype(t);
-            bytes = (size_t)n_key * LaKeys<TT, decltype(d)::value>::BYTES + (size_t)n_head * (LaLayout<TT>::HEAD_BYTES + 64);
+            bytes = (size_t)n_key * LaKeys<TT, decltype(d)::value>::BYTES + (size_t)n_head * (LaLayout::HEAD_BYTES + 64);
             return 0;
         });
     });
@@ -1034,7 +1032,7 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
                 const int64_t wgs = ((int64_t)A.n_long * A.n_key + 7) / 8 * 8 * A.share * (a->dim_v / 16);
                 const unsigned grid = (unsigned)(wgs < 2048 ? wgs : 2048);
                 A.heads = A.keys + (size_t)A.n_tile * (size_t)A.n_key * LaKeys<TT, DK>::BYTES;
-                A.left = (int *)(A.heads + (size_t)A.n_tile * (size_t)A.n_head * LaLayout<TT>::HEAD_BYTES);
+                A.left = (int *)(A.heads + (size_t)A.n_tile * (size_t)A.n_head * LaLayout::HEAD_BYTES);
                 A.carry_in = carry + (odd ? state / sizeof(float) : 0);
                 A.carry_out = carry + (odd ? 0 : state / sizeof(float));
                 const unsigned tiles = (unsigned)A.n_tile * (unsigned)A.n_key;
