@@ -198,6 +198,21 @@ template <class T> constexpr int LA_PARTS = 3;
 template <> constexpr int LA_PARTS<TF16> = 2;
 template <> constexpr int LA_PARTS<TBF16> = 1;
 
+// What the chunks' products hold; anything else goes token by token, from the row that has it or, for a state, the chunk
+// ahead of which it has grown so.  K and Q are multiplied as they are read, their norms' inverses come after, so that
+//   K S, Q S          |k| |s| sqrt(dim_k) <= 2^(40 + 80 + 4)
+// is what stays in fp32's range by the least.  With k', q' the keys and queries that the formula has (normalised or not),
+// and b |k'|^2 <= 2.01 for the delta rule, whose b |k'| is then 2^10.5 at most, and whose state so at most doubles in a chunk:
+//   U                 b (|v| + |k'| |S|) <= 2^96 (2^60 without the delta rule); its terms in T X 64 times 2^97
+//   u_j |k'_j|        2^86 (2^80), and as much is added to the state; divided by |k_j|, as it meets K, 2^116
+//   P U               64 scale |q'| 2^86 <= 2^122
+// and none of it is above 2^124.  From the smallest k', q' and scale on P's third part is above bf16's smallest, 2^-133.
+constexpr float LA_MOST_ROW = 0x1p80f;           // |k|^2, |q|^2 as they are read
+constexpr float LA_MOST_KEY = 0x1p40f, LA_LEAST_KEY = 0x1p-80f;      // |k'|^2, |q'|^2 that are not 0
+constexpr float LA_LEAST_ROW = 0x1p-60f;         // with the norm, |k|^2 and |q|^2 that are not 0: squares lose digits
+constexpr float LA_MOST_BETA = 0x1p20f, LA_MOST_V = 0x1p40f, LA_MOST_STATE = 0x1p80f;
+constexpr float LA_MOST_SCALE = 0x1p10f, LA_LEAST_SCALE = 0x1p-30f;
+
 // Operands lie in the workspace as the matrix cores take them: 64 lanes of 16 bytes.
 constexpr int LA_FRAG = 1024;
 constexpr int LA_TRI = 6;             // operands of a lower triangle: 16 rows by 32 columns, those all above it left out
@@ -397,9 +412,10 @@ __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kern
     const int64_t row0 = at.rows.first + 64 * (int64_t)at.chunk;
 
     uint8_t *mine = A.keys + ((int64_t)tile * A.n_key + key) * LaKeys<T, DK>::BYTES;
-    // rows of K and Q as operands, their sums of squares
+    // rows of K and Q as operands, their sums of squares, and the bits that any of their values has
     bf168 kf[NKB][NP], qf[NKB][NP];
     float kk = 0.0f, qq = 0.0f;
+    uint32_t kn = 0, qn = 0;
     const int my = 16 * w + l16;
     const S *kp = (const S *)A.k.p + (row0 + min(my, n - 1)) * A.k.ts + key * A.k.hs + 8 * g;
     const S *qp = (const S *)A.q.p + (row0 + min(my, n - 1)) * A.q.ts + key * A.q.hs + 8 * g;
@@ -418,6 +434,8 @@ __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kern
         for (int e = 0; e < 8; e++) {
             kk = fmaf(x[e], x[e], kk);
             qq = fmaf(y[e], y[e], qq);
+            kn |= __float_as_uint(x[e]);
+            qn |= __float_as_uint(y[e]);
         }
         la_split8<NP>(x, kf[kb]);
         la_split8<NP>(y, qf[kb]);
@@ -431,15 +449,21 @@ __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kern
     kk = la_sum4(kk);
     qq = la_sum4(qq);
     const bool norm = A.norm_eps > 0.0f;
+    // whether the row, which four lanes have, is other than zeros (whose squares' sum is 0 too where they are small)
+    constexpr uint64_t ROW_LANES = 0x0001000100010001ull;
+    const bool some_k = (__ballot(kn << 1 != 0) >> l16 & ROW_LANES) != 0, some_q = (__ballot(qn << 1 != 0) >> l16 & ROW_LANES) != 0;
     if (lane < 16) {
+        // (a key of zeros adds nothing whatever it is multiplied by)
         s_kk[my] = norm ? kk / (kk + A.norm_eps) : kk;
-        s_fk[my] = norm ? rsqrtf(kk + A.norm_eps) : 1.0f;
-        s_fq[my] = norm ? rsqrtf(qq + A.norm_eps) : 1.0f;
+        s_fk[my] = !some_k ? 0.0f : norm ? rsqrtf(kk + A.norm_eps) : 1.0f;
+        s_fq[my] = !some_q ? 0.0f : norm ? rsqrtf(qq + A.norm_eps) : 1.0f;
     }
-    // From a row whose values the products' fp32 sums, or the sums of squares, do not hold on the chunk goes token by
-    // token; the rows ahead of it are as if there were none behind.
-    constexpr float MOST = 0x1p80f, LEAST = 0x1p-60f;
-    const uint64_t odd = __ballot(!(kk <= MOST) || !(qq <= MOST) || (norm && ((kk > 0.0f && kk < LEAST) || (qq > 0.0f && qq < LEAST))));
+    // From a row that is not held on the chunk goes token by token; the rows ahead of it are as if there were none behind.
+    auto held = [&](float sum, bool some) {
+        const float key = norm ? sum / (sum + A.norm_eps) : sum;
+        return !some || (sum <= LA_MOST_ROW && (!norm || sum >= LA_LEAST_ROW) && key <= LA_MOST_KEY && key >= LA_LEAST_KEY);
+    };
+    const uint64_t odd = __ballot(!held(kk, some_k) || !held(qq, some_q));
     if (lane == 0) s_odd[w] = odd ? 16 * w + (__ffsll((unsigned long long)odd) - 1) % 16 : 64;
     __syncthreads();
     const int even = min(min(s_odd[0], s_odd[1]), min(s_odd[2], s_odd[3]));
@@ -481,7 +505,7 @@ __global__ void __launch_bounds__(256, (LA_CHUNK_WGS<T, DK>)) linattn_chunk_kern
             const double all = __shfl(sum, 63);
             const float bk = b * s_kk[lane];
             // the delta rule grows past b |k|^2 = 2, and its inverse with it
-            const bool out = none || (DELTA ? !(bk >= 0.0f && bk <= 2.01f) || !(b <= 0x1p60f) : !(fabsf(b) <= 0x1p40f));
+            const bool out = none || !(fabsf(b) <= LA_MOST_BETA) || (DELTA && !(bk >= 0.0f && bk <= 2.01f));
             const uint64_t bad = __ballot(out);
             s_g[w][lane] = sum;
             s_b[w][lane] = b;
@@ -641,7 +665,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 for (int r = 0; r < 4; r++) {
                     s[o][h][r] = 0.0f;
                     if (chain && kb < NKB && st.from) s[o][h][r] = ldg(st.from + (int64_t)(32 * kb + 8 * g + 4 * h + r) * A.dim_v + c0 + l16);
-                    odd |= !(fabsf(s[o][h][r]) <= 0x1p100f);
+                    odd |= !(fabsf(s[o][h][r]) <= LA_MOST_STATE);
                 }
         }
         auto publish = [&]() {
@@ -660,6 +684,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
         };
         publish();
         int c = 0, upto = 0;                              // the first chunk that is not done, the first such row of it
+        bool wide = false;                                // the wave's part of the state is not held any more
         const bool go = !__syncthreads_or(odd);
         auto heads = [&](int i) { return A.heads + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_head + head) * Y::HEAD_BYTES; };
         auto keys = [&](int i) { return A.keys + ((int64_t)(tile0 + min(i, chunks - 1)) * A.n_key + key) * X::BYTES; };
@@ -708,7 +733,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                 for (int r = 0; r < 4; r++) {
                     // (b is 0 behind the sequence's end)
                     x[r] = bt[r] * (DELTA ? fmaf(-kd[r], acc[r], v[r]) : v[r]);
-                    odd |= !(fabsf(v[r]) <= 0x1p60f);
+                    odd |= !(fabsf(v[r]) <= LA_MOST_V);
                 }
                 int bad = 64;
                 if (__ballot(odd)) {
@@ -716,7 +741,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
 #pragma unroll
                     for (int r = 3; r >= 0; r--) {
                         const int row = 16 * rt + g4 + r;
-                        const bool fine = fabsf(v[r]) <= 0x1p60f;
+                        const bool fine = fabsf(v[r]) <= LA_MOST_V;
                         if (row < left && !fine) bad = min(bad, row);
                         if (row >= left || !fine) x[r] = 0.0f;              // not even times 0 in the rows ahead
                     }
@@ -728,7 +753,7 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
 #pragma unroll
                     for (int i = 0; i < 3; i++) *(s16x4 *)&s_x[rt >> 1][i][half] = *(const s16x4 *)p[i];
                 }
-                if (lane == 0) s_bad[rt] = bad;
+                if (lane == 0) s_bad[rt] = wide ? 0 : bad;            // a chunk from a state that is not held is left out
                 if constexpr (DELTA) {
                     __syncthreads();
                     f32x4 us[2] = {};
@@ -789,6 +814,14 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
                             la_mac(av, b, s[o][h]);
                         }
                 }
+                float most = 0.0f;
+#pragma unroll
+                for (int o = 0; o < OWN; o++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) most = fmaxf(most, fabsf(s[o][h][r]));
+                wide = __ballot(most > LA_MOST_STATE) != 0;
                 publish();
                 __syncthreads();
                 if constexpr (BUFS == 1) __syncthreads();
@@ -898,8 +931,9 @@ __global__ void __launch_bounds__(512, (2 * LaRoom<T, DK>::WGS)) linattn_chain_k
             }
         }
         // a row with values that the products do not hold, or a state: all is left as it was from there on
-        if (threadIdx.x == 0) A.left[((int64_t)tile0 * A.n_head + head) * slices + c0 / 16] = c < chunks ? 64 * c + upto : -1;
-        if (c >= chunks && chain && st.to) {
+        const bool grown = __syncthreads_or(wide);
+        if (threadIdx.x == 0) A.left[((int64_t)tile0 * A.n_head + head) * slices + c0 / 16] = c < chunks ? 64 * c + upto : grown ? rows.n : -1;
+        if (c >= chunks && !grown && chain && st.to) {
 #pragma unroll
             for (int o = 0; o < OWN; o++)
 #pragma unroll
@@ -996,7 +1030,7 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
     const int64_t slices = (int64_t)n_seq * a->n_head * (a->dim_v / 16);
     // prompts in chunks; few tokens to a sequence one after another
     A.brief = la_brief(slices, type == QMAG_TYPE_F32);
-    const bool chunks = la_cut(T, n_seq, A.brief);
+    const bool chunks = la_cut(T, n_seq, A.brief) && fabsf(scale) >= LA_LEAST_SCALE && fabsf(scale) <= LA_MOST_SCALE;
     size_t state = 0;
     int window = 0;
     if (chunks) {
