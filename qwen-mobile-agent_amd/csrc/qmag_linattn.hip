@@ -44,6 +44,7 @@
 //   workgroups to a CU at 3.2 us each.
 //   Not kept in the walk, at 200 us for fp32 and 245 for bf16: operands by transfers
 //   straight to LDS, by 4 waves more (227, 325); Q and K split into parts there (244, 395).
+#include <float.h>
 #include <math.h>
 
 #include "qmag_rows.h"
@@ -149,12 +150,28 @@ __device__ void la_recurrence(const LaArgs &A, int head, int c0, int first, int 
         if (A.norm_eps > 0.0f) {
             // ahead of the products: a large key's would leave fp32's range
             float kk = 0.0f, qq = 0.0f;
+            auto squares = [&]() {
+                kk = qq = 0.0f;
 #pragma unroll
-            for (int r = 0; r < N; r++) {
-                kk = fmaf(x.k[r], x.k[r], kk);
-                qq = fmaf(x.q[r], x.q[r], qq);
+                for (int r = 0; r < N; r++) {
+                    kk = fmaf(x.k[r], x.k[r], kk);
+                    qq = fmaf(x.q[r], x.q[r], qq);
+                }
+                kk = group_sum<16>(kk);
+                qq = group_sum<16>(qq);
+            };
+            squares();
+            float ek = A.norm_eps, eq = A.norm_eps;
+            if (__ballot(!(kk + qq <= FLT_MAX))) {
+                // a row whose squares do so themselves is taken times 2^-70, and its eps with it
+                const float fk = kk <= FLT_MAX ? 1.0f : 0x1p-70f, fq = qq <= FLT_MAX ? 1.0f : 0x1p-70f;
+#pragma unroll
+                for (int r = 0; r < N; r++) x.k[r] *= fk, x.q[r] *= fq;
+                ek = ek * fk * fk;
+                eq = eq * fq * fq;
+                squares();
             }
-            const float rk = rsqrtf(group_sum<16>(kk) + A.norm_eps), rq = rsqrtf(group_sum<16>(qq) + A.norm_eps);
+            const float rk = rsqrtf(kk + ek), rq = rsqrtf(qq + eq);
 #pragma unroll
             for (int r = 0; r < N; r++) x.k[r] *= rk, x.q[r] *= rq;
         }
