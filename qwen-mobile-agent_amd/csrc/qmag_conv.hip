@@ -53,11 +53,14 @@ __device__ __forceinline__ void store_some(typename T::S *p, int n, const float 
     }
 }
 
-// y / (1 + e^-y), both sides times 2^-64, so that what is divided by has no reciprocal below fp32's normal numbers
-// while the result has
+// y / (1 + e^-y), e^-y as a square, so that it does not leave fp32's range where the result is above its smallest normal
+// number (y of -92), both sides times 2^-8, so that what is divided by has a normal reciprocal there; y itself loses
+// digits to that below 2^-118 only, 2^-143 at most.  (Two scales chosen by a comparison: 24.4 us for 5003 tokens of 4100
+// bf16 channels against 23.)
 __device__ __forceinline__ float conv_silu(float y)
 {
-    return (y * 0x1p-64f) * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(y * -1.44269504088896340736f), 0x1p-64f, 0x1p-64f));
+    const float half = __builtin_amdgcn_exp2f(y * -0.72134752044448170368f) * 0x1p-4f;      // e^(-y/2) / 16
+    return (y * 0x1p-8f) * __builtin_amdgcn_rcpf(fmaf(half, half, 0x1p-8f));
 }
 
 // a tile's channels from c0 on: V of them, or the row's last nc.  Rows are asked for 16 values ahead of those at work:
