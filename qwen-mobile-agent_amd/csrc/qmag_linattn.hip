@@ -239,6 +239,7 @@ constexpr int la_tri(int rt, int tb) { return rt < 2 ? rt : 2 * rt - 2 + tb; }
 template <class T, int DK>
 struct LaKeys {
     static constexpr int K = 0, PLANE = 64 * DK * 2, Q = LA_PARTS<T> * PLANE, BYTES = 2 * Q;
+    static_assert(BYTES == la_key_bytes(LA_PARTS<T>, DK));
 };
 // Where 16 bytes of a row of K lie, in 16 bytes: 16 rows' of one piece in different banks, and so four rows' of four
 // pieces side by side, which a transposing read takes.
@@ -254,6 +255,7 @@ struct LaLayout {
     static constexpr int KD = 0, KE = 64, B = 128, END = 192, BAD = 193;     // floats of VEC; END: e^G_63; BAD: the first row the form does not hold, 64: none
     static constexpr int HEAD_BYTES = QD + 256;
 };
+static_assert(LaLayout::HEAD_BYTES == LA_HEAD_BYTES);
 
 // x as N parts, the first the nearest bf16 to it, each other to what those ahead leave
 template <int N, int V>
@@ -970,22 +972,6 @@ static int with_dim_k(int dim, F f)
     return f(std::integral_constant<int, 256>{});
 }
 
-constexpr size_t LA_WORKSPACE = (size_t)1 << 30;
-
-// bytes of the workspace for a chunk number
-static size_t la_tile_bytes(int type, int dim_k, int n_key, int n_head)
-{
-    size_t bytes = 0;
-    with_type(type, [&](auto t) {
-        return with_dim_k(dim_k, [&](auto d) {
-            using TT = decltype(t);
-            bytes = (size_t)n_key * LaKeys<TT, decltype(d)::value>::BYTES + (size_t)n_head * (LaLayout::HEAD_BYTES + 64);
-            return 0;
-        });
-    });
-    return bytes;
-}
-
 }  // namespace qmag
 
 using namespace qmag;
@@ -1047,16 +1033,14 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
     const int64_t slices = (int64_t)n_seq * a->n_head * (a->dim_v / 16);
     // prompts in chunks; few tokens to a sequence one after another
     A.brief = la_brief(slices, type == QMAG_TYPE_F32);
-    const bool chunks = la_cut(T, n_seq, A.brief) && fabsf(scale) >= LA_LEAST_SCALE && fabsf(scale) <= LA_MOST_SCALE;
-    size_t state = 0;
-    int window = 0;
+    const int parts = with_type(type, [](auto t) { return LA_PARTS<decltype(t)>; });
+    const size_t tile = la_tile_bytes(parts, a->dim_k, q->n_head, a->n_head);
+    const size_t state = sizeof(float) * (size_t)a->n_head * (size_t)a->dim_k * (size_t)a->dim_v;
+    const bool cut = la_cut(T, n_seq, A.brief) && fabsf(scale) >= LA_LEAST_SCALE && fabsf(scale) <= LA_MOST_SCALE;
+    const int window = cut ? la_window(T, n_seq, A.brief, tile, state) : 0;
+    const bool chunks = window > 0;
     if (chunks) {
-        // windows that keep the workspace under a bound
-        const size_t per = la_tile_bytes(type, a->dim_k, q->n_head, a->n_head);
-        state = sizeof(float) * (size_t)a->n_head * (size_t)a->dim_k * (size_t)a->dim_v;
-        window = (int)(((int64_t)T + LA_CHUNK - 1) / LA_CHUNK < (1 << 20) ? (T + LA_CHUNK - 1) / LA_CHUNK * LA_CHUNK : 1 << 26);
-        while (window > 4 * LA_CHUNK && (size_t)la_most_tiles(window, n_seq, A.brief) * per > LA_WORKSPACE) window = window / (2 * LA_CHUNK) * LA_CHUNK;
-        uint8_t *p = (uint8_t *)workspace(WS_LINATTN, (size_t)la_most_tiles(window, n_seq, A.brief) * per + (T > window ? 2 * state : 0), &st);
+        uint8_t *p = (uint8_t *)workspace(WS_LINATTN, la_workspace(window, T, n_seq, A.brief, tile, state), &st);
         if (st) return st;
         A.carry_in = (float *)p;
         A.keys = p + (T > window ? 2 * state : 0);

@@ -9,6 +9,7 @@
 // ceil(n / 64) <= (n >> 6) + 1, so that no two share a number.
 #pragma once
 
+#include <stddef.h>
 #include <stdint.h>
 
 #include "qmag_seq.h"
@@ -59,6 +60,34 @@ constexpr int la_most_tiles(int rows, int n_seq, int brief) { return (rows >> LA
 constexpr bool la_room(int rank, int tile0, int chunks, int most_long, int most_tiles)
 {
     return rank < most_long && tile0 + chunks <= most_tiles;
+}
+
+
+// ------------------------------------------------------------- workspace --
+// What a chunk has there, in bytes: for each key head K's and Q's parts (three bf16 of an fp32 value, two of an fp16 one,
+// one of a bf16 one); for each head the triangle's inverse and P, three parts of 6 operands of 1 KB each, 1280 bytes of
+// vectors, and 64 for a row's place in each of up to 16 slices of columns.
+constexpr size_t la_key_bytes(int parts, int dim_k) { return (size_t)2 * parts * LA_CHUNK * dim_k * 2; }
+constexpr size_t LA_HEAD_BYTES = 2 * 6 * 3 * 1024 + 1280;
+constexpr size_t la_tile_bytes(int parts, int dim_k, int n_key, int n_head)
+{
+    return (size_t)n_key * la_key_bytes(parts, dim_k) + (size_t)n_head * (LA_HEAD_BYTES + 64);
+}
+
+// A call's workspace is at most this; calls of more rows than it holds the chunks of go window by window, and have two
+// states of `state` bytes there to hand on.
+constexpr size_t LA_WORKSPACE = (size_t)1 << 30;
+constexpr size_t la_workspace(int window, int T, int n_seq, int brief, size_t tile, size_t state)
+{
+    return (size_t)la_most_tiles(window, n_seq, brief) * tile + (T > window ? 2 * state : 0);
+}
+// The rows of a window, whole chunks; 0: not even two chunks are held (heads by the thousand, whose sequences fill the
+// chip token by token, which takes no workspace).
+constexpr int la_window(int T, int n_seq, int brief, size_t tile, size_t state)
+{
+    int window = ((int64_t)T + LA_CHUNK - 1) / LA_CHUNK < (1 << 20) ? (T + LA_CHUNK - 1) / LA_CHUNK * LA_CHUNK : 1 << 26;
+    while (window > 0 && la_workspace(window, T, n_seq, brief, tile, state) > LA_WORKSPACE) window = window / (2 * LA_CHUNK) * LA_CHUNK;
+    return window >= 2 * LA_CHUNK || window >= T ? window : 0;
 }
 
 }  // namespace qmag
