@@ -1032,8 +1032,8 @@ extern "C" int qmag_linattn_dev(const qmag_linattn *a, int type, const qmag_head
     hipStream_t s = ctx().stream;
     const int64_t slices = (int64_t)n_seq * a->n_head * (a->dim_v / 16);
     // prompts in chunks; few tokens to a sequence one after another
-    A.brief = la_brief(slices, type == QMAG_TYPE_F32);
     const int parts = with_type(type, [](auto t) { return LA_PARTS<decltype(t)>; });
+    A.brief = la_brief(slices, parts);
     const size_t tile = la_tile_bytes(parts, a->dim_k, q->n_head, a->n_head);
     const size_t state = sizeof(float) * (size_t)a->n_head * (size_t)a->dim_k * (size_t)a->dim_v;
     const bool cut = la_cut(T, n_seq, A.brief) && fabsf(scale) >= LA_LEAST_SCALE && fabsf(scale) <= LA_MOST_SCALE;

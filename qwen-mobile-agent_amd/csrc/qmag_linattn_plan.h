@@ -22,10 +22,17 @@ constexpr int LA_CHUNK = 64, LA_SHIFT = 6;
 // columns of a head and sequence each.  Few waves wait for one another's sums, some 0.7 us
 // a token, and a chunk takes 26 us whatever rows it has (one sequence of 32 heads and 128
 // channels fp32, tokens and a chunk: 27 us and 26 for 32 rows, 50 and 26 for 64).  Where
-// the chip is full a token costs what it computes, and a chunk what begins and ends it: 64
-// such sequences in fp32, one workgroup to a CU, of 64 rows 468 and 638, of 96 689 and 830,
-// of 128 910 and 840; in bf16, two to a CU, of 32 rows 242 and 293, of 48 350 and 307.
-constexpr int la_brief(int64_t waves, bool wide) { return waves <= 1024 ? 32 : wide ? 96 : 40; }
+// the chip is full a token costs what it computes, and a chunk what its type's bf16 parts
+// (3, 2 or 1) make of it.  Sequences alike, us token by token (4 to 15 more where the call
+// is cut all the same) and in chunks:
+//   heads, channels           fp32 64 rows  96 rows   fp16 48 rows  56 rows   bf16 40 rows  48 rows
+//   64 of 32 over 16, 64         187  278  274  368      145  173  166  178     123  155  148  155
+//   64 of 32 over 16, 128        480  624  699  826      381  523  446  525     330  330  381  330
+//   64 of 8 over 4, 256          452  442  641  691      339  349  395  340     294  271  335  272
+//   16 of 32 over 16, 64          64   77   93   93       51   57   59   57      42   52   49   52
+//   16 of 32 over 16, 128        144  150  208  189      116  132  132  133      99   92  117   92
+//   16 of 8 over 4, 256          131  129  186  175      100  107  115  108      86   87  100   86
+constexpr int la_brief(int64_t waves, int parts) { return waves <= 1024 ? 32 : parts == 3 ? 96 : parts == 2 ? 48 : 40; }
 // Whether a call is cut: its sequences have more rows than that on average, or one of them
 // may have many more, the others a row each.  A prompt of 512 tokens beside 31 single
 // ones takes 81 us, token by token 436; where none is long after all, the launches that

@@ -18,7 +18,7 @@ class Wide:
 
     def __init__(self, qm, t, delta, dk, n_seq=4, slots=(3, 1, 0, 2)):
         r = rng_of(t, delta, dk, 51)
-        (self.window, _, self.brief), = windows([(ROWS, n_seq, HEADS, HEADS, dk, DV, PARTS[t], t == F32)])
+        (self.window, _, self.brief), = windows([(ROWS, n_seq, HEADS, HEADS, dk, DV, PARTS[t])])
         self.n_windows = -(-ROWS // self.window)
         assert self.n_windows >= 3
         # the second sequence ends in the last window but one, a few rows behind its border; the third begins there
