@@ -53,7 +53,7 @@ METRIC = "MoE FFN decode tokens/s + achieved HBM GB/s (% of peak), Q4_K/Q6_K, 1 
 FUSED_TRAFFIC = {"bytes": 869.5e6, "profile": "profiles/moe_decode_kernel_c4_hbm_counters.md",
                  "sources": ["qwen-mobile-agent_amd/csrc/qmag_fused.hip", "qwen-mobile-agent_amd/csrc/qmag_device.h",
                              "qwen-mobile-agent_amd/csrc/qmag_internal.h"],
-                 "source_sha16": "60ab1d2219df97f2"}
+                 "source_sha16": "8d2fe082e4646f54"}
 
 
 def fused_source_sha16():
