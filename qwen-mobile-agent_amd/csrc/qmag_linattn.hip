@@ -40,8 +40,8 @@
 //   prompts, fp32, 4096 tokens: 54 us for all chunks' matrices, 179 MB written and read
 //   back, and 183 for the walk, 64 chunks in a row of 2.9 us: three products of 6 pairs
 //   of parts that wait for one another through LDS, with a barrier after each.
-//   8192 tokens of 7 prompts, bf16: 60 and 206 us, the chip full of chunks of two
-//   workgroups to a CU at 3.2 us each.
+//   8192 tokens of 7 prompts, bf16: 65 and 237 us, the chip full of chunks of two
+//   workgroups to a CU at 3.7 us each (two parts of what a 16-bit result is made of: 206).
 //   Not kept in the walk, at 200 us for fp32 and 245 for bf16: operands by transfers
 //   straight to LDS, by 4 waves more (227, 325); Q and K split into parts there (244, 395).
 #include <float.h>
@@ -407,7 +407,8 @@ constexpr double LOG2E = 1.4426950408889634;
 __device__ __forceinline__ float la_power(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
 // workgroups to a CU, as many as their LDS leaves, three at most: more than two waves to a SIMD take fewer registers than
-// the compiler would (8192 tokens bf16 60 us with three, 72 with two)
+// the compiler would (8192 tokens bf16, three: 146 registers, two: 159, which leave three workgroups their places too and
+// take as long, 65 us; with more than 168 they took 72)
 template <class T, int DK>
 constexpr int LA_CHUNK_WGS = 160 * 1024 / (LA_PARTS<T> * 128 * (DK + 8) + 28 * 1024) < 3 ? 160 * 1024 / (LA_PARTS<T> * 128 * (DK + 8) + 28 * 1024) : 3;
 
