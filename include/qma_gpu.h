@@ -711,8 +711,9 @@ int qmag_conv_dev(const qmag_conv *c, int type, const void *x, int64_t x_stride,
    forgets all there was), or NULL: none.  beta: f32 [T][n_head], or NULL: 1.  With
    norm_eps > 0, q and k are taken times (sum of their squares + norm_eps)^-1/2.
    All in fp32, a 16-bit result rounded once from it: products on the matrix cores
-   hold 2^-22 and better of each operand.  Prompts take a workspace (at most 1 GiB,
-   kept), a window of them at a time.
+   hold 2^-22 and better of each operand.  q . k and the products of q and k with
+   the state are such numbers: where one leaves fp32's range, its results do.
+   Prompts take a workspace (at most 1 GiB, kept), a window of them at a time.
    A NaN or infinity at a token has no effect on tokens ahead of it, on other
    heads' states or other sequences; what follows it is as the recurrence has it.
    q, k and v may be views of one buffer; out overlaps nothing that is read, the

@@ -1,4 +1,5 @@
 """The host's arithmetic of linear attention's chunks (qmag_linattn_plan.h), compiled for the tests."""
+import atexit
 import os
 import shutil
 import subprocess
@@ -37,6 +38,7 @@ def windows(calls):
         pytest.skip("no host compiler")
     if _exe is None:
         d = tempfile.mkdtemp(prefix="linattn_plan")
+        atexit.register(shutil.rmtree, d, ignore_errors=True)
         src = os.path.join(d, "ask.cpp")
         with open(src, "w") as f:
             f.write(ASK)
